@@ -146,6 +146,8 @@ def lib() -> ctypes.CDLL:
     L.hipgemm_quantize_rows_e4m3.argtypes = [vp, ci, ci, ci, ctypes.c_longlong,
                                              vp, vp, vp]
     L.hipgemm_quantize_rows_e4m3.restype = ci
+    L.hipgemm_w4_gemm.argtypes = [ctypes.c_void_p, vp]
+    L.hipgemm_w4_gemm.restype = ci
     L.hipgemm_workspace_size.argtypes = [ci, ci, ci, ci]
     L.hipgemm_workspace_size.restype = ctypes.c_size_t
     L.hipgemm_fp8_gemm_4wave_256x256x128.argtypes = [vp, vp, vp, ci, ci, ci,
@@ -640,3 +642,10 @@ def fp8_gemm_4wave_256x256x128(A, B_T, C, stream=None):
         stream.cuda_stream or None))
     _check(code, "hipgemm_fp8_gemm_4wave_256x256x128")
     return C
+
+
+# (after everything that it uses of this module)
+from .serving import *  # noqa: E402,F401,F403
+from . import serving as _serving  # noqa: E402
+
+__all__ += _serving.__all__

@@ -1,0 +1,15 @@
+// Products of f16 activations with int4 weights.
+#include "kw4.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* w4_vec_f16_int4(int s, int rows) {
+  return w4_vec_of<detail::kInF16, detail::kWInt4>(s, rows);
+}
+const void* w4_rows_f16_int4(int s, int mode, int mt) {
+  return w4_rows_of<detail::kInF16, detail::kWInt4>(s, mode, mt);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

@@ -1,0 +1,140 @@
+"""Operators of LLM serving with quantised weights and 16-bit activations
+(include/hipgemm.h: hipgemm_w4_gemm and its neighbours), on torch tensors.
+
+w4_gemm      products with 4-bit weights and group scales
+
+Like the rest of the package these run on the GPU only, on the current stream
+or the one given, and raise HipGemmError for arguments that they do not take.
+None of them records a gradient.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+
+from . import (ACTIVATIONS, OUT_BF16, OUT_F16, OUT_F32, HipGemmError, _check,
+               _torch, hipErrorInvalidValue, lib)
+
+__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "W4_FORMATS"]
+
+# include/hipgemm.h codes
+W4_FORMATS = {"int4": 0, "fp4": 1}
+_vp, _ci, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+
+
+class W4Desc(ctypes.Structure):
+    """hipgemm_w4_desc (include/hipgemm.h)."""
+    _fields_ = [("size", ctypes.c_size_t), ("x", _vp), ("weight", _vp),
+                ("scales", _vp), ("zeros", _vp), ("y", _vp), ("bias", _vp),
+                ("M", _ci), ("N", _ci), ("K", _ci), ("group_size", _ci),
+                ("ldx", _ll), ("ldw", _ll), ("lds", _ll), ("ldy", _ll),
+                ("x_type", _ci), ("format", _ci), ("scale_type", _ci),
+                ("out_dtype", _ci), ("activation", _ci)]
+
+
+_W4_BYTES = ctypes.sizeof(W4Desc)
+
+
+@functools.lru_cache(maxsize=1)
+def _types():
+    """Codes by dtype: activations, scales, outputs."""
+    t = _torch()
+    return ({t.bfloat16: 1, t.float16: 2},
+            {t.float32: 0, t.bfloat16: 1, t.float16: 2, t.uint8: 3},
+            {t.bfloat16: OUT_BF16, t.float16: OUT_F16, t.float32: OUT_F32})
+
+
+def _bad(msg: str):
+    raise HipGemmError(msg, hipErrorInvalidValue)
+
+
+def _stream_handle(t, stream) -> int:
+    if stream is not None:
+        return stream.cuda_stream
+    return _torch()._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def w4_gemm_raw(desc: "W4Desc", stream: int = 0) -> int:
+    """Call hipgemm_w4_gemm; returns hipError_t."""
+    return int(lib().hipgemm_w4_gemm(ctypes.byref(desc), stream or None))
+
+
+def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
+            group_size: int = 128, bias=None, activation=None, out_dtype=None,
+            out=None, stream=None):
+    """out[m, n] = round(act(sum_k x[m, k] w[n, k] + bias[n])) with 4-bit
+    weights: w[n, k] = (q[n, k] - zeros[n, k // group_size]) *
+    scales[n, k // group_size] ("int4", q 0-15, zeros 8 where None), or
+    e2m1(q[n, k]) * scales[...] ("fp4").
+
+    x (M, K): bfloat16 or float16, K a multiple of 32.  weight (N, K / 2): uint8,
+    element 2i in the low nibble of byte i (or float4_e2m1fn_x2).  scales
+    (N, ceil(K / group_size)): bfloat16, float16, float32, or uint8 for E8M0
+    (2^(e - 127)); zeros: uint8 of that shape and strides.  group_size: a
+    multiple of 32.  bias: float32 (N).  activation as for gemm().  out_dtype:
+    bfloat16, float16 or float32, x's where None.  Rows have unit stride; those
+    of x and weight start on 16 bytes.  Sums are fp32, weights are not rounded.
+    """
+    torch = _torch()
+    x_types, s_types, o_types = _types()
+    if x.dim() != 2 or weight.dim() != 2 or scales.dim() != 2:
+        _bad("x, weight and scales must be 2-D")
+    (M, K), N = x.shape, weight.shape[0]
+    xt = x_types.get(x.dtype)
+    if xt is None:
+        _bad(f"x must be bfloat16 or float16, got {x.dtype}")
+    fmt = W4_FORMATS.get(format)
+    if fmt is None:
+        _bad(f"format must be one of {sorted(W4_FORMATS)}")
+    if weight.dtype != torch.uint8:
+        if weight.dtype != torch.float4_e2m1fn_x2 or fmt != 1:
+            _bad(f"weight must be uint8 (or float4_e2m1fn_x2 for fp4), got {weight.dtype}")
+    if 2 * weight.shape[1] != K:
+        _bad(f"K mismatch: x has {K}, weight {2 * weight.shape[1]}")
+    if group_size <= 0 or group_size % 32 or K % 32:
+        _bad("K and group_size must be multiples of 32")
+    groups = -(-K // group_size)
+    st = s_types.get(scales.dtype)
+    if st is None or tuple(scales.shape) != (N, groups):
+        _bad(f"scales must be ({N}, {groups}) bfloat16, float16, float32 or uint8, "
+             f"got {tuple(scales.shape)} {scales.dtype}")
+    lds = scales.stride(0) if N > 1 else groups
+    zp = 0
+    if zeros is not None:
+        if fmt != 0:
+            _bad("zeros belong to int4")
+        if zeros.dtype != torch.uint8 or zeros.shape != scales.shape or not zeros.is_cuda:
+            _bad("zeros must be uint8 of the shape of scales, on the GPU")
+        if zeros.stride() != scales.stride() and zeros.numel() > 1:
+            zeros = torch.empty_strided(scales.shape, scales.stride(), dtype=torch.uint8,
+                                        device=zeros.device).copy_(zeros)
+        zp = zeros.data_ptr()
+    if not (x.is_cuda and weight.is_cuda and scales.is_cuda):
+        _bad("x, weight and scales must be device tensors")
+    if ((K > 1 and x.stride(1) != 1) or (K > 2 and weight.stride(1) != 1)
+            or (groups > 1 and scales.stride(1) != 1)):
+        _bad("x, weight and scales must have unit stride along K")
+    if activation not in ACTIVATIONS:
+        _bad(f"activation must be one of {sorted(k for k in ACTIVATIONS if k)}")
+    out_dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    ot = o_types.get(out_dtype)
+    if ot is None:
+        _bad("out_dtype must be bfloat16, float16 or float32")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    elif (out.dtype != out_dtype or tuple(out.shape) != (M, N) or not out.is_cuda
+          or (N > 1 and out.stride(1) != 1)):
+        _bad(f"out must be a ({M}, {N}) {out_dtype} device tensor with unit column stride")
+    bp = 0
+    if bias is not None:
+        if not (bias.is_cuda and bias.dtype == torch.float32 and tuple(bias.shape) == (N,)
+                and (N <= 1 or bias.stride(0) == 1)):
+            _bad(f"bias must be a contiguous float32 device vector of {N} elements")
+        bp = bias.data_ptr()
+    d = W4Desc(_W4_BYTES, x.data_ptr(), weight.data_ptr(), scales.data_ptr(), zp,
+               out.data_ptr(), bp, M, N, K, group_size,
+               x.stride(0) if M > 1 else K, weight.stride(0) if N > 1 else K // 2,
+               lds, out.stride(0) if M > 1 else N, xt, fmt, st, ot,
+               ACTIVATIONS[activation])
+    _check(lib().hipgemm_w4_gemm(ctypes.byref(d), _stream_handle(x, stream)), "hipgemm_w4_gemm")
+    return out

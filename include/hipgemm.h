@@ -362,6 +362,48 @@ hipError_t hipgemm_quantize_rows_e4m3(const void *x, int type, int M, int K,
                                       long long ldx, void *q, float *s,
                                       hipStream_t stream);
 
+/*
+ * Products of 16-bit activations with 4-bit weights:
+ *
+ *   y[m, n] = round_out(activation(sum_k x[m, k] w[n, k] + bias[n]))
+ *   int4: w[n, k] = (q[n, k] - z[n, k / G]) s[n, k / G]
+ *   fp4:  w[n, k] = e2m1(q[n, k]) s[n, k / G]
+ *
+ * x is M x K, bf16 or fp16; q the N x K codes, two per byte, element 2i in the
+ * low nibble of byte i of a row; one scale s (and zero point z, a byte, 8 where
+ * zeros is NULL) per G = group_size neighbouring elements of a row, N x
+ * ceil(K / G).  Products and sums are fp32 and the weights are not rounded: the
+ * scale multiplies the fp32 sum over its group.  bias: N floats or NULL.
+ * Rows of x, q, scales and zeros are contiguous, with the strides given.
+ * Requirements: K % 32 == 0, K <= 2^26, G % 32 == 0, x and q 16-byte aligned
+ * with strides of a multiple of 16 bytes, the others aligned to their element;
+ * out_dtype BF16, F16 or F32.  M == 0 or N == 0 is a no-op, K == 0 gives
+ * activation(bias).  No workspace, no allocation: one launch on `stream`.
+ * Zero-initialise the struct and set `size`.  No reference counterpart (the
+ * reference has e4m3 operands only).
+ */
+enum { HIPGEMM_W4_INT4 = 0, HIPGEMM_W4_FP4 = 1 };
+/* Scale types: HIPGEMM_IN_F32, _BF16, _F16, or E8M0 bytes, 2^(e - 127), 255 NaN. */
+enum { HIPGEMM_SCALE_E8M0 = 3 };
+typedef struct hipgemm_w4_desc {
+  size_t size;
+  const void *x, *weight, *scales;
+  const unsigned char *zeros; /* or NULL */
+  void *y;
+  const float *bias; /* or NULL */
+  int M, N, K, group_size;
+  long long ldx;    /* elements */
+  long long ldw;    /* bytes */
+  long long lds;    /* elements, of zeros too */
+  long long ldy;    /* elements */
+  int x_type;       /* HIPGEMM_IN_BF16 or HIPGEMM_IN_F16 */
+  int format;       /* HIPGEMM_W4_* */
+  int scale_type;   /* HIPGEMM_IN_* or HIPGEMM_SCALE_E8M0 */
+  int out_dtype;    /* HIPGEMM_OUT_* */
+  int activation;   /* HIPGEMM_ACT_* */
+} hipgemm_w4_desc;
+hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc *desc, hipStream_t stream);
+
 /* Workspace bytes hipgemm_fp8_gemm_bf16_ws needs for this shape and variant
  * on the current device (0: none).  No GPU work.  No reference counterpart. */
 size_t hipgemm_workspace_size(int M, int N, int K, int variant);

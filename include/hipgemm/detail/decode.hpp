@@ -1,0 +1,154 @@
+// Quantised weights as 16-bit MFMA operands, for products with 16-bit
+// activations: int4 and fp4 (E2M1) with one scale per group along K, and e4m3.
+//
+// Decoding is exact: every code's value has at most 8 significand bits, so it
+// is a bf16 and an fp16 number, and scales are applied in fp32 after the
+// products.  int4 codes q (0-15, value q - z) are not decoded to q - z, which
+// would cost an addition per pair, but to q + kBias by placing the nibble in
+// the significand of a constant of fixed exponent (one and-or for two): 128 + q
+// in bf16 (significand steps of 1 from 128 up), 64 + q in fp16.  The product's
+// excess is (kBias + z) times the sum of x over the group, which is formed once
+// per group and row of x and subtracted in fp32.
+//
+// The pairs come out in the order (0, 4), (1, 5), (2, 6), (3, 7) of a dword's
+// eight codes, so int4's activations are taken in that order too (pair_order);
+// the sums are the same.
+#pragma once
+
+#include "arch.hpp"
+
+namespace hipgemm {
+namespace detail {
+
+using bf16x8_t = __bf16 __attribute__((ext_vector_type(8)));
+using f16x8_t = _Float16 __attribute__((ext_vector_type(8)));
+using f16x2_t = _Float16 __attribute__((ext_vector_type(2)));
+
+// Types of activations and scales (HIPGEMM_IN_* and HIPGEMM_SCALE_E8M0).
+constexpr int kInF32 = 0, kInBf16 = 1, kInF16 = 2, kScaleE8M0 = 3;
+__host__ __device__ constexpr int type_bytes(int t) {
+  return t == kInF32 ? 4 : t == kScaleE8M0 ? 1 : 2;
+}
+// Weight formats.
+constexpr int kWInt4 = 0, kWFp4 = 1, kWE4M3 = 2;
+
+// The offset that an int4 code carries after decoding to type kX.
+template <int kX>
+constexpr float kInt4Bias = kX == kInBf16 ? 128.0f : 64.0f;
+
+template <int kX>
+__device__ __forceinline__ f32x4 mfma_16x16x32(i32x4 a, i32x4 b, f32x4 c) {
+  if constexpr (kX == kInBf16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        __builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// a.lo * b.lo + a.hi * b.hi + c of two packed pairs, in fp32.
+template <int kX>
+__device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
+  if constexpr (kX == kInBf16)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, a),
+                                           __builtin_bit_cast(bf16x2_t, b), c, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, a),
+                                  __builtin_bit_cast(f16x2_t, b), c, false);
+}
+
+// One packed pair as two floats.
+template <int kX>
+__device__ __forceinline__ f32x2 unpack2(uint32_t a) {
+  if constexpr (kX == kInBf16)
+    return f32x2{__builtin_bit_cast(float, a << 16),
+                 __builtin_bit_cast(float, a & 0xffff0000u)};
+  const f16x2_t h = __builtin_bit_cast(f16x2_t, a);
+  return f32x2{(float)h[0], (float)h[1]};
+}
+
+// 1.0 twice.
+template <int kX>
+constexpr uint32_t kOnes2 = kX == kInBf16 ? 0x3f803f80u : 0x3c003c00u;
+
+// A scale as fp32.  E8M0: 2^(e - 127), 255 is NaN.
+template <int kS>
+__device__ __forceinline__ float scale_at(const void* p, long long i) {
+  if constexpr (kS == kInF32) {
+    return static_cast<const float*>(p)[i];
+  } else if constexpr (kS == kInBf16) {
+    return __builtin_bit_cast(float, (uint32_t) static_cast<const uint16_t*>(p)[i] << 16);
+  } else if constexpr (kS == kInF16) {
+    return (float)static_cast<const _Float16*>(p)[i];
+  } else {
+    const uint32_t e = static_cast<const uint8_t*>(p)[i];
+    return __builtin_bit_cast(float, e == 255u ? 0x7fc00000u : e == 0u ? 0x00400000u : e << 23);
+  }
+}
+
+// Eight codes of a dword (eight bytes for e4m3: lo, hi) as a 16-bit fragment;
+// for fp4 and e4m3 times `scale`, a power of two that the result holds exactly.
+template <int kX, int kW>
+__device__ __forceinline__ i32x4 decode8(uint32_t lo, uint32_t hi, float scale) {
+  i32x4 r;
+  if constexpr (kW == kWInt4) {
+    if constexpr (kX == kInBf16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        r[i] = (int)(((lo >> (4 * i)) & 0x000f000fu) | 0x43004300u);
+    } else {
+      r[0] = (int)(((lo << 4) & 0x00f000f0u) | 0x54005400u);
+      r[1] = (int)((lo & 0x00f000f0u) | 0x54005400u);
+      r[2] = (int)(((lo >> 4) & 0x00f000f0u) | 0x54005400u);
+      r[3] = (int)(((lo >> 8) & 0x00f000f0u) | 0x54005400u);
+    }
+  } else if constexpr (kW == kWFp4) {
+    if constexpr (kX == kInBf16) {
+      r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(lo, scale, 0));
+      r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(lo, scale, 1));
+      r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(lo, scale, 2));
+      r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(lo, scale, 3));
+    } else {
+      r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(lo, scale, 0));
+      r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(lo, scale, 1));
+      r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(lo, scale, 2));
+      r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(lo, scale, 3));
+    }
+  } else {
+    if constexpr (kX == kInBf16) {
+      r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+      r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+      r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+      r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    } else {
+      r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false));
+      r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true));
+      r[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false));
+      r[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true));
+    }
+  }
+  return r;
+}
+
+// Eight activations (four pairs of neighbours) in the order of decode8's pairs.
+template <int kW>
+__device__ __forceinline__ i32x4 pair_order(i32x4 x) {
+  if constexpr (kW != kWInt4) return x;
+  return i32x4{(int)__builtin_amdgcn_perm((uint32_t)x[2], (uint32_t)x[0], 0x05040100u),
+               (int)__builtin_amdgcn_perm((uint32_t)x[2], (uint32_t)x[0], 0x07060302u),
+               (int)__builtin_amdgcn_perm((uint32_t)x[3], (uint32_t)x[1], 0x05040100u),
+               (int)__builtin_amdgcn_perm((uint32_t)x[3], (uint32_t)x[1], 0x07060302u)};
+}
+
+// The value of one 4-bit code, scale excluded (rare paths).
+template <int kW>
+__device__ __forceinline__ float code_value(uint32_t q, float z) {
+  if constexpr (kW == kWInt4) return (float)q - z;
+  const uint32_t m = q & 7u;
+  const float v = m < 2u ? 0.5f * (float)m
+                         : __builtin_bit_cast(float, ((126u + (m >> 1)) << 23) | ((m & 1u) << 22));
+  return q & 8u ? -v : v;
+}
+
+}  // namespace detail
+}  // namespace hipgemm
