@@ -1,0 +1,220 @@
+// The router's choice: for each token the k experts of largest logit, and their
+// weights.
+//
+// Ordering: logits become 32-bit keys whose unsigned order is theirs (-0 as +0,
+// NaN above infinity, -inf as 0: never chosen), kV of them in each of a token's
+// kL lanes, neighbours in one lane.  A round takes the lanes' maxima (three at a
+// time: v_max3_u32), reduces them over the kL lanes by DPP, finds the first lane
+// that has it (so equal logits go to the lowest expert) and clears it there;
+// lane j keeps the j-th result.  Weights are then computed once, in lanes 0 to
+// k - 1.
+//
+// What bounds it: one token is the latency of k rounds; many are instructions,
+// about 5 kV + 12 per round for 64 / kL tokens at once, so that a token's values
+// go to 16 lanes where there are tokens enough to fill the CUs (fewer exchanges
+// per value), to all 64 where there are not.
+#include "hipgemm.h"
+
+#include "kernels.hpp"
+
+#include "hipgemm/detail/decode.hpp"
+
+namespace hipgemm {
+namespace kernels {
+namespace {
+
+using namespace detail;
+
+struct RouteArgs {
+  const uint8_t* logits;
+  float* weights;
+  int* ids;
+  long long ld;  // bytes
+  int T, E, k;
+  int sigmoid, renormalize, vec;
+  float scale;
+};
+
+__device__ __forceinline__ uint32_t key_of(float f) {
+  f += 0.0f;  // -0 -> +0
+  uint32_t b = __builtin_bit_cast(uint32_t, f);
+  if (f != f) b = 0x7fc00000u;
+  b = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return f == -__builtin_inff() ? 0u : b;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  const uint32_t b = key & 0x80000000u ? key & 0x7fffffffu : ~key;
+  return key == 0u ? -__builtin_inff() : __builtin_bit_cast(float, b);
+}
+
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, true);
+}
+// All lanes of a group of kL (16 or 64) get op over the group: exchanges with
+// the neighbour, the pair, the mirrored half row and the mirrored row, then with
+// the other rows.
+template <int kL, class F>
+__device__ __forceinline__ uint32_t all_lanes(uint32_t v, F&& op) {
+  v = op(v, dpp<0xb1>(v));   // quad_perm 1, 0, 3, 2
+  v = op(v, dpp<0x4e>(v));   // quad_perm 2, 3, 0, 1
+  v = op(v, dpp<0x141>(v));  // row_half_mirror
+  v = op(v, dpp<0x140>(v));  // row_mirror
+  if constexpr (kL == 64) {
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(b[0], b[1]);
+  }
+  return v;
+}
+template <int kL>
+__device__ __forceinline__ float sum_lanes(float f) {
+  return __builtin_bit_cast(
+      float, all_lanes<kL>(__builtin_bit_cast(uint32_t, f), [](uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(
+            uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+      }));
+}
+
+template <int kType>
+__device__ __forceinline__ float logit(const uint8_t* p, int i) {
+  if constexpr (kType == kInF32) return reinterpret_cast<const float*>(p)[i];
+  else if constexpr (kType == kInBf16)
+    return __builtin_bit_cast(float, (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << 16);
+  else return (float)reinterpret_cast<const _Float16*>(p)[i];
+}
+
+template <int kType, int kL, int kV>
+__global__ __launch_bounds__(256) void k_route(RouteArgs g) {
+  constexpr int kBytes = type_bytes(kType), kPer = 16 / kBytes;
+  const int gl = (int)threadIdx.x % kL;  // lane of the token's group
+  const int t = (int)blockIdx.x * (256 / kL) + (int)threadIdx.x / kL;
+  const bool live = t < g.T;
+  const uint8_t* p = g.logits + (long long)(live ? t : g.T - 1) * g.ld;
+  const int e0 = gl * kV;
+
+  uint32_t key[kV];
+  if (kV * kBytes >= 16 && g.vec) {
+#pragma unroll
+    for (int c = 0; c < kV / kPer; ++c) {
+      i32x4 v = {};
+      const bool in = e0 + c * kPer < g.E;
+      if (in) v = *reinterpret_cast<const i32x4*>(p + (e0 + c * kPer) * kBytes);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        float f;
+        // (an element goes through an integer: bit_cast of a vector element takes element 0)
+        if constexpr (kType == kInF32) f = __builtin_bit_cast(float, (uint32_t)v[i]);
+        else if constexpr (kType == kInBf16)
+          f = __builtin_bit_cast(float, (uint32_t)v[i / 2] << (i & 1 ? 0 : 16) & 0xffff0000u);
+        else f = (float)__builtin_bit_cast(_Float16, (uint16_t)((uint32_t)v[i / 2] >> (16 * (i & 1))));
+        key[c * kPer + i] = in ? key_of(f) : 0u;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) key[i] = e0 + i < g.E ? key_of(logit<kType>(p, e0 + i)) : 0u;
+  }
+
+  auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  uint32_t top = 0;        // the largest key
+  float total = 1.0f;      // sum of all exponentials, where it is asked for
+  uint32_t mine_key = 0;
+  int mine_id = -1;
+  for (int j = 0; j < g.k; ++j) {
+    uint32_t m = key[0];
+#pragma unroll
+    for (int i = 1; i < kV; ++i) m = larger(m, key[i]);
+    const uint32_t best = all_lanes<kL>(m, larger);
+    if (j == 0) {
+      top = best;
+      if (!g.sigmoid && !g.renormalize) {
+        const float ref = value_of(top);
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kV; ++i) s += key[i] ? expf(value_of(key[i]) - ref) : 0.0f;
+        total = sum_lanes<kL>(s);
+      }
+    }
+    // The first lane of the group whose maximum it is, and its first value.
+    const uint64_t has = __builtin_amdgcn_ballot_w64(m == best);
+    const int base = lane_id() & ~(kL - 1);
+    const uint64_t in_group = kL == 64 ? has : (has >> base) & ((1ull << kL) - 1ull);
+    const int owner = __builtin_ctzll(in_group);
+    int at = 0;
+#pragma unroll
+    for (int i = kV - 1; i >= 0; --i) at = key[i] == best ? i : at;
+    const bool own = gl == owner;
+#pragma unroll
+    for (int i = 0; i < kV; ++i) key[i] = own && at == i ? 0u : key[i];
+    const int id = owner * kV + __shfl(at, base + owner, kWave);
+    if (gl == j && best != 0u) {
+      mine_key = best;
+      mine_id = id;
+    }
+  }
+
+  const float v = value_of(mine_key);
+  float w = 0.0f;
+  if (mine_id >= 0) w = g.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - value_of(top));
+  if (g.renormalize) total = sum_lanes<kL>(w);
+  w = mine_id >= 0 ? w / total * g.scale : 0.0f;
+  if (live && gl < g.k) {
+    g.weights[(long long)t * g.k + gl] = w;
+    g.ids[(long long)t * g.k + gl] = mine_id;
+  }
+}
+
+template <int kType, int kL>
+const void* route_of(int v) {
+  switch (v) {
+    case 1: return (const void*)&k_route<kType, kL, 1>;
+    case 2: return (const void*)&k_route<kType, kL, 2>;
+    case 4: return (const void*)&k_route<kType, kL, 4>;
+    case 8: return (const void*)&k_route<kType, kL, 8>;
+    case 16: return (const void*)&k_route<kType, kL, 16>;
+    default:
+      if constexpr (kL == 16) return v == 32 ? (const void*)&k_route<kType, kL, 32> : nullptr;
+      return nullptr;
+  }
+}
+template <int kL>
+const void* route_fn(int type, int v) {
+  return type == kInF32 ? route_of<kInF32, kL>(v)
+                        : type == kInBf16 ? route_of<kInBf16, kL>(v) : route_of<kInF16, kL>(v);
+}
+
+}  // namespace
+}  // namespace kernels
+}  // namespace hipgemm
+
+extern "C" hipError_t hipgemm_moe_route(const void* logits, int type, int T, int E, int k,
+                                        long long ld, int scoring, int renormalize, float scale,
+                                        float* weights, int* ids, hipStream_t stream) {
+  using namespace hipgemm::kernels;
+  if (T < 0 || E < 1 || E > HIPGEMM_MOE_MAX_EXPERTS || k < 1 || k > E || k > 64 ||
+      type < HIPGEMM_IN_F32 || type > HIPGEMM_IN_F16 ||
+      (scoring != HIPGEMM_MOE_SOFTMAX && scoring != HIPGEMM_MOE_SIGMOID))
+    return hipErrorInvalidValue;
+  if (T == 0) return hipSuccess;
+  const int es = type == HIPGEMM_IN_F32 ? 4 : 2;
+  auto aligned = [](const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; };
+  if (!logits || !weights || !ids || ld < E || !aligned(logits, es) || !aligned(weights, 4) ||
+      !aligned(ids, 4))
+    return hipErrorInvalidValue;
+  RouteArgs g{static_cast<const uint8_t*>(logits), weights, ids, ld * es, T, E, k,
+              scoring == HIPGEMM_MOE_SIGMOID, renormalize != 0, 0, scale};
+  g.vec = aligned(logits, 16) && g.ld % 16 == 0 && E % (16 / es) == 0;
+  // 16 lanes per token from the tokens on that give every SIMD a wave so (4 x
+  // 256 SIMDs).
+  const bool narrow = k <= 16 && E <= 512 && T >= 4096;
+  const int lanes = narrow ? 16 : 64;
+  int v = 1;
+  while (v * lanes < E) v *= 2;
+  const void* fn = narrow ? route_fn<16>(type, v) : route_fn<64>(type, v);
+  if (!fn) return hipErrorInvalidValue;
+  void* args[] = {&g};
+  const int per = 256 / lanes;
+  return hipLaunchKernel(fn, dim3((unsigned)((T + per - 1) / per)), dim3(256), args, 0, stream);
+}

@@ -2,6 +2,7 @@
 (include/hipgemm.h: hipgemm_w4_gemm and its neighbours), on torch tensors.
 
 w4_gemm      products with 4-bit weights and group scales
+moe_route    a router's choice of experts for each token
 
 Like the rest of the package these run on the GPU only, on the current stream
 or the one given, and raise HipGemmError for arguments that they do not take.
@@ -15,10 +16,12 @@ import functools
 from . import (ACTIVATIONS, OUT_BF16, OUT_F16, OUT_F32, HipGemmError, _check,
                _torch, hipErrorInvalidValue, lib)
 
-__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "W4_FORMATS"]
+__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "W4_FORMATS",
+           "moe_route", "MOE_SCORING"]
 
 # include/hipgemm.h codes
 W4_FORMATS = {"int4": 0, "fp4": 1}
+MOE_SCORING = {"softmax": 0, "sigmoid": 1}
 _vp, _ci, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 
 
@@ -138,3 +141,35 @@ def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
                ACTIVATIONS[activation])
     _check(lib().hipgemm_w4_gemm(ctypes.byref(d), _stream_handle(x, stream)), "hipgemm_w4_gemm")
     return out
+
+
+def moe_route(logits, k: int, *, scoring: str = "softmax", renormalize: bool = True,
+              scale: float = 1.0, stream=None):
+    """The k experts of largest logit for each token, in order (equal logits: the
+    lower index first), and their weights: (weights (T, k) float32, ids (T, k)
+    int32).
+
+    logits (T, E): float32, bfloat16 or float16, unit stride along E.  scoring:
+    "softmax" over all experts, or "sigmoid" of each; renormalize divides a
+    token's k weights by their sum; scale multiplies them.  A logit of -inf is
+    never chosen: a token with fewer than k others gets id -1 and weight 0 in the
+    remaining places.  Up to 1024 experts, k up to 64."""
+    torch = _torch()
+    if logits.dim() != 2 or not logits.is_cuda:
+        _bad("logits must be a 2-D device tensor")
+    kind = _types()[1].get(logits.dtype)
+    if kind is None or kind > 2:
+        _bad(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    T, E = logits.shape
+    if E > 1 and logits.stride(1) != 1:
+        _bad("logits must have unit stride along the experts")
+    code = MOE_SCORING.get(scoring)
+    if code is None:
+        _bad(f"scoring must be one of {sorted(MOE_SCORING)}")
+    weights = torch.empty((T, max(k, 0)), dtype=torch.float32, device=logits.device)
+    ids = torch.empty((T, max(k, 0)), dtype=torch.int32, device=logits.device)
+    _check(lib().hipgemm_moe_route(
+        logits.data_ptr(), kind, T, E, k, logits.stride(0) if T > 1 else E, code,
+        int(renormalize), scale, weights.data_ptr(), ids.data_ptr(),
+        _stream_handle(logits, stream)), "hipgemm_moe_route")
+    return weights, ids

@@ -404,6 +404,26 @@ typedef struct hipgemm_w4_desc {
 } hipgemm_w4_desc;
 hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc *desc, hipStream_t stream);
 
+/*
+ * The router's choice of a mixture-of-experts layer: for each of T rows of E
+ * logits (device, of type HIPGEMM_IN_*, row stride ld elements) the k largest,
+ * in order, equal ones by the lower index:
+ *
+ *   softmax: p = exp(l - max l) / sum exp(l - max l);  sigmoid: p = 1 / (1 + exp(-l))
+ *   weights[t, j] = scale * p[ids[t, j]]   [ / sum over j, if renormalize ]
+ *
+ * weights (float) and ids (int) are T x k, packed.  A logit of -inf is never
+ * chosen: where fewer than k others are left, the rest of the row gets id -1 and
+ * weight 0.  A NaN ranks above +inf.  1 <= k <= min(E, 64), E <=
+ * HIPGEMM_MOE_MAX_EXPERTS.  One launch, no workspace.  No reference counterpart.
+ */
+#define HIPGEMM_MOE_MAX_EXPERTS 1024
+enum { HIPGEMM_MOE_SOFTMAX = 0, HIPGEMM_MOE_SIGMOID = 1 };
+hipError_t hipgemm_moe_route(const void *logits, int type, int T, int E, int k,
+                             long long ld, int scoring, int renormalize,
+                             float scale, float *weights, int *ids,
+                             hipStream_t stream);
+
 /* Workspace bytes hipgemm_fp8_gemm_bf16_ws needs for this shape and variant
  * on the current device (0: none).  No GPU work.  No reference counterpart. */
 size_t hipgemm_workspace_size(int M, int N, int K, int variant);
