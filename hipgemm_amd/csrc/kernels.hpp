@@ -77,6 +77,9 @@ hipError_t quantize_rows(const void* x, int type, int M, int K, long long ldx,
 // type; rows: 1, 2 or 4; mode: detail::kCoarse, kFine or kInline; mt: 1 or 2.
 const void* w4_vec(int x, int w, int s, int rows);
 const void* w4_rows(int x, int w, int s, int mode, int mt);
+// The experts' products (kmoe_*.hip); mode as above or detail::kNone.
+const void* moe_up(int x, int w, int s, int mode, int mt);
+const void* moe_down(int w, int s, int mode);
 // Packs [rows][ceil(K/32)] E8M0 scales (row stride ld) into MxArgs' layout.
 hipError_t mx_pack(const uint8_t* src, int rows, int K, int ld, uint8_t* dst,
                    hipStream_t stream);

@@ -1,0 +1,162 @@
+// hipgemm_moe_experts: arguments and launches.
+#include "hipgemm.h"
+
+#include "kernels.hpp"
+
+#include "hipgemm/detail/moe.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* moe_up_int4(int x, int s, int mode, int mt);
+const void* moe_up_fp4(int x, int s, int mode, int mt);
+const void* moe_up_e4m3(int x, int s, int mode, int mt);
+const void* moe_down_int4(int s, int mode);
+const void* moe_down_fp4(int s, int mode);
+const void* moe_down_e4m3(int s, int mode);
+
+const void* moe_up(int x, int w, int s, int mode, int mt) {
+  return w == detail::kWInt4  ? moe_up_int4(x, s, mode, mt)
+         : w == detail::kWFp4 ? moe_up_fp4(x, s, mode, mt)
+                              : moe_up_e4m3(x, s, mode, mt);
+}
+const void* moe_down(int w, int s, int mode) {
+  return w == detail::kWInt4 ? moe_down_int4(s, mode)
+         : w == detail::kWFp4 ? moe_down_fp4(s, mode)
+                              : moe_down_e4m3(s, mode);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm
+
+namespace {
+
+using namespace hipgemm::detail;
+namespace hk = hipgemm::kernels;
+
+static_assert(HIPGEMM_W8_E4M3 == kWE4M3 && HIPGEMM_MOE_MAX_PAIRS == kMoePairs, "codes");
+
+bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+constexpr int kMaxDim = 1 << 26;  // Stream's group index
+
+// Tokens of one turn, and its slots.
+int turn_tokens(int T, int k) { return T < kMoePairs / k ? T : kMoePairs / k; }
+int turn_slots(int T, int k, int E) { return T * k < E ? T * k : E < kMoePairs ? E : kMoePairs; }
+
+size_t table_bytes(int slots) { return ((size_t)slots * kMoeTable * sizeof(int) + 15) / 16 * 16; }
+
+int mode_of(int x_type, int format, int scale_type, int group) {
+  if (format == kWE4M3) return kNone;
+  if (format == kWFp4 && scale_type == kScaleE8M0 && x_type == kInBf16) return kInline;
+  return group % 128 == 0 ? kCoarse : kFine;
+}
+
+bool matrix_ok(const hipgemm_moe_matrix& m, int rows, int K, const hipgemm_moe_desc& d) {
+  const bool e4m3 = d.format == HIPGEMM_W8_E4M3;
+  const long long row = e4m3 ? K : K / 2;
+  const long long groups = e4m3 ? 1 : (K + d.group_size - 1) / d.group_size;
+  return m.weight && m.scales && aligned(m.weight, 16) &&
+         aligned(m.scales, type_bytes(d.scale_type)) && m.ldw >= row && m.ldw % 16 == 0 &&
+         m.expert_w % 16 == 0 && (d.E == 1 || m.expert_w >= (rows - 1) * m.ldw + row) &&
+         m.lds >= groups && (d.E == 1 || m.expert_s >= (rows - 1) * m.lds + groups) &&
+         (!m.zeros || d.format == HIPGEMM_W4_INT4);
+}
+
+hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
+  const int pairs = g.T * g.k;
+  g.by_pair = pairs < g.E;
+  g.slots = turn_slots(g.T, g.k, g.E);
+  // Tiles of 16 tokens, two at a time where experts have more on average.
+  const int mt = pairs > 12 * g.E ? 2 : 1;
+  void* args[] = {&g};
+  const void* up = hk::moe_up(d.x_type, d.format, d.scale_type,
+                              mode_of(d.x_type, d.format, d.scale_type, d.group_size), mt);
+  const void* down = hk::moe_down(d.format, d.scale_type,
+                                  mode_of(kInBf16, d.format, d.scale_type, d.group_size));
+  if (!up || !down) return hipErrorInvalidValue;
+  // LDS of the second kernel: parts x pairs x 16 floats, up to 48 KiB.
+  g.max_parts = 768 / pairs < 1 ? 1 : 768 / pairs > 16 ? 16 : 768 / pairs;
+  hipError_t e = hipLaunchKernel(up, dim3((unsigned)(g.F / 16), (unsigned)g.slots), dim3(512),
+                                 args, 0, stream);
+  if (e != hipSuccess) return e;
+  return hipLaunchKernel(down, dim3((unsigned)(g.D / 16)), dim3(512), args,
+                         (size_t)g.max_parts * pairs * 64, stream);
+}
+
+}  // namespace
+
+extern "C" size_t hipgemm_moe_workspace_size(int T, int k, int E, int F) {
+  if (T <= 0 || k <= 0 || k > 64 || E <= 0 || F <= 0) return 0;
+  const int t = turn_tokens(T, k);
+  return table_bytes(turn_slots(t, k, E)) + (size_t)t * k * F * 4;
+}
+
+extern "C" hipError_t hipgemm_moe_experts(const hipgemm_moe_desc* desc, hipStream_t stream) {
+  if (!desc || desc->size != sizeof(hipgemm_moe_desc)) return hipErrorInvalidValue;
+  const hipgemm_moe_desc& d = *desc;
+  const bool e4m3 = d.format == HIPGEMM_W8_E4M3;
+  if (d.T < 0 || d.k < 1 || d.k > 64 || d.E < 1 || d.E > HIPGEMM_MOE_MAX_PAIRS || d.D < 32 ||
+      d.F < 32 || d.D % 32 != 0 || d.F % 32 != 0 || d.D > kMaxDim || d.F > kMaxDim / 2 ||
+      d.format < 0 || d.format > HIPGEMM_W8_E4M3 ||
+      (d.x_type != HIPGEMM_IN_BF16 && d.x_type != HIPGEMM_IN_F16) || d.out_dtype < 0 ||
+      d.out_dtype > HIPGEMM_OUT_F32 || d.activation < 0 || d.activation > HIPGEMM_ACT_SILU)
+    return hipErrorInvalidValue;
+  if (e4m3 ? d.scale_type != HIPGEMM_IN_F32
+           : d.scale_type < 0 || d.scale_type > HIPGEMM_SCALE_E8M0 || d.group_size <= 0 ||
+                 d.group_size % 32 != 0)
+    return hipErrorInvalidValue;
+  if (d.T == 0) return hipSuccess;
+  if (!d.x || !d.ids || !d.weights || !d.y || !aligned(d.x, 16) || !aligned(d.ids, 4) ||
+      !aligned(d.weights, 4) || !aligned(d.y, out_bytes(d.out_dtype)) || d.ldx < d.D ||
+      d.ldx % 8 != 0 || d.ldy < d.D || !matrix_ok(d.w13, 2 * d.F, d.D, d) ||
+      !matrix_ok(d.w2, d.D, d.F, d))
+    return hipErrorInvalidValue;
+  if (!d.workspace || !aligned(d.workspace, 16) ||
+      d.workspace_bytes < hipgemm_moe_workspace_size(d.T, d.k, d.E, d.F))
+    return hipErrorInvalidValue;
+
+  MoeArgs g{};
+  const int ss = type_bytes(d.scale_type), ys = out_bytes(d.out_dtype);
+  g.w13 = static_cast<const uint8_t*>(d.w13.weight);
+  g.s13 = static_cast<const uint8_t*>(d.w13.scales);
+  g.z13 = d.w13.zeros;
+  g.w2 = static_cast<const uint8_t*>(d.w2.weight);
+  g.s2 = static_cast<const uint8_t*>(d.w2.scales);
+  g.z2 = d.w2.zeros;
+  g.ldx = 2 * d.ldx;
+  g.ldy = d.ldy;
+  g.w13_row = d.w13.ldw;
+  g.w13_expert = d.w13.expert_w;
+  g.s13_row = d.w13.lds * ss;
+  g.s13_expert = d.w13.expert_s * ss;
+  g.z13_row = d.w13.lds;
+  g.z13_expert = d.w13.expert_s;
+  g.w2_row = d.w2.ldw;
+  g.w2_expert = d.w2.expert_w;
+  g.s2_row = d.w2.lds * ss;
+  g.s2_expert = d.w2.expert_s * ss;
+  g.z2_row = d.w2.lds;
+  g.z2_expert = d.w2.expert_s;
+  g.k = d.k;
+  g.E = d.E;
+  g.D = d.D;
+  g.F = d.F;
+  g.G13 = g.G2 = e4m3 ? 32 : d.group_size;
+  g.act = d.activation;
+  g.out = d.out_dtype;
+  const int most = turn_tokens(d.T, d.k);
+  g.table = static_cast<int*>(d.workspace);
+  g.h = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(d.workspace) +
+                                    table_bytes(turn_slots(most, d.k, d.E)));
+  for (int t = 0; t < d.T; t += most) {
+    g.T = d.T - t < most ? d.T - t : most;
+    g.x = static_cast<const uint8_t*>(d.x) + (long long)t * g.ldx;
+    g.ids = d.ids + (long long)t * d.k;
+    g.weights = d.weights + (long long)t * d.k;
+    g.y = static_cast<uint8_t*>(d.y) + (long long)t * d.ldy * ys;
+    const hipError_t e = turn(g, d, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}

@@ -3,6 +3,7 @@
 
 w4_gemm      products with 4-bit weights and group scales
 moe_route    a router's choice of experts for each token
+moe_experts  the experts' gated MLPs of a few tokens, e4m3 or 4-bit weights
 
 Like the rest of the package these run on the GPU only, on the current stream
 or the one given, and raise HipGemmError for arguments that they do not take.
@@ -17,10 +18,12 @@ from . import (ACTIVATIONS, OUT_BF16, OUT_F16, OUT_F32, HipGemmError, _check,
                _torch, hipErrorInvalidValue, lib)
 
 __all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "W4_FORMATS",
-           "moe_route", "MOE_SCORING"]
+           "moe_route", "MOE_SCORING", "moe_experts", "MoeDesc", "MoeMatrix",
+           "moe_experts_raw", "moe_workspace_size", "MOE_FORMATS"]
 
 # include/hipgemm.h codes
 W4_FORMATS = {"int4": 0, "fp4": 1}
+MOE_FORMATS = {**W4_FORMATS, "e4m3": 2}
 MOE_SCORING = {"softmax": 0, "sigmoid": 1}
 _vp, _ci, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 
@@ -35,6 +38,24 @@ class W4Desc(ctypes.Structure):
                 ("out_dtype", _ci), ("activation", _ci)]
 
 
+class MoeMatrix(ctypes.Structure):
+    """hipgemm_moe_matrix (include/hipgemm.h)."""
+    _fields_ = [("weight", _vp), ("scales", _vp), ("zeros", _vp), ("ldw", _ll),
+                ("expert_w", _ll), ("lds", _ll), ("expert_s", _ll)]
+
+
+class MoeDesc(ctypes.Structure):
+    """hipgemm_moe_desc (include/hipgemm.h)."""
+    _fields_ = [("size", ctypes.c_size_t), ("x", _vp), ("ids", _vp),
+                ("weights", _vp), ("w13", MoeMatrix), ("w2", MoeMatrix),
+                ("y", _vp), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t), ("ldx", _ll), ("ldy", _ll),
+                ("T", _ci), ("k", _ci), ("E", _ci), ("D", _ci), ("F", _ci),
+                ("group_size", _ci), ("x_type", _ci), ("format", _ci),
+                ("scale_type", _ci), ("out_dtype", _ci), ("activation", _ci)]
+
+
+_MOE_BYTES = ctypes.sizeof(MoeDesc)
 _W4_BYTES = ctypes.sizeof(W4Desc)
 
 
@@ -173,3 +194,121 @@ def moe_route(logits, k: int, *, scoring: str = "softmax", renormalize: bool = T
         int(renormalize), scale, weights.data_ptr(), ids.data_ptr(),
         _stream_handle(logits, stream)), "hipgemm_moe_route")
     return weights, ids
+
+
+def moe_experts_raw(desc: "MoeDesc", stream: int = 0) -> int:
+    """Call hipgemm_moe_experts; returns hipError_t."""
+    return int(lib().hipgemm_moe_experts(ctypes.byref(desc), stream or None))
+
+
+def moe_workspace_size(T: int, k: int, E: int, F: int) -> int:
+    """Workspace bytes hipgemm_moe_experts needs."""
+    return int(lib().hipgemm_moe_workspace_size(T, k, E, F))
+
+
+_moe_ws_bytes = functools.lru_cache(maxsize=1024)(moe_workspace_size)
+
+
+def _moe_matrix(name, w, s, z, shape, fmt, group):
+    """The matrix' pointers and strides, and its scales' type; shape: (E, rows, K)."""
+    torch = _torch()
+    E, rows, K = shape
+    if fmt == 2:
+        dtypes, width, groups = (torch.float8_e4m3fn,), K, None
+    else:
+        dtypes = (torch.uint8, torch.float4_e2m1fn_x2) if fmt == 1 else (torch.uint8,)
+        width, groups = K // 2, -(-K // group)
+    if w.dtype not in dtypes or tuple(w.shape) != (E, rows, width) or not w.is_cuda \
+            or w.stride(2) != 1:
+        _bad(f"{name} must be a ({E}, {rows}, {width}) {dtypes[0]} device tensor with unit "
+             f"stride along the last dimension, got {tuple(w.shape)} {w.dtype}")
+    want = (E, rows) if groups is None else (E, rows, groups)
+    st = _types()[1].get(s.dtype)
+    if st is None or (fmt == 2 and st != 0) or tuple(s.shape) != want or not s.is_cuda:
+        _bad(f"scales of {name} must be {want}" + (" float32" if fmt == 2 else
+             " bfloat16, float16, float32 or uint8") + f", got {tuple(s.shape)} {s.dtype}")
+    if groups is not None and groups > 1 and s.stride(2) != 1:
+        _bad(f"scales of {name} must have unit stride along the groups")
+    zp = 0
+    if z is not None:
+        if fmt != 0:
+            _bad("zeros belong to int4")
+        if z.dtype != torch.uint8 or tuple(z.shape) != want or not z.is_cuda \
+                or z.stride() != s.stride():
+            _bad(f"zeros of {name} must be uint8 of the shape and strides of its scales")
+        zp = z.data_ptr()
+    return MoeMatrix(w.data_ptr(), s.data_ptr(), zp, w.stride(1), w.stride(0),
+                     s.stride(1), s.stride(0)), st
+
+
+def moe_experts(x, ids, weights, w13, scales13, w2, scales2, *, zeros13=None,
+                zeros2=None, format: str = "e4m3", group_size: int = 128,
+                activation="silu", out_dtype=None, out=None, workspace=None, stream=None):
+    """The experts of a mixture-of-experts layer on a few tokens:
+
+        h[t, j] = act(x[t] @ W13[e, :F].T) * (x[t] @ W13[e, F:].T),  e = ids[t, j]
+        out[t]  = round(sum_j weights[t, j] * (h[t, j] @ W2[e].T))
+
+    x (T, D): bfloat16 or float16.  ids (T, k) int32 and weights (T, k) float32 as
+    moe_route gives them; an id outside [0, E) is skipped.  w13 (E, 2F, D) (gate
+    rows, then up rows) and w2 (E, D, F): float8_e4m3fn with float32 scales (E, 2F)
+    and (E, D) ("e4m3"), or 4-bit codes (last dimension halved) with scales per
+    group_size elements of a row, (E, rows, groups), as for w4_gemm ("int4",
+    "fp4").  D, F and group_size are multiples of 32.  activation: of the gate
+    (None, "relu", "gelu_tanh", "silu").  out_dtype: bfloat16, float16 or float32,
+    x's where None.  Made for up to 64 tokens (each expert's weights are read once
+    for up to 16 of its tokens); any number works.  workspace: a uint8 device
+    tensor of moe_workspace_size bytes; allocated per call where None."""
+    torch = _torch()
+    x_types, _, o_types = _types()
+    xt, fmt = x_types.get(x.dtype), MOE_FORMATS.get(format)
+    if xt is None or x.dim() != 2 or not x.is_cuda:
+        _bad(f"x must be a 2-D bfloat16 or float16 device tensor, got {x.dtype}")
+    if fmt is None:
+        _bad(f"format must be one of {sorted(MOE_FORMATS)}")
+    if w13.dim() != 3 or ids.dim() != 2:
+        _bad("w13 must be 3-D, ids 2-D")
+    (T, D), (E, F2, _), k = x.shape, w13.shape, ids.shape[1]
+    F = F2 // 2
+    if F2 % 2 or D % 32 or F % 32:
+        _bad("D and F must be multiples of 32")
+    if fmt != 2 and (group_size <= 0 or group_size % 32):
+        _bad("group_size must be a multiple of 32")
+    if D > 1 and x.stride(1) != 1:
+        _bad("x must have unit stride along D")
+    for t, dtype, name in ((ids, torch.int32, "ids"), (weights, torch.float32, "weights")):
+        if t.dtype != dtype or tuple(t.shape) != (T, k) or not t.is_cuda \
+                or not t.is_contiguous():
+            _bad(f"{name} must be a contiguous ({T}, {k}) {dtype} device tensor")
+    if activation not in ACTIVATIONS:
+        _bad(f"activation must be one of {sorted(a for a in ACTIVATIONS if a)}")
+    m13, s13 = _moe_matrix("w13", w13, scales13, zeros13, (E, F2, D), fmt, group_size)
+    m2, s2 = _moe_matrix("w2", w2, scales2, zeros2, (E, D, F), fmt, group_size)
+    if s13 != s2:
+        _bad("scales13 and scales2 must have one dtype")
+    out_dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    ot = o_types.get(out_dtype)
+    if ot is None:
+        _bad("out_dtype must be bfloat16, float16 or float32")
+    if out is None:
+        out = torch.empty((T, D), dtype=out_dtype, device=x.device)
+    elif (out.dtype != out_dtype or tuple(out.shape) != (T, D) or not out.is_cuda
+          or out.stride(1) != 1):
+        _bad(f"out must be a ({T}, {D}) {out_dtype} device tensor with unit column stride")
+    need = _moe_ws_bytes(T, k, E, F)
+    if workspace is None:
+        if stream is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        else:
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_cuda \
+            or not workspace.is_contiguous() or workspace.numel() < need:
+        _bad(f"workspace must be a contiguous uint8 device tensor of {need} bytes")
+    d = MoeDesc(_MOE_BYTES, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), m13, m2,
+                out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                x.stride(0) if T > 1 else D, out.stride(0) if T > 1 else D, T, k, E, D, F,
+                group_size, xt, fmt, s13, ot, ACTIVATIONS[activation])
+    _check(lib().hipgemm_moe_experts(ctypes.byref(d), _stream_handle(x, stream)),
+           "hipgemm_moe_experts")
+    return out

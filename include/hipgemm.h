@@ -424,6 +424,56 @@ hipError_t hipgemm_moe_route(const void *logits, int type, int T, int E, int k,
                              float scale, float *weights, int *ids,
                              hipStream_t stream);
 
+/*
+ * The experts of a mixture-of-experts layer for a few tokens:
+ *
+ *   h[t, j] = act(x[t] W13[e][:F]^T) * (x[t] W13[e][F:]^T),  e = ids[t, j]
+ *   y[t]    = round_out(sum_j weights[t, j] (h[t, j] W2[e]^T))
+ *
+ * x: T x D, bf16 or fp16; ids (int), weights (float): T x k, packed.  W13: E x
+ * 2F x D (gate rows, then up rows), W2: E x D x F, in one weight format:
+ * HIPGEMM_W4_INT4 or _FP4 with scales (and zeros) per group_size elements of a
+ * row as in hipgemm_w4_gemm, or HIPGEMM_W8_E4M3 with one float scale per row
+ * (scale_type F32, lds 1: E x 2F and E x D).  An id outside [0, E) is skipped: a
+ * token without any gives zeros.  Sums are fp32; h is held to 16 significant
+ * bits between the two kernels.  Each chosen expert's weights are read once for
+ * up to 16 of its tokens, so it is made for a few tokens (up to 64); more go in
+ * turns of at most HIPGEMM_MOE_MAX_PAIRS / k.
+ * D, F, group_size multiples of 32; matrices 16-byte aligned, with row and
+ * expert strides of multiples of 16 bytes; k <= 64.  Workspace:
+ * hipgemm_moe_workspace_size bytes, 16-byte aligned, of any content; calls that
+ * may run concurrently must not share one.  Two launches per turn on `stream`.
+ * Zero-initialise the struct and set `size`.  No reference counterpart.
+ */
+enum { HIPGEMM_W8_E4M3 = 2 };
+#define HIPGEMM_MOE_MAX_PAIRS 512
+typedef struct hipgemm_moe_matrix {
+  const void *weight, *scales;
+  const unsigned char *zeros;          /* or NULL */
+  long long ldw, expert_w;             /* bytes: a row, an expert */
+  long long lds, expert_s;             /* elements, of zeros too */
+} hipgemm_moe_matrix;
+typedef struct hipgemm_moe_desc {
+  size_t size;
+  const void *x;
+  const int *ids;
+  const float *weights;
+  hipgemm_moe_matrix w13, w2;
+  void *y;
+  void *workspace;
+  size_t workspace_bytes;
+  long long ldx, ldy; /* elements */
+  int T, k, E, D, F;
+  int group_size;     /* not for e4m3 */
+  int x_type;         /* HIPGEMM_IN_BF16 or HIPGEMM_IN_F16 */
+  int format;         /* HIPGEMM_W4_* or HIPGEMM_W8_E4M3 */
+  int scale_type;     /* HIPGEMM_IN_* or HIPGEMM_SCALE_E8M0 */
+  int out_dtype;      /* HIPGEMM_OUT_BF16, _F16 or _F32 */
+  int activation;     /* HIPGEMM_ACT_* */
+} hipgemm_moe_desc;
+size_t hipgemm_moe_workspace_size(int T, int k, int E, int F);
+hipError_t hipgemm_moe_experts(const hipgemm_moe_desc *desc, hipStream_t stream);
+
 /* Workspace bytes hipgemm_fp8_gemm_bf16_ws needs for this shape and variant
  * on the current device (0: none).  No GPU work.  No reference counterpart. */
 size_t hipgemm_workspace_size(int M, int N, int K, int variant);

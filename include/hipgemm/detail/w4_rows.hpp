@@ -47,7 +47,7 @@ __global__ __launch_bounds__(512, 2) void k_w4_rows(W4Args g) {
 #pragma unroll
   for (int m = 0; m < kMT; ++m)
     st.x[m] = g.x + (long long)min(m0 + 16 * m + (lane & 15), g.M - 1) * g.ldx;
-  st.run(wave, waves);
+  st.run(wave, st.pairs(), waves);
 
   // Lane l, element e of tile (n, m): row 16 m + 4 (l / 16) + e, column 16 n + l % 16.
   __shared__ f32x4 part[8 * kNT * kMT * kWave];

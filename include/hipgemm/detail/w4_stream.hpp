@@ -226,17 +226,16 @@ struct Stream {
     }
   }
 
-  // Blocks first, first + 1, first + 2 * step, ...: two neighbours (the halves
-  // of 128-byte lines), then 2 * step on.
-  __device__ __forceinline__ void run(int pair, int step) {
-    const int pairs = (K + 255) >> 8;
+  // Pairs of blocks first, first + step, ... below end (a pair is 256 of K: the
+  // halves of 4-bit weights' 128-byte lines).
+  __device__ __forceinline__ void run(int first, int end, int step) {
+    if (first >= end) return;
     Block b[2], c[2];
-    if (pair >= pairs) return;
-    load(b[0], pair * 256);
-    load(b[1], pair * 256 + 128);
-    for (; pair < pairs; pair += step) {
+    load(b[0], first * 256);
+    load(b[1], first * 256 + 128);
+    for (int pair = first; pair < end; pair += step) {
       // (past the end: the last weights again, not used)
-      const int next = min(pair + step, pairs - 1);
+      const int next = min(pair + step, end - 1);
       load(c[0], next * 256);
       load(c[1], next * 256 + 128);
       mul(b[0], pair * 256);
@@ -245,6 +244,7 @@ struct Stream {
       b[1] = c[1];
     }
   }
+  __device__ __forceinline__ int pairs() const { return (K + 255) >> 8; }
 };
 
 }  // namespace detail
