@@ -73,13 +73,16 @@ void* noalloc_scratch(hipStream_t stream, hipError_t* err);
 // Per-row e4m3 quantisation (kquant.hip); type: HIPGEMM_IN_*.
 hipError_t quantize_rows(const void* x, int type, int M, int K, long long ldx,
                          void* q, float* s, hipStream_t stream);
-// Products with 4-bit weights (kw4_*.hip).  x, w, s: detail::kIn*, kW*, scale
-// type; rows: 1, 2 or 4; mode: detail::kCoarse, kFine or kInline; mt: 1 or 2.
-const void* w4_vec(int x, int w, int s, int rows);
+// Products of 16-bit activations with quantised weights (kw4_*.hip, kmoe_*.hip).
+// x: activations' type, w: detail::kW*, s: scales' type, mode: detail::kNone,
+// kCoarse, kFine or kInline; rows: 1, 2 or 4, lk: 16
+// or 64 lanes of a row; mt: tiles of 16 rows of x (1, 2, for
+// w4_rows also 4).
+const void* w4_vec(int x, int w, int s, int rows, int lk);
 const void* w4_rows(int x, int w, int s, int mode, int mt);
-// The experts' products (kmoe_*.hip); mode as above or detail::kNone.
+const void* w4_sum(int x, int w, int s);
 const void* moe_up(int x, int w, int s, int mode, int mt);
-const void* moe_down(int w, int s, int mode);
+const void* moe_down(int w, int s, int mode, int mt);
 // Packs [rows][ceil(K/32)] E8M0 scales (row stride ld) into MxArgs' layout.
 hipError_t mx_pack(const uint8_t* src, int rows, int K, int ld, uint8_t* dst,
                    hipStream_t stream);

@@ -1,0 +1,12 @@
+// The experts' down products with e4m3 weights.
+#include "kw4.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* moe_down_e4m3(int s, int mode, int mt) {
+  return moe_down_of<detail::kWE4M3>(s, mode, mt);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

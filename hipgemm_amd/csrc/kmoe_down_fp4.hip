@@ -1,0 +1,12 @@
+// The experts' down products with fp4 weights.
+#include "kw4.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* moe_down_fp4(int s, int mode, int mt) {
+  return moe_down_of<detail::kWFp4>(s, mode, mt);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

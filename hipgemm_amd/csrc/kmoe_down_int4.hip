@@ -1,0 +1,12 @@
+// The experts' down products with int4 weights.
+#include "kw4.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* moe_down_int4(int s, int mode, int mt) {
+  return moe_down_of<detail::kWInt4>(s, mode, mt);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

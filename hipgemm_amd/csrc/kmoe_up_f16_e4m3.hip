@@ -1,0 +1,12 @@
+// The experts' gate and up products, f16 activations, e4m3 weights.
+#include "kw4.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* moe_up_f16_e4m3(int s, int mode, int mt) {
+  return moe_up_of<detail::kInF16, detail::kWE4M3>(s, mode, mt);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

@@ -1,53 +1,83 @@
-// Instantiations of the kernels with 4-bit weights for one activation type and
-// weight format (kw4_*.hip).
+// Instantiations of the kernels with quantised weights and 16-bit activations
+// for one weight format (kw4_*.hip, kmoe_*.hip).
 #pragma once
 
 #include "kernels.hpp"
 
+#include "hipgemm/detail/moe.hpp"
 #include "hipgemm/detail/w4_rows.hpp"
 
 namespace hipgemm {
 namespace kernels {
 
-template <class F>
-const void* sel_scale(int s, F&& f) {
-  return sel4(s, f);
+// f(scale type, mode) with the combination's constants, where it is built: e4m3
+// has row scales; fp4 with E8M0 scales and bf16 activations takes kInline alone.
+template <int kX, int kW, class F>
+const void* sel_scales(int s, int mode, F&& f) {
+  using namespace detail;
+  if constexpr (kW == kWE4M3) {
+    return s == kInF32 && mode == kNone ? f(ic<kInF32>{}, ic<kNone>{}) : nullptr;
+  } else {
+    return sel4(s, [&](auto S) -> const void* {
+      if constexpr (kX == kInBf16 && kW == kWFp4 && decltype(S)::value == kScaleE8M0)
+        return mode == kInline ? f(S, ic<kInline>{}) : nullptr;
+      else
+        return mode == kCoarse ? f(S, ic<kCoarse>{}) : mode == kFine ? f(S, ic<kFine>{}) : nullptr;
+    });
+  }
+}
+template <int kX, int kW>
+const void* w4_vec_of(int s, int rows, int lk) {
+  using namespace detail;
+  return sel4(s, [&](auto S) -> const void* {
+    constexpr int kS = decltype(S)::value;
+    auto by_lk = [&](auto M) {
+      constexpr int kM = decltype(M)::value;
+      return lk == 64 ? (const void*)&k_w4_vec<kX, kW, kS, kM, 64>
+                      : (const void*)&k_w4_vec<kX, kW, kS, kM, 16>;
+    };
+    return rows == 1 ? by_lk(ic<1>{}) : rows == 2 ? by_lk(ic<2>{}) : by_lk(ic<4>{});
+  });
 }
 
-template <int kX, int kW>
-const void* w4_vec_of(int s, int rows) {
-  using namespace detail;
-  return sel_scale(s, [&](auto S) -> const void* {
-    constexpr int kS = decltype(S)::value;
-    switch (rows) {
-      case 1: return (const void*)&k_w4_vec<kX, kW, kS, 1>;
-      case 2: return (const void*)&k_w4_vec<kX, kW, kS, 2>;
-      case 4: return (const void*)&k_w4_vec<kX, kW, kS, 4>;
-      default: return nullptr;
-    }
-  });
+// f(tiles of 16 rows of x).
+template <class F>
+const void* sel_mt(int mt, F&& f) {
+  return mt == 1 ? f(ic<1>{}) : mt == 2 ? f(ic<2>{}) : nullptr;
 }
 
 template <int kX, int kW>
 const void* w4_rows_of(int s, int mode, int mt) {
-  using namespace detail;
-  return sel_scale(s, [&](auto S) -> const void* {
-    constexpr int kS = decltype(S)::value;
-    // fp4 with E8M0 scales and bf16 activations takes kInline alone.
-    constexpr bool kOnlyInline = kX == kInBf16 && kW == kWFp4 && kS == kScaleE8M0;
-    auto by_mt = [&](auto Mode) -> const void* {
-      constexpr int kMode = decltype(Mode)::value;
-      switch (mt) {
-        case 1: return (const void*)&k_w4_rows<kX, kW, kS, kMode, 2, 1>;
-        case 2: return (const void*)&k_w4_rows<kX, kW, kS, kMode, 2, 2>;
-        default: return nullptr;
-      }
+  return sel_scales<kX, kW>(s, mode, [&](auto S, auto Mode) {
+    auto f = [&](auto MT) {
+      return (const void*)&detail::k_w4_rows<kX, kW, decltype(S)::value, decltype(Mode)::value,
+                                             decltype(MT)::value>;
     };
-    if constexpr (kOnlyInline) {
-      return mode == kInline ? by_mt(ic<kInline>{}) : nullptr;
-    } else {
-      return mode == kCoarse ? by_mt(ic<kCoarse>{}) : mode == kFine ? by_mt(ic<kFine>{}) : nullptr;
-    }
+    return mt == 4 ? f(ic<4>{}) : sel_mt(mt, f);
+  });
+}
+template <int kX, int kW>
+const void* w4_sum_of(int s) {
+  return sel4(s, [](auto S) { return (const void*)&detail::k_w4_sum<kX, kW, decltype(S)::value>; });
+}
+
+template <int kX, int kW>
+const void* moe_up_of(int s, int mode, int mt) {
+  return sel_scales<kX, kW>(s, mode, [&](auto S, auto Mode) {
+    return sel_mt(mt, [&](auto MT) {
+      return (const void*)&detail::k_moe_up<kX, kW, decltype(S)::value, decltype(Mode)::value,
+                                            decltype(MT)::value>;
+    });
+  });
+}
+
+template <int kW>
+const void* moe_down_of(int s, int mode, int mt) {
+  return sel_scales<detail::kInBf16, kW>(s, mode, [&](auto S, auto Mode) {
+    return sel_mt(mt, [&](auto MT) {
+      return (const void*)&detail::k_moe_down<kW, decltype(S)::value, decltype(Mode)::value,
+                                              decltype(MT)::value>;
+    });
   });
 }
 

@@ -1,0 +1,16 @@
+// Products of bf16 activations with int4z weights.
+#include "kw4.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* w4_vec_bf16_int4z(int s, int rows, int lk) {
+  return w4_vec_of<detail::kInBf16, detail::kWInt4Z>(s, rows, lk);
+}
+const void* w4_rows_bf16_int4z(int s, int mode, int mt) {
+  return w4_rows_of<detail::kInBf16, detail::kWInt4Z>(s, mode, mt);
+}
+const void* w4_sum_bf16_int4z(int s) { return w4_sum_of<detail::kInBf16, detail::kWInt4Z>(s); }
+
+}  // namespace kernels
+}  // namespace hipgemm

@@ -4,12 +4,13 @@
 namespace hipgemm {
 namespace kernels {
 
-const void* w4_vec_f16_fp4(int s, int rows) {
-  return w4_vec_of<detail::kInF16, detail::kWFp4>(s, rows);
+const void* w4_vec_f16_fp4(int s, int rows, int lk) {
+  return w4_vec_of<detail::kInF16, detail::kWFp4>(s, rows, lk);
 }
 const void* w4_rows_f16_fp4(int s, int mode, int mt) {
   return w4_rows_of<detail::kInF16, detail::kWFp4>(s, mode, mt);
 }
+const void* w4_sum_f16_fp4(int s) { return w4_sum_of<detail::kInF16, detail::kWFp4>(s); }
 
 }  // namespace kernels
 }  // namespace hipgemm

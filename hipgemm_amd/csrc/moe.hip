@@ -8,22 +8,33 @@
 namespace hipgemm {
 namespace kernels {
 
-const void* moe_up_int4(int x, int s, int mode, int mt);
-const void* moe_up_fp4(int x, int s, int mode, int mt);
-const void* moe_up_e4m3(int x, int s, int mode, int mt);
-const void* moe_down_int4(int s, int mode);
-const void* moe_down_fp4(int s, int mode);
-const void* moe_down_e4m3(int s, int mode);
+#define HIPGEMM_MOE(W)                                            \
+  const void* moe_up_bf16_##W(int s, int mode, int mt);   \
+  const void* moe_up_f16_##W(int s, int mode, int mt);    \
+  const void* moe_down_##W(int s, int mode, int mt);
+HIPGEMM_MOE(int4)
+HIPGEMM_MOE(int4z)
+HIPGEMM_MOE(fp4)
+HIPGEMM_MOE(e4m3)
+#undef HIPGEMM_MOE
 
 const void* moe_up(int x, int w, int s, int mode, int mt) {
-  return w == detail::kWInt4  ? moe_up_int4(x, s, mode, mt)
-         : w == detail::kWFp4 ? moe_up_fp4(x, s, mode, mt)
-                              : moe_up_e4m3(x, s, mode, mt);
+  const bool b = x == detail::kInBf16;
+  switch (w) {
+    case detail::kWInt4: return b ? moe_up_bf16_int4(s, mode, mt) : moe_up_f16_int4(s, mode, mt);
+    case detail::kWInt4Z:
+      return b ? moe_up_bf16_int4z(s, mode, mt) : moe_up_f16_int4z(s, mode, mt);
+    case detail::kWFp4: return b ? moe_up_bf16_fp4(s, mode, mt) : moe_up_f16_fp4(s, mode, mt);
+    default: return b ? moe_up_bf16_e4m3(s, mode, mt) : moe_up_f16_e4m3(s, mode, mt);
+  }
 }
-const void* moe_down(int w, int s, int mode) {
-  return w == detail::kWInt4 ? moe_down_int4(s, mode)
-         : w == detail::kWFp4 ? moe_down_fp4(s, mode)
-                              : moe_down_e4m3(s, mode);
+const void* moe_down(int w, int s, int mode, int mt) {
+  switch (w) {
+    case detail::kWInt4: return moe_down_int4(s, mode, mt);
+    case detail::kWInt4Z: return moe_down_int4z(s, mode, mt);
+    case detail::kWFp4: return moe_down_fp4(s, mode, mt);
+    default: return moe_down_e4m3(s, mode, mt);
+  }
 }
 
 }  // namespace kernels
@@ -34,17 +45,32 @@ namespace {
 using namespace hipgemm::detail;
 namespace hk = hipgemm::kernels;
 
-static_assert(HIPGEMM_W8_E4M3 == kWE4M3 && HIPGEMM_MOE_MAX_PAIRS == kMoePairs, "codes");
+static_assert(HIPGEMM_W8_E4M3 == kWE4M3 && HIPGEMM_MOE_MAX_PAIRS == kMoePairs &&
+                  HIPGEMM_MOE_MAX_EXPERTS == kMoeExperts, "codes");
+
+// Four columns of one token per thread.
+__global__ __launch_bounds__(256) void k_moe_sum(MoeArgs g) {
+  const int i = (int)blockIdx.x * 256 + (int)threadIdx.x, per = g.D / 4;
+  const int t = i / per, d = i % per * 4;
+  if (t >= g.T) return;
+  const long long pairs = g.T * g.k;
+  f32x4 v = {};
+  for (int j = 0; j < g.k; ++j) {
+    const int p = t * g.k + j, e = g.ids[p];
+    if (e < 0 || e >= g.E) continue;
+    for (int q = 0; q < g.parts; ++q)
+      v += *reinterpret_cast<const f32x4*>(g.o + (q * pairs + p) * g.D + d);
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) store_result(g.y, t * g.ldy + d + c, g.out, v[c]);
+}
 
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 constexpr int kMaxDim = 1 << 26;  // Stream's group index
 
-// Tokens of one turn, and its slots.
+// Tokens of one turn.
 int turn_tokens(int T, int k) { return T < kMoePairs / k ? T : kMoePairs / k; }
-int turn_slots(int T, int k, int E) { return T * k < E ? T * k : E < kMoePairs ? E : kMoePairs; }
-
-size_t table_bytes(int slots) { return ((size_t)slots * kMoeTable * sizeof(int) + 15) / 16 * 16; }
 
 int mode_of(int x_type, int format, int scale_type, int group) {
   if (format == kWE4M3) return kNone;
@@ -63,40 +89,61 @@ bool matrix_ok(const hipgemm_moe_matrix& m, int rows, int K, const hipgemm_moe_d
          (!m.zeros || d.format == HIPGEMM_W4_INT4);
 }
 
+// Parts of F in the down product, of part_len (a multiple of 256).
+int down_parts(int T, int k, int E, int D, int F, int* part_len) {
+  const int chosen = T * k < E ? T * k : E;  // experts at most
+  const int tiles = chosen * ((D + 63) / 64), steps = (F + 255) / 256;
+  int parts = tiles >= 512 ? 1 : (512 + tiles - 1) / tiles;
+  if (parts > (steps + 7) / 8) parts = (steps + 7) / 8;
+  const int len = (steps + parts - 1) / parts;
+  *part_len = 256 * len;
+  return (steps + len - 1) / len;
+}
+
+hipError_t launch(const void* fn, dim3 grid, int threads, MoeArgs& g, hipStream_t stream) {
+  if (!fn) return hipErrorInvalidValue;
+  void* args[] = {&g};
+  return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, stream);
+}
+
 hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   const int pairs = g.T * g.k;
-  g.by_pair = pairs < g.E;
-  g.slots = turn_slots(g.T, g.k, g.E);
   // Tiles of 16 tokens, two at a time where experts have more on average.
   const int mt = pairs > 12 * g.E ? 2 : 1;
-  void* args[] = {&g};
-  const void* up = hk::moe_up(d.x_type, d.format, d.scale_type,
-                              mode_of(d.x_type, d.format, d.scale_type, d.group_size), mt);
-  const void* down = hk::moe_down(d.format, d.scale_type,
-                                  mode_of(kInBf16, d.format, d.scale_type, d.group_size));
-  if (!up || !down) return hipErrorInvalidValue;
-  // LDS of the second kernel: parts x pairs x 16 floats, up to 48 KiB.
-  g.max_parts = 768 / pairs < 1 ? 1 : 768 / pairs > 16 ? 16 : 768 / pairs;
-  hipError_t e = hipLaunchKernel(up, dim3((unsigned)(g.F / 16), (unsigned)g.slots), dim3(512),
-                                 args, 0, stream);
+  g.parts = down_parts(g.T, g.k, g.E, g.D, g.F, &g.part_len);
+  const int cus = 256;
+  hipError_t e = launch(hk::moe_up(d.x_type, d.w13.zeros ? kWInt4Z : d.format, d.scale_type,
+                                   mode_of(d.x_type, d.format, d.scale_type, d.group_size), mt),
+                        dim3((unsigned)cus), 1024, g, stream);
   if (e != hipSuccess) return e;
-  return hipLaunchKernel(down, dim3((unsigned)(g.D / 16)), dim3(512), args,
-                         (size_t)g.max_parts * pairs * 64, stream);
+  e = launch(hk::moe_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type,
+                          mode_of(kInBf16, d.format, d.scale_type, d.group_size), mt),
+             dim3((unsigned)cus), 1024, g, stream);
+  if (e != hipSuccess) return e;
+  return launch((const void*)&k_moe_sum, dim3((unsigned)((g.T * (g.D / 4) + 255) / 256)), 256, g,
+                stream);
 }
 
 }  // namespace
 
-extern "C" size_t hipgemm_moe_workspace_size(int T, int k, int E, int F) {
-  if (T <= 0 || k <= 0 || k > 64 || E <= 0 || F <= 0) return 0;
+extern "C" size_t hipgemm_moe_workspace_size(int T, int k, int E, int D, int F) {
+  if (T <= 0 || k <= 0 || k > 64 || E <= 0 || D <= 0 || F <= 0) return 0;
   const int t = turn_tokens(T, k);
-  return table_bytes(turn_slots(t, k, E)) + (size_t)t * k * F * 4;
+  int len;
+  // (a last turn of fewer tokens can have more parts)
+  size_t o = 0;
+  for (int u : {t, T % t}) {
+    const size_t n = u == 0 ? 0 : (size_t)down_parts(u, k, E, D, F, &len) * u * k;
+    if (n > o) o = n;
+  }
+  return (size_t)t * k * F * 4 + o * D * 4;
 }
 
 extern "C" hipError_t hipgemm_moe_experts(const hipgemm_moe_desc* desc, hipStream_t stream) {
   if (!desc || desc->size != sizeof(hipgemm_moe_desc)) return hipErrorInvalidValue;
   const hipgemm_moe_desc& d = *desc;
   const bool e4m3 = d.format == HIPGEMM_W8_E4M3;
-  if (d.T < 0 || d.k < 1 || d.k > 64 || d.E < 1 || d.E > HIPGEMM_MOE_MAX_PAIRS || d.D < 32 ||
+  if (d.T < 0 || d.k < 1 || d.k > 64 || d.E < 1 || d.E > HIPGEMM_MOE_MAX_EXPERTS || d.D < 32 ||
       d.F < 32 || d.D % 32 != 0 || d.F % 32 != 0 || d.D > kMaxDim || d.F > kMaxDim / 2 ||
       d.format < 0 || d.format > HIPGEMM_W8_E4M3 ||
       (d.x_type != HIPGEMM_IN_BF16 && d.x_type != HIPGEMM_IN_F16) || d.out_dtype < 0 ||
@@ -113,7 +160,7 @@ extern "C" hipError_t hipgemm_moe_experts(const hipgemm_moe_desc* desc, hipStrea
       !matrix_ok(d.w2, d.D, d.F, d))
     return hipErrorInvalidValue;
   if (!d.workspace || !aligned(d.workspace, 16) ||
-      d.workspace_bytes < hipgemm_moe_workspace_size(d.T, d.k, d.E, d.F))
+      d.workspace_bytes < hipgemm_moe_workspace_size(d.T, d.k, d.E, d.D, d.F))
     return hipErrorInvalidValue;
 
   MoeArgs g{};
@@ -142,13 +189,12 @@ extern "C" hipError_t hipgemm_moe_experts(const hipgemm_moe_desc* desc, hipStrea
   g.E = d.E;
   g.D = d.D;
   g.F = d.F;
-  g.G13 = g.G2 = e4m3 ? 32 : d.group_size;
+  g.G = e4m3 ? 32 : d.group_size;
   g.act = d.activation;
   g.out = d.out_dtype;
   const int most = turn_tokens(d.T, d.k);
-  g.table = static_cast<int*>(d.workspace);
-  g.h = reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(d.workspace) +
-                                    table_bytes(turn_slots(most, d.k, d.E)));
+  g.h = static_cast<uint16_t*>(d.workspace);
+  g.o = reinterpret_cast<float*>(g.h + (size_t)most * d.k * 2 * d.F);
   for (int t = 0; t < d.T; t += most) {
     g.T = d.T - t < most ? d.T - t : most;
     g.x = static_cast<const uint8_t*>(d.x) + (long long)t * g.ldx;

@@ -3,30 +3,48 @@
 
 #include "kernels.hpp"
 
-#include "hipgemm/detail/w4_vec.hpp"
-#include "hipgemm/detail/w4_stream.hpp"
+#include "hipgemm/detail/w4_rows.hpp"
 
 namespace hipgemm {
 namespace kernels {
 
-const void* w4_vec_bf16_int4(int s, int rows);
-const void* w4_vec_bf16_fp4(int s, int rows);
-const void* w4_vec_f16_int4(int s, int rows);
-const void* w4_vec_f16_fp4(int s, int rows);
-const void* w4_rows_bf16_int4(int s, int mode, int mt);
-const void* w4_rows_bf16_fp4(int s, int mode, int mt);
-const void* w4_rows_f16_int4(int s, int mode, int mt);
-const void* w4_rows_f16_fp4(int s, int mode, int mt);
+#define HIPGEMM_W4(X, W)                      \
+  const void* w4_vec_##X##_##W(int s, int rows, int lk); \
+  const void* w4_rows_##X##_##W(int s, int mode, int mt); \
+  const void* w4_sum_##X##_##W(int s);
+HIPGEMM_W4(bf16, int4)
+HIPGEMM_W4(bf16, int4z)
+HIPGEMM_W4(bf16, fp4)
+HIPGEMM_W4(f16, int4)
+HIPGEMM_W4(f16, int4z)
+HIPGEMM_W4(f16, fp4)
+#undef HIPGEMM_W4
 
-const void* w4_vec(int x, int w, int s, int rows) {
-  if (x == detail::kInBf16)
-    return w == detail::kWInt4 ? w4_vec_bf16_int4(s, rows) : w4_vec_bf16_fp4(s, rows);
-  return w == detail::kWInt4 ? w4_vec_f16_int4(s, rows) : w4_vec_f16_fp4(s, rows);
+const void* w4_vec(int x, int w, int s, int rows, int lk) {
+  const bool b = x == detail::kInBf16;
+  switch (w) {
+    case detail::kWInt4: return b ? w4_vec_bf16_int4(s, rows, lk) : w4_vec_f16_int4(s, rows, lk);
+    case detail::kWInt4Z: return b ? w4_vec_bf16_int4z(s, rows, lk) : w4_vec_f16_int4z(s, rows, lk);
+    default: return b ? w4_vec_bf16_fp4(s, rows, lk) : w4_vec_f16_fp4(s, rows, lk);
+  }
 }
 const void* w4_rows(int x, int w, int s, int mode, int mt) {
-  if (x == detail::kInBf16)
-    return w == detail::kWInt4 ? w4_rows_bf16_int4(s, mode, mt) : w4_rows_bf16_fp4(s, mode, mt);
-  return w == detail::kWInt4 ? w4_rows_f16_int4(s, mode, mt) : w4_rows_f16_fp4(s, mode, mt);
+  const bool b = x == detail::kInBf16;
+  switch (w) {
+    case detail::kWInt4:
+      return b ? w4_rows_bf16_int4(s, mode, mt) : w4_rows_f16_int4(s, mode, mt);
+    case detail::kWInt4Z:
+      return b ? w4_rows_bf16_int4z(s, mode, mt) : w4_rows_f16_int4z(s, mode, mt);
+    default: return b ? w4_rows_bf16_fp4(s, mode, mt) : w4_rows_f16_fp4(s, mode, mt);
+  }
+}
+const void* w4_sum(int x, int w, int s) {
+  const bool b = x == detail::kInBf16;
+  switch (w) {
+    case detail::kWInt4: return b ? w4_sum_bf16_int4(s) : w4_sum_f16_int4(s);
+    case detail::kWInt4Z: return b ? w4_sum_bf16_int4z(s) : w4_sum_f16_int4z(s);
+    default: return b ? w4_sum_bf16_fp4(s) : w4_sum_f16_fp4(s);
+  }
 }
 
 }  // namespace kernels
@@ -45,27 +63,60 @@ static_assert(HIPGEMM_IN_F32 == kInF32 && HIPGEMM_IN_BF16 == kInBf16 &&
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 constexpr int kMaxK = 1 << 26;
+constexpr long long kMaxRow = 1 << 25;  // 32 rows in a buffer's range
 
-hipError_t launch(const void* fn, dim3 grid, int threads, W4Args& g, hipStream_t stream) {
+template <class Args>
+hipError_t launch(const void* fn, dim3 grid, int threads, Args& g, hipStream_t stream) {
   if (!fn) return hipErrorInvalidValue;
   void* args[] = {&g};
   return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, stream);
 }
 
-// Lanes along K of a step, waves along K and rows of a workgroup.  lk: the
-// widest that leaves few lanes without codes in the last chunk.
-void vec_shape(int K, int* lk, int* waves_k, int* waves_r) {
-  const int units = K / 32;
-  int best = 64;
-  for (int l = 64; l >= 8; l /= 2) {
-    const int covered = (units + l - 1) / l * l, least = (units + best - 1) / best * best;
-    if (covered * 5 < least * 4) best = l;
+// The plan of k_w4_rows.  The activations of an item's rows and part of K lie in
+// LDS; parts of K are as many as that takes.
+struct RowsPlan {
+  int mt, rows_max, parts, len;
+};
+RowsPlan rows_plan(int M, int N, int K) {
+  RowsPlan p;
+  p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  auto fit = [&](int len) {
+    return p.mt == 1 ? Stream<kInBf16, kWFp4, kInF32, kCoarse, 1, false, 8>::rows_that_fit(len)
+         : p.mt == 2 ? Stream<kInBf16, kWFp4, kInF32, kCoarse, 2, false, 8>::rows_that_fit(len)
+                     : Stream<kInBf16, kWFp4, kInF32, kCoarse, 4, false, 8>::rows_that_fit(len);
+  };
+  const int steps = (K + 255) / 256, rows = M < 16 * p.mt ? M : 16 * p.mt;
+  for (p.parts = 1;; ++p.parts) {
+    const int len = (steps + p.parts - 1) / p.parts;
+    p.len = 256 * len;
+    p.rows_max = fit(p.len);
+    if (p.rows_max >= rows || len <= 1) break;
   }
-  const int chunks = units > best ? (units + best - 1) / best : 1;
+  p.parts = (steps + p.len / 256 - 1) / (p.len / 256);
+  if (p.parts < 1) p.parts = 1;
+  return p;
+}
+
+// k_w4_vec: lanes of a row, and the waves along K and rows of a workgroup.
+// 16 lanes where a chunk of 64 would leave half of the lanes idle or more.
+struct VecPlan {
+  int lk, waves_k, waves_r, rows, wave_rows;
+};
+VecPlan vec_plan(int N, int K) {
+  VecPlan p;
+  const int units = K / 32;
+  p.lk = units > 32 && (units + 63) / 64 * 64 * 3 < units * 4 ? 64 : 16;
+  const int chunks = units > p.lk ? (units + p.lk - 1) / p.lk : 1;
   const int turns = (chunks + 7) / 8;
-  *lk = best;
-  *waves_k = (chunks + turns - 1) / turns;
-  *waves_r = *waves_k >= 4 ? 1 : 4 / *waves_k;
+  p.waves_k = (chunks + turns - 1) / turns;
+  p.waves_r = p.waves_k >= 4 ? 1 : 4 / p.waves_k;
+  // Rows: two workgroups per CU, in whole steps of the waves.
+  const int step = kVecRows * (kWave / p.lk);
+  int steps = (N + 512 * step * p.waves_r - 1) / (512 * step * p.waves_r);
+  if (steps * step > kVecMaxRows) steps = kVecMaxRows / step;
+  p.wave_rows = steps * step;
+  p.rows = p.wave_rows * p.waves_r;
+  return p;
 }
 
 hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
@@ -87,12 +138,14 @@ hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
   g.G = d.group_size;
   g.act = d.activation;
   g.out = d.out_dtype;
+  const int w = d.zeros ? kWInt4Z : d.format;
   if (d.M <= 4) {
-    int waves_r;
-    vec_shape(d.K, &g.lk, &g.waves_k, &waves_r);
-    const int rows = kVecSteps * (kWave / g.lk) * waves_r;
-    return launch(hk::w4_vec(d.x_type, d.format, d.scale_type, d.M == 3 ? 4 : d.M),
-                  dim3((unsigned)((d.N + rows - 1) / rows)), kWave * g.waves_k * waves_r, g,
+    const VecPlan p = vec_plan(d.N, d.K);
+    g.waves_k = p.waves_k;
+    g.rows = p.rows;
+    g.wave_rows = p.wave_rows;
+    return launch(hk::w4_vec(d.x_type, w, d.scale_type, d.M == 3 ? 4 : d.M, p.lk),
+                  dim3((unsigned)((d.N + p.rows - 1) / p.rows)), kWave * p.waves_k * p.waves_r, g,
                   stream);
   }
   const int mode = d.format == HIPGEMM_W4_FP4 && d.scale_type == HIPGEMM_SCALE_E8M0 &&
@@ -100,13 +153,28 @@ hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
                        ? kInline
                    : d.group_size % 128 == 0 ? kCoarse
                                              : kFine;
-  const int mt = d.M <= 16 ? 1 : 2;
-  const unsigned tiles_m = (unsigned)((d.M + 16 * mt - 1) / (16 * mt));
-  return launch(hk::w4_rows(d.x_type, d.format, d.scale_type, mode, mt),
-                dim3((unsigned)((d.N + 31) / 32), tiles_m), 512, g, stream);
+  if (d.K == 0) {  // no parts to sum
+    W4RowsArgs r{g, nullptr, 1, 0, 0};
+    return launch(hk::w4_sum(d.x_type, w, d.scale_type),
+                  dim3((unsigned)((d.N + 255) / 256), (unsigned)d.M), 256, r, stream);
+  }
+  const RowsPlan p = rows_plan(d.M, d.N, d.K);
+  W4RowsArgs r{g, static_cast<float*>(d.workspace), p.rows_max, p.parts, p.len};
+  const int items = (d.M + p.rows_max - 1) / p.rows_max * p.parts * ((d.N + 31) / 32);
+  const hipError_t e = launch(hk::w4_rows(d.x_type, w, d.scale_type, mode, p.mt),
+                              dim3((unsigned)(items < 256 ? items : 256)), 512, r, stream);
+  if (e != hipSuccess || p.parts == 1) return e;
+  return launch(hk::w4_sum(d.x_type, w, d.scale_type),
+                dim3((unsigned)((d.N + 255) / 256), (unsigned)d.M), 256, r, stream);
 }
 
 }  // namespace
+
+extern "C" size_t hipgemm_w4_workspace_size(int M, int N, int K) {
+  if (M <= 4 || N <= 0 || K <= 0) return 0;
+  const RowsPlan p = rows_plan(M, N, K);
+  return p.parts == 1 ? 0 : (size_t)p.parts * M * N * 4;
+}
 
 extern "C" hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc* desc, hipStream_t stream) {
   if (!desc || desc->size != sizeof(hipgemm_w4_desc)) return hipErrorInvalidValue;
@@ -129,8 +197,12 @@ extern "C" hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc* desc, hipStream_t s
         !aligned(d.scales, type_bytes(d.scale_type)))
       return hipErrorInvalidValue;
     if (d.ldx < d.K || d.ldx % 8 != 0 || d.ldw < d.K / 2 || d.ldw % 16 != 0 ||
+        d.ldw > kMaxRow || d.lds > kMaxRow ||
         d.lds < (d.K + d.group_size - 1) / d.group_size)
       return hipErrorInvalidValue;
   }
+  const size_t need = hipgemm_w4_workspace_size(d.M, d.N, d.K);
+  if (need && (!d.workspace || !aligned(d.workspace, 16) || d.workspace_bytes < need))
+    return hipErrorInvalidValue;
   return run(d, stream);
 }

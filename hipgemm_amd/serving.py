@@ -17,7 +17,7 @@ import functools
 from . import (ACTIVATIONS, OUT_BF16, OUT_F16, OUT_F32, HipGemmError, _check,
                _torch, hipErrorInvalidValue, lib)
 
-__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "W4_FORMATS",
+__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "w4_workspace_size", "W4_FORMATS",
            "moe_route", "MOE_SCORING", "moe_experts", "MoeDesc", "MoeMatrix",
            "moe_experts_raw", "moe_workspace_size", "MOE_FORMATS"]
 
@@ -35,7 +35,8 @@ class W4Desc(ctypes.Structure):
                 ("M", _ci), ("N", _ci), ("K", _ci), ("group_size", _ci),
                 ("ldx", _ll), ("ldw", _ll), ("lds", _ll), ("ldy", _ll),
                 ("x_type", _ci), ("format", _ci), ("scale_type", _ci),
-                ("out_dtype", _ci), ("activation", _ci)]
+                ("out_dtype", _ci), ("activation", _ci), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t)]
 
 
 class MoeMatrix(ctypes.Structure):
@@ -76,6 +77,23 @@ def _stream_handle(t, stream) -> int:
     if stream is not None:
         return stream.cuda_stream
     return _torch()._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _scratch(nbytes: int, device, stream):
+    """Scratch memory for one call on `stream` (None: the current one)."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def w4_workspace_size(M: int, N: int, K: int) -> int:
+    """Workspace bytes hipgemm_w4_gemm needs (0: none)."""
+    return int(lib().hipgemm_w4_workspace_size(M, N, K))
+
+
+_w4_ws_bytes = functools.lru_cache(maxsize=1024)(w4_workspace_size)
 
 
 def w4_gemm_raw(desc: "W4Desc", stream: int = 0) -> int:
@@ -155,11 +173,14 @@ def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
                 and (N <= 1 or bias.stride(0) == 1)):
             _bad(f"bias must be a contiguous float32 device vector of {N} elements")
         bp = bias.data_ptr()
+    need = _w4_ws_bytes(M, N, K) if M > 4 else 0
+    if need:
+        ws = _scratch(need, x.device, stream)
     d = W4Desc(_W4_BYTES, x.data_ptr(), weight.data_ptr(), scales.data_ptr(), zp,
                out.data_ptr(), bp, M, N, K, group_size,
                x.stride(0) if M > 1 else K, weight.stride(0) if N > 1 else K // 2,
                lds, out.stride(0) if M > 1 else N, xt, fmt, st, ot,
-               ACTIVATIONS[activation])
+               ACTIVATIONS[activation], ws.data_ptr() if need else 0, need)
     _check(lib().hipgemm_w4_gemm(ctypes.byref(d), _stream_handle(x, stream)), "hipgemm_w4_gemm")
     return out
 
@@ -201,9 +222,9 @@ def moe_experts_raw(desc: "MoeDesc", stream: int = 0) -> int:
     return int(lib().hipgemm_moe_experts(ctypes.byref(desc), stream or None))
 
 
-def moe_workspace_size(T: int, k: int, E: int, F: int) -> int:
+def moe_workspace_size(T: int, k: int, E: int, D: int, F: int) -> int:
     """Workspace bytes hipgemm_moe_experts needs."""
-    return int(lib().hipgemm_moe_workspace_size(T, k, E, F))
+    return int(lib().hipgemm_moe_workspace_size(T, k, E, D, F))
 
 
 _moe_ws_bytes = functools.lru_cache(maxsize=1024)(moe_workspace_size)
@@ -295,13 +316,9 @@ def moe_experts(x, ids, weights, w13, scales13, w2, scales2, *, zeros13=None,
     elif (out.dtype != out_dtype or tuple(out.shape) != (T, D) or not out.is_cuda
           or out.stride(1) != 1):
         _bad(f"out must be a ({T}, {D}) {out_dtype} device tensor with unit column stride")
-    need = _moe_ws_bytes(T, k, E, F)
+    need = _moe_ws_bytes(T, k, E, D, F)
     if workspace is None:
-        if stream is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-        else:
-            with torch.cuda.stream(stream):
-                workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        workspace = _scratch(need, x.device, stream)
     elif workspace.dtype != torch.uint8 or not workspace.is_cuda \
             or not workspace.is_contiguous() or workspace.numel() < need:
         _bad(f"workspace must be a contiguous uint8 device tensor of {need} bytes")

@@ -29,8 +29,10 @@ constexpr int kInF32 = 0, kInBf16 = 1, kInF16 = 2, kScaleE8M0 = 3;
 __host__ __device__ constexpr int type_bytes(int t) {
   return t == kInF32 ? 4 : t == kScaleE8M0 ? 1 : 2;
 }
-// Weight formats.
-constexpr int kWInt4 = 0, kWFp4 = 1, kWE4M3 = 2;
+// Weight formats (HIPGEMM_W4_*, HIPGEMM_W8_E4M3; int4 with zero points is a
+// format of its own to the kernels).
+constexpr int kWInt4 = 0, kWFp4 = 1, kWE4M3 = 2, kWInt4Z = 3;
+__host__ __device__ constexpr bool is_int4(int w) { return w == kWInt4 || w == kWInt4Z; }
 
 // The offset that an int4 code carries after decoding to type kX.
 template <int kX>
@@ -71,19 +73,27 @@ __device__ __forceinline__ f32x2 unpack2(uint32_t a) {
 template <int kX>
 constexpr uint32_t kOnes2 = kX == kInBf16 ? 0x3f803f80u : 0x3c003c00u;
 
-// A scale as fp32.  E8M0: 2^(e - 127), 255 is NaN.
+// A scale as fp32, from its bits.  E8M0: 2^(e - 127), 255 is NaN.
+template <int kS>
+__device__ __forceinline__ float scale_of(uint32_t r) {
+  if constexpr (kS == kInF32) return __builtin_bit_cast(float, r);
+  else if constexpr (kS == kInBf16) return __builtin_bit_cast(float, r << 16);
+  else if constexpr (kS == kInF16) return (float)__builtin_bit_cast(_Float16, (uint16_t)r);
+  else
+    return __builtin_bit_cast(float, r == 255u ? 0x7fc00000u : r == 0u ? 0x00400000u : r << 23);
+}
+
+// The scale group of unit u of 32 weights, inv = 1 / (units per group): exact
+// for u < 2^21 (the quotient is 0.5 / group or more from an integer, its error
+// below u / group 2^-22).
+__device__ __forceinline__ int group_of(int u, float inv) {
+  return (int)(((float)u + 0.5f) * inv);
+}
 template <int kS>
 __device__ __forceinline__ float scale_at(const void* p, long long i) {
-  if constexpr (kS == kInF32) {
-    return static_cast<const float*>(p)[i];
-  } else if constexpr (kS == kInBf16) {
-    return __builtin_bit_cast(float, (uint32_t) static_cast<const uint16_t*>(p)[i] << 16);
-  } else if constexpr (kS == kInF16) {
-    return (float)static_cast<const _Float16*>(p)[i];
-  } else {
-    const uint32_t e = static_cast<const uint8_t*>(p)[i];
-    return __builtin_bit_cast(float, e == 255u ? 0x7fc00000u : e == 0u ? 0x00400000u : e << 23);
-  }
+  if constexpr (type_bytes(kS) == 4) return scale_of<kS>(static_cast<const uint32_t*>(p)[i]);
+  else if constexpr (type_bytes(kS) == 2) return scale_of<kS>(static_cast<const uint16_t*>(p)[i]);
+  else return scale_of<kS>(static_cast<const uint8_t*>(p)[i]);
 }
 
 // Eight codes of a dword (eight bytes for e4m3: lo, hi) as a 16-bit fragment;
@@ -91,7 +101,7 @@ __device__ __forceinline__ float scale_at(const void* p, long long i) {
 template <int kX, int kW>
 __device__ __forceinline__ i32x4 decode8(uint32_t lo, uint32_t hi, float scale) {
   i32x4 r;
-  if constexpr (kW == kWInt4) {
+  if constexpr (is_int4(kW)) {
     if constexpr (kX == kInBf16) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -133,7 +143,7 @@ __device__ __forceinline__ i32x4 decode8(uint32_t lo, uint32_t hi, float scale) 
 // Eight activations (four pairs of neighbours) in the order of decode8's pairs.
 template <int kW>
 __device__ __forceinline__ i32x4 pair_order(i32x4 x) {
-  if constexpr (kW != kWInt4) return x;
+  if constexpr (!is_int4(kW)) return x;
   return i32x4{(int)__builtin_amdgcn_perm((uint32_t)x[2], (uint32_t)x[0], 0x05040100u),
                (int)__builtin_amdgcn_perm((uint32_t)x[2], (uint32_t)x[0], 0x07060302u),
                (int)__builtin_amdgcn_perm((uint32_t)x[3], (uint32_t)x[1], 0x05040100u),
@@ -143,7 +153,7 @@ __device__ __forceinline__ i32x4 pair_order(i32x4 x) {
 // The value of one 4-bit code, scale excluded (rare paths).
 template <int kW>
 __device__ __forceinline__ float code_value(uint32_t q, float z) {
-  if constexpr (kW == kWInt4) return (float)q - z;
+  if constexpr (is_int4(kW)) return (float)q - z;
   const uint32_t m = q & 7u;
   const float v = m < 2u ? 0.5f * (float)m
                          : __builtin_bit_cast(float, ((126u + (m >> 1)) << 23) | ((m & 1u) << 22));

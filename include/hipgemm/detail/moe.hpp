@@ -1,24 +1,19 @@
-// The experts of a mixture-of-experts layer for a few tokens, in two kernels:
+// The experts of a mixture-of-experts layer for a few tokens:
 //
 //   k_moe_up    h[p] = weights[p] act(x[t] W13[e][:F]^T) (x[t] W13[e][F:]^T)
 //               for each pair p = (token t, its j-th choice), e = ids[p]
-//   k_moe_down  y[t] = sum_j h[t k + j] W2[e]^T
+//   k_moe_down  o[q][p] = h[p] W2[e]^T over the q-th part of F
+//   k_moe_sum   y[t] = sum_j sum_q o[q][t k + j]
 //
 // What bounds it: each chosen expert's weights are read once, whatever the
-// number of its tokens, so both stream weights past the few rows that need them
-// (w4_stream.hpp: Stream).
+// number of its tokens, so the first two stream weights past the few rows that
+// need them (w4_stream.hpp: Stream), one workgroup per CU, which share the work
+// evenly: all tiles of weights of all chosen experts, in order, cut into as many
+// pieces as there are workgroups.  Which experts those are, and their pairs, each
+// workgroup finds from the ids (at most kMoePairs) by itself, by counting.
 //
-// k_moe_up: a workgroup takes an expert and 16 of its F columns, gate and up,
-// and deals K to its waves.  The experts in question are found from the ids by
-// the workgroup itself (a ballot over at most kMoePairs ids): blockIdx.y names a
-// pair, which does the work if it is the first of its expert, or, where there are
-// more pairs than experts, the expert.  What it found goes to a table for the
-// second kernel.
-//
-// k_moe_down: a workgroup takes 16 columns of y for all chosen experts, dealt to
-// its waves by expert and part of K, so that all contributions to an output meet
-// in one workgroup's LDS, by pair, and are summed in the order of j: no atomics,
-// the same result every time.
+// The contributions to an output are written apart, by pair and part, and summed
+// in their order: no atomics, the same result every time.
 //
 // h is held as the sum of two bf16 numbers (16 significand bits; one rounding to
 // bf16 would leave an error as large as the output's own), and the second
@@ -31,7 +26,8 @@
 namespace hipgemm {
 namespace detail {
 
-constexpr int kMoePairs = 512;  // of one launch
+constexpr int kMoePairs = 512;     // of one launch
+constexpr int kMoeExperts = 1024;  // one per thread
 
 // Strides in bytes, but ldy in elements.
 struct MoeArgs {
@@ -44,172 +40,206 @@ struct MoeArgs {
   long long w2_row, w2_expert, s2_row, s2_expert, z2_row, z2_expert;
   uint8_t* y;
   uint16_t* h;  // pairs x 2 x F: high parts, low parts
-  int* table;   // per slot: pairs, expert, kMoePairs of list
-  int T, k, E, D, F, G13, G2;
+  float* o;     // parts x pairs x D
+  int T, k, E, D, F, G;
   int act, out;
-  int by_pair;    // slots are pairs (else experts)
-  int slots;
-  int max_parts;  // k_moe_down: parts of K at most
+  int parts, part_len;  // k_moe_down: of F
 };
 
-constexpr int kMoeTable = 2 + kMoePairs;
+// The pairs by expert: groups of up to rows_max pairs of one expert.
+struct MoeGroups {
+  uint16_t expert[kMoePairs], begin[kMoePairs], rows[kMoePairs];
+  // Pairs, by group (their experts while they are counted).
+  __attribute__((aligned(16))) uint16_t list[kMoePairs];
+};
 
-template <int kX, int kW, int kS, int kMode, int kMT>
-__global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
-  const int wave = wave_id(), lane = lane_id(), tid = (int)threadIdx.x;
-  const int slot = (int)blockIdx.y, f0 = (int)blockIdx.x * 16;
-  __shared__ uint64_t match[8];
-  __shared__ int list[kMoePairs];
+// Fills t, by all 1024 threads; count: LDS of kMoeExperts + 16 ints, free after.
+// Returns the number of groups.  A pair's place among its expert's is where the
+// counting put it, which may differ between workgroups: nothing depends on the
+// order within a group.  Where an expert has several groups, all workgroups have
+// to agree on them, and places go by the pairs' order.
+__device__ __forceinline__ int moe_groups(const MoeArgs& g, int rows_max, MoeGroups& t,
+                                          __attribute__((address_space(3))) int* count) {
+  const int tid = (int)threadIdx.x, wave = wave_id(), lane = lane_id();
   const int pairs = g.T * g.k;
-  const int e = g.by_pair ? g.ids[slot] : slot;
-  const bool valid = e >= 0 && e < g.E;
-  const bool mine = valid && tid < pairs && g.ids[tid] == e;
-  const uint64_t here = __builtin_amdgcn_ballot_w64(mine);
-  if (lane == 0) match[wave] = here;
+  auto* totals = count + kMoeExperts;
+  count[tid] = 0;
   __syncthreads();
-  int count = 0, before = 0, first = kMoePairs;
-#pragma unroll
-  for (int w = 7; w >= 0; --w) {
-    const uint64_t m = match[w];
-    count += __builtin_popcountll(m);
-    if (w < wave) before += __builtin_popcountll(m);
-    if (m) first = 64 * w + __builtin_ctzll(m);
-  }
-  if (g.by_pair && first != slot) count = 0;
-  if (mine) list[before + __builtin_popcountll(here & ((1ull << lane) - 1ull))] = tid;
+  const int id = tid < pairs ? g.ids[tid] : -1;
+  const bool on = id >= 0 && id < g.E;
+  int rank = 0;
+  if (on) rank = __hip_atomic_fetch_add(&count[id], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  if (tid < kMoePairs) t.list[tid] = (uint16_t)(on ? id : 0xffff);
   __syncthreads();
-  if (blockIdx.x == 0) {
-    int* t = g.table + (long long)slot * kMoeTable;
-    if (tid == 0) {
-      t[0] = count;
-      t[1] = e;
-    }
-    if (tid < count) t[2 + tid] = list[tid];
+  // Both sums at once: pairs above, groups below.
+  const int n = count[tid], groups = (n + rows_max - 1) / rows_max;
+  const int mine = n << 16 | groups;
+  int sum = mine;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int v = __shfl_up(sum, d, kWave);
+    if (lane >= d) sum += v;
   }
-  if (count == 0) return;
-
-  Stream<kX, kW, kS, kMode, 2, kMT, false> st;
-  st.K = g.D;
-  st.lo = 0;
-  st.inv = 32.0f / (float)g.G13;
+  if (lane == kWave - 1) totals[wave] = sum;
+  const bool several = __syncthreads_or(groups > 1);
+  if (several && on) {
+    rank = 0;
+    for (int j = 0; j < 64 * (wave + 1); j += 8) {
+      const i32x4 v = *reinterpret_cast<const i32x4*>(t.list + j);
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const long long r = n * g.F + f0 + (lane & 15);
-    st.w[n] = g.w13 + e * g.w13_expert + r * g.w13_row;
-    st.s[n] = g.s13 + e * g.s13_expert + r * g.s13_row;
-    st.z[n] = g.z13 ? g.z13 + e * g.z13_expert + r * g.z13_row : nullptr;
-  }
-  __shared__ float part[8][2][kMT][kWave * 4];
-  for (int m0 = 0; m0 < count; m0 += 16 * kMT) {
-#pragma unroll
-    for (int m = 0; m < kMT; ++m) {
-      st.x[m] = g.x + (long long)(list[min(m0 + 16 * m + (lane & 15), count - 1)] / g.k) * g.ldx;
-      st.acc[0][m] = st.acc[1][m] = f32x4{};
-    }
-    st.run(wave, st.pairs(), 8);
-    if (m0) __syncthreads();
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int m = 0; m < kMT; ++m)
-        *reinterpret_cast<f32x4*>(&part[wave][n][m][4 * lane]) = st.acc[n][m];
-    __syncthreads();
-    // One value per thread: 16 columns of a row in neighbouring threads.
-    for (int t = tid; t < 256 * kMT; t += 512) {
-      const int m = t >> 8, row = (t >> 4) & 15, col = t & 15;
-      const int at = 4 * (16 * (row >> 2) + col) + (row & 3);
-      float a = 0.0f, b = 0.0f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        a += part[w][0][m][at];
-        b += part[w][1][m][at];
+      for (int i = 0; i < 8; ++i) {
+        const int other = (int)((uint32_t)v[i / 2] >> (16 * (i & 1)) & 0xffffu);
+        rank += other == id && j + i < tid;
       }
-      const int r = m0 + 16 * m + row;
-      if (r >= count) continue;
-      const int f = f0 + col;
-      if constexpr (kW == kWE4M3) {
-        const uint8_t* s = g.s13 + e * g.s13_expert;
-        a *= *reinterpret_cast<const float*>(s + f * g.s13_row);
-        b *= *reinterpret_cast<const float*>(s + (g.F + f) * g.s13_row);
-      }
-      const int p = list[r];
-      const float v = activate(a, g.act) * b * g.weights[p];
-      const __bf16 hi = (__bf16)v;
-      const float rest = v - (float)hi;
-      // (an infinite h has no rest)
-      const __bf16 lo = (__bf16)(rest == rest ? rest : 0.0f);
-      uint16_t* h = g.h + (long long)p * 2 * g.F + f;
-      h[0] = __builtin_bit_cast(uint16_t, hi);
-      h[g.F] = __builtin_bit_cast(uint16_t, lo);
     }
   }
+  int all = 0;
+  for (int w = 0; w < 16; ++w) {
+    const int v = totals[w];
+    if (w < wave) sum += v;
+    all += v;
+  }
+  const int before = sum - mine, at = before >> 16;
+  for (int i = 0; i < groups; ++i) {
+    const int q = (before & 0xffff) + i;
+    t.expert[q] = (uint16_t)tid;
+    t.begin[q] = (uint16_t)(at + i * rows_max);
+    t.rows[q] = (uint16_t)min(rows_max, n - i * rows_max);
+  }
+  count[tid] = at;
+  __syncthreads();
+  if (on) t.list[count[id] + rank] = (uint16_t)tid;
+  __syncthreads();
+  return all & 0xffff;
 }
 
-template <int kW, int kS, int kMode>
-__global__ __launch_bounds__(512) void k_moe_down(MoeArgs g) {
-  const int wave = wave_id(), lane = lane_id(), tid = (int)threadIdx.x;
-  const int waves = (int)blockDim.x / kWave;
-  const int d0 = (int)blockIdx.x * 16;
-  const int pairs = g.T * g.k;
-  extern __shared__ float sums[];  // max_parts x pairs x 16
-  __shared__ uint64_t have[8];
-  __shared__ int active[kMoePairs];
-  // The slots that have pairs, in order.
-  const bool on = tid < g.slots && g.table[(long long)tid * kMoeTable] > 0;
-  const uint64_t here = __builtin_amdgcn_ballot_w64(on);
-  if (wave < 8 && lane == 0) have[wave] = here;
-  for (int i = tid; i < g.max_parts * pairs * 4; i += (int)blockDim.x)
-    reinterpret_cast<f32x4*>(sums)[i] = f32x4{};
-  __syncthreads();
-  int n_active = 0, before = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const uint64_t m = w < waves ? have[w] : 0ull;
-    n_active += __builtin_popcountll(m);
-    if (w < wave) before += __builtin_popcountll(m);
-  }
-  if (on) active[before + __builtin_popcountll(here & ((1ull << lane) - 1ull))] = tid;
-  __syncthreads();
+// This workgroup's share of items.
+__device__ __forceinline__ void share(int items, int* first, int* last) {
+  *first = (int)((long long)items * blockIdx.x / gridDim.x);
+  *last = (int)((long long)items * (blockIdx.x + 1) / gridDim.x);
+}
 
-  Stream<kInBf16, kW, kS, kMode, 1, 1, true> st;
-  st.K = g.F;
-  st.lo = 2ll * g.F;
-  st.inv = 32.0f / (float)g.G2;
-  // Parts of K: as many as leave every wave something to do.
-  const int steps = st.pairs();
-  int parts = 1;
-  while (2 * parts <= g.max_parts && 2 * parts <= steps && n_active * parts < waves) parts *= 2;
-  for (int item = wave; item < n_active * parts; item += waves) {
-    const int part = item % parts;
-    const int* t = g.table + (long long)__builtin_amdgcn_readfirstlane(active[item / parts]) * kMoeTable;
-    const int count = t[0], e = t[1];
-    const long long r = d0 + (lane & 15);
-    st.w[0] = g.w2 + e * g.w2_expert + r * g.w2_row;
-    st.s[0] = g.s2 + e * g.s2_expert + r * g.s2_row;
-    st.z[0] = g.z2 ? g.z2 + e * g.z2_expert + r * g.z2_row : nullptr;
-    float row_scale = 1.0f;
-    if constexpr (kW == kWE4M3) row_scale = *reinterpret_cast<const float*>(st.s[0]);
-    for (int m0 = 0; m0 < count; m0 += 16) {
-      st.x[0] = reinterpret_cast<const uint8_t*>(
-          g.h + (long long)t[2 + min(m0 + (lane & 15), count - 1)] * 2 * g.F);
-      st.acc[0][0] = f32x4{};
-      st.run(part * steps / parts, (part + 1) * steps / parts, 1);
+template <int kX, int kW, int kS, int kMode, int kMT>
+__global__ __launch_bounds__(1024) void k_moe_up(MoeArgs g) {
+  using S = Stream<kX, kW, kS, kMode, kMT, false, 16>;
+  constexpr int kCols = 16 * S::kWN;  // of F, of an item: gate and up rows
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kLdsBytes];
+  __shared__ MoeGroups t;
+  const int n_groups = moe_groups(g, S::rows_that_fit(g.D), t,
+                                  (__attribute__((address_space(3))) int*)(lds_u8*)lds);
+  const int tiles = (g.F + kCols - 1) / kCols;
+
+  struct Policy {
+    S st;
+    const MoeArgs& g;
+    const MoeGroups& t;
+    int tiles;
+    __device__ __forceinline__ int group(int item) const { return item / tiles; }
+    __device__ __forceinline__ int k_begin(int) const { return 0; }
+    __device__ __forceinline__ int rows(int q) const {
+      return __builtin_amdgcn_readfirstlane(t.rows[q]);
+    }
+    __device__ __forceinline__ int pair(int q, int m) const { return t.list[t.begin[q] + m]; }
+    __device__ __forceinline__ const uint8_t* row_at(int q, int, int m) const {
+      return g.x + (long long)(__builtin_amdgcn_readfirstlane(pair(q, m)) / g.k) * g.ldx;
+    }
+    __device__ __forceinline__ void weights(int item) {
+      const int q = item / tiles, e = __builtin_amdgcn_readfirstlane(t.expert[q]);
+      const int f = (item - q * tiles) * kCols + 16 * (wave_id() / S::kWK) + (lane_id() & 15);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = m0 + 4 * (lane >> 4) + i;
-        if (row < count)
-          sums[(part * pairs + t[2 + row]) * 16 + (lane & 15)] = st.acc[0][0][i] * row_scale;
+      for (int n = 0; n < 2; ++n) {
+        const long long r = n * g.F + min(f, g.F - 1);
+        st.w[n] = g.w13 + e * g.w13_expert + r * g.w13_row;
+        st.s[n] = g.s13 + e * g.s13_expert + r * g.s13_row;
+        if constexpr (kW == kWInt4Z) st.z[n] = g.z13 + e * g.z13_expert + r * g.z13_row;
       }
     }
-  }
-  __syncthreads();
-  for (int i = tid; i < g.T * 16; i += (int)blockDim.x) {
-    const int tok = i >> 4, col = i & 15;
-    float v = 0.0f;
-    for (int j = 0; j < g.k; ++j)
-      for (int q = 0; q < parts; ++q) v += sums[(q * pairs + tok * g.k + j) * 16 + col];
-    store_result(g.y, tok * g.ldy + d0 + col, g.out, v);
-  }
+    __device__ __forceinline__ void finish(int item) {
+      const int q = item / tiles, f0 = (item - q * tiles) * kCols, n_rows = rows(q);
+      // One value per thread and turn: neighbouring columns in neighbouring threads.
+      for (int i = (int)threadIdx.x; i < n_rows * kCols; i += S::kThreads) {
+        const int c = i % kCols, r = i / kCols, f = f0 + c;
+        if (f >= g.F) continue;
+        const float a = st.sum_of(c / 16, 0, r / 16, r % 16, c % 16);
+        const float b = st.sum_of(c / 16, 1, r / 16, r % 16, c % 16);
+        const int p = pair(q, r);
+        const float v = activate(a, g.act) * b * g.weights[p];
+        const __bf16 hi = (__bf16)v;
+        const float rest = v - (float)hi;
+        // (an infinite h has no rest)
+        const __bf16 lo = (__bf16)(rest == rest ? rest : 0.0f);
+        uint16_t* h = g.h + (long long)p * 2 * g.F + f;
+        h[0] = __builtin_bit_cast(uint16_t, hi);
+        h[g.F] = __builtin_bit_cast(uint16_t, lo);
+      }
+    }
+  };
+  Policy p{{}, g, t, tiles};
+  p.st.lds = (lds_u8*)lds;
+  p.st.K = g.D;
+  p.st.inv = 32.0f / (float)g.G;
+  int first, last;
+  share(n_groups * tiles, &first, &last);
+  p.st.run(first, last, g.D, p);
+}
+
+template <int kW, int kS, int kMode, int kMT>
+__global__ __launch_bounds__(1024) void k_moe_down(MoeArgs g) {
+  using S = Stream<kInBf16, kW, kS, kMode, kMT, true, 16>;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kLdsBytes];
+  __shared__ MoeGroups t;
+  const int n_groups = moe_groups(g, S::rows_that_fit(g.part_len), t,
+                                  (__attribute__((address_space(3))) int*)(lds_u8*)lds);
+  const int tiles = (g.D + S::kTile - 1) / S::kTile;
+
+  struct Policy {
+    S st;
+    const MoeArgs& g;
+    const MoeGroups& t;
+    int tiles;
+    // Groups here: an expert's rows over a part of F.
+    __device__ __forceinline__ int group(int item) const { return item / tiles; }
+    __device__ __forceinline__ int k_begin(int item) const {
+      return item / tiles % g.parts * g.part_len;
+    }
+    __device__ __forceinline__ int rows(int q) const {
+      return __builtin_amdgcn_readfirstlane(t.rows[q / g.parts]);
+    }
+    __device__ __forceinline__ int pair(int q, int m) const {
+      return t.list[t.begin[q / g.parts] + m];
+    }
+    __device__ __forceinline__ const uint8_t* row_at(int q, int part, int m) const {
+      return reinterpret_cast<const uint8_t*>(
+          g.h + ((long long)__builtin_amdgcn_readfirstlane(pair(q, m)) * 2 + part) * g.F);
+    }
+    __device__ __forceinline__ void weights(int item) {
+      const int q = item / tiles, e = __builtin_amdgcn_readfirstlane(t.expert[q / g.parts]);
+      const int d = (item - q * tiles) * S::kTile + 32 * (wave_id() / S::kWK) + (lane_id() & 15);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const long long r = min(d + 16 * n, g.D - 1);
+        st.w[n] = g.w2 + e * g.w2_expert + r * g.w2_row;
+        st.s[n] = g.s2 + e * g.s2_expert + r * g.s2_row;
+        if constexpr (kW == kWInt4Z) st.z[n] = g.z2 + e * g.z2_expert + r * g.z2_row;
+      }
+    }
+    __device__ __forceinline__ void finish(int item) {
+      const int q = item / tiles, d0 = (item - q * tiles) * S::kTile, n_rows = rows(q);
+      for (int i = (int)threadIdx.x; i < n_rows * S::kTile; i += S::kThreads) {
+        const int c = i % S::kTile, r = i / S::kTile, d = d0 + c;
+        if (d >= g.D) continue;
+        g.o[((long long)(q % g.parts) * (g.T * g.k) + pair(q, r)) * g.D + d] =
+            st.sum_of(c / 32, c / 16 % 2, r / 16, r % 16, c % 16);
+      }
+    }
+  };
+  Policy p{{}, g, t, tiles};
+  p.st.lds = (lds_u8*)lds;
+  p.st.K = g.F;
+  p.st.inv = 32.0f / (float)g.G;
+  int first, last;
+  share(n_groups * g.parts * tiles, &first, &last);
+  p.st.run(first, last, g.part_len, p);
 }
 
 }  // namespace detail

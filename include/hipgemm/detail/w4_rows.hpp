@@ -1,6 +1,5 @@
 // Products of 5 rows of 16-bit activations and more with 4-bit weights, while
-// the weights' bytes are what they cost: Stream over all of K, K dealt to the
-// waves of a workgroup and summed in LDS.
+// the weights' bytes are what they cost: Stream over all of K.
 #pragma once
 
 #include "w4_stream.hpp"
@@ -29,49 +28,77 @@ __device__ __forceinline__ float slow_row(const W4Args& g, int m, int n) {
   return sum;
 }
 
-template <int kX, int kW, int kS, int kMode, int kNT, int kMT>
-__global__ __launch_bounds__(512, 2) void k_w4_rows(W4Args g) {
-  const int wave = wave_id(), lane = lane_id(), waves = (int)(blockDim.x / kWave);
-  const int n0 = (int)blockIdx.x * 16 * kNT, m0 = (int)blockIdx.y * 16 * kMT;
-  Stream<kX, kW, kS, kMode, kNT, kMT, false> st;
-  st.K = g.K;
-  st.lo = 0;
-  st.inv = 32.0f / (float)g.G;
-#pragma unroll
-  for (int n = 0; n < kNT; ++n) {
-    const long long r = min(n0 + 16 * n + (lane & 15), g.N - 1);
-    st.w[n] = g.w + r * g.ldw;
-    st.s[n] = g.s + r * g.lds;
-    st.z[n] = g.z ? g.z + r * g.ldz : nullptr;
-  }
-#pragma unroll
-  for (int m = 0; m < kMT; ++m)
-    st.x[m] = g.x + (long long)min(m0 + 16 * m + (lane & 15), g.M - 1) * g.ldx;
-  st.run(wave, st.pairs(), waves);
+// Items: m tiles of up to rows_max rows, parts of K (len), 32 columns of y.  With
+// more than one part the sums go to o (parts x M x N) and k_w4_sum ends the work.
+struct W4RowsArgs {
+  W4Args a;
+  float* o;
+  int rows_max, parts, len;
+};
 
-  // Lane l, element e of tile (n, m): row 16 m + 4 (l / 16) + e, column 16 n + l % 16.
-  __shared__ f32x4 part[8 * kNT * kMT * kWave];
-#pragma unroll
-  for (int n = 0; n < kNT; ++n)
-#pragma unroll
-    for (int m = 0; m < kMT; ++m) part[(wave * kNT * kMT + n * kMT + m) * kWave + lane] = st.acc[n][m];
-  __syncthreads();
-  for (int t = wave; t < kNT * kMT; t += waves) {
-    f32x4 v = part[t * kWave + lane];
-    for (int w = 1; w < waves; ++w) v += part[(w * kNT * kMT + t) * kWave + lane];
-    const int n = n0 + 16 * (t / kMT) + (lane & 15);
-    const int m = m0 + 16 * (t % kMT) + 4 * (lane >> 4);
-    if (n >= g.N) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (m + e >= g.M) break;
-      float f = v[e];
-      if (!(__builtin_fabsf(f) < __builtin_inff()))
-        f = slow_row<kX, kW, kS>(g, m + e, n);
-      if (g.bias) f += g.bias[n];
-      store_result(g.y, (m + e) * g.ldy + n, g.out, activate(f, g.act));
+template <int kX, int kW, int kS>
+__device__ __forceinline__ void finish_w4(const W4Args& g, int m, int n, float f) {
+  if (!(__builtin_fabsf(f) < __builtin_inff())) f = slow_row<kX, kW, kS>(g, m, n);
+  if (g.bias) f += g.bias[n];
+  store_result(g.y, m * g.ldy + n, g.out, activate(f, g.act));
+}
+
+template <int kX, int kW, int kS, int kMode, int kMT>
+__global__ __launch_bounds__(512) void k_w4_rows(W4RowsArgs r) {
+  using S = Stream<kX, kW, kS, kMode, kMT, false, 8>;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kLdsBytes];
+  struct Policy {
+    S st;
+    const W4RowsArgs& r;
+    int tiles;
+    __device__ __forceinline__ int group(int item) const { return item / tiles; }
+    __device__ __forceinline__ int k_begin(int item) const {
+      return item / tiles % r.parts * r.len;
     }
-  }
+    __device__ __forceinline__ int m_begin(int q) const { return q / r.parts * r.rows_max; }
+    __device__ __forceinline__ int rows(int q) const {
+      return min(r.a.M - m_begin(q), r.rows_max);
+    }
+    __device__ __forceinline__ const uint8_t* row_at(int q, int, int m) const {
+      return r.a.x + (long long)(m_begin(q) + m) * r.a.ldx;
+    }
+    __device__ __forceinline__ void weights(int item) {
+      const int n0 = item % tiles * S::kTile + (lane_id() & 15);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const long long row = min(n0 + 16 * n, r.a.N - 1);
+        st.w[n] = r.a.w + row * r.a.ldw;
+        st.s[n] = r.a.s + row * r.a.lds;
+        if constexpr (kW == kWInt4Z) st.z[n] = r.a.z + row * r.a.ldz;
+      }
+    }
+    __device__ __forceinline__ void finish(int item) {
+      const int q = item / tiles, n0 = (item - q * tiles) * S::kTile, n_rows = rows(q);
+      for (int i = (int)threadIdx.x; i < n_rows * S::kTile; i += S::kThreads) {
+        const int c = i % S::kTile, row = i / S::kTile, n = n0 + c, m = m_begin(q) + row;
+        if (n >= r.a.N) continue;
+        const float f = st.sum_of(0, c / 16, row / 16, row % 16, c % 16);
+        if (r.parts > 1) r.o[((long long)(q % r.parts) * r.a.M + m) * r.a.N + n] = f;
+        else finish_w4<kX, kW, kS>(r.a, m, n, f);
+      }
+    }
+  };
+  Policy p{{}, r, (r.a.N + S::kTile - 1) / S::kTile};
+  p.st.lds = (lds_u8*)lds;
+  p.st.K = r.a.K;
+  p.st.inv = 32.0f / (float)r.a.G;
+  const int items = (r.a.M + r.rows_max - 1) / r.rows_max * r.parts * p.tiles;
+  p.st.run((int)((long long)items * blockIdx.x / gridDim.x),
+           (int)((long long)items * (blockIdx.x + 1) / gridDim.x), r.len, p);
+}
+
+template <int kX, int kW, int kS>
+__global__ __launch_bounds__(256) void k_w4_sum(W4RowsArgs r) {
+  const int n = (int)blockIdx.x * 256 + (int)threadIdx.x, m = (int)blockIdx.y;
+  if (n >= r.a.N) return;
+  float f = 0.0f;
+  for (int q = 0; q < r.parts; ++q) f += r.o[((long long)q * r.a.M + m) * r.a.N + n];
+  finish_w4<kX, kW, kS>(r.a, m, n, f);
 }
 
 }  // namespace detail

@@ -1,16 +1,15 @@
-// Products of up to four rows of 16-bit activations with 4-bit weights:
-// y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]).
+// Products of a few rows of 16-bit activations with quantised weights, a pass
+// over the weights' rows: y[m, n] = act(sum_k x[m, k] w[n, k] + bias[n]).
 //
-// A pass over the weights: each wave takes a chunk of 32 * lk codes of K (lk
-// lanes of 16 bytes, so one load reads lk * 16 consecutive bytes of a row; 1 KiB
-// at the usual 64), holds the activations of its chunk in registers, and runs
-// down kVecSteps rows with them.  So a weight costs its own load and nothing
-// else (the matrix unit's tiles would ask for a load of activations per load of
-// weights), and a lane's 32 codes lie in one scale group, whose scale multiplies
-// the lane's partial sum.  Products by the two-element dot instructions in
-// fp32.  Chunks are dealt to the waves_k waves of a row group; partial sums meet
-// in a transposed butterfly over the lanes (rows are halved as lanes are: 10
-// exchanges for 8 rows instead of 48) and then in LDS.
+// Each wave takes a chunk of K, 16 bytes of weights per lane (kLk lanes of a row:
+// 1 KiB of one row at the usual 64), holds the activations of its chunk in
+// registers, and runs down its rows with them, eight loads at a time and eight
+// ahead.  So a weight costs its own load and nothing else (the matrix unit's
+// tiles would ask for a read of activations per load of weights), memory is read
+// in the longest pieces there are, and a lane's weights lie in one scale group,
+// whose scale multiplies the lane's partial sum.  Products by the two-element dot
+// instructions in fp32.  The lanes' sums meet in a butterfly that halves the rows
+// as it halves the lanes, those of the chunks in LDS.
 //
 // The int4 excess (decode.hpp) is (bias + z) times the lane's sum of x.  Where
 // x is so large that the unscaled sums could overflow, or infinite, the wave
@@ -36,7 +35,7 @@ struct W4Args {
   long long ldx, ldw, lds, ldz, ldy;
   int M, N, K, G;
   int act, out;
-  int lk, waves_k;  // k_w4_vec only
+  int waves_k, rows, wave_rows;  // k_w4_vec: of a workgroup, of a wave
 };
 
 __device__ __forceinline__ float activate(float v, int act) {
@@ -55,157 +54,246 @@ __device__ __forceinline__ void store_result(uint8_t* y, long long i, int out, f
   else reinterpret_cast<__bf16*>(y)[i] = (__bf16)v;
 }
 
-constexpr int kVecSteps = 8;
-
-// One lane's 32 weights (at w) times its 32 activations, one by one and scaled
-// first.
-template <int kX, int kW>
-__device__ __forceinline__ float slow_dot32(const uint8_t* x, const uint8_t* w, float s, float z) {
-  float sum = 0.0f;
-#pragma unroll 1
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t c = w[i];
-    const f32x2 v = unpack2<kX>(reinterpret_cast<const uint32_t*>(x)[i]);
-    sum = __builtin_fmaf(v[0], s * code_value<kW>(c & 15u, z), sum);
-    sum = __builtin_fmaf(v[1], s * code_value<kW>(c >> 4, z), sum);
-  }
-  return sum;
-}
-
 // Magnitudes of x whose products with codes, and their sums, cannot overflow.
 constexpr float kSafeSum = 0x1p112f;
+constexpr int kVecRows = 8;       // loads of a step
+constexpr int kVecMaxRows = 128;  // of a workgroup
 
-template <int kX, int kW, int kS, int kM>
-__global__ __launch_bounds__(512) void k_w4_vec(W4Args g) {
-  const int wave = wave_id(), lane = lane_id();
-  const int lk = g.lk, per = kWave / lk;  // rows per step
-  const int wk = wave % g.waves_k, wr = wave / g.waves_k;
-  const int waves_r = (int)(blockDim.x / kWave) / g.waves_k;
-  const int rows = kVecSteps * per;  // of a wave
-  const int row0 = ((int)blockIdx.x * waves_r + wr) * rows;
-  const int kl = lane & (lk - 1), rl = lane / lk;
+// One wave's part: kM rows of x by rows of one matrix, over one chunk of K.
+template <int kX, int kW, int kS, int kM, int kLk>
+struct Vec {
+  static constexpr int kPer = kWave / kLk;              // rows of a load
+  static constexpr int kStep = kVecRows * kPer;         // rows of a step
+  static constexpr int kElems = kW == kWE4M3 ? 16 : 32;  // of a lane
+  static constexpr int kWords = kElems / 8;
+  static constexpr int kChunk = kLk * kElems;
+  static constexpr bool kScaled = kW != kWE4M3;  // by groups
 
-  float acc[kM][kVecSteps] = {};
-  for (int k0 = (wk * lk + kl) * 32; k0 - kl * 32 < g.K; k0 += g.waves_k * lk * 32) {
-    const bool in = k0 < g.K;
-    // Weights, scales and zero points of this chunk's rows first: all of them
-    // are in flight while the activations are read.
-    i32x4 w[kVecSteps];
-    float s[kVecSteps], z[kVecSteps];
-    const unsigned grp = in ? (unsigned)k0 / (unsigned)g.G : 0u;
+  i32x4 x[kM][kWords];
+  float xs[kM];
+  bool odd;        // the wave's x is out of the ordinary
+  int k;           // this lane's first element, or its last valid start
+  bool in;
+  uint32_t grp;
+
+  struct Rows {
+    i32x4 w[kVecRows];
+    uint32_t s[kVecRows], z[kVecRows];
+  };
+
+  // The chunk at k0 of a K long row; xr(m): row m of x.
+  template <class F>
+  __device__ __forceinline__ void begin(int k0, int K, int group, F&& xr) {
+    k = k0 + (lane_id() & (kLk - 1)) * kElems;
+    in = k < K;
+    grp = kScaled ? (uint32_t)group_of(min(k, K - 32) >> 5, 32.0f / (float)group) : 0u;
+    i32x4 v[kM][kWords];
 #pragma unroll
-    for (int i = 0; i < kVecSteps; ++i) {
-      const int r = min(row0 + i * per + rl, g.N - 1);
-      w[i] = in ? __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(
-                      g.w + r * g.ldw + (k0 >> 1)))
-                : i32x4{};
-    }
+    for (int m = 0; m < kM; ++m)
 #pragma unroll
-    for (int i = 0; i < kVecSteps; ++i) {
-      const int r = min(row0 + i * per + rl, g.N - 1);
-      s[i] = scale_at<kS>(g.s + r * g.lds, grp);
-      if constexpr (kW == kWInt4) z[i] = g.z ? (float)g.z[r * g.ldz + grp] : 8.0f;
-      else z[i] = 0.0f;
-    }
-    i32x4 x[kM][4];
-    float xs[kM];
-    bool odd = false;
+      for (int j = 0; j < kWords; ++j)
+        v[m][j] = *reinterpret_cast<const i32x4*>(xr(m) + 2ll * min(k + 8 * j, K - 8));
+    bool any = false;
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
-      const uint8_t* p = g.x + min(m, g.M - 1) * g.ldx + 2ll * k0;
+      float ss = 0.0f;
       xs[m] = 0.0f;
-      float mag = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const i32x4 v = in ? reinterpret_cast<const i32x4*>(p)[j] : i32x4{};
+      for (int j = 0; j < kWords; ++j) {
+        if (!in) v[m][j] = i32x4{};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (kW == kWInt4) xs[m] = dot2<kX>((uint32_t)v[e], kOnes2<kX>, xs[m]);
-          const f32x2 f = unpack2<kX>((uint32_t)v[e]);
-          mag = fmaxf(mag, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
+          const uint32_t u = (uint32_t)v[m][j][e];
+          if constexpr (is_int4(kW)) xs[m] = dot2<kX>(u, kOnes2<kX>, xs[m]);
+          if constexpr (kScaled) {
+            const f32x2 f = unpack2<kX>(u);
+            ss = fmaxf(ss, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
+          }
         }
-        x[m][j] = pair_order<kW>(v);
+        x[m][j] = pair_order<kW>(v[m][j]);
       }
       // (fp16 stays below it unless infinite; the maximum ignores a NaN, which
       // comes out as one either way)
-      odd |= !(mag < kSafeSum);
+      any |= !(ss < kSafeSum);
     }
-    const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0;
-    if (!any_odd) {
+    odd = kScaled && __builtin_amdgcn_ballot_w64(any) != 0;
+  }
+
+  // Rows row to below end of a matrix of `row_bytes`-byte rows (zeros past end).
+  __device__ __forceinline__ void load(Rows& r, const uint8_t* w, long long ldw, const uint8_t* s,
+                                       long long lds, const uint8_t* z, long long ldz, int row,
+                                       int end) const {
+    const int left = max(min(end - row, kStep), 0), rl = lane_id() / kLk;
+    const auto wb = make_rsrc(w + row * ldw, (uint32_t)(left * ldw));
+    const uint32_t wo = in ? (uint32_t)(rl * ldw) + (kW == kWE4M3 ? k : k >> 1) : kOobOffset;
 #pragma unroll
-      for (int i = 0; i < kVecSteps; ++i) {
+    for (int i = 0; i < kVecRows; ++i)
+      r.w[i] = __builtin_amdgcn_raw_buffer_load_b128(wb, wo, (uint32_t)(i * kPer * ldw), kStoreC);
+    if constexpr (kScaled) {
+      const auto sb = make_rsrc(s + row * lds, (uint32_t)(left * lds));
+      const uint32_t so = (uint32_t)(rl * lds) + grp * type_bytes(kS);
+#pragma unroll
+      for (int i = 0; i < kVecRows; ++i) {
+        const uint32_t at = (uint32_t)(i * kPer * lds);
+        if constexpr (type_bytes(kS) == 4) r.s[i] = __builtin_amdgcn_raw_buffer_load_b32(sb, so, at, 0);
+        else if constexpr (type_bytes(kS) == 2)
+          r.s[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sb, so, at, 0);
+        else r.s[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(sb, so, at, 0);
+      }
+      if constexpr (kW == kWInt4Z) {
+        const auto zb = make_rsrc(z + row * ldz, (uint32_t)(left * ldz));
+        const uint32_t zo = (uint32_t)(rl * ldz) + grp;
+#pragma unroll
+        for (int i = 0; i < kVecRows; ++i)
+          r.z[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zb, zo, (uint32_t)(i * kPer * ldz), 0);
+      }
+    }
+  }
+
+  // The lane's sums over its part of the chunk.
+  template <class F>
+  __device__ __forceinline__ void dot(const Rows& r, int K, F&& xr, float (&sum)[kM][kVecRows]) const {
+    if (!odd) {
+#pragma unroll
+      for (int i = 0; i < kVecRows; ++i) {
         float d[kM] = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const i32x4 b = decode8<kX, kW>((uint32_t)w[i][j], 0u, 1.0f);
+        for (int j = 0; j < kWords; ++j) {
+          const i32x4 b = kW == kWE4M3
+                              ? decode8<kX, kW>((uint32_t)r.w[i][2 * j % 4], (uint32_t)r.w[i][(2 * j + 1) % 4], 1.0f)
+                              : decode8<kX, kW>((uint32_t)r.w[i][j], 0u, 1.0f);
 #pragma unroll
           for (int m = 0; m < kM; ++m)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               d[m] = dot2<kX>((uint32_t)x[m][j][e], (uint32_t)b[e], d[m]);
         }
+        float sc = 1.0f, off = -(kInt4Bias<kX> + 8.0f);
+        if constexpr (kScaled) sc = scale_of<kS>(r.s[i]);
+        if constexpr (kW == kWInt4Z) off = -(kInt4Bias<kX> + (float)r.z[i]);
 #pragma unroll
         for (int m = 0; m < kM; ++m) {
-          if constexpr (kW == kWInt4)
-            d[m] = __builtin_fmaf(-(kInt4Bias<kX> + z[i]), xs[m], d[m]);
-          if (in) acc[m][i] = __builtin_fmaf(s[i], d[m], acc[m][i]);
+          if constexpr (is_int4(kW)) d[m] = __builtin_fmaf(off, xs[m], d[m]);
+          sum[m][i] = !kScaled ? d[m] : in ? sc * d[m] : 0.0f;
         }
-        sched_fence();  // one step's decoded codes at a time in registers
+        sched_fence();  // one row's decoded weights at a time in registers
       }
-    } else if (in) {
-#pragma unroll 1
-      for (int i = 0; i < kVecSteps; ++i) {
-        const int r = min(row0 + i * per + rl, g.N - 1);
-        const float sc = scale_at<kS>(g.s + r * g.lds, grp);
-        const float zp = g.z ? (float)g.z[r * g.ldz + grp] : 8.0f;
+    } else {
+      // One by one, and scaled first.
+#pragma unroll
+      for (int i = 0; i < kVecRows; ++i) {
+        const float sc = kScaled ? scale_of<kS>(r.s[i]) : 1.0f;
+        const float z = kW == kWInt4Z ? (float)r.z[i] : 8.0f;
 #pragma unroll
         for (int m = 0; m < kM; ++m) {
-          const float v = slow_dot32<kX, kW>(g.x + min(m, g.M - 1) * g.ldx + 2ll * k0,
-                                             g.w + r * g.ldw + (k0 >> 1), sc, zp);
-#pragma unroll
-          for (int e = 0; e < kVecSteps; ++e) acc[m][e] = e == i ? acc[m][e] + v : acc[m][e];
+          float d = 0.0f;
+          if (in) {
+#pragma unroll 1
+            for (int j = 0; j < kElems / 2; ++j) {
+              const uint32_t q = (uint32_t)(j < 4 ? r.w[i][0] : j < 8 ? r.w[i][1] : j < 12 ? r.w[i][2] : r.w[i][3]);
+              const uint32_t c = q >> (8 * (j & 3)) & 255u;
+              const f32x2 v = unpack2<kX>(*reinterpret_cast<const uint32_t*>(xr(m) + 2ll * k + 4 * j));
+              d = __builtin_fmaf(v[0], sc * code_value<kW>(c & 15u, z), d);
+              d = __builtin_fmaf(v[1], sc * code_value<kW>(c >> 4, z), d);
+            }
+          }
+          sum[m][i] = d;
         }
       }
     }
   }
 
-  // Sum over the lk lanes of a row: three steps that halve the rows a lane
-  // holds (lane bits 0-2 choose the row step), then plain ones.
-  __shared__ float part[8 * kVecSteps * 8 * kM];
+  // Adds the rows' sums over the lanes to to[row of the step].
+  __device__ __forceinline__ void gather(float (&v)[kVecRows], float* to) const {
+    const int lane = lane_id();
+    if constexpr (kLk == 64) {
+      // Half of the rows to the other 32 lanes, half of those to the other 16.
 #pragma unroll
-  for (int m = 0; m < kM; ++m) {
-    float v[kVecSteps];
+      for (int i = 0; i < 4; ++i) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v[i]),
+                                                        __builtin_bit_cast(uint32_t, v[i + 4]), false, false);
+        v[i] = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
+      }
 #pragma unroll
-    for (int i = 0; i < kVecSteps; ++i) v[i] = acc[m][i];
-#pragma unroll
-    for (int b = 0, n = kVecSteps; b < 3; ++b) {
-      n /= 2;
-      const bool up = (lane >> b) & 1;
-#pragma unroll
-      for (int i = 0; i < n; ++i) {
-        const float give = up ? v[i] : v[i + n];
-        const float keep = up ? v[i + n] : v[i];
-        v[i] = keep + __shfl_xor(give, 1 << b, kWave);
+      for (int i = 0; i < 2; ++i) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v[i]),
+                                                        __builtin_bit_cast(uint32_t, v[i + 2]), false, false);
+        v[i] = __builtin_bit_cast(float, (uint32_t)p[0]) + __builtin_bit_cast(float, (uint32_t)p[1]);
       }
     }
-    for (int b = 8; b < lk; b *= 2) v[0] += __shfl_xor(v[0], b, kWave);
-    // Lane bits 0, 1, 2 are bits 2, 1, 0 of the step whose row it holds.
-    if (kl < 8) {
-      const int step = ((kl & 1) << 2) | (kl & 2) | ((kl >> 2) & 1);
-      part[((wr * g.waves_k + wk) * kM + m) * rows + step * per + rl] = v[0];
+    constexpr int kLeft = kLk == 64 ? 2 : kVecRows;
+#pragma unroll
+    for (int i = 0; i < kLeft; ++i) {
+      v[i] += dpp_f<0xb1>(v[i]);   // quad_perm 1, 0, 3, 2
+      v[i] += dpp_f<0x4e>(v[i]);   // quad_perm 2, 3, 0, 1
+      v[i] += dpp_f<0x141>(v[i]);  // row_half_mirror
+      v[i] += dpp_f<0x140>(v[i]);  // row_mirror
+    }
+    if ((lane & 15) == 0) {
+#pragma unroll
+      for (int i = 0; i < kLeft; ++i) {
+        // 64 lanes: lane bit 5 is bit 2 of the row, bit 4 bit 1.  16: rows i kPer + l / 16.
+        const int row = kLk == 64 ? i + 2 * (lane >> 4 & 1) + 4 * (lane >> 5) : i * kPer + (lane >> 4);
+        to[row] += v[i];
+      }
     }
   }
-  __syncthreads();
-  const int total = waves_r * kM * rows;
-  for (int i = threadIdx.x; i < total; i += blockDim.x) {
-    const int r = i % rows, m = i / rows % kM, q = i / (rows * kM);
-    const int n = ((int)blockIdx.x * waves_r + q) * rows + r;
-    float v = 0.0f;
-    for (int w = 0; w < g.waves_k; ++w) v += part[((q * g.waves_k + w) * kM + m) * rows + r];
-    if (n < g.N && m < g.M) {
-      if (g.bias) v += g.bias[n];
-      store_result(g.y, m * g.ldy + n, g.out, activate(v, g.act));
+  template <int kCtrl>
+  __device__ static float dpp_f(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                                         0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, true));
+  }
+
+  // Rows r0 to below r1 of one matrix, with the x of begin(): adds to
+  // to[m * kVecMaxRows + row - r0], which is this wave's own.
+  template <class F>
+  __device__ __forceinline__ void rows(const uint8_t* w, long long ldw, const uint8_t* s, long long lds,
+                                       const uint8_t* z, long long ldz, int K, int r0, int r1, F&& xr,
+                                       float* to) const {
+    Rows ring[2];
+    load(ring[0], w, ldw, s, lds, z, ldz, r0, r1);
+    for (int row = r0; row < r1; row += 2 * kStep) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int at = row + u * kStep;
+        if (at >= r1) break;
+        load(ring[1 - u], w, ldw, s, lds, z, ldz, at + kStep, r1);
+        float sum[kM][kVecRows];
+        dot(ring[u], K, xr, sum);
+#pragma unroll
+        for (int m = 0; m < kM; ++m) gather(sum[m], to + m * kVecMaxRows + at - r0);
+      }
     }
+  }
+};
+
+template <int kX, int kW, int kS, int kM, int kLk>
+__global__ __launch_bounds__(512) void k_w4_vec(W4Args g) {
+  using V = Vec<kX, kW, kS, kM, kLk>;
+  const int wave = wave_id(), tid = (int)threadIdx.x;
+  const int wk = wave % g.waves_k, wr = wave / g.waves_k;
+  // A workgroup's rows, and this wave's.
+  const int n0 = (int)blockIdx.x * g.rows;
+  const int r0 = n0 + wr * g.wave_rows, r1 = min(min(r0 + g.wave_rows, n0 + g.rows), g.N);
+  __shared__ float part[8][kM * kVecMaxRows];
+  for (int i = tid; i < 8 * kM * kVecMaxRows; i += (int)blockDim.x) (&part[0][0])[i] = 0.0f;
+  __syncthreads();
+  auto xr = [&](int m) { return g.x + min(m, g.M - 1) * g.ldx; };
+  V v;
+  for (int k0 = wk * V::kChunk; k0 < g.K; k0 += g.waves_k * V::kChunk) {
+    v.begin(k0, g.K, g.G, xr);
+    if (r0 < r1) v.rows(g.w, g.ldw, g.s, g.lds, g.z, g.ldz, g.K, r0, r1, xr, part[wave]);
+  }
+  __syncthreads();
+  for (int i = tid; i < kM * g.rows; i += (int)blockDim.x) {
+    const int r = i % g.rows, m = i / g.rows, n = n0 + r;
+    if (n >= g.N || m >= g.M) continue;
+    const int q = r / g.wave_rows;
+    float f = 0.0f;
+    for (int w = 0; w < g.waves_k; ++w)
+      f += part[q * g.waves_k + w][m * kVecMaxRows + r - q * g.wave_rows];
+    if (g.bias) f += g.bias[n];
+    store_result(g.y, m * g.ldy + n, g.out, activate(f, g.act));
   }
 }
 

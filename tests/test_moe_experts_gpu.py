@@ -196,7 +196,7 @@ def test_other_stream_graph_and_workspace(hg):
     hg.moe_experts(**a, format="int4", out=y, stream=side)
     torch.cuda.synchronize()
     assert torch.equal(y, ref)
-    ws = torch.full((hg.moe_workspace_size(4, 4, 16, 256),), 255, dtype=torch.uint8,
+    ws = torch.full((hg.moe_workspace_size(4, 4, 16, 512, 256),), 255, dtype=torch.uint8,
                     device="cuda")
     assert torch.equal(hg.moe_experts(**a, format="int4", workspace=ws), ref)
     graph = torch.cuda.CUDAGraph()
@@ -252,6 +252,6 @@ def test_refusals(hg, change):
 
 def test_refuses_small_workspace(hg):
     a = make(2, 3, 4, 2, 64, 96)
-    ws = torch.empty(hg.moe_workspace_size(3, 2, 4, 96) - 1, dtype=torch.uint8, device="cuda")
+    ws = torch.empty(hg.moe_workspace_size(3, 2, 4, 64, 96) - 1, dtype=torch.uint8, device="cuda")
     with pytest.raises(hg.HipGemmError):
         hg.moe_experts(**a, workspace=ws)
