@@ -83,6 +83,8 @@ const void* w4_rows(int x, int w, int s, int mode, int mt);
 const void* w4_sum(int x, int w, int s);
 const void* moe_up(int x, int w, int s, int mode, int mt);
 const void* moe_down(int w, int s, int mode, int mt);
+const void* moe_vec_up(int x, int w, int s, int lk);
+const void* moe_vec_down(int w, int s, int lk);
 // Packs [rows][ceil(K/32)] E8M0 scales (row stride ld) into MxArgs' layout.
 hipError_t mx_pack(const uint8_t* src, int rows, int K, int ld, uint8_t* dst,
                    hipStream_t stream);

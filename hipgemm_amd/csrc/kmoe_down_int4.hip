@@ -7,6 +7,9 @@ namespace kernels {
 const void* moe_down_int4(int s, int mode, int mt) {
   return moe_down_of<detail::kWInt4>(s, mode, mt);
 }
+const void* moe_vec_down_int4(int s, int lk) {
+  return moe_vec_down_of<detail::kWInt4>(s, lk);
+}
 
 }  // namespace kernels
 }  // namespace hipgemm

@@ -7,6 +7,9 @@ namespace kernels {
 const void* moe_up_f16_fp4(int s, int mode, int mt) {
   return moe_up_of<detail::kInF16, detail::kWFp4>(s, mode, mt);
 }
+const void* moe_vec_up_f16_fp4(int s, int lk) {
+  return moe_vec_up_of<detail::kInF16, detail::kWFp4>(s, lk);
+}
 
 }  // namespace kernels
 }  // namespace hipgemm

@@ -4,7 +4,7 @@
 
 #include "kernels.hpp"
 
-#include "hipgemm/detail/moe.hpp"
+#include "hipgemm/detail/moe_vec.hpp"
 #include "hipgemm/detail/w4_rows.hpp"
 
 namespace hipgemm {
@@ -68,6 +68,27 @@ const void* moe_up_of(int s, int mode, int mt) {
       return (const void*)&detail::k_moe_up<kX, kW, decltype(S)::value, decltype(Mode)::value,
                                             decltype(MT)::value>;
     });
+  });
+}
+
+// Scale types as above, whatever the mode.
+template <int kW, class F>
+const void* sel_vec(int s, int lk, F&& f) {
+  using namespace detail;
+  auto by_lk = [&](auto S) { return lk == 64 ? f(S, ic<64>{}) : f(S, ic<16>{}); };
+  if constexpr (kW == kWE4M3) return s == kInF32 ? by_lk(ic<kInF32>{}) : nullptr;
+  else return sel4(s, by_lk);
+}
+template <int kX, int kW>
+const void* moe_vec_up_of(int s, int lk) {
+  return sel_vec<kW>(s, lk, [](auto S, auto L) {
+    return (const void*)&detail::k_moe_vec_up<kX, kW, decltype(S)::value, decltype(L)::value>;
+  });
+}
+template <int kW>
+const void* moe_vec_down_of(int s, int lk) {
+  return sel_vec<kW>(s, lk, [](auto S, auto L) {
+    return (const void*)&detail::k_moe_vec_down<kW, decltype(S)::value, decltype(L)::value>;
   });
 }
 

@@ -3,15 +3,18 @@
 
 #include "kernels.hpp"
 
-#include "hipgemm/detail/moe.hpp"
+#include "hipgemm/detail/moe_vec.hpp"
 
 namespace hipgemm {
 namespace kernels {
 
-#define HIPGEMM_MOE(W)                                            \
-  const void* moe_up_bf16_##W(int s, int mode, int mt);   \
-  const void* moe_up_f16_##W(int s, int mode, int mt);    \
-  const void* moe_down_##W(int s, int mode, int mt);
+#define HIPGEMM_MOE(W)                                  \
+  const void* moe_up_bf16_##W(int s, int mode, int mt); \
+  const void* moe_up_f16_##W(int s, int mode, int mt);  \
+  const void* moe_down_##W(int s, int mode, int mt);    \
+  const void* moe_vec_up_bf16_##W(int s, int lk);       \
+  const void* moe_vec_up_f16_##W(int s, int lk);        \
+  const void* moe_vec_down_##W(int s, int lk);
 HIPGEMM_MOE(int4)
 HIPGEMM_MOE(int4z)
 HIPGEMM_MOE(fp4)
@@ -34,6 +37,23 @@ const void* moe_down(int w, int s, int mode, int mt) {
     case detail::kWInt4Z: return moe_down_int4z(s, mode, mt);
     case detail::kWFp4: return moe_down_fp4(s, mode, mt);
     default: return moe_down_e4m3(s, mode, mt);
+  }
+}
+const void* moe_vec_up(int x, int w, int s, int lk) {
+  const bool b = x == detail::kInBf16;
+  switch (w) {
+    case detail::kWInt4: return b ? moe_vec_up_bf16_int4(s, lk) : moe_vec_up_f16_int4(s, lk);
+    case detail::kWInt4Z: return b ? moe_vec_up_bf16_int4z(s, lk) : moe_vec_up_f16_int4z(s, lk);
+    case detail::kWFp4: return b ? moe_vec_up_bf16_fp4(s, lk) : moe_vec_up_f16_fp4(s, lk);
+    default: return b ? moe_vec_up_bf16_e4m3(s, lk) : moe_vec_up_f16_e4m3(s, lk);
+  }
+}
+const void* moe_vec_down(int w, int s, int lk) {
+  switch (w) {
+    case detail::kWInt4: return moe_vec_down_int4(s, lk);
+    case detail::kWInt4Z: return moe_vec_down_int4z(s, lk);
+    case detail::kWFp4: return moe_vec_down_fp4(s, lk);
+    default: return moe_vec_down_e4m3(s, lk);
   }
 }
 
@@ -106,8 +126,48 @@ hipError_t launch(const void* fn, dim3 grid, int threads, MoeArgs& g, hipStream_
   return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, stream);
 }
 
+// Lanes of a row for rows of K elements (16 bytes of weights a lane): 16 where 64
+// would leave a quarter of the lanes idle or more.
+int vec_lanes(int K, int per_lane) {
+  const int units = K / per_lane;
+  return units > 32 && (units + 63) / 64 * 64 * 3 < units * 4 ? 64 : 16;
+}
+int chunks_of(int K, int per_lane, int lk) {
+  return (K + per_lane * lk - 1) / (per_lane * lk);
+}
+
+hipError_t vec_turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
+  const int per_lane = d.format == HIPGEMM_W8_E4M3 ? 16 : 32;
+  auto steps_of = [](int rows, int groups, int step) {  // of a wave: 512 workgroups
+    const int s = (rows + 512 * step / groups - 1) / (512 * step / groups > 0 ? 512 * step / groups : 1);
+    const int most = kVecMaxRows / step;
+    return s < 1 ? 1 : s > most ? most : s;
+  };
+  {
+    const int lk = vec_lanes(g.D, per_lane), chunks = chunks_of(g.D, per_lane, lk);
+    const int step = kVecRows * (kWave / lk), turns = (chunks + 3) / 4;
+    g.waves_k = (chunks + turns - 1) / turns;
+    const int waves_r = g.waves_k > 2 ? 1 : 4 / g.waves_k;  // pairs of gate and up
+    g.wave_rows = step * steps_of((g.F + waves_r - 1) / waves_r, g.T * g.k, step);
+    g.rows = g.wave_rows * waves_r;
+    if (g.rows > kVecMaxRows * waves_r) return hipErrorInvalidValue;
+    const hipError_t e = launch(
+        hk::moe_vec_up(d.x_type, d.w13.zeros ? kWInt4Z : d.format, d.scale_type, lk),
+        dim3((unsigned)((g.F + g.rows - 1) / g.rows), (unsigned)(g.T * g.k)),
+        kWave * g.waves_k * 2 * waves_r, g, stream);
+    if (e != hipSuccess) return e;
+  }
+  const int lk = vec_lanes(g.F, per_lane), chunks = chunks_of(g.F, per_lane, lk);
+  const int items = chunks * g.k, turns = (items + 7) / 8;
+  g.rows = kVecRows * (kWave / lk) * steps_of(g.D, g.T, kVecRows * (kWave / lk));
+  return launch(hk::moe_vec_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type, lk),
+                dim3((unsigned)((g.D + g.rows - 1) / g.rows), (unsigned)g.T),
+                kWave * ((items + turns - 1) / turns), g, stream);
+}
+
 hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   const int pairs = g.T * g.k;
+  if (g.T == 1) return vec_turn(g, d, stream);
   // Tiles of 16 tokens, two at a time where experts have more on average.
   const int mt = pairs > 12 * g.E ? 2 : 1;
   g.parts = down_parts(g.T, g.k, g.E, g.D, g.F, &g.part_len);

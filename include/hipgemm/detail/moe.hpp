@@ -44,7 +44,18 @@ struct MoeArgs {
   int T, k, E, D, F, G;
   int act, out;
   int parts, part_len;  // k_moe_down: of F
+  int waves_k, rows, wave_rows;  // k_moe_vec_*: of a workgroup, of a wave
 };
+
+// One value of h, in two parts (an infinite one has no rest).
+__device__ __forceinline__ void store_h(const MoeArgs& g, int pair, int f, float v) {
+  const __bf16 hi = (__bf16)v;
+  const float rest = v - (float)hi;
+  const __bf16 lo = (__bf16)(rest == rest ? rest : 0.0f);
+  uint16_t* h = g.h + (long long)pair * 2 * g.F + f;
+  h[0] = __builtin_bit_cast(uint16_t, hi);
+  h[g.F] = __builtin_bit_cast(uint16_t, lo);
+}
 
 // The pairs by expert: groups of up to rows_max pairs of one expert.
 struct MoeGroups {
@@ -163,14 +174,7 @@ __global__ __launch_bounds__(1024) void k_moe_up(MoeArgs g) {
         const float a = st.sum_of(c / 16, 0, r / 16, r % 16, c % 16);
         const float b = st.sum_of(c / 16, 1, r / 16, r % 16, c % 16);
         const int p = pair(q, r);
-        const float v = activate(a, g.act) * b * g.weights[p];
-        const __bf16 hi = (__bf16)v;
-        const float rest = v - (float)hi;
-        // (an infinite h has no rest)
-        const __bf16 lo = (__bf16)(rest == rest ? rest : 0.0f);
-        uint16_t* h = g.h + (long long)p * 2 * g.F + f;
-        h[0] = __builtin_bit_cast(uint16_t, hi);
-        h[g.F] = __builtin_bit_cast(uint16_t, lo);
+        store_h(g, p, f, activate(a, g.act) * b * g.weights[p]);
       }
     }
   };

@@ -67,7 +67,8 @@ struct Vec {
   static constexpr int kElems = kW == kWE4M3 ? 16 : 32;  // of a lane
   static constexpr int kWords = kElems / 8;
   static constexpr int kChunk = kLk * kElems;
-  static constexpr bool kScaled = kW != kWE4M3;  // by groups
+  // (e4m3 rows have one scale each: group 0)
+  static constexpr bool kGroups = kW != kWE4M3;
 
   i32x4 x[kM][kWords];
   float xs[kM];
@@ -81,22 +82,12 @@ struct Vec {
     uint32_t s[kVecRows], z[kVecRows];
   };
 
-  // The chunk at k0 of a K long row; xr(m): row m of x.
-  template <class F>
-  __device__ __forceinline__ void begin(int k0, int K, int group, F&& xr) {
-    k = k0 + (lane_id() & (kLk - 1)) * kElems;
-    in = k < K;
-    grp = kScaled ? (uint32_t)group_of(min(k, K - 32) >> 5, 32.0f / (float)group) : 0u;
-    i32x4 v[kM][kWords];
-#pragma unroll
-    for (int m = 0; m < kM; ++m)
-#pragma unroll
-      for (int j = 0; j < kWords; ++j)
-        v[m][j] = *reinterpret_cast<const i32x4*>(xr(m) + 2ll * min(k + 8 * j, K - 8));
+  // The chunk's activations, loaded to v, into the form that dot takes.
+  __device__ __forceinline__ void take(i32x4 (&v)[kM][kWords]) {
     bool any = false;
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
-      float ss = 0.0f;
+      float top = 0.0f;
       xs[m] = 0.0f;
 #pragma unroll
       for (int j = 0; j < kWords; ++j) {
@@ -105,18 +96,18 @@ struct Vec {
         for (int e = 0; e < 4; ++e) {
           const uint32_t u = (uint32_t)v[m][j][e];
           if constexpr (is_int4(kW)) xs[m] = dot2<kX>(u, kOnes2<kX>, xs[m]);
-          if constexpr (kScaled) {
+          if constexpr (kGroups) {
             const f32x2 f = unpack2<kX>(u);
-            ss = fmaxf(ss, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
+            top = fmaxf(top, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
           }
         }
         x[m][j] = pair_order<kW>(v[m][j]);
       }
       // (fp16 stays below it unless infinite; the maximum ignores a NaN, which
       // comes out as one either way)
-      any |= !(ss < kSafeSum);
+      any |= !(top < kSafeSum);
     }
-    odd = kScaled && __builtin_amdgcn_ballot_w64(any) != 0;
+    odd = kGroups && __builtin_amdgcn_ballot_w64(any) != 0;
   }
 
   // Rows row to below end of a matrix of `row_bytes`-byte rows (zeros past end).
@@ -129,7 +120,7 @@ struct Vec {
 #pragma unroll
     for (int i = 0; i < kVecRows; ++i)
       r.w[i] = __builtin_amdgcn_raw_buffer_load_b128(wb, wo, (uint32_t)(i * kPer * ldw), kStoreC);
-    if constexpr (kScaled) {
+    {
       const auto sb = make_rsrc(s + row * lds, (uint32_t)(left * lds));
       const uint32_t so = (uint32_t)(rl * lds) + grp * type_bytes(kS);
 #pragma unroll
@@ -168,13 +159,13 @@ struct Vec {
             for (int e = 0; e < 4; ++e)
               d[m] = dot2<kX>((uint32_t)x[m][j][e], (uint32_t)b[e], d[m]);
         }
-        float sc = 1.0f, off = -(kInt4Bias<kX> + 8.0f);
-        if constexpr (kScaled) sc = scale_of<kS>(r.s[i]);
+        const float sc = scale_of<kS>(r.s[i]);
+        float off = -(kInt4Bias<kX> + 8.0f);
         if constexpr (kW == kWInt4Z) off = -(kInt4Bias<kX> + (float)r.z[i]);
 #pragma unroll
         for (int m = 0; m < kM; ++m) {
           if constexpr (is_int4(kW)) d[m] = __builtin_fmaf(off, xs[m], d[m]);
-          sum[m][i] = !kScaled ? d[m] : in ? sc * d[m] : 0.0f;
+          sum[m][i] = in ? sc * d[m] : 0.0f;
         }
         sched_fence();  // one row's decoded weights at a time in registers
       }
@@ -182,7 +173,7 @@ struct Vec {
       // One by one, and scaled first.
 #pragma unroll
       for (int i = 0; i < kVecRows; ++i) {
-        const float sc = kScaled ? scale_of<kS>(r.s[i]) : 1.0f;
+        const float sc = scale_of<kS>(r.s[i]);
         const float z = kW == kWInt4Z ? (float)r.z[i] : 8.0f;
 #pragma unroll
         for (int m = 0; m < kM; ++m) {
@@ -244,14 +235,26 @@ struct Vec {
                                          0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, true));
   }
 
-  // Rows r0 to below r1 of one matrix, with the x of begin(): adds to
-  // to[m * kVecMaxRows + row - r0], which is this wave's own.
+  // Rows r0 to below r1 of one matrix (rows of K) by the chunk at k0 of the rows
+  // of x, xr(m); adds to to[m * kVecMaxRows + row - r0], which is this wave's own.
   template <class F>
-  __device__ __forceinline__ void rows(const uint8_t* w, long long ldw, const uint8_t* s, long long lds,
-                                       const uint8_t* z, long long ldz, int K, int r0, int r1, F&& xr,
-                                       float* to) const {
+  __device__ __forceinline__ void pass(int k0, int K, int group, F&& xr, const uint8_t* w,
+                                       long long ldw, const uint8_t* s, long long lds,
+                                       const uint8_t* z, long long ldz, int r0, int r1, float* to) {
+    k = k0 + (lane_id() & (kLk - 1)) * kElems;
+    in = k < K;
+    grp = kGroups ? (uint32_t)group_of(min(k, K - 32) >> 5, 32.0f / (float)group) : 0u;
+    i32x4 v[kM][kWords];
+#pragma unroll
+    for (int m = 0; m < kM; ++m)
+#pragma unroll
+      for (int j = 0; j < kWords; ++j)
+        v[m][j] = *reinterpret_cast<const i32x4*>(xr(m) + 2ll * min(k + 8 * j, K - 8));
+    sched_fence();
     Rows ring[2];
     load(ring[0], w, ldw, s, lds, z, ldz, r0, r1);
+    sched_fence();
+    take(v);
     for (int row = r0; row < r1; row += 2 * kStep) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -281,8 +284,8 @@ __global__ __launch_bounds__(512) void k_w4_vec(W4Args g) {
   auto xr = [&](int m) { return g.x + min(m, g.M - 1) * g.ldx; };
   V v;
   for (int k0 = wk * V::kChunk; k0 < g.K; k0 += g.waves_k * V::kChunk) {
-    v.begin(k0, g.K, g.G, xr);
-    if (r0 < r1) v.rows(g.w, g.ldw, g.s, g.lds, g.z, g.ldz, g.K, r0, r1, xr, part[wave]);
+    if (r0 < r1)
+      v.pass(k0, g.K, g.G, xr, g.w, g.ldw, g.s, g.lds, g.z, g.ldz, r0, r1, part[wave]);
   }
   __syncthreads();
   for (int i = tid; i < kM * g.rows; i += (int)blockDim.x) {
