@@ -76,8 +76,7 @@ hipError_t quantize_rows(const void* x, int type, int M, int K, long long ldx,
 // Products of 16-bit activations with quantised weights (kw4_*.hip, kmoe_*.hip).
 // x: activations' type, w: detail::kW*, s: scales' type, mode: detail::kNone,
 // kCoarse, kFine or kInline; rows: 1, 2 or 4, lk: 16
-// or 64 lanes of a row; mt: tiles of 16 rows of x (1, 2, for
-// w4_rows also 4).
+// or 64 lanes of a row; mt: tiles of 16 rows of x (1, 2).
 const void* w4_vec(int x, int w, int s, int rows, int lk);
 const void* w4_rows(int x, int w, int s, int mode, int mt);
 const void* w4_sum(int x, int w, int s);

@@ -49,11 +49,10 @@ const void* sel_mt(int mt, F&& f) {
 template <int kX, int kW>
 const void* w4_rows_of(int s, int mode, int mt) {
   return sel_scales<kX, kW>(s, mode, [&](auto S, auto Mode) {
-    auto f = [&](auto MT) {
+    return sel_mt(mt, [&](auto MT) {
       return (const void*)&detail::k_w4_rows<kX, kW, decltype(S)::value, decltype(Mode)::value,
                                              decltype(MT)::value>;
-    };
-    return mt == 4 ? f(ic<4>{}) : sel_mt(mt, f);
+    });
   });
 }
 template <int kX, int kW>

@@ -87,7 +87,8 @@ __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs g) {
 
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-constexpr int kMaxDim = 1 << 26;  // Stream's group index
+constexpr int kMaxDim = 1 << 26;           // Stream's group index
+constexpr long long kMaxRow = 1 << 25;  // 32 rows in a buffer's range
 
 // Tokens of one turn.
 int turn_tokens(int T, int k) { return T < kMoePairs / k ? T : kMoePairs / k; }
@@ -102,7 +103,7 @@ bool matrix_ok(const hipgemm_moe_matrix& m, int rows, int K, const hipgemm_moe_d
   const bool e4m3 = d.format == HIPGEMM_W8_E4M3;
   const long long row = e4m3 ? K : K / 2;
   const long long groups = e4m3 ? 1 : (K + d.group_size - 1) / d.group_size;
-  return m.weight && m.scales && aligned(m.weight, 16) &&
+  return m.weight && m.scales && aligned(m.weight, 16) && m.ldw <= kMaxRow && m.lds <= kMaxRow &&
          aligned(m.scales, type_bytes(d.scale_type)) && m.ldw >= row && m.ldw % 16 == 0 &&
          m.expert_w % 16 == 0 && (d.E == 1 || m.expert_w >= (rows - 1) * m.ldw + row) &&
          m.lds >= groups && (d.E == 1 || m.expert_s >= (rows - 1) * m.lds + groups) &&
@@ -174,11 +175,11 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   const int cus = 256;
   hipError_t e = launch(hk::moe_up(d.x_type, d.w13.zeros ? kWInt4Z : d.format, d.scale_type,
                                    mode_of(d.x_type, d.format, d.scale_type, d.group_size), mt),
-                        dim3((unsigned)cus), 1024, g, stream);
+                        dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   e = launch(hk::moe_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type,
                           mode_of(kInBf16, d.format, d.scale_type, d.group_size), mt),
-             dim3((unsigned)cus), 1024, g, stream);
+             dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   return launch((const void*)&k_moe_sum, dim3((unsigned)((g.T * (g.D / 4) + 255) / 256)), 256, g,
                 stream);

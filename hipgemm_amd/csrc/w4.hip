@@ -79,11 +79,10 @@ struct RowsPlan {
 };
 RowsPlan rows_plan(int M, int N, int K) {
   RowsPlan p;
-  p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  p.mt = M <= 16 ? 1 : 2;
   auto fit = [&](int len) {
-    return p.mt == 1 ? Stream<kInBf16, kWFp4, kInF32, kCoarse, 1, false, 8>::rows_that_fit(len)
-         : p.mt == 2 ? Stream<kInBf16, kWFp4, kInF32, kCoarse, 2, false, 8>::rows_that_fit(len)
-                     : Stream<kInBf16, kWFp4, kInF32, kCoarse, 4, false, 8>::rows_that_fit(len);
+    return p.mt == 1 ? Stream<kInBf16, kWFp4, kInF32, kCoarse, 1, false>::rows_that_fit(len)
+                     : Stream<kInBf16, kWFp4, kInF32, kCoarse, 2, false>::rows_that_fit(len);
   };
   const int steps = (K + 255) / 256, rows = M < 16 * p.mt ? M : 16 * p.mt;
   for (p.parts = 1;; ++p.parts) {

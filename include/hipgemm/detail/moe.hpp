@@ -27,7 +27,7 @@ namespace hipgemm {
 namespace detail {
 
 constexpr int kMoePairs = 512;     // of one launch
-constexpr int kMoeExperts = 1024;  // one per thread
+constexpr int kMoeExperts = 1024;  // two per thread
 
 // Strides in bytes, but ldy in elements.
 struct MoeArgs {
@@ -62,9 +62,11 @@ struct MoeGroups {
   uint16_t expert[kMoePairs], begin[kMoePairs], rows[kMoePairs];
   // Pairs, by group (their experts while they are counted).
   __attribute__((aligned(16))) uint16_t list[kMoePairs];
+  // By pair (a load of memory at an item's end would wait for the weights ahead).
+  float weight[kMoePairs];
 };
 
-// Fills t, by all 1024 threads; count: LDS of kMoeExperts + 16 ints, free after.
+// Fills t, by all 512 threads; count: LDS of kMoeExperts + 8 ints, free after.
 // Returns the number of groups.  A pair's place among its expert's is where the
 // counting put it, which may differ between workgroups: nothing depends on the
 // order within a group.  Where an expert has several groups, all workgroups have
@@ -74,17 +76,19 @@ __device__ __forceinline__ int moe_groups(const MoeArgs& g, int rows_max, MoeGro
   const int tid = (int)threadIdx.x, wave = wave_id(), lane = lane_id();
   const int pairs = g.T * g.k;
   auto* totals = count + kMoeExperts;
-  count[tid] = 0;
-  __syncthreads();
   const int id = tid < pairs ? g.ids[tid] : -1;
   const bool on = id >= 0 && id < g.E;
+  count[2 * tid] = count[2 * tid + 1] = 0;
+  __syncthreads();
   int rank = 0;
   if (on) rank = __hip_atomic_fetch_add(&count[id], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-  if (tid < kMoePairs) t.list[tid] = (uint16_t)(on ? id : 0xffff);
+  t.list[tid] = (uint16_t)(on ? id : 0xffff);
+  t.weight[tid] = on ? g.weights[tid] : 0.0f;
   __syncthreads();
-  // Both sums at once: pairs above, groups below.
-  const int n = count[tid], groups = (n + rows_max - 1) / rows_max;
-  const int mine = n << 16 | groups;
+  // A thread's two experts; both sums at once: pairs above, groups below.
+  const int n[2] = {count[2 * tid], count[2 * tid + 1]};
+  const int groups[2] = {(n[0] + rows_max - 1) / rows_max, (n[1] + rows_max - 1) / rows_max};
+  const int mine = (n[0] + n[1]) << 16 | (groups[0] + groups[1]);
   int sum = mine;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
@@ -92,7 +96,7 @@ __device__ __forceinline__ int moe_groups(const MoeArgs& g, int rows_max, MoeGro
     if (lane >= d) sum += v;
   }
   if (lane == kWave - 1) totals[wave] = sum;
-  const bool several = __syncthreads_or(groups > 1);
+  const bool several = __syncthreads_or(groups[0] > 1 || groups[1] > 1);
   if (several && on) {
     rank = 0;
     for (int j = 0; j < 64 * (wave + 1); j += 8) {
@@ -105,19 +109,24 @@ __device__ __forceinline__ int moe_groups(const MoeArgs& g, int rows_max, MoeGro
     }
   }
   int all = 0;
-  for (int w = 0; w < 16; ++w) {
+  for (int w = 0; w < 8; ++w) {
     const int v = totals[w];
     if (w < wave) sum += v;
     all += v;
   }
-  const int before = sum - mine, at = before >> 16;
-  for (int i = 0; i < groups; ++i) {
-    const int q = (before & 0xffff) + i;
-    t.expert[q] = (uint16_t)tid;
-    t.begin[q] = (uint16_t)(at + i * rows_max);
-    t.rows[q] = (uint16_t)min(rows_max, n - i * rows_max);
+  int before = sum - mine;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const int at = before >> 16;
+    for (int i = 0; i < groups[x]; ++i) {
+      const int q = (before & 0xffff) + i;
+      t.expert[q] = (uint16_t)(2 * tid + x);
+      t.begin[q] = (uint16_t)(at + i * rows_max);
+      t.rows[q] = (uint16_t)min(rows_max, n[x] - i * rows_max);
+    }
+    count[2 * tid + x] = at;
+    before += n[x] << 16 | groups[x];
   }
-  count[tid] = at;
   __syncthreads();
   if (on) t.list[count[id] + rank] = (uint16_t)tid;
   __syncthreads();
@@ -131,10 +140,12 @@ __device__ __forceinline__ void share(int items, int* first, int* last) {
 }
 
 template <int kX, int kW, int kS, int kMode, int kMT>
-__global__ __launch_bounds__(1024) void k_moe_up(MoeArgs g) {
-  using S = Stream<kX, kW, kS, kMode, kMT, false, 16>;
-  constexpr int kCols = 16 * S::kWN;  // of F, of an item: gate and up rows
-  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kLdsBytes];
+__global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
+  using S = Stream<kX, kW, kS, kMode, kMT, false>;
+  constexpr int kCols = 16;  // of F, of an item: gate and up rows
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kXBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t rings[S::kRingBytes];
+  __shared__ float sums[S::kSums];
   __shared__ MoeGroups t;
   const int n_groups = moe_groups(g, S::rows_that_fit(g.D), t,
                                   (__attribute__((address_space(3))) int*)(lds_u8*)lds);
@@ -156,13 +167,13 @@ __global__ __launch_bounds__(1024) void k_moe_up(MoeArgs g) {
     }
     __device__ __forceinline__ void weights(int item) {
       const int q = item / tiles, e = __builtin_amdgcn_readfirstlane(t.expert[q]);
-      const int f = (item - q * tiles) * kCols + 16 * (wave_id() / S::kWK) + (lane_id() & 15);
+      const int f0 = (item - q * tiles) * kCols;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const long long r = n * g.F + min(f, g.F - 1);
-        st.w[n] = g.w13 + e * g.w13_expert + r * g.w13_row;
-        st.s[n] = g.s13 + e * g.s13_expert + r * g.s13_row;
-        if constexpr (kW == kWInt4Z) st.z[n] = g.z13 + e * g.z13_expert + r * g.z13_row;
+        st.set_tile(n, g.w13 + e * g.w13_expert + ((long long)n * g.F + f0) * g.w13_row, g.F - f0);
+        const long long r = (long long)st.scale_tile(n) * g.F + min(f0 + (lane_id() & 15), g.F - 1);
+        st.sp[n] = g.s13 + e * g.s13_expert + r * g.s13_row;
+        if constexpr (kW == kWInt4Z) st.zp[n] = g.z13 + e * g.z13_expert + r * g.z13_row;
       }
     }
     __device__ __forceinline__ void finish(int item) {
@@ -171,16 +182,19 @@ __global__ __launch_bounds__(1024) void k_moe_up(MoeArgs g) {
       for (int i = (int)threadIdx.x; i < n_rows * kCols; i += S::kThreads) {
         const int c = i % kCols, r = i / kCols, f = f0 + c;
         if (f >= g.F) continue;
-        const float a = st.sum_of(c / 16, 0, r / 16, r % 16, c % 16);
-        const float b = st.sum_of(c / 16, 1, r / 16, r % 16, c % 16);
+        const float a = st.sum_of(0, r / 16, r % 16, c);
+        const float b = st.sum_of(1, r / 16, r % 16, c);
         const int p = pair(q, r);
-        store_h(g, p, f, activate(a, g.act) * b * g.weights[p]);
+        store_h(g, p, f, activate(a, g.act) * b * t.weight[p]);
       }
     }
   };
   Policy p{{}, g, t, tiles};
   p.st.lds = (lds_u8*)lds;
+  p.st.rings = (lds_u8*)rings;
+  p.st.sums = (__attribute__((address_space(3))) float*)sums;
   p.st.K = g.D;
+  p.st.ldw = (uint32_t)g.w13_row;
   p.st.inv = 32.0f / (float)g.G;
   int first, last;
   share(n_groups * tiles, &first, &last);
@@ -188,9 +202,11 @@ __global__ __launch_bounds__(1024) void k_moe_up(MoeArgs g) {
 }
 
 template <int kW, int kS, int kMode, int kMT>
-__global__ __launch_bounds__(1024) void k_moe_down(MoeArgs g) {
-  using S = Stream<kInBf16, kW, kS, kMode, kMT, true, 16>;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kLdsBytes];
+__global__ __launch_bounds__(512) void k_moe_down(MoeArgs g) {
+  using S = Stream<kInBf16, kW, kS, kMode, kMT, true>;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kXBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t rings[S::kRingBytes];
+  __shared__ float sums[S::kSums];
   __shared__ MoeGroups t;
   const int n_groups = moe_groups(g, S::rows_that_fit(g.part_len), t,
                                   (__attribute__((address_space(3))) int*)(lds_u8*)lds);
@@ -218,13 +234,14 @@ __global__ __launch_bounds__(1024) void k_moe_down(MoeArgs g) {
     }
     __device__ __forceinline__ void weights(int item) {
       const int q = item / tiles, e = __builtin_amdgcn_readfirstlane(t.expert[q / g.parts]);
-      const int d = (item - q * tiles) * S::kTile + 32 * (wave_id() / S::kWK) + (lane_id() & 15);
+      const int d0 = (item - q * tiles) * S::kTile;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const long long r = min(d + 16 * n, g.D - 1);
-        st.w[n] = g.w2 + e * g.w2_expert + r * g.w2_row;
-        st.s[n] = g.s2 + e * g.s2_expert + r * g.s2_row;
-        if constexpr (kW == kWInt4Z) st.z[n] = g.z2 + e * g.z2_expert + r * g.z2_row;
+        // (D is a multiple of 32: tiles are whole)
+        st.set_tile(n, g.w2 + e * g.w2_expert + (long long)(d0 + 16 * n) * g.w2_row, 16);
+        const long long r = d0 + 16 * st.scale_tile(n) + (lane_id() & 15);
+        st.sp[n] = g.s2 + e * g.s2_expert + r * g.s2_row;
+        if constexpr (kW == kWInt4Z) st.zp[n] = g.z2 + e * g.z2_expert + r * g.z2_row;
       }
     }
     __device__ __forceinline__ void finish(int item) {
@@ -233,13 +250,16 @@ __global__ __launch_bounds__(1024) void k_moe_down(MoeArgs g) {
         const int c = i % S::kTile, r = i / S::kTile, d = d0 + c;
         if (d >= g.D) continue;
         g.o[((long long)(q % g.parts) * (g.T * g.k) + pair(q, r)) * g.D + d] =
-            st.sum_of(c / 32, c / 16 % 2, r / 16, r % 16, c % 16);
+            st.sum_of(c / 16, r / 16, r % 16, c % 16);
       }
     }
   };
   Policy p{{}, g, t, tiles};
   p.st.lds = (lds_u8*)lds;
+  p.st.rings = (lds_u8*)rings;
+  p.st.sums = (__attribute__((address_space(3))) float*)sums;
   p.st.K = g.F;
+  p.st.ldw = (uint32_t)g.w2_row;
   p.st.inv = 32.0f / (float)g.G;
   int first, last;
   share(n_groups * g.parts * tiles, &first, &last);

@@ -45,8 +45,10 @@ __device__ __forceinline__ void finish_w4(const W4Args& g, int m, int n, float f
 
 template <int kX, int kW, int kS, int kMode, int kMT>
 __global__ __launch_bounds__(512) void k_w4_rows(W4RowsArgs r) {
-  using S = Stream<kX, kW, kS, kMode, kMT, false, 8>;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kLdsBytes];
+  using S = Stream<kX, kW, kS, kMode, kMT, false>;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::kXBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t rings[S::kRingBytes];
+  __shared__ float sums[S::kSums];
   struct Policy {
     S st;
     const W4RowsArgs& r;
@@ -63,13 +65,15 @@ __global__ __launch_bounds__(512) void k_w4_rows(W4RowsArgs r) {
       return r.a.x + (long long)(m_begin(q) + m) * r.a.ldx;
     }
     __device__ __forceinline__ void weights(int item) {
-      const int n0 = item % tiles * S::kTile + (lane_id() & 15);
+      const int n0 = item % tiles * S::kTile;
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const long long row = min(n0 + 16 * n, r.a.N - 1);
-        st.w[n] = r.a.w + row * r.a.ldw;
-        st.s[n] = r.a.s + row * r.a.lds;
-        if constexpr (kW == kWInt4Z) st.z[n] = r.a.z + row * r.a.ldz;
+        // (a second tile that is not there: the first one again, not used)
+        const int first = min(n0 + 16 * n, (r.a.N - 1) & ~15);
+        st.set_tile(n, r.a.w + (long long)first * r.a.ldw, r.a.N - first);
+        const long long row = min(n0 + 16 * st.scale_tile(n) + (lane_id() & 15), r.a.N - 1);
+        st.sp[n] = r.a.s + row * r.a.lds;
+        if constexpr (kW == kWInt4Z) st.zp[n] = r.a.z + row * r.a.ldz;
       }
     }
     __device__ __forceinline__ void finish(int item) {
@@ -77,7 +81,7 @@ __global__ __launch_bounds__(512) void k_w4_rows(W4RowsArgs r) {
       for (int i = (int)threadIdx.x; i < n_rows * S::kTile; i += S::kThreads) {
         const int c = i % S::kTile, row = i / S::kTile, n = n0 + c, m = m_begin(q) + row;
         if (n >= r.a.N) continue;
-        const float f = st.sum_of(0, c / 16, row / 16, row % 16, c % 16);
+        const float f = st.sum_of(c / 16, row / 16, row % 16, c % 16);
         if (r.parts > 1) r.o[((long long)(q % r.parts) * r.a.M + m) * r.a.N + n] = f;
         else finish_w4<kX, kW, kS>(r.a, m, n, f);
       }
@@ -85,7 +89,10 @@ __global__ __launch_bounds__(512) void k_w4_rows(W4RowsArgs r) {
   };
   Policy p{{}, r, (r.a.N + S::kTile - 1) / S::kTile};
   p.st.lds = (lds_u8*)lds;
+  p.st.rings = (lds_u8*)rings;
+  p.st.sums = (__attribute__((address_space(3))) float*)sums;
   p.st.K = r.a.K;
+  p.st.ldw = (uint32_t)r.a.ldw;
   p.st.inv = 32.0f / (float)r.a.G;
   const int items = (r.a.M + r.rows_max - 1) / r.rows_max * r.parts * p.tiles;
   p.st.run((int)((long long)items * blockIdx.x / gridDim.x),
