@@ -76,12 +76,12 @@ hipError_t quantize_rows(const void* x, int type, int M, int K, long long ldx,
 // Products of 16-bit activations with quantised weights (kw4_*.hip, kmoe_*.hip).
 // x: activations' type, w: detail::kW*, s: scales' type, mode: detail::kNone,
 // kCoarse, kFine or kInline; rows: 1, 2 or 4, lk: 16
-// or 64 lanes of a row; mt: tiles of 16 rows of x (1, 2).
+// or 64 lanes of a row; mt: tiles of 16 rows of x (1, 2);
+// wk: waves that share a row's K (2, 8).
 const void* w4_vec(int x, int w, int s, int rows, int lk);
 const void* w4_rows(int x, int w, int s, int mode, int mt);
-const void* w4_sum(int x, int w, int s);
-const void* moe_up(int x, int w, int s, int mode, int mt);
-const void* moe_down(int w, int s, int mode, int mt);
+const void* moe_up(int x, int w, int s, int mode, int mt, int wk);
+const void* moe_down(int w, int s, int mode, int mt, int wk);
 const void* moe_vec_up(int x, int w, int s, int lk);
 const void* moe_vec_down(int w, int s, int lk);
 // Packs [rows][ceil(K/32)] E8M0 scales (row stride ld) into MxArgs' layout.

@@ -4,8 +4,8 @@
 namespace hipgemm {
 namespace kernels {
 
-const void* moe_up_bf16_int4(int s, int mode, int mt) {
-  return moe_up_of<detail::kInBf16, detail::kWInt4>(s, mode, mt);
+const void* moe_up_bf16_int4(int s, int mode, int mt, int wk) {
+  return moe_up_of<detail::kInBf16, detail::kWInt4>(s, mode, mt, wk);
 }
 const void* moe_vec_up_bf16_int4(int s, int lk) {
   return moe_vec_up_of<detail::kInBf16, detail::kWInt4>(s, lk);

@@ -56,16 +56,13 @@ const void* w4_rows_of(int s, int mode, int mt) {
   });
 }
 template <int kX, int kW>
-const void* w4_sum_of(int s) {
-  return sel4(s, [](auto S) { return (const void*)&detail::k_w4_sum<kX, kW, decltype(S)::value>; });
-}
-
-template <int kX, int kW>
-const void* moe_up_of(int s, int mode, int mt) {
+const void* moe_up_of(int s, int mode, int mt, int wk) {
   return sel_scales<kX, kW>(s, mode, [&](auto S, auto Mode) {
     return sel_mt(mt, [&](auto MT) {
-      return (const void*)&detail::k_moe_up<kX, kW, decltype(S)::value, decltype(Mode)::value,
-                                            decltype(MT)::value>;
+      constexpr int kS = decltype(S)::value, kMode = decltype(Mode)::value;
+      constexpr int kMT = decltype(MT)::value;
+      return wk == 8 ? (const void*)&detail::k_moe_up<kX, kW, kS, kMode, kMT, 8>
+                     : (const void*)&detail::k_moe_up<kX, kW, kS, kMode, kMT, 2>;
     });
   });
 }
@@ -92,11 +89,13 @@ const void* moe_vec_down_of(int s, int lk) {
 }
 
 template <int kW>
-const void* moe_down_of(int s, int mode, int mt) {
+const void* moe_down_of(int s, int mode, int mt, int wk) {
   return sel_scales<detail::kInBf16, kW>(s, mode, [&](auto S, auto Mode) {
     return sel_mt(mt, [&](auto MT) {
-      return (const void*)&detail::k_moe_down<kW, decltype(S)::value, decltype(Mode)::value,
-                                              decltype(MT)::value>;
+      constexpr int kS = decltype(S)::value, kMode = decltype(Mode)::value;
+      constexpr int kMT = decltype(MT)::value;
+      return wk == 8 ? (const void*)&detail::k_moe_down<kW, kS, kMode, kMT, 8>
+                     : (const void*)&detail::k_moe_down<kW, kS, kMode, kMT, 2>;
     });
   });
 }

@@ -10,7 +10,6 @@ const void* w4_vec_f16_int4(int s, int rows, int lk) {
 const void* w4_rows_f16_int4(int s, int mode, int mt) {
   return w4_rows_of<detail::kInF16, detail::kWInt4>(s, mode, mt);
 }
-const void* w4_sum_f16_int4(int s) { return w4_sum_of<detail::kInF16, detail::kWInt4>(s); }
 
 }  // namespace kernels
 }  // namespace hipgemm

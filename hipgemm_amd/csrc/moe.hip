@@ -1,6 +1,8 @@
 // hipgemm_moe_experts: arguments and launches.
 #include "hipgemm.h"
 
+#include <cmath>
+
 #include "kernels.hpp"
 
 #include "hipgemm/detail/moe_vec.hpp"
@@ -9,9 +11,9 @@ namespace hipgemm {
 namespace kernels {
 
 #define HIPGEMM_MOE(W)                                  \
-  const void* moe_up_bf16_##W(int s, int mode, int mt); \
-  const void* moe_up_f16_##W(int s, int mode, int mt);  \
-  const void* moe_down_##W(int s, int mode, int mt);    \
+  const void* moe_up_bf16_##W(int s, int mode, int mt, int wk); \
+  const void* moe_up_f16_##W(int s, int mode, int mt, int wk);  \
+  const void* moe_down_##W(int s, int mode, int mt, int wk);    \
   const void* moe_vec_up_bf16_##W(int s, int lk);       \
   const void* moe_vec_up_f16_##W(int s, int lk);        \
   const void* moe_vec_down_##W(int s, int lk);
@@ -21,22 +23,22 @@ HIPGEMM_MOE(fp4)
 HIPGEMM_MOE(e4m3)
 #undef HIPGEMM_MOE
 
-const void* moe_up(int x, int w, int s, int mode, int mt) {
+const void* moe_up(int x, int w, int s, int mode, int mt, int wk) {
   const bool b = x == detail::kInBf16;
   switch (w) {
-    case detail::kWInt4: return b ? moe_up_bf16_int4(s, mode, mt) : moe_up_f16_int4(s, mode, mt);
+    case detail::kWInt4: return b ? moe_up_bf16_int4(s, mode, mt, wk) : moe_up_f16_int4(s, mode, mt, wk);
     case detail::kWInt4Z:
-      return b ? moe_up_bf16_int4z(s, mode, mt) : moe_up_f16_int4z(s, mode, mt);
-    case detail::kWFp4: return b ? moe_up_bf16_fp4(s, mode, mt) : moe_up_f16_fp4(s, mode, mt);
-    default: return b ? moe_up_bf16_e4m3(s, mode, mt) : moe_up_f16_e4m3(s, mode, mt);
+      return b ? moe_up_bf16_int4z(s, mode, mt, wk) : moe_up_f16_int4z(s, mode, mt, wk);
+    case detail::kWFp4: return b ? moe_up_bf16_fp4(s, mode, mt, wk) : moe_up_f16_fp4(s, mode, mt, wk);
+    default: return b ? moe_up_bf16_e4m3(s, mode, mt, wk) : moe_up_f16_e4m3(s, mode, mt, wk);
   }
 }
-const void* moe_down(int w, int s, int mode, int mt) {
+const void* moe_down(int w, int s, int mode, int mt, int wk) {
   switch (w) {
-    case detail::kWInt4: return moe_down_int4(s, mode, mt);
-    case detail::kWInt4Z: return moe_down_int4z(s, mode, mt);
-    case detail::kWFp4: return moe_down_fp4(s, mode, mt);
-    default: return moe_down_e4m3(s, mode, mt);
+    case detail::kWInt4: return moe_down_int4(s, mode, mt, wk);
+    case detail::kWInt4Z: return moe_down_int4z(s, mode, mt, wk);
+    case detail::kWFp4: return moe_down_fp4(s, mode, mt, wk);
+    default: return moe_down_e4m3(s, mode, mt, wk);
   }
 }
 const void* moe_vec_up(int x, int w, int s, int lk) {
@@ -68,18 +70,30 @@ namespace hk = hipgemm::kernels;
 static_assert(HIPGEMM_W8_E4M3 == kWE4M3 && HIPGEMM_MOE_MAX_PAIRS == kMoePairs &&
                   HIPGEMM_MOE_MAX_EXPERTS == kMoeExperts, "codes");
 
-// Four columns of one token per thread.
+// Four columns of one token per thread, eight pairs' loads at a time.
 __global__ __launch_bounds__(256) void k_moe_sum(MoeArgs g) {
   const int i = (int)blockIdx.x * 256 + (int)threadIdx.x, per = g.D / 4;
   const int t = i / per, d = i % per * 4;
   if (t >= g.T) return;
   const long long pairs = g.T * g.k;
   f32x4 v = {};
-  for (int j = 0; j < g.k; ++j) {
-    const int p = t * g.k + j, e = g.ids[p];
-    if (e < 0 || e >= g.E) continue;
-    for (int q = 0; q < g.parts; ++q)
-      v += *reinterpret_cast<const f32x4*>(g.o + (q * pairs + p) * g.D + d);
+  for (int j0 = 0; j0 < g.k; j0 += 8) {
+    bool on[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = g.ids[t * g.k + min(j0 + j, g.k - 1)];
+      on[j] = j0 + j < g.k && e >= 0 && e < g.E;
+    }
+    for (int q = 0; q < g.parts; ++q) {
+      f32x4 o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        o[j] = *reinterpret_cast<const f32x4*>(
+            g.o + (q * pairs + t * g.k + min(j0 + j, g.k - 1)) * g.D + d);
+      // (what was not written may be anything)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v = on[j] ? v + o[j] : v;
+    }
   }
 #pragma unroll
   for (int c = 0; c < 4; ++c) store_result(g.y, t * g.ldy + d + c, g.out, v[c]);
@@ -128,11 +142,8 @@ hipError_t launch(const void* fn, dim3 grid, int threads, MoeArgs& g, hipStream_
 }
 
 // Lanes of a row for rows of K elements (16 bytes of weights a lane): 16 where 64
-// would leave a quarter of the lanes idle or more.
-int vec_lanes(int K, int per_lane) {
-  const int units = K / per_lane;
-  return units > 32 && (units + 63) / 64 * 64 * 3 < units * 4 ? 64 : 16;
-}
+// would leave most of them idle.
+int vec_lanes(int K, int per_lane) { return K / per_lane > 24 ? 64 : 16; }
 int chunks_of(int K, int per_lane, int lk) {
   return (K + per_lane * lk - 1) / (per_lane * lk);
 }
@@ -172,13 +183,19 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   // Tiles of 16 tokens, two at a time where experts have more on average.
   const int mt = pairs > 12 * g.E ? 2 : 1;
   g.parts = down_parts(g.T, g.k, g.E, g.D, g.F, &g.part_len);
+  // Experts chosen at all, if all are chosen alike.
+  const double chosen = g.E * (1.0 - std::pow(1.0 - 1.0 / g.E, pairs));
+  // Tiles of 128 rows with two waves to a row's K where each CU has ten or more of
+  // them (fewer ends of tiles per byte), of 32 rows with eight where not.
+  const int wku = chosen * g.F / 64 >= 2560 ? 2 : 8;
+  const int wkd = chosen * g.D / 128 * g.parts >= 2560 ? 2 : 8;
   const int cus = 256;
   hipError_t e = launch(hk::moe_up(d.x_type, d.w13.zeros ? kWInt4Z : d.format, d.scale_type,
-                                   mode_of(d.x_type, d.format, d.scale_type, d.group_size), mt),
+                                   mode_of(d.x_type, d.format, d.scale_type, d.group_size), mt, wku),
                         dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   e = launch(hk::moe_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type,
-                          mode_of(kInBf16, d.format, d.scale_type, d.group_size), mt),
+                          mode_of(kInBf16, d.format, d.scale_type, d.group_size), mt, wkd),
              dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   return launch((const void*)&k_moe_sum, dim3((unsigned)((g.T * (g.D / 4) + 255) / 256)), 256, g,

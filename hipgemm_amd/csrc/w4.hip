@@ -10,8 +10,7 @@ namespace kernels {
 
 #define HIPGEMM_W4(X, W)                      \
   const void* w4_vec_##X##_##W(int s, int rows, int lk); \
-  const void* w4_rows_##X##_##W(int s, int mode, int mt); \
-  const void* w4_sum_##X##_##W(int s);
+  const void* w4_rows_##X##_##W(int s, int mode, int mt);
 HIPGEMM_W4(bf16, int4)
 HIPGEMM_W4(bf16, int4z)
 HIPGEMM_W4(bf16, fp4)
@@ -36,14 +35,6 @@ const void* w4_rows(int x, int w, int s, int mode, int mt) {
     case detail::kWInt4Z:
       return b ? w4_rows_bf16_int4z(s, mode, mt) : w4_rows_f16_int4z(s, mode, mt);
     default: return b ? w4_rows_bf16_fp4(s, mode, mt) : w4_rows_f16_fp4(s, mode, mt);
-  }
-}
-const void* w4_sum(int x, int w, int s) {
-  const bool b = x == detail::kInBf16;
-  switch (w) {
-    case detail::kWInt4: return b ? w4_sum_bf16_int4(s) : w4_sum_f16_int4(s);
-    case detail::kWInt4Z: return b ? w4_sum_bf16_int4z(s) : w4_sum_f16_int4z(s);
-    default: return b ? w4_sum_bf16_fp4(s) : w4_sum_f16_fp4(s);
   }
 }
 
@@ -72,39 +63,39 @@ hipError_t launch(const void* fn, dim3 grid, int threads, Args& g, hipStream_t s
   return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, stream);
 }
 
-// The plan of k_w4_rows.  The activations of an item's rows and part of K lie in
-// LDS; parts of K are as many as that takes.
+// The plan of k_w4_rows: the rows of x that go together, and as many parts of K as
+// LDS makes it for them.
 struct RowsPlan {
   int mt, rows_max, parts, len;
 };
-RowsPlan rows_plan(int M, int N, int K) {
+RowsPlan rows_plan(int M, int K) {
   RowsPlan p;
   p.mt = M <= 16 ? 1 : 2;
-  auto fit = [&](int len) {
-    return p.mt == 1 ? Stream<kInBf16, kWFp4, kInF32, kCoarse, 1, false>::rows_that_fit(len)
-                     : Stream<kInBf16, kWFp4, kInF32, kCoarse, 2, false>::rows_that_fit(len);
-  };
-  const int steps = (K + 255) / 256, rows = M < 16 * p.mt ? M : 16 * p.mt;
-  for (p.parts = 1;; ++p.parts) {
-    const int len = (steps + p.parts - 1) / p.parts;
-    p.len = 256 * len;
-    p.rows_max = fit(p.len);
-    if (p.rows_max >= rows || len <= 1) break;
+  const int groups = (M + 16 * p.mt - 1) / (16 * p.mt);
+  p.rows_max = (M + groups - 1) / groups;
+  const int steps = (K + 255) / 256;
+  for (p.parts = 1; p.parts < steps; ++p.parts) {
+    const int len = 256 * ((steps + p.parts - 1) / p.parts);
+    if ((p.mt == 1 ? W4Stream<kInBf16, kWFp4, kInF32, kCoarse, 1>::rows_that_fit(len)
+                   : W4Stream<kInBf16, kWFp4, kInF32, kCoarse, 2>::rows_that_fit(len)) >=
+        p.rows_max)
+      break;
   }
-  p.parts = (steps + p.len / 256 - 1) / (p.len / 256);
-  if (p.parts < 1) p.parts = 1;
+  const int len = (steps + p.parts - 1) / p.parts;
+  p.len = 256 * len;
+  p.parts = (steps + len - 1) / len;
   return p;
 }
 
 // k_w4_vec: lanes of a row, and the waves along K and rows of a workgroup.
-// 16 lanes where a chunk of 64 would leave half of the lanes idle or more.
+// 16 lanes where 64 would be idle for the most part.
 struct VecPlan {
   int lk, waves_k, waves_r, rows, wave_rows;
 };
 VecPlan vec_plan(int N, int K) {
   VecPlan p;
   const int units = K / 32;
-  p.lk = units > 32 && (units + 63) / 64 * 64 * 3 < units * 4 ? 64 : 16;
+  p.lk = units > 24 ? 64 : 16;
   const int chunks = units > p.lk ? (units + p.lk - 1) / p.lk : 1;
   const int turns = (chunks + 7) / 8;
   p.waves_k = (chunks + turns - 1) / turns;
@@ -138,42 +129,36 @@ hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
   g.act = d.activation;
   g.out = d.out_dtype;
   const int w = d.zeros ? kWInt4Z : d.format;
-  if (d.M <= 4) {
+  if (d.M <= 4 || d.K == 0) {
     const VecPlan p = vec_plan(d.N, d.K);
     g.waves_k = p.waves_k;
     g.rows = p.rows;
     g.wave_rows = p.wave_rows;
-    return launch(hk::w4_vec(d.x_type, w, d.scale_type, d.M == 3 ? 4 : d.M, p.lk),
-                  dim3((unsigned)((d.N + p.rows - 1) / p.rows)), kWave * p.waves_k * p.waves_r, g,
-                  stream);
+    for (int m = 0; m < d.M; m += 4) {  // (more than four rows only without any K)
+      g.M = d.M - m < 4 ? d.M - m : 4;
+      const hipError_t e =
+          launch(hk::w4_vec(d.x_type, w, d.scale_type, g.M == 3 ? 4 : g.M, p.lk),
+                 dim3((unsigned)((d.N + p.rows - 1) / p.rows)), kWave * p.waves_k * p.waves_r, g,
+                 stream);
+      if (e != hipSuccess) return e;
+      g.y += 4 * d.ldy * out_bytes(d.out_dtype);
+    }
+    return hipSuccess;
   }
   const int mode = d.format == HIPGEMM_W4_FP4 && d.scale_type == HIPGEMM_SCALE_E8M0 &&
                            d.x_type == HIPGEMM_IN_BF16
                        ? kInline
                    : d.group_size % 128 == 0 ? kCoarse
                                              : kFine;
-  if (d.K == 0) {  // no parts to sum
-    W4RowsArgs r{g, nullptr, 1, 0, 0};
-    return launch(hk::w4_sum(d.x_type, w, d.scale_type),
-                  dim3((unsigned)((d.N + 255) / 256), (unsigned)d.M), 256, r, stream);
-  }
-  const RowsPlan p = rows_plan(d.M, d.N, d.K);
-  W4RowsArgs r{g, static_cast<float*>(d.workspace), p.rows_max, p.parts, p.len};
-  const int items = (d.M + p.rows_max - 1) / p.rows_max * p.parts * ((d.N + 31) / 32);
-  const hipError_t e = launch(hk::w4_rows(d.x_type, w, d.scale_type, mode, p.mt),
-                              dim3((unsigned)(items < 256 ? items : 256)), 512, r, stream);
-  if (e != hipSuccess || p.parts == 1) return e;
-  return launch(hk::w4_sum(d.x_type, w, d.scale_type),
-                dim3((unsigned)((d.N + 255) / 256), (unsigned)d.M), 256, r, stream);
+  const RowsPlan p = rows_plan(d.M, d.K);
+  W4RowsArgs r{g, p.rows_max, p.parts, p.len};
+  const long long tiles =
+      (long long)((d.M + p.rows_max - 1) / p.rows_max) * ((d.N + 31) / 32);
+  return launch(hk::w4_rows(d.x_type, w, d.scale_type, mode, p.mt),
+                dim3((unsigned)(tiles < 256 ? tiles : 256)), 512, r, stream);
 }
 
 }  // namespace
-
-extern "C" size_t hipgemm_w4_workspace_size(int M, int N, int K) {
-  if (M <= 4 || N <= 0 || K <= 0) return 0;
-  const RowsPlan p = rows_plan(M, N, K);
-  return p.parts == 1 ? 0 : (size_t)p.parts * M * N * 4;
-}
 
 extern "C" hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc* desc, hipStream_t stream) {
   if (!desc || desc->size != sizeof(hipgemm_w4_desc)) return hipErrorInvalidValue;
@@ -200,8 +185,5 @@ extern "C" hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc* desc, hipStream_t s
         d.lds < (d.K + d.group_size - 1) / d.group_size)
       return hipErrorInvalidValue;
   }
-  const size_t need = hipgemm_w4_workspace_size(d.M, d.N, d.K);
-  if (need && (!d.workspace || !aligned(d.workspace, 16) || d.workspace_bytes < need))
-    return hipErrorInvalidValue;
   return run(d, stream);
 }

@@ -17,7 +17,7 @@ import functools
 from . import (ACTIVATIONS, OUT_BF16, OUT_F16, OUT_F32, HipGemmError, _check,
                _torch, hipErrorInvalidValue, lib)
 
-__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "w4_workspace_size", "W4_FORMATS",
+__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "W4_FORMATS",
            "moe_route", "MOE_SCORING", "moe_experts", "MoeDesc", "MoeMatrix",
            "moe_experts_raw", "moe_workspace_size", "MOE_FORMATS"]
 
@@ -35,8 +35,7 @@ class W4Desc(ctypes.Structure):
                 ("M", _ci), ("N", _ci), ("K", _ci), ("group_size", _ci),
                 ("ldx", _ll), ("ldw", _ll), ("lds", _ll), ("ldy", _ll),
                 ("x_type", _ci), ("format", _ci), ("scale_type", _ci),
-                ("out_dtype", _ci), ("activation", _ci), ("workspace", _vp),
-                ("workspace_bytes", ctypes.c_size_t)]
+                ("out_dtype", _ci), ("activation", _ci)]
 
 
 class MoeMatrix(ctypes.Structure):
@@ -86,14 +85,6 @@ def _scratch(nbytes: int, device, stream):
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     with torch.cuda.stream(stream):
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-
-
-def w4_workspace_size(M: int, N: int, K: int) -> int:
-    """Workspace bytes hipgemm_w4_gemm needs (0: none)."""
-    return int(lib().hipgemm_w4_workspace_size(M, N, K))
-
-
-_w4_ws_bytes = functools.lru_cache(maxsize=1024)(w4_workspace_size)
 
 
 def w4_gemm_raw(desc: "W4Desc", stream: int = 0) -> int:
@@ -173,14 +164,11 @@ def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
                 and (N <= 1 or bias.stride(0) == 1)):
             _bad(f"bias must be a contiguous float32 device vector of {N} elements")
         bp = bias.data_ptr()
-    need = _w4_ws_bytes(M, N, K) if M > 4 else 0
-    if need:
-        ws = _scratch(need, x.device, stream)
     d = W4Desc(_W4_BYTES, x.data_ptr(), weight.data_ptr(), scales.data_ptr(), zp,
                out.data_ptr(), bp, M, N, K, group_size,
                x.stride(0) if M > 1 else K, weight.stride(0) if N > 1 else K // 2,
                lds, out.stride(0) if M > 1 else N, xt, fmt, st, ot,
-               ACTIVATIONS[activation], ws.data_ptr() if need else 0, need)
+               ACTIVATIONS[activation])
     _check(lib().hipgemm_w4_gemm(ctypes.byref(d), _stream_handle(x, stream)), "hipgemm_w4_gemm")
     return out
 

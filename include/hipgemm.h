@@ -378,9 +378,7 @@ hipError_t hipgemm_quantize_rows_e4m3(const void *x, int type, int M, int K,
  * Requirements: K % 32 == 0, K <= 2^26, G % 32 == 0, x and q 16-byte aligned
  * with strides of a multiple of 16 bytes, the others aligned to their element;
  * out_dtype BF16, F16 or F32.  M == 0 or N == 0 is a no-op, K == 0 gives
- * activation(bias).  Workspace: hipgemm_w4_workspace_size bytes (0 for most
- * sizes), 16-byte aligned, of any content; calls that may run concurrently must
- * not share one.  Zero-initialise the struct and set `size`.  No reference counterpart (the
+ * activation(bias).  One launch on `stream`, no workspace.  Zero-initialise the struct and set `size`.  No reference counterpart (the
  * reference has e4m3 operands only).
  */
 enum { HIPGEMM_W4_INT4 = 0, HIPGEMM_W4_FP4 = 1 };
@@ -402,10 +400,7 @@ typedef struct hipgemm_w4_desc {
   int scale_type;   /* HIPGEMM_IN_* or HIPGEMM_SCALE_E8M0 */
   int out_dtype;    /* HIPGEMM_OUT_* */
   int activation;   /* HIPGEMM_ACT_* */
-  void *workspace;
-  size_t workspace_bytes;
 } hipgemm_w4_desc;
-size_t hipgemm_w4_workspace_size(int M, int N, int K);
 hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc *desc, hipStream_t stream);
 
 /*

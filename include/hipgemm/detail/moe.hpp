@@ -66,6 +66,9 @@ struct MoeGroups {
   float weight[kMoePairs];
 };
 
+constexpr int kMoeTables = 7 << 10;
+static_assert(sizeof(MoeGroups) <= kMoeTables - 512, "room for the tables");
+
 // Fills t, by all 512 threads; count: LDS of kMoeExperts + 8 ints, free after.
 // Returns the number of groups.  A pair's place among its expert's is where the
 // counting put it, which may differ between workgroups: nothing depends on the
@@ -139,10 +142,10 @@ __device__ __forceinline__ void share(int items, int* first, int* last) {
   *last = (int)((long long)items * (blockIdx.x + 1) / gridDim.x);
 }
 
-template <int kX, int kW, int kS, int kMode, int kMT>
+template <int kX, int kW, int kS, int kMode, int kMT, int kWK>
 __global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
-  using S = Stream<kX, kW, kS, kMode, kMT, false>;
-  constexpr int kCols = 16;  // of F, of an item: gate and up rows
+  using S = Stream<kX, kW, kS, kMode, kMT, false, kWK, kMoeTables>;
+  constexpr int kCols = 16 * S::kWN;  // of F, of an item: gate and up rows
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::kXBytes];
   __shared__ __attribute__((aligned(1024))) uint8_t rings[S::kRingBytes];
   __shared__ float sums[S::kSums];
@@ -167,11 +170,12 @@ __global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
     }
     __device__ __forceinline__ void weights(int item) {
       const int q = item / tiles, e = __builtin_amdgcn_readfirstlane(t.expert[q]);
-      const int f0 = (item - q * tiles) * kCols;
+      // (a set past the end: the last columns again, not used)
+      const int f0 = min((item - q * tiles) * kCols + 16 * st.set(), g.F - 16);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        st.set_tile(n, g.w13 + e * g.w13_expert + ((long long)n * g.F + f0) * g.w13_row, g.F - f0);
-        const long long r = (long long)st.scale_tile(n) * g.F + min(f0 + (lane_id() & 15), g.F - 1);
+        st.set_tile(n, g.w13 + e * g.w13_expert + ((long long)n * g.F + f0) * g.w13_row, 16);
+        const long long r = (long long)st.scale_tile(n) * g.F + f0 + (lane_id() & 15);
         st.sp[n] = g.s13 + e * g.s13_expert + r * g.s13_row;
         if constexpr (kW == kWInt4Z) st.zp[n] = g.z13 + e * g.z13_expert + r * g.z13_row;
       }
@@ -182,8 +186,8 @@ __global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
       for (int i = (int)threadIdx.x; i < n_rows * kCols; i += S::kThreads) {
         const int c = i % kCols, r = i / kCols, f = f0 + c;
         if (f >= g.F) continue;
-        const float a = st.sum_of(0, r / 16, r % 16, c);
-        const float b = st.sum_of(1, r / 16, r % 16, c);
+        const float a = st.sum_of(c / 16, 0, r / 16, r % 16, c % 16);
+        const float b = st.sum_of(c / 16, 1, r / 16, r % 16, c % 16);
         const int p = pair(q, r);
         store_h(g, p, f, activate(a, g.act) * b * t.weight[p]);
       }
@@ -201,9 +205,9 @@ __global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
   p.st.run(first, last, g.D, p);
 }
 
-template <int kW, int kS, int kMode, int kMT>
+template <int kW, int kS, int kMode, int kMT, int kWK>
 __global__ __launch_bounds__(512) void k_moe_down(MoeArgs g) {
-  using S = Stream<kInBf16, kW, kS, kMode, kMT, true>;
+  using S = Stream<kInBf16, kW, kS, kMode, kMT, true, kWK, kMoeTables>;
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::kXBytes];
   __shared__ __attribute__((aligned(1024))) uint8_t rings[S::kRingBytes];
   __shared__ float sums[S::kSums];
@@ -234,10 +238,9 @@ __global__ __launch_bounds__(512) void k_moe_down(MoeArgs g) {
     }
     __device__ __forceinline__ void weights(int item) {
       const int q = item / tiles, e = __builtin_amdgcn_readfirstlane(t.expert[q / g.parts]);
-      const int d0 = (item - q * tiles) * S::kTile;
+      const int d0 = min((item - q * tiles) * S::kTile + 32 * st.set(), g.D - 32);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        // (D is a multiple of 32: tiles are whole)
         st.set_tile(n, g.w2 + e * g.w2_expert + (long long)(d0 + 16 * n) * g.w2_row, 16);
         const long long r = d0 + 16 * st.scale_tile(n) + (lane_id() & 15);
         st.sp[n] = g.s2 + e * g.s2_expert + r * g.s2_row;
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(512) void k_moe_down(MoeArgs g) {
         const int c = i % S::kTile, r = i / S::kTile, d = d0 + c;
         if (d >= g.D) continue;
         g.o[((long long)(q % g.parts) * (g.T * g.k) + pair(q, r)) * g.D + d] =
-            st.sum_of(c / 16, r / 16, r % 16, c % 16);
+            st.sum_of(c / 32, c / 16 % 2, r / 16, r % 16, c % 16);
       }
     }
   };

@@ -5,8 +5,9 @@
 // What bounds it is the weights' bytes, 9 per CU and cycle at most, so all that
 // matters is that enough of them are on their way all the time, from the first
 // instruction to the last.  One workgroup per CU works off a list of items (32
-// rows of weights times a group of rows of x); its eight waves take turns over K,
-// and their sums meet in LDS at an item's end.  Each wave brings its own weights
+// kWN rows of weights times a group of rows of x); kWK of its eight waves take
+// turns over K, and their sums meet in LDS at an item's end, kWN = 8 / kWK sets of
+// them have 32 rows of weights of their own.  Each wave brings its own weights
 // into its own ring of LDS by DMA, two units of 4 KiB ahead, across the items'
 // ends, and has hardly any other loads of memory in between.  Activations lie in
 // LDS, all of the item's K, and stay there for all items of a group.
@@ -77,23 +78,25 @@ __device__ __forceinline__ uint32_t scale_raw(const uint8_t* p, int i) {
   else return p[i];
 }
 // kLo: activations in two parts, x = hi + lo (16 bits each).
-template <int kX, int kW, int kS, int kMode, int kMT, bool kLo>
+// kTables: bytes of LDS that the kernel keeps for itself.
+template <int kX, int kW, int kS, int kMode, int kMT, bool kLo, int kWK, int kTables>
 struct Stream {
   static constexpr int kWaves = 8, kThreads = kWaves * kWave, kNT = 2;
   static constexpr int kParts = kLo ? 2 : 1;
   static constexpr int kRows = 16 * kMT;
-  static constexpr int kTile = 32;  // rows of weights of an item
+  static constexpr int kWN = kWaves / kWK;
+  static constexpr int kTile = 32 * kWN;  // rows of weights of an item
   static constexpr int kBlocks = kW == kWE4M3 ? 1 : 2;  // of 128 of K, of a unit
   static constexpr int kUnit = 128 * kBlocks;
   static constexpr int kUnitBytes = 4096;
   static constexpr int kRing = 2;
   // LDS: activations (rows x parts of K, each row 16 bytes longer, so that the 16
-  // rows' pieces of an MFMA operand lie on all banks), rings, the waves' sums; 7
-  // of 160 KiB are left to the kernel's own tables.
+  // rows' pieces of an MFMA operand lie on all banks), rings, the waves' sums, the
+  // kernel's tables: 160 KiB in all.
   static constexpr int kRingBytes = kWaves * kRing * kUnitBytes;
   static constexpr int kSumBytes = kWaves * kNT * kMT * kWave * 16;
   static constexpr int kPadBytes = kRows * kParts * 16;
-  static constexpr int kElems = ((153 << 10) - kRingBytes - kSumBytes - kPadBytes) / 512 * 256;
+  static constexpr int kElems = ((160 << 10) - kTables - kRingBytes - kSumBytes - kPadBytes) / 512 * 256;
   static constexpr int kXBytes = 2 * kElems + kPadBytes;
   static constexpr int kSums = kSumBytes / 4;
   // Rows of a group whose K elements fit.
@@ -124,6 +127,8 @@ struct Stream {
     uint32_t s[kSc], z[kSc];
   };
 
+  // This wave's set of rows.
+  __device__ static int set() { return wave_id() / kWK; }
   // The tile of this lane's scales: one load each for both tiles, or one in all.
   __device__ static int scale_tile(int n) {
     const int g = lane_id() >> 4;
@@ -345,23 +350,23 @@ struct Stream {
   template <class P>
   __device__ __forceinline__ void run(int first, int last, int len, P& p) {
     if (first >= last) return;
-    const int wave = wave_id();
+    const int wave = wave_id(), wk = wave % kWK;
     lds_u8* ring = rings + wave * kRing * kUnitBytes;
-    const int turns = ((len + kUnit - 1) / kUnit + kWaves - 1) / kWaves;  // a wave's units of an item
+    const int turns = ((len + kUnit - 1) / kUnit + kWK - 1) / kWK;  // a wave's units of an item
     int li = first, lu = 0, lk = 0, lend = 0;  // the item and unit that is loaded next
     auto next_item = [&]() {
       if (li < last) {
         p.weights(li);
         lk = p.k_begin(li);
         lend = min(lk + len, K);
-        lk += wave * kUnit;
+        lk += wk * kUnit;
       } else {
         lend = 0;
       }
     };
     next_item();
     auto fetch = [&](Scales& b, int slot) {
-      load(b, ring + slot * kUnitBytes, lk + lu * kWaves * kUnit, lend);
+      load(b, ring + slot * kUnitBytes, lk + lu * kWK * kUnit, lend);
       if (++lu == turns) {
         lu = 0;
         ++li;
@@ -408,7 +413,7 @@ struct Stream {
         // the youngest, may be under way.
         wait_vmcnt<(kRing - 1) * kLoads>();
         Scales& b = scales[slot];
-        const int kb = k0 + (u * kWaves + wave) * kUnit;
+        const int kb = k0 + (u * kWK + wk) * kUnit;
         if (kb < k1) {
           uint32_t sc[kNT][4], zs[kNT][4];
 #pragma unroll
@@ -443,7 +448,7 @@ struct Stream {
   }
 
   // The waves' accumulators to LDS: [wave][n][m][row][column], 16 x 16 floats a
-  // tile.
+  // tile (wave = wn kWK + wk).
   __device__ __forceinline__ void spill_sums(int wave) const {
     barrier();  // the item before has been finished
     const int r = lane_id() & 15, g = lane_id() >> 4;
@@ -457,12 +462,12 @@ struct Stream {
     wait_lgkmcnt<0>();
     barrier();
   }
-  // The sum over K of tile n.
-  __device__ __forceinline__ float sum_of(int n, int m, int row, int col) const {
+  // The sum over K of set wn's tile n.
+  __device__ __forceinline__ float sum_of(int wn, int n, int m, int row, int col) const {
     float v = 0.0f;
 #pragma unroll
-    for (int q = 0; q < kWaves; ++q)
-      v += sums[(((q * kNT + n) * kMT + m) * 16 + row) * 16 + col];
+    for (int q = 0; q < kWK; ++q)
+      v += sums[((((wn * kWK + q) * kNT + n) * kMT + m) * 16 + row) * 16 + col];
     return v;
   }
 };
