@@ -79,7 +79,8 @@ hipError_t quantize_rows(const void* x, int type, int M, int K, long long ldx,
 // or 64 lanes of a row; mt: tiles of 16 rows of x (1, 2);
 // wk: waves that share a row's K (2, 8).
 const void* w4_vec(int x, int w, int s, int rows, int lk);
-const void* w4_rows(int x, int w, int s, int mode, int mt);
+const void* w4_tile(int x, int w, int s, int mode);
+const void* w4_split(int x, int w, int s, int mode, int mt, int nt);
 const void* moe_up(int x, int w, int s, int mode, int mt, int wk);
 const void* moe_down(int w, int s, int mode, int mt, int wk);
 const void* moe_vec_up(int x, int w, int s, int lk);

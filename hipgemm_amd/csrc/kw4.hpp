@@ -5,7 +5,7 @@
 #include "kernels.hpp"
 
 #include "hipgemm/detail/moe_vec.hpp"
-#include "hipgemm/detail/w4_rows.hpp"
+#include "hipgemm/detail/w4_tile.hpp"
 
 namespace hipgemm {
 namespace kernels {
@@ -47,14 +47,29 @@ const void* sel_mt(int mt, F&& f) {
 }
 
 template <int kX, int kW>
-const void* w4_rows_of(int s, int mode, int mt) {
-  return sel_scales<kX, kW>(s, mode, [&](auto S, auto Mode) {
-    return sel_mt(mt, [&](auto MT) {
-      return (const void*)&detail::k_w4_rows<kX, kW, decltype(S)::value, decltype(Mode)::value,
-                                             decltype(MT)::value>;
-    });
+const void* w4_tile_of(int s, int mode) {
+  return sel_scales<kX, kW>(s, mode, [](auto S, auto Mode) {
+    return (const void*)&detail::k_w4_tile<kX, kW, decltype(S)::value, decltype(Mode)::value>;
   });
 }
+
+template <int kX, int kW>
+const void* w4_split_of(int s, int mode, int mt, int nt) {
+  return sel_scales<kX, kW>(s, mode, [mt, nt](auto S, auto Mode) -> const void* {
+    constexpr int kS = decltype(S)::value, kMode = decltype(Mode)::value;
+    switch (mt) {
+      case 1: return nt == 2 ? (const void*)&detail::k_w4_split<kX, kW, kS, kMode, 1, 2>
+                            : (const void*)&detail::k_w4_split<kX, kW, kS, kMode, 1, 4>;
+      case 2: return nt == 2 ? (const void*)&detail::k_w4_split<kX, kW, kS, kMode, 2, 2>
+                            : (const void*)&detail::k_w4_split<kX, kW, kS, kMode, 2, 4>;
+      case 3: return nt == 2 ? (const void*)&detail::k_w4_split<kX, kW, kS, kMode, 3, 2>
+                            : (const void*)&detail::k_w4_split<kX, kW, kS, kMode, 3, 4>;
+      default: return nt == 2 ? (const void*)&detail::k_w4_split<kX, kW, kS, kMode, 4, 2>
+                            : (const void*)&detail::k_w4_split<kX, kW, kS, kMode, 4, 4>;
+    }
+  });
+}
+
 template <int kX, int kW>
 const void* moe_up_of(int s, int mode, int mt, int wk) {
   return sel_scales<kX, kW>(s, mode, [&](auto S, auto Mode) {

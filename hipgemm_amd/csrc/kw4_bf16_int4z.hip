@@ -7,8 +7,11 @@ namespace kernels {
 const void* w4_vec_bf16_int4z(int s, int rows, int lk) {
   return w4_vec_of<detail::kInBf16, detail::kWInt4Z>(s, rows, lk);
 }
-const void* w4_rows_bf16_int4z(int s, int mode, int mt) {
-  return w4_rows_of<detail::kInBf16, detail::kWInt4Z>(s, mode, mt);
+const void* w4_tile_bf16_int4z(int s, int mode) {
+  return w4_tile_of<detail::kInBf16, detail::kWInt4Z>(s, mode);
+}
+const void* w4_split_bf16_int4z(int s, int mode, int mt, int nt) {
+  return w4_split_of<detail::kInBf16, detail::kWInt4Z>(s, mode, mt, nt);
 }
 
 }  // namespace kernels

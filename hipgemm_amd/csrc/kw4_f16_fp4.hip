@@ -7,8 +7,11 @@ namespace kernels {
 const void* w4_vec_f16_fp4(int s, int rows, int lk) {
   return w4_vec_of<detail::kInF16, detail::kWFp4>(s, rows, lk);
 }
-const void* w4_rows_f16_fp4(int s, int mode, int mt) {
-  return w4_rows_of<detail::kInF16, detail::kWFp4>(s, mode, mt);
+const void* w4_tile_f16_fp4(int s, int mode) {
+  return w4_tile_of<detail::kInF16, detail::kWFp4>(s, mode);
+}
+const void* w4_split_f16_fp4(int s, int mode, int mt, int nt) {
+  return w4_split_of<detail::kInF16, detail::kWFp4>(s, mode, mt, nt);
 }
 
 }  // namespace kernels

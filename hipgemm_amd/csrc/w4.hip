@@ -3,14 +3,15 @@
 
 #include "kernels.hpp"
 
-#include "hipgemm/detail/w4_rows.hpp"
+#include "hipgemm/detail/w4_tile.hpp"
 
 namespace hipgemm {
 namespace kernels {
 
 #define HIPGEMM_W4(X, W)                      \
   const void* w4_vec_##X##_##W(int s, int rows, int lk); \
-  const void* w4_rows_##X##_##W(int s, int mode, int mt);
+  const void* w4_tile_##X##_##W(int s, int mode); \
+  const void* w4_split_##X##_##W(int s, int mode, int mt, int nt);
 HIPGEMM_W4(bf16, int4)
 HIPGEMM_W4(bf16, int4z)
 HIPGEMM_W4(bf16, fp4)
@@ -27,14 +28,22 @@ const void* w4_vec(int x, int w, int s, int rows, int lk) {
     default: return b ? w4_vec_bf16_fp4(s, rows, lk) : w4_vec_f16_fp4(s, rows, lk);
   }
 }
-const void* w4_rows(int x, int w, int s, int mode, int mt) {
+const void* w4_tile(int x, int w, int s, int mode) {
+  const bool b = x == detail::kInBf16;
+  switch (w) {
+    case detail::kWInt4: return b ? w4_tile_bf16_int4(s, mode) : w4_tile_f16_int4(s, mode);
+    case detail::kWInt4Z: return b ? w4_tile_bf16_int4z(s, mode) : w4_tile_f16_int4z(s, mode);
+    default: return b ? w4_tile_bf16_fp4(s, mode) : w4_tile_f16_fp4(s, mode);
+  }
+}
+const void* w4_split(int x, int w, int s, int mode, int mt, int nt) {
   const bool b = x == detail::kInBf16;
   switch (w) {
     case detail::kWInt4:
-      return b ? w4_rows_bf16_int4(s, mode, mt) : w4_rows_f16_int4(s, mode, mt);
+      return b ? w4_split_bf16_int4(s, mode, mt, nt) : w4_split_f16_int4(s, mode, mt, nt);
     case detail::kWInt4Z:
-      return b ? w4_rows_bf16_int4z(s, mode, mt) : w4_rows_f16_int4z(s, mode, mt);
-    default: return b ? w4_rows_bf16_fp4(s, mode, mt) : w4_rows_f16_fp4(s, mode, mt);
+      return b ? w4_split_bf16_int4z(s, mode, mt, nt) : w4_split_f16_int4z(s, mode, mt, nt);
+    default: return b ? w4_split_bf16_fp4(s, mode, mt, nt) : w4_split_f16_fp4(s, mode, mt, nt);
   }
 }
 
@@ -54,7 +63,8 @@ static_assert(HIPGEMM_IN_F32 == kInF32 && HIPGEMM_IN_BF16 == kInBf16 &&
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 constexpr int kMaxK = 1 << 26;
-constexpr long long kMaxRow = 1 << 25;  // 32 rows in a buffer's range
+constexpr long long kMaxTileRow = 1 << 23;  // 128 rows' bytes in a buffer's range
+constexpr long long kMaxRow = 1 << 25;      // 64 rows' bytes
 
 template <class Args>
 hipError_t launch(const void* fn, dim3 grid, int threads, Args& g, hipStream_t stream) {
@@ -63,27 +73,35 @@ hipError_t launch(const void* fn, dim3 grid, int threads, Args& g, hipStream_t s
   return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, stream);
 }
 
-// The plan of k_w4_rows: the rows of x that go together, and as many parts of K as
-// LDS makes it for them.
-struct RowsPlan {
-  int mt, rows_max, parts, len;
+// k_w4_split and k_w4_tile.  us in a graph, split / tile, group 128, by M:
+//   N x K            96       128       192       256
+//   5000 x 3584    32/112    39/114    40/114    71/114
+//   4096 x 4096    16/65     18/67     23/67     24/67
+//   14336 x 4096   36/66     42/68     61/68     80/68
+//   28672 x 8192  116/116   134/120   198/169   238/174
+// (tile: 40, 32, 112, 224 tiles and twice that from 192 rows): tiles from three
+// quarters of the CUs on, not of fewer rows than three quarters of a tile.
+bool by_tiles(const hipgemm_w4_desc& d) {
+  const long long tiles = (long long)((d.M + kW4TileM - 1) / kW4TileM) *
+                          ((d.N + kW4TileN - 1) / kW4TileN);
+  return d.M > 96 && tiles >= 192 && 2 * d.ldx <= kMaxTileRow && d.ldw <= kMaxTileRow &&
+         d.lds <= kMaxTileRow;
+}
+
+// k_w4_split: groups of up to 64 rows of even lengths, and 32 columns where that
+// leaves a workgroup for each CU (16 rows, 4096 x 4096: 9.8 us for 13.4;  14336 x
+// 4096, 448 tiles: 19.6 for 16.0).
+struct SplitPlan {
+  int mt, nt;
+  long long tiles;
 };
-RowsPlan rows_plan(int M, int K) {
-  RowsPlan p;
-  p.mt = M <= 16 ? 1 : 2;
-  const int groups = (M + 16 * p.mt - 1) / (16 * p.mt);
-  p.rows_max = (M + groups - 1) / groups;
-  const int steps = (K + 255) / 256;
-  for (p.parts = 1; p.parts < steps; ++p.parts) {
-    const int len = 256 * ((steps + p.parts - 1) / p.parts);
-    if ((p.mt == 1 ? W4Stream<kInBf16, kWFp4, kInF32, kCoarse, 1>::rows_that_fit(len)
-                   : W4Stream<kInBf16, kWFp4, kInF32, kCoarse, 2>::rows_that_fit(len)) >=
-        p.rows_max)
-      break;
-  }
-  const int len = (steps + p.parts - 1) / p.parts;
-  p.len = 256 * len;
-  p.parts = (steps + len - 1) / len;
+SplitPlan split_plan(int M, int N) {
+  SplitPlan p;
+  const int groups = (M + 63) / 64;
+  p.mt = ((M + groups - 1) / groups + 15) / 16;
+  const long long tm = (M + 16 * p.mt - 1) / (16 * p.mt);
+  p.nt = tm * ((N + 31) / 32) <= 256 ? 2 : 4;
+  p.tiles = tm * ((N + 16 * p.nt - 1) / (16 * p.nt));
   return p;
 }
 
@@ -129,18 +147,21 @@ hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
   g.act = d.activation;
   g.out = d.out_dtype;
   const int w = d.zeros ? kWInt4Z : d.format;
-  if (d.M <= 4 || d.K == 0) {
+  // Up to four rows;  and, four at a time, without any K or where rows of x lie so
+  // far apart that 64 are not in a buffer's range.
+  if (d.M <= 4 || d.K == 0 || 2 * d.ldx > kMaxRow) {
     const VecPlan p = vec_plan(d.N, d.K);
     g.waves_k = p.waves_k;
     g.rows = p.rows;
     g.wave_rows = p.wave_rows;
-    for (int m = 0; m < d.M; m += 4) {  // (more than four rows only without any K)
+    for (int m = 0; m < d.M; m += 4) {
       g.M = d.M - m < 4 ? d.M - m : 4;
       const hipError_t e =
           launch(hk::w4_vec(d.x_type, w, d.scale_type, g.M == 3 ? 4 : g.M, p.lk),
                  dim3((unsigned)((d.N + p.rows - 1) / p.rows)), kWave * p.waves_k * p.waves_r, g,
                  stream);
       if (e != hipSuccess) return e;
+      g.x += 4 * g.ldx;
       g.y += 4 * d.ldy * out_bytes(d.out_dtype);
     }
     return hipSuccess;
@@ -150,12 +171,15 @@ hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
                        ? kInline
                    : d.group_size % 128 == 0 ? kCoarse
                                              : kFine;
-  const RowsPlan p = rows_plan(d.M, d.K);
-  W4RowsArgs r{g, p.rows_max, p.parts, p.len};
-  const long long tiles =
-      (long long)((d.M + p.rows_max - 1) / p.rows_max) * ((d.N + 31) / 32);
-  return launch(hk::w4_rows(d.x_type, w, d.scale_type, mode, p.mt),
-                dim3((unsigned)(tiles < 256 ? tiles : 256)), 512, r, stream);
+  if (by_tiles(d)) {
+    const long long tiles = (long long)((d.M + kW4TileM - 1) / kW4TileM) *
+                            ((d.N + kW4TileN - 1) / kW4TileN);
+    return launch(hk::w4_tile(d.x_type, w, d.scale_type, mode),
+                  dim3((unsigned)(tiles < 512 ? tiles : 512)), 256, g, stream);
+  }
+  const SplitPlan p = split_plan(d.M, d.N);
+  return launch(hk::w4_split(d.x_type, w, d.scale_type, mode, p.mt, p.nt),
+                dim3((unsigned)(p.tiles < 256 ? p.tiles : 256)), 256, g, stream);
 }
 
 }  // namespace

@@ -1,0 +1,443 @@
+// Products of 5 rows of 16-bit activations and more with 4-bit weights, by MFMA.  A
+// wave multiplies 16 kMT rows of x by 16 kNT of weights (W4Wave), 128 of K at a
+// time: x (256 bytes of a row) and weights (64 bytes) come by DMA into stages of
+// LDS, weights are decoded in registers on their way to the matrix unit.
+//
+// k_w4_split, some rows: what bounds it is the weights' and x's way into a CU, and
+// for few steps the first loads' latency.  Four waves take every fourth step of
+// one tile each, with stages of their own, so nobody waits for anybody until the
+// sums are added; up to 160 KiB of stages are on their way.  bf16, us in a graph:
+// 16 x 14336 x 4096 fp4 in groups of 32 16.1 (2.0 TB/s), 16 x 28672 x 8192 int4 52,
+// 64 x 14336 x 4096 int4 24, 37 x 5000 x 3584 int4 in groups of 64 21.  (With all of
+// x of a group in LDS and the weights streaming past it the same took 18.6, 53, 104,
+// 35: x came in again for every 32 columns.)
+//
+// k_w4_tile, many rows: bound by the matrix unit and by what surrounds it.  Tiles of
+// 128 x 128 by four waves, 64 x 64 each, two stages of 40 KiB that they share, two
+// workgroups to a CU, so that one's arithmetic hides the other's waits.  2048 x 14336
+// x 4096 int4, group 128, bf16: 321 us, 750 TFLOP/s (628 by k_w4_split).
+//
+// Per wave of 64 x 64 and step there are 64 MFMAs of 16 cycles each; the decoding
+// takes 9 instructions per 8 weights and lane (16 x 9), int4 with one scale per step
+// and row one FMA per accumulator (64): all told about as many issue slots as the
+// matrix unit takes, so neither may grow.  Hence:
+//   * int4 codes are decoded exactly, q (0-15), not q plus an offset: the code's
+//     nibble is the e4m3 number q 2^-9 (subnormal below 8, the first binade from
+//     there), so unpacked nibbles go through the e4m3 conversion with scale 2^9.
+//     They come out in their own order, and the activations need no reordering,
+//     which would cost as much as the decoding (16 operands against 16).
+//   * the zero point's share, -z sum(x), is the accumulator that a step's MFMAs
+//     start from: without zero points it is the same for all columns.
+// Scales as in w4_stream.hpp (kCoarse, kFine, kInline), loaded with the stage by the
+// lanes that need them.
+//
+// A row of x's chunk c (16 bytes) lies at slot c ^ (row % 16), one of weights (16
+// bytes, four to a row) at slot c ^ (row / 2 % 4): the 16 rows that an operand's
+// read takes one chunk of lie on all banks.
+#pragma once
+
+#include "layout.hpp"
+#include "w4_stream.hpp"
+#include "w4_vec.hpp"
+
+namespace hipgemm {
+namespace detail {
+
+constexpr int kW4TileM = 128, kW4TileN = 128, kW4TileK = 128;
+
+// Eight codes in their own order, exactly (int4: q).
+template <int kX, int kW>
+__device__ __forceinline__ i32x4 decode8_exact(uint32_t q, float scale) {
+  if constexpr (!is_int4(kW)) {
+    return decode8<kX, kW>(q, 0u, scale);
+  } else {
+    const uint32_t lo = q & 0x0f0f0f0fu, hi = (q >> 4) & 0x0f0f0f0fu;
+    return decode8<kX, kWE4M3>(__builtin_amdgcn_perm(hi, lo, 0x05010400u),
+                               __builtin_amdgcn_perm(hi, lo, 0x07030602u), 512.0f);
+  }
+}
+
+// One output by its definition, weight by weight, where the sum came out
+// infinite or NaN: int4's excess (decode.hpp) makes inf - inf of an infinite x,
+// and the sums before the scale can overflow for one near the largest, where the
+// definition has an infinity or a number.
+template <int kX, int kW, int kS>
+__device__ __forceinline__ float slow_row(const W4Args& g, int m, int n) {
+  float sum = 0.0f;
+#pragma unroll 1
+  for (int k = 0; k < g.K; k += 2) {
+    const int grp = k / g.G;
+    const uint32_t c = g.w[n * g.ldw + (k >> 1)];
+    const f32x2 x = unpack2<kX>(reinterpret_cast<const uint32_t*>(g.x + m * g.ldx)[k >> 1]);
+    const float s = scale_at<kS>(g.s + n * g.lds, grp);
+    const float z = g.z ? (float)g.z[n * g.ldz + grp] : 8.0f;
+    sum = __builtin_fmaf(x[0], s * code_value<kW>(c & 15u, z), sum);
+    sum = __builtin_fmaf(x[1], s * code_value<kW>(c >> 4, z), sum);
+  }
+  return sum;
+}
+
+// What a wave multiplies: 16 kMT rows of x by 16 kNT of weights, 128 of K.
+template <int kX, int kW, int kS, int kMode, int kMT, int kNT>
+struct W4Wave {
+  static constexpr bool kZ = kW == kWInt4Z;
+  f32x4 acc[kNT][kMT];  // [n][m]
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int m = 0; m < kMT; ++m) acc[n][m] = f32x4{};
+  }
+
+  // Reads of LDS in assembly, with their waits (w4_stream.hpp: read_x): 16 bytes
+  // each of rows r, 16 + r, ...
+  __device__ __forceinline__ static void read_x(const lds_u8* p, i32x4 (&v)[kMT]) {
+    if constexpr (kMT == 1)
+      asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(v[0]) : "v"(p) : "memory");
+    else if constexpr (kMT == 2)
+      asm volatile(
+          "ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:4096\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(v[0]), "=&v"(v[1])
+          : "v"(p)
+          : "memory");
+    else if constexpr (kMT == 3)
+      asm volatile(
+          "ds_read_b128 %0, %3\n\tds_read_b128 %1, %3 offset:4096\n\t"
+          "ds_read_b128 %2, %3 offset:8192\n\ts_waitcnt lgkmcnt(0)"
+          : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2])
+          : "v"(p)
+          : "memory");
+    else
+      asm volatile(
+          "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:4096\n\t"
+          "ds_read_b128 %2, %4 offset:8192\n\tds_read_b128 %3, %4 offset:12288\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+          : "v"(p)
+          : "memory");
+  }
+  __device__ __forceinline__ static void read_w(const lds_u8* p, i32x4 (&v)[kNT]) {
+    if constexpr (kNT == 2)
+      asm volatile(
+          "ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:1024\n\ts_waitcnt lgkmcnt(0)"
+          : "=&v"(v[0]), "=&v"(v[1])
+          : "v"(p)
+          : "memory");
+    else
+      asm volatile(
+          "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:1024\n\t"
+          "ds_read_b128 %2, %4 offset:2048\n\tds_read_b128 %3, %4 offset:3072\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+          : "v"(p)
+          : "memory");
+  }
+
+  // x and w: the wave's first rows in a stage;  s, z: raw scales and zero points of
+  // rows 16 n + r.
+  __device__ __forceinline__ void multiply(const lds_u8* x, const lds_u8* w_, const uint32_t (&s)[kNT],
+                                           const uint32_t (&z)[kNT]) {
+    i32x4 q[kNT];
+    const int r = lane_id() & 15, gq = lane_id() >> 4;
+    read_w(w_ + r * 64 + 16 * (gq ^ ((r >> 1) & 3)), q);
+    const lds_u8* ap = x + r * 256;
+    const int one = (int)kOnes2<kX>;
+    const i32x4 ones{one, one, one, one};
+    if constexpr (kMode == kFine) {
+      // MFMA j: the lane's k = 32 j + 8 gq, one scale for all of it.
+      uint32_t w[kNT][4], s4[kNT][4], z4[kNT][4];
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[n][i] = (uint32_t)q[n][i];
+        transpose4(w[n]);
+        spread4(s[n], s4[n]);
+        if constexpr (kZ) spread4(z[n], z4[n]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        i32x4 a[kMT];
+        read_x(ap + 16 * ((4 * j + gq) ^ r), a);
+        f32x4 xs[kMT];
+        if constexpr (is_int4(kW)) {
+#pragma unroll
+          for (int m = 0; m < kMT; ++m) {
+            xs[m] = mfma_16x16x32<kX>(a[m], ones, f32x4{});
+            if constexpr (!kZ) xs[m] *= -8.0f;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) {
+          const i32x4 b = decode8_exact<kX, kW>(w[n][j], 1.0f);
+          const float c = scale_of<kS>(s4[n][j]);
+#pragma unroll
+          for (int m = 0; m < kMT; ++m) {
+            f32x4 p = f32x4{};
+            if constexpr (kZ) p = xs[m] * -(float)z4[n][j];
+            else if constexpr (is_int4(kW)) p = xs[m];
+            p = mfma_16x16x32<kX>(a[m], b, p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n][m][e] = __builtin_fmaf(c, p[e], acc[n][m][e]);
+          }
+        }
+      }
+    } else {
+      // MFMA j: the lane's k = 32 gq + 8 j.
+      i32x4 a[4][kMT];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) read_x(ap + 16 * ((4 * gq + j) ^ r), a[j]);
+      f32x4 xs[kMT];
+      if constexpr (is_int4(kW)) {
+#pragma unroll
+        for (int m = 0; m < kMT; ++m) {
+          xs[m] = f32x4{};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) xs[m] = mfma_16x16x32<kX>(a[j][m], ones, xs[m]);
+          if constexpr (!kZ) xs[m] *= -8.0f;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n) {
+        const float c = scale_of<kS>(s[n]);
+        i32x4 b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          b[j] = decode8_exact<kX, kW>((uint32_t)q[n][j], kMode == kInline ? c : 1.0f);
+#pragma unroll
+        for (int m = 0; m < kMT; ++m) {
+          if constexpr (kMode == kInline) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[n][m] = mfma_16x16x32<kX>(a[j][m], b[j], acc[n][m]);
+          } else {
+            f32x4 p = f32x4{};
+            if constexpr (kZ) p = xs[m] * -(float)z[n];
+            else if constexpr (is_int4(kW)) p = xs[m];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p = mfma_16x16x32<kX>(a[j][m], b[j], p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n][m][e] = __builtin_fmaf(c, p[e], acc[n][m][e]);
+          }
+        }
+      }
+    }
+  }
+};
+
+// The loads of W4Wave's scales.
+template <int kW, int kS, int kMode, int kNT>
+struct W4Scales {
+  static constexpr bool kZ = kW == kWInt4Z;
+  static constexpr int kLoads = kZ ? 2 * kNT : kNT;
+  const uint8_t *s, *z;
+  uint32_t row[kNT];
+  int K;
+  float inv;
+
+  // Rows n0 + 16 n + r.
+  __device__ __forceinline__ void set(const W4Args& g, int n0) {
+    n0 = min(n0, g.N - 1);
+    s = g.s + (long long)n0 * g.lds;
+    z = kZ ? g.z + (long long)n0 * g.ldz : nullptr;
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+      row[n] = (uint32_t)min(16 * n + (lane_id() & 15), g.N - 1 - n0) * (uint32_t)g.ldz;
+    K = g.K;
+    inv = 32.0f / (float)g.G;
+  }
+  __device__ __forceinline__ void load(int k, uint32_t (&sv)[kNT], uint32_t (&zv)[kNT]) const {
+    const int own = kMode == kCoarse ? k : k + 32 * (lane_id() >> 4);
+    const uint32_t at = (uint32_t)group_of(min(own, K - 32) >> 5, inv);
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      sv[n] = scale_raw<kS>(s, row[n] + at);
+      if constexpr (kZ) zv[n] = z[row[n] + at];
+    }
+  }
+};
+
+// One column of results: rows m0 + 16 m + 4 gq + e.
+template <int kX, int kW, int kS, int kMT>
+__device__ __forceinline__ void w4_store(const W4Args& g, int m0, int col, const f32x4 (&v)[kMT]) {
+  if (col >= g.N) return;
+  const float b = g.bias ? g.bias[col] : 0.0f;
+#pragma unroll
+  for (int m = 0; m < kMT; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int row = m0 + 16 * m + 4 * (lane_id() >> 4) + e;
+      if (row >= g.M) continue;
+      float f = v[m][e];
+      if (!(__builtin_fabsf(f) < __builtin_inff())) f = slow_row<kX, kW, kS>(g, row, col);
+      if (g.bias) f += b;
+      store_result(g.y, row * g.ldy + col, g.out, activate(f, g.act));
+    }
+}
+
+template <int kX, int kW, int kS, int kMode>
+__global__ __launch_bounds__(256, 2) void k_w4_tile(W4Args g) {
+  constexpr int kStageA = kW4TileM * 256, kStageB = kW4TileN * 64;
+  constexpr int kStage = kStageA + kStageB;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds_[2 * kStage];
+  lds_u8* lds = (lds_u8*)lds_;
+  const int wave = wave_id(), lane = lane_id();
+  const int wm = wave & 1, wn = wave >> 1;
+  const int r = lane & 15;
+
+  const int tiles_m = (g.M + kW4TileM - 1) / kW4TileM, tiles_n = (g.N + kW4TileN - 1) / kW4TileN;
+  const TileWalk walk = tile_walk((int)blockIdx.x, (int)gridDim.x, tiles_m * tiles_n);
+  const uint32_t ldx = (uint32_t)g.ldx, ldw = (uint32_t)g.ldw;
+  const int steps = (g.K + kW4TileK - 1) / kW4TileK;
+
+  for (int tile = walk.first; tile < walk.end; tile += walk.stride) {
+    const TileCoord tc = grouped_tile_u(tile, tiles_m, tiles_n, 8);
+    const int m0 = tc.m * kW4TileM, n0 = tc.n * kW4TileN;
+    const auto xb = make_rsrc(g.x + (long long)m0 * g.ldx, (uint32_t)min(g.M - m0, kW4TileM) * ldx);
+    const auto wb = make_rsrc(g.w + (long long)n0 * g.ldw, (uint32_t)min(g.N - n0, kW4TileN) * ldw);
+    // DMA lanes: x, instruction i (of 32, 8 per wave): rows 4 i .. + 3, lane l row l
+    // / 16, slot l % 16;  weights, instruction i (of 8, 2 per wave): rows 16 i .. +
+    // 15, lane l row l / 4, slot l % 4.
+    auto dma = [&](int k, lds_u8* to) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = 4 * (8 * wave + i) + (lane >> 4);
+        const int c = (lane & 15) ^ (row & 15);
+        const int kc = k + 8 * c;
+        dma16(xb, to + 1024 * (8 * wave + i), kc < g.K ? (uint32_t)row * ldx + 2 * kc : kOobOffset, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = 16 * (2 * wave + i) + (lane >> 2);
+        const int c = (lane & 3) ^ ((row >> 1) & 3);
+        const int kc = k + 32 * c;
+        dma16(wb, to + kStageA + 1024 * (2 * wave + i),
+              kc < g.K ? (uint32_t)row * ldw + (kc >> 1) : kOobOffset, 0);
+      }
+    };
+    W4Scales<kW, kS, kMode, 4> sc;
+    sc.set(g, n0 + 64 * wn);
+    constexpr int kLoads = 10 + W4Scales<kW, kS, kMode, 4>::kLoads;
+    W4Wave<kX, kW, kS, kMode, 4, 4> wv;
+    wv.clear();
+    const int xo = 64 * wm * 256, wo = kStageA + 64 * wn * 64;
+
+    // Step t in stage t % 2; the next step's loads go out before it is waited for.
+    uint32_t s[2][4], z[2][4];
+    dma(0, lds);
+    sc.load(0, s[0], z[0]);
+    for (int t = 0; t < steps; t += 2) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (t + u >= steps) break;
+        compiler_fence();
+        sched_fence();
+        dma((t + u + 1) * kW4TileK, lds + (1 - u) * kStage);  // (past K: zeros)
+        sc.load((t + u + 1) * kW4TileK, s[1 - u], z[1 - u]);
+        wait_vmcnt<kLoads>();
+        barrier();
+        wv.multiply(lds + u * kStage + xo, lds + u * kStage + wo, s[u], z[u]);
+        wait_lgkmcnt<0>();
+        barrier();
+      }
+    }
+    // (the last step's zeros have to land before the stages are used again)
+    wait_vmcnt<0>();
+    barrier();
+
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      w4_store<kX, kW, kS, 4>(g, m0 + 64 * wm, n0 + 64 * wn + 16 * n + r, wv.acc[n]);
+  }
+}
+
+// Some rows: tiles of 16 kMT x 16 kNT, of whose K the four waves take every fourth 128
+// each, with stages of their own and no barrier until their sums are added.
+template <int kMT, int kNT>
+constexpr int kW4SplitStages = (40 << 10) / (kMT * 4096 + kNT * 1024) > 4
+                                   ? 4
+                                   : (40 << 10) / (kMT * 4096 + kNT * 1024);
+
+template <int kX, int kW, int kS, int kMode, int kMT, int kNT>
+__global__ __launch_bounds__(256, 1) void k_w4_split(W4Args g) {
+  constexpr int kStageA = kMT * 4096, kStage = kStageA + kNT * 1024, kStages = kW4SplitStages<kMT, kNT>;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds_[4 * kStages * kStage];
+  const int wave = wave_id(), lane = lane_id();
+  lds_u8* lds = (lds_u8*)lds_ + wave * (kStages * kStage);
+  const int r = lane & 15;
+  const int tiles_m = (g.M + 16 * kMT - 1) / (16 * kMT), tiles_n = (g.N + 16 * kNT - 1) / (16 * kNT);
+  const TileWalk walk = tile_walk((int)blockIdx.x, (int)gridDim.x, tiles_m * tiles_n);
+  const uint32_t ldx = (uint32_t)g.ldx, ldw = (uint32_t)g.ldw;
+  const int steps = ((g.K + 127) / 128 + 3 - wave) / 4;
+
+  for (int tile = walk.first; tile < walk.end; tile += walk.stride) {
+    const int m0 = tile % tiles_m * (16 * kMT), n0 = tile / tiles_m * (16 * kNT);
+    const auto xb = make_rsrc(g.x + (long long)m0 * g.ldx, (uint32_t)min(g.M - m0, 16 * kMT) * ldx);
+    const auto wb = make_rsrc(g.w + (long long)n0 * g.ldw, (uint32_t)min(g.N - n0, 16 * kNT) * ldw);
+    auto dma = [&](int k, lds_u8* to) {
+#pragma unroll
+      for (int i = 0; i < 4 * kMT; ++i) {
+        const int row = 4 * i + (lane >> 4);
+        const int kc = k + 8 * ((lane & 15) ^ (row & 15));
+        dma16(xb, to + 1024 * i, kc < g.K ? (uint32_t)row * ldx + 2 * kc : kOobOffset, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        const int row = 16 * i + (lane >> 2);
+        const int kc = k + 32 * ((lane & 3) ^ ((row >> 1) & 3));
+        dma16_nt(wb, to + kStageA + 1024 * i, kc < g.K ? (uint32_t)row * ldw + (kc >> 1) : kOobOffset, 0);
+      }
+    };
+    W4Scales<kW, kS, kMode, kNT> sc;
+    sc.set(g, n0);
+    constexpr int kLoads = 4 * kMT + kNT + W4Scales<kW, kS, kMode, kNT>::kLoads;
+    W4Wave<kX, kW, kS, kMode, kMT, kNT> wv;
+    wv.clear();
+
+    // Step t of this wave in stage t % kStages, kStages - 1 of them ahead.
+    uint32_t s[kStages][kNT], z[kStages][kNT];
+    auto load = [&](int t, int u) __attribute__((always_inline)) {
+      compiler_fence();
+      sched_fence();
+      const int k = 512 * t + 128 * wave;
+      dma(k, lds + u * kStage);  // (past K: zeros)
+      sc.load(k, s[u], z[u]);
+    };
+#pragma unroll
+    for (int u = 0; u < kStages - 1; ++u) load(u, u);
+    for (int t = 0; t < steps; t += kStages) {
+#pragma unroll
+      for (int u = 0; u < kStages; ++u) {
+        if (t + u >= steps) break;
+        load(t + u + kStages - 1, (u + kStages - 1) % kStages);
+        wait_vmcnt<(kStages - 1) * kLoads>();
+        compiler_fence();
+        sched_fence();
+        wv.multiply(lds + u * kStage, lds + u * kStage + kStageA, s[u], z[u]);
+      }
+    }
+    // The waves' sums, added in their order; wave w stores columns 16 w + r.
+    wait_vmcnt<0>();
+    auto sum = (__attribute__((address_space(3))) f32x4*)(lds_u8*)lds_;
+    constexpr int kPer = kStages * kStage / 16;
+#pragma unroll
+    for (int n = 0; n < kNT; ++n)
+#pragma unroll
+      for (int m = 0; m < kMT; ++m) sum[wave * kPer + (n * kMT + m) * kWave + lane] = wv.acc[n][m];
+    __syncthreads();
+    for (int n = wave; n < kNT; n += 4) {
+      f32x4 v[kMT];
+#pragma unroll
+      for (int m = 0; m < kMT; ++m) {
+        v[m] = sum[(n * kMT + m) * kWave + lane];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) v[m] += sum[i * kPer + (n * kMT + m) * kWave + lane];
+      }
+      w4_store<kX, kW, kS, kMT>(g, m0, n0 + 16 * n + r, v);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace detail
+}  // namespace hipgemm
