@@ -257,22 +257,19 @@ struct W4Scales {
   }
 };
 
-// One column of results: rows m0 + 16 m + 4 gq + e.
-template <int kX, int kW, int kS, int kMT>
-__device__ __forceinline__ void w4_store(const W4Args& g, int m0, int col, const f32x4 (&v)[kMT]) {
+// Rows row .. + 3 of a column.
+template <int kX, int kW, int kS>
+__device__ __forceinline__ void w4_store(const W4Args& g, int row, int col, const f32x4& v) {
   if (col >= g.N) return;
   const float b = g.bias ? g.bias[col] : 0.0f;
 #pragma unroll
-  for (int m = 0; m < kMT; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = m0 + 16 * m + 4 * (lane_id() >> 4) + e;
-      if (row >= g.M) continue;
-      float f = v[m][e];
-      if (!(__builtin_fabsf(f) < __builtin_inff())) f = slow_row<kX, kW, kS>(g, row, col);
-      if (g.bias) f += b;
-      store_result(g.y, row * g.ldy + col, g.out, activate(f, g.act));
-    }
+  for (int e = 0; e < 4; ++e) {
+    if (row + e >= g.M) break;
+    float f = v[e];
+    if (!(__builtin_fabsf(f) < __builtin_inff())) f = slow_row<kX, kW, kS>(g, row + e, col);
+    if (g.bias) f += b;
+    store_result(g.y, (row + e) * g.ldy + col, g.out, activate(f, g.act));
+  }
 }
 
 template <int kX, int kW, int kS, int kMode>
@@ -283,7 +280,6 @@ __global__ __launch_bounds__(256, 2) void k_w4_tile(W4Args g) {
   lds_u8* lds = (lds_u8*)lds_;
   const int wave = wave_id(), lane = lane_id();
   const int wm = wave & 1, wn = wave >> 1;
-  const int r = lane & 15;
 
   const int tiles_m = (g.M + kW4TileM - 1) / kW4TileM, tiles_n = (g.N + kW4TileN - 1) / kW4TileN;
   const TileWalk walk = tile_walk((int)blockIdx.x, (int)gridDim.x, tiles_m * tiles_n);
@@ -345,9 +341,19 @@ __global__ __launch_bounds__(256, 2) void k_w4_tile(W4Args g) {
     wait_vmcnt<0>();
     barrier();
 
+    // Each wave's sums through its quarter of the stages, from columns in lanes'
+    // registers to whole lines of a row.
+    auto sum = (__attribute__((address_space(3))) f32x4*)lds + wave * (2 * kStage / 64);
 #pragma unroll
     for (int n = 0; n < 4; ++n)
-      w4_store<kX, kW, kS, 4>(g, m0 + 64 * wm, n0 + 64 * wn + 16 * n + r, wv.acc[n]);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) sum[(n * 4 + m) * kWave + lane] = wv.acc[n][m];
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {  // rows 4 i .. + 3, column of the lane
+      const f32x4 v = sum[((lane >> 4) * 4 + (i >> 2)) * kWave + (i & 3) * 16 + (lane & 15)];
+      w4_store<kX, kW, kS>(g, m0 + 64 * wm + 4 * i, n0 + 64 * wn + lane, v);
+    }
+    barrier();
   }
 }
 
@@ -416,7 +422,7 @@ __global__ __launch_bounds__(256, 1) void k_w4_split(W4Args g) {
         wv.multiply(lds + u * kStage, lds + u * kStage + kStageA, s[u], z[u]);
       }
     }
-    // The waves' sums, added in their order; wave w stores columns 16 w + r.
+    // The waves' sums, added in their order.
     wait_vmcnt<0>();
     auto sum = (__attribute__((address_space(3))) f32x4*)(lds_u8*)lds_;
     constexpr int kPer = kStages * kStage / 16;
@@ -425,15 +431,13 @@ __global__ __launch_bounds__(256, 1) void k_w4_split(W4Args g) {
 #pragma unroll
       for (int m = 0; m < kMT; ++m) sum[wave * kPer + (n * kMT + m) * kWave + lane] = wv.acc[n][m];
     __syncthreads();
-    for (int n = wave; n < kNT; n += 4) {
-      f32x4 v[kMT];
+    // (16 x 16 at a time: rows 4 gq .. + 3 of column r in a lane)
+#pragma unroll 1
+    for (int i = wave; i < kNT * kMT; i += 4) {
+      f32x4 v = sum[i * kWave + lane];
 #pragma unroll
-      for (int m = 0; m < kMT; ++m) {
-        v[m] = sum[(n * kMT + m) * kWave + lane];
-#pragma unroll
-        for (int i = 1; i < 4; ++i) v[m] += sum[i * kPer + (n * kMT + m) * kWave + lane];
-      }
-      w4_store<kX, kW, kS, kMT>(g, m0, n0 + 16 * n + r, v);
+      for (int w = 1; w < 4; ++w) v += sum[w * kPer + i * kWave + lane];
+      w4_store<kX, kW, kS>(g, m0 + 16 * (i % kMT) + 4 * (lane >> 4), n0 + 16 * (i / kMT) + r, v);
     }
     __syncthreads();
   }

@@ -144,32 +144,32 @@ struct Vec {
   // The lane's sums over its part of the chunk.
   template <class F>
   __device__ __forceinline__ void dot(const Rows& r, int K, F&& xr, float (&sum)[kM][kVecRows]) const {
-    if (!odd) {
 #pragma unroll
-      for (int i = 0; i < kVecRows; ++i) {
-        float d[kM] = {};
+    for (int i = 0; i < kVecRows; ++i) {
+      float d[kM] = {};
 #pragma unroll
-        for (int j = 0; j < kWords; ++j) {
-          const i32x4 b = kW == kWE4M3
-                              ? decode8<kX, kW>((uint32_t)r.w[i][2 * j % 4], (uint32_t)r.w[i][(2 * j + 1) % 4], 1.0f)
-                              : decode8<kX, kW>((uint32_t)r.w[i][j], 0u, 1.0f);
+      for (int j = 0; j < kWords; ++j) {
+        const i32x4 b = kW == kWE4M3
+                            ? decode8<kX, kW>((uint32_t)r.w[i][2 * j % 4], (uint32_t)r.w[i][(2 * j + 1) % 4], 1.0f)
+                            : decode8<kX, kW>((uint32_t)r.w[i][j], 0u, 1.0f);
 #pragma unroll
-          for (int m = 0; m < kM; ++m)
+        for (int m = 0; m < kM; ++m)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              d[m] = dot2<kX>((uint32_t)x[m][j][e], (uint32_t)b[e], d[m]);
-        }
-        const float sc = scale_of<kS>(r.s[i]);
-        float off = -(kInt4Bias<kX> + 8.0f);
-        if constexpr (kW == kWInt4Z) off = -(kInt4Bias<kX> + (float)r.z[i]);
-#pragma unroll
-        for (int m = 0; m < kM; ++m) {
-          if constexpr (is_int4(kW)) d[m] = __builtin_fmaf(off, xs[m], d[m]);
-          sum[m][i] = in ? sc * d[m] : 0.0f;
-        }
-        sched_fence();  // one row's decoded weights at a time in registers
+          for (int e = 0; e < 4; ++e)
+            d[m] = dot2<kX>((uint32_t)x[m][j][e], (uint32_t)b[e], d[m]);
       }
-    } else {
+      const float sc = scale_of<kS>(r.s[i]);
+      float off = -(kInt4Bias<kX> + 8.0f);
+      if constexpr (kW == kWInt4Z) off = -(kInt4Bias<kX> + (float)r.z[i]);
+#pragma unroll
+      for (int m = 0; m < kM; ++m) {
+        if constexpr (is_int4(kW)) d[m] = __builtin_fmaf(off, xs[m], d[m]);
+        sum[m][i] = in ? sc * d[m] : 0.0f;
+      }
+      sched_fence();  // one row's decoded weights at a time in registers
+    }
+    // (Not as an else: that would make the loop's branches ones on the lanes.)
+    if (__builtin_amdgcn_readfirstlane((int)odd)) {
       // One by one, and scaled first.
 #pragma unroll
       for (int i = 0; i < kVecRows; ++i) {
@@ -230,7 +230,7 @@ struct Vec {
     }
   }
   template <int kCtrl>
-  __device__ static float dpp_f(float v) {
+  __device__ __forceinline__ static float dpp_f(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
                                          0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, true));
   }
