@@ -179,12 +179,18 @@ hipError_t vec_turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
 
 hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   const int pairs = g.T * g.k;
-  if (g.T == 1) return vec_turn(g, d, stream);
+  // Experts chosen at all, if all are chosen alike.
+  const double chosen = g.E * (1.0 - std::pow(1.0 - (g.k < g.E ? (double)g.k / g.E : 1.0), g.T));
+  // Pair by pair while few experts are read twice.  us in a graph, pairs / grouped,
+  // by tokens: int4, 8 of 64 experts of 2048 x 1024, 2 24/37, 6 55/58, 12 87/73; 8 of
+  // 128 of 4096 x 1536, 4 71/90, 8 124/140, 16 237/175;  fp4, 3 of 30 of 2336 x 1056,
+  // 5 24/44, 12 43/56;  e4m3, 4 of 64 of 4096 x 2048, 2 41/51, 4 71/80, 8 126/115; 2
+  // of 8 of 4096 x 14336, 1 66/71, 2 121/116.  (Grouped, 4-bit weights stream at 3 to
+  // 4.6 TB/s, e4m3 ones at 5 to 5.8.)
+  if (pairs <= chosen * (d.format == HIPGEMM_W8_E4M3 ? 1.13 : 1.5)) return vec_turn(g, d, stream);
   // Tiles of 16 tokens, two at a time where experts have more on average.
   const int mt = pairs > 12 * g.E ? 2 : 1;
   g.parts = down_parts(g.T, g.k, g.E, g.D, g.F, &g.part_len);
-  // Experts chosen at all, if all are chosen alike.
-  const double chosen = g.E * (1.0 - std::pow(1.0 - 1.0 / g.E, pairs));
   // Tiles of 128 rows with two waves to a row's K where each CU has ten or more of
   // them (fewer ends of tiles per byte), of 32 rows with eight where not.
   const int wku = chosen * g.F / 64 >= 2560 ? 2 : 8;

@@ -442,7 +442,7 @@ hipError_t hipgemm_moe_route(const void *logits, int type, int T, int E, int k,
  * D, F, group_size multiples of 32; matrices 16-byte aligned, with row and
  * expert strides of multiples of 16 bytes; k <= 64.  Workspace:
  * hipgemm_moe_workspace_size bytes, 16-byte aligned, of any content; calls that
- * may run concurrently must not share one.  Three launches per turn on `stream`.
+ * may run concurrently must not share one.  Two or three launches per turn on `stream`.
  * Zero-initialise the struct and set `size`.  No reference counterpart.
  */
 enum { HIPGEMM_W8_E4M3 = 2 };

@@ -1,4 +1,4 @@
-// The experts of one token (or a few), in two kernels of w4_vec.hpp's kind:
+// The experts of a few tokens that share few of them, in two kernels of w4_vec.hpp's kind:
 //
 //   k_moe_vec_up    h[p] = weights[p] act(x W13[e][:F]^T) (x W13[e][F:]^T)
 //   k_moe_vec_down  y[t] = sum_j h[t k + j] W2[e]^T

@@ -31,9 +31,11 @@
 // Scales as in w4_stream.hpp (kCoarse, kFine, kInline), loaded with the stage by the
 // lanes that need them.
 //
-// A row of x's chunk c (16 bytes) lies at slot c ^ (row % 16), one of weights (16
-// bytes, four to a row) at slot c ^ (row / 2 % 4): the 16 rows that an operand's
-// read takes one chunk of lie on all banks.
+// A row of x's chunk c (16 bytes) lies at slot c ^ x_slot(row), one of weights (16
+// bytes, four to a row) at slot c ^ (row / 2 % 4).  A read of 16 bytes per lane takes
+// lanes 0-3, 12-15, 20-27 together, and so on: eight rows of one chunk and the
+// other eight of the next or the fourth from it, which have to lie on all banks.
+// (With c ^ (row % 16) 43% of the LDS cycles were conflicts.)
 #pragma once
 
 #include "layout.hpp"
@@ -44,6 +46,9 @@ namespace hipgemm {
 namespace detail {
 
 constexpr int kW4TileM = 128, kW4TileN = 128, kW4TileK = 128;
+
+// (rows 0-3, 12-15 have slots 0-7, the others 8-15: xor 1 or 4 stays in these)
+__device__ __forceinline__ int x_slot(int row) { return (row + 4) & 15; }
 
 // Eight codes in their own order, exactly (int4: q).
 template <int kX, int kW>
@@ -159,7 +164,7 @@ struct W4Wave {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         i32x4 a[kMT];
-        read_x(ap + 16 * ((4 * j + gq) ^ r), a);
+        read_x(ap + 16 * ((4 * j + gq) ^ x_slot(r)), a);
         f32x4 xs[kMT];
         if constexpr (is_int4(kW)) {
 #pragma unroll
@@ -184,40 +189,47 @@ struct W4Wave {
         }
       }
     } else {
-      // MFMA j: the lane's k = 32 gq + 8 j.
+      // MFMA j: the lane's k = 32 gq + 8 j.  One accumulator after the other: four
+      // MFMAs that depend on each other would wait for each other.
       i32x4 a[4][kMT];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) read_x(ap + 16 * ((4 * gq + j) ^ r), a[j]);
+      for (int j = 0; j < 4; ++j) read_x(ap + 16 * ((4 * gq + j) ^ x_slot(r)), a[j]);
       f32x4 xs[kMT];
       if constexpr (is_int4(kW)) {
 #pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          xs[m] = f32x4{};
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) xs[m] = mfma_16x16x32<kX>(a[j][m], ones, xs[m]);
-          if constexpr (!kZ) xs[m] *= -8.0f;
+          for (int m = 0; m < kMT; ++m)
+            xs[m] = mfma_16x16x32<kX>(a[j][m], ones, j == 0 ? f32x4{} : xs[m]);
+        if constexpr (!kZ) {
+#pragma unroll
+          for (int m = 0; m < kMT; ++m) xs[m] *= -8.0f;
         }
       }
 #pragma unroll
       for (int n = 0; n < kNT; ++n) {
         const float c = scale_of<kS>(s[n]);
-        i32x4 b[4];
+        f32x4 p[kMT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          b[j] = decode8_exact<kX, kW>((uint32_t)q[n][j], kMode == kInline ? c : 1.0f);
+        for (int m = 0; m < kMT; ++m) {
+          if constexpr (kMode == kInline) p[m] = acc[n][m];
+          else if constexpr (kZ) p[m] = xs[m] * -(float)z[n];
+          else if constexpr (is_int4(kW)) p[m] = xs[m];
+          else p[m] = f32x4{};
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const i32x4 b = decode8_exact<kX, kW>((uint32_t)q[n][j], kMode == kInline ? c : 1.0f);
+#pragma unroll
+          for (int m = 0; m < kMT; ++m) p[m] = mfma_16x16x32<kX>(a[j][m], b, p[m]);
+        }
 #pragma unroll
         for (int m = 0; m < kMT; ++m) {
           if constexpr (kMode == kInline) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[n][m] = mfma_16x16x32<kX>(a[j][m], b[j], acc[n][m]);
+            acc[n][m] = p[m];
           } else {
-            f32x4 p = f32x4{};
-            if constexpr (kZ) p = xs[m] * -(float)z[n];
-            else if constexpr (is_int4(kW)) p = xs[m];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p = mfma_16x16x32<kX>(a[j][m], b[j], p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[n][m][e] = __builtin_fmaf(c, p[e], acc[n][m][e]);
+            for (int e = 0; e < 4; ++e) acc[n][m][e] = __builtin_fmaf(c, p[m][e], acc[n][m][e]);
           }
         }
       }
@@ -298,7 +310,7 @@ __global__ __launch_bounds__(256, 2) void k_w4_tile(W4Args g) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int row = 4 * (8 * wave + i) + (lane >> 4);
-        const int c = (lane & 15) ^ (row & 15);
+        const int c = (lane & 15) ^ x_slot(row);
         const int kc = k + 8 * c;
         dma16(xb, to + 1024 * (8 * wave + i), kc < g.K ? (uint32_t)row * ldx + 2 * kc : kOobOffset, 0);
       }
@@ -384,7 +396,7 @@ __global__ __launch_bounds__(256, 1) void k_w4_split(W4Args g) {
 #pragma unroll
       for (int i = 0; i < 4 * kMT; ++i) {
         const int row = 4 * i + (lane >> 4);
-        const int kc = k + 8 * ((lane & 15) ^ (row & 15));
+        const int kc = k + 8 * ((lane & 15) ^ x_slot(row));
         dma16(xb, to + 1024 * i, kc < g.K ? (uint32_t)row * ldx + 2 * kc : kOobOffset, 0);
       }
 #pragma unroll
