@@ -128,7 +128,7 @@ def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
         _bad("K and group_size must be multiples of 32")
     groups = -(-K // group_size)
     st = s_types.get(scales.dtype)
-    if st is None or tuple(scales.shape) != (N, groups):
+    if st is None or scales.shape != (N, groups):
         _bad(f"scales must be ({N}, {groups}) bfloat16, float16, float32 or uint8, "
              f"got {tuple(scales.shape)} {scales.dtype}")
     lds = scales.stride(0) if N > 1 else groups
@@ -154,7 +154,9 @@ def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
     if ot is None:
         _bad("out_dtype must be bfloat16, float16 or float32")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        # (a bare new_empty is the quickest there is, by 0.3 us of 8)
+        out = (x.new_empty((M, N)) if out_dtype is x.dtype else
+               x.new_empty((M, N), dtype=out_dtype))
     elif (out.dtype != out_dtype or tuple(out.shape) != (M, N) or not out.is_cuda
           or (N > 1 and out.stride(1) != 1)):
         _bad(f"out must be a ({M}, {N}) {out_dtype} device tensor with unit column stride")
@@ -196,8 +198,10 @@ def moe_route(logits, k: int, *, scoring: str = "softmax", renormalize: bool = T
     code = MOE_SCORING.get(scoring)
     if code is None:
         _bad(f"scoring must be one of {sorted(MOE_SCORING)}")
-    weights = torch.empty((T, max(k, 0)), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((T, max(k, 0)), dtype=torch.int32, device=logits.device)
+    shape = (T, k if k > 0 else 0)
+    weights = (logits.new_empty(shape) if kind == 0 else
+               logits.new_empty(shape, dtype=torch.float32))
+    ids = logits.new_empty(shape, dtype=torch.int32)
     _check(lib().hipgemm_moe_route(
         logits.data_ptr(), kind, T, E, k, logits.stride(0) if T > 1 else E, code,
         int(renormalize), scale, weights.data_ptr(), ids.data_ptr(),
