@@ -4,15 +4,17 @@
 // Ordering: logits become 32-bit keys whose unsigned order is theirs (-0 as +0,
 // NaN above infinity, -inf as 0: never chosen), kV of them in each of a token's
 // kL lanes, neighbours in one lane.  A round takes the lanes' maxima (three at a
-// time: v_max3_u32), reduces them over the kL lanes by DPP, finds the first lane
-// that has it (so equal logits go to the lowest expert) and clears it there;
-// lane j keeps the j-th result.  Weights are then computed once, in lanes 0 to
-// k - 1.
+// time: v_max3_u32), reduces them over the kL lanes by DPP and clears the key that
+// it found; lane j keeps the j-th result.  Equal logits go to the lowest expert:
+// keys of 16-bit logits hold it (and so say themselves whose they are), for fp32 it
+// is the first lane that has the maximum and its first value.  Weights are then
+// computed once, in lanes 0 to k - 1.
 //
 // What bounds it: one token is the latency of k rounds; many are instructions,
-// about 5 kV + 12 per round for 64 / kL tokens at once, so that a token's values
-// go to 16 lanes where there are tokens enough to fill the CUs (fewer exchanges
-// per value), to all 64 where there are not.
+// about 5 kV + 12 per round (16 bits: 3 kV + 12) for 64 / kL tokens at once, so
+// that a token's values go to 16 lanes where there are tokens enough to fill the CUs
+// (fewer exchanges per value), to all 64 where there are not.  us in a graph: one
+// token, 8 of 64, fp32 2.7; 16384 tokens, 8 of 256, bf16 7.2 (9.1 with fp32's keys).
 #include "hipgemm.h"
 
 #include "kernels.hpp"
@@ -35,6 +37,7 @@ struct RouteArgs {
   float scale;
 };
 
+// fp32: the key is the logit's alone.
 __device__ __forceinline__ uint32_t key_of(float f) {
   f += 0.0f;  // -0 -> +0
   uint32_t b = __builtin_bit_cast(uint32_t, f);
@@ -45,6 +48,29 @@ __device__ __forceinline__ uint32_t key_of(float f) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   const uint32_t b = key & 0x80000000u ? key & 0x7fffffffu : ~key;
   return key == 0u ? -__builtin_inff() : __builtin_bit_cast(float, b);
+}
+
+// 16 bits: the logit's order above, 0xffff - expert below, so that no two keys of a
+// token are equal but 0.
+template <int kType>
+__device__ __forceinline__ uint32_t key16_of(uint32_t b, int e) {
+  constexpr uint32_t kInf = kType == kInBf16 ? 0x7f80u : 0x7c00u;
+  const uint32_t mag = b & 0x7fffu;
+  const bool never = b == (0x8000u | kInf);
+  b = mag == 0u ? 0u : mag > kInf ? 0x7fffu : b;
+  b ^= b & 0x8000u ? 0xffffu : 0x8000u;
+  return never ? 0u : b << 16 | (0xffffu - (uint32_t)e);
+}
+template <int kType>
+__device__ __forceinline__ float value_of(uint32_t key) {
+  if constexpr (kType == kInF32) {
+    return value_of(key);
+  } else {
+    const uint32_t o = key >> 16, b = o & 0x8000u ? o & 0x7fffu : o ^ 0xffffu;
+    const float f = kType == kInBf16 ? __builtin_bit_cast(float, b << 16)
+                                     : (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+    return key == 0u ? -__builtin_inff() : f;
+  }
 }
 
 template <int kCtrl>
@@ -78,11 +104,9 @@ __device__ __forceinline__ float sum_lanes(float f) {
 }
 
 template <int kType>
-__device__ __forceinline__ float logit(const uint8_t* p, int i) {
-  if constexpr (kType == kInF32) return reinterpret_cast<const float*>(p)[i];
-  else if constexpr (kType == kInBf16)
-    return __builtin_bit_cast(float, (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << 16);
-  else return (float)reinterpret_cast<const _Float16*>(p)[i];
+__device__ __forceinline__ uint32_t key_at(const uint8_t* p, int i) {
+  if constexpr (kType == kInF32) return key_of(reinterpret_cast<const float*>(p)[i]);
+  else return key16_of<kType>(reinterpret_cast<const uint16_t*>(p)[i], i);
 }
 
 template <int kType, int kL, int kV>
@@ -103,18 +127,16 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs g) {
       if (in) v = *reinterpret_cast<const i32x4*>(p + (e0 + c * kPer) * kBytes);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        float f;
         // (an element goes through an integer: bit_cast of a vector element takes element 0)
-        if constexpr (kType == kInF32) f = __builtin_bit_cast(float, (uint32_t)v[i]);
-        else if constexpr (kType == kInBf16)
-          f = __builtin_bit_cast(float, (uint32_t)v[i / 2] << (i & 1 ? 0 : 16) & 0xffff0000u);
-        else f = (float)__builtin_bit_cast(_Float16, (uint16_t)((uint32_t)v[i / 2] >> (16 * (i & 1))));
-        key[c * kPer + i] = in ? key_of(f) : 0u;
+        uint32_t q;
+        if constexpr (kType == kInF32) q = key_of(__builtin_bit_cast(float, (uint32_t)v[i]));
+        else q = key16_of<kType>((uint32_t)v[i / 2] >> (16 * (i & 1)) & 0xffffu, e0 + c * kPer + i);
+        key[c * kPer + i] = in ? q : 0u;
       }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kV; ++i) key[i] = e0 + i < g.E ? key_of(logit<kType>(p, e0 + i)) : 0u;
+    for (int i = 0; i < kV; ++i) key[i] = e0 + i < g.E ? key_at<kType>(p, e0 + i) : 0u;
   }
 
   auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
@@ -130,34 +152,41 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs g) {
     if (j == 0) {
       top = best;
       if (!g.sigmoid && !g.renormalize) {
-        const float ref = value_of(top);
+        const float ref = value_of<kType>(top);
         float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kV; ++i) s += key[i] ? expf(value_of(key[i]) - ref) : 0.0f;
+        for (int i = 0; i < kV; ++i) s += key[i] ? expf(value_of<kType>(key[i]) - ref) : 0.0f;
         total = sum_lanes<kL>(s);
       }
     }
-    // The first lane of the group whose maximum it is, and its first value.
-    const uint64_t has = __builtin_amdgcn_ballot_w64(m == best);
-    const int base = lane_id() & ~(kL - 1);
-    const uint64_t in_group = kL == 64 ? has : (has >> base) & ((1ull << kL) - 1ull);
-    const int owner = __builtin_ctzll(in_group);
-    int at = 0;
+    int id;
+    if constexpr (kType == kInF32) {
+      // The first lane of the group whose maximum it is, and its first value.
+      const uint64_t has = __builtin_amdgcn_ballot_w64(m == best);
+      const int base = lane_id() & ~(kL - 1);
+      const uint64_t in_group = kL == 64 ? has : (has >> base) & ((1ull << kL) - 1ull);
+      const int owner = __builtin_ctzll(in_group);
+      int at = 0;
+  #pragma unroll
+      for (int i = kV - 1; i >= 0; --i) at = key[i] == best ? i : at;
+      const bool own = gl == owner;
+  #pragma unroll
+      for (int i = 0; i < kV; ++i) key[i] = own && at == i ? 0u : key[i];
+      id = owner * kV + __shfl(at, base + owner, kWave);
+    } else {
+      id = 0xffff - (int)(best & 0xffffu);
 #pragma unroll
-    for (int i = kV - 1; i >= 0; --i) at = key[i] == best ? i : at;
-    const bool own = gl == owner;
-#pragma unroll
-    for (int i = 0; i < kV; ++i) key[i] = own && at == i ? 0u : key[i];
-    const int id = owner * kV + __shfl(at, base + owner, kWave);
+      for (int i = 0; i < kV; ++i) key[i] = key[i] == best ? 0u : key[i];
+    }
     if (gl == j && best != 0u) {
       mine_key = best;
       mine_id = id;
     }
   }
 
-  const float v = value_of(mine_key);
+  const float v = value_of<kType>(mine_key);
   float w = 0.0f;
-  if (mine_id >= 0) w = g.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - value_of(top));
+  if (mine_id >= 0) w = g.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - value_of<kType>(top));
   if (g.renormalize) total = sum_lanes<kL>(w);
   w = mine_id >= 0 ? w / total * g.scale : 0.0f;
   if (live && gl < g.k) {
