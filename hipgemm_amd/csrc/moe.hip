@@ -117,22 +117,59 @@ bool matrix_ok(const hipgemm_moe_matrix& m, int rows, int K, const hipgemm_moe_d
   const bool e4m3 = d.format == HIPGEMM_W8_E4M3;
   const long long row = e4m3 ? K : K / 2;
   const long long groups = e4m3 ? 1 : (K + d.group_size - 1) / d.group_size;
-  return m.weight && m.scales && aligned(m.weight, 16) && m.ldw <= kMaxRow && m.lds <= kMaxRow &&
+  return m.weight && m.scales && aligned(m.weight, 16) && m.ldw <= kMaxRow &&
+         m.lds <= kMaxRow / type_bytes(d.scale_type) &&
          aligned(m.scales, type_bytes(d.scale_type)) && m.ldw >= row && m.ldw % 16 == 0 &&
          m.expert_w % 16 == 0 && (d.E == 1 || m.expert_w >= (rows - 1) * m.ldw + row) &&
          m.lds >= groups && (d.E == 1 || m.expert_s >= (rows - 1) * m.lds + groups) &&
          (!m.zeros || d.format == HIPGEMM_W4_INT4);
 }
 
-// Parts of F in the down product, of part_len (a multiple of 256).
-int down_parts(int T, int k, int E, int D, int F, int* part_len) {
-  const int chosen = T * k < E ? T * k : E;  // experts at most
-  const int tiles = chosen * ((D + 63) / 64), steps = (F + 255) / 256;
+// Experts that are chosen, if all are chosen alike.
+double chosen_experts(int T, int k, int E) {
+  return E * (1.0 - std::pow(1.0 - (k < E ? (double)k / E : 1.0), T));
+}
+
+// What a workgroup of the grouped kernels keeps in LDS is the same for all formats.
+template <int kMT, bool kLo>
+using AnyStream = Stream<kInBf16, kWE4M3, kInF32, kNone, kMT, kLo, 8, kMoeTables>;
+// Rows of x (of D elements) going up.
+int up_rows(int mt, int D) {
+  return mt == 2 ? AnyStream<2, false>::rows_that_fit(D) : AnyStream<1, false>::rows_that_fit(D);
+}
+// Elements of h going down, over all rows.
+int down_elems(int mt) {
+  return (mt == 2 ? AnyStream<2, true>::kElems : AnyStream<1, true>::kElems) / 2;
+}
+
+// Whether the grouped kernels take the sizes: a row of x in LDS going up, and going
+// down no more parts than 64.
+bool grouped(int D, int F) { return up_rows(1, D) >= 1 && F <= 1 << 16; }
+
+// The down product: tiles of 16 rows of h per group, and parts of F, of len (a
+// multiple of 256).
+struct DownPlan {
+  int mt, parts, len;
+};
+DownPlan down_plan(int T, int k, int E, int D, int F) {
+  const int pairs = T * k, steps = (F + 255) / 256;
+  // Parts so short that the rows of an expert, up to half as many again as there are on
+  // average, lie in LDS together: its weights are read once for them.  Not below
+  // 1024, and of 32 rows only where more than 16 fit.
+  const double rows = std::ceil(1.5 * pairs / chosen_experts(T, k, E));
+  int mt = pairs > 12 * E ? 2 : 1, fit;
+  for (;; mt = 1) {
+    fit = (int)(down_elems(mt) / (rows < 16 * mt ? rows : 16 * mt)) / 256;
+    if (fit < 4) fit = 4;
+    if (mt == 1 || down_elems(2) / (256 * (fit < steps ? fit : steps)) > 16) break;
+  }
+  const int chosen = pairs < E ? pairs : E;  // experts at most
+  const int tiles = chosen * ((D + 63) / 64);
   int parts = tiles >= 512 ? 1 : (512 + tiles - 1) / tiles;
   if (parts > (steps + 7) / 8) parts = (steps + 7) / 8;
+  if (parts < (steps + fit - 1) / fit) parts = (steps + fit - 1) / fit;
   const int len = (steps + parts - 1) / parts;
-  *part_len = 256 * len;
-  return (steps + len - 1) / len;
+  return {mt, (steps + len - 1) / len, 256 * len};
 }
 
 hipError_t launch(const void* fn, dim3 grid, int threads, MoeArgs& g, hipStream_t stream) {
@@ -179,18 +216,21 @@ hipError_t vec_turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
 
 hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   const int pairs = g.T * g.k;
-  // Experts chosen at all, if all are chosen alike.
-  const double chosen = g.E * (1.0 - std::pow(1.0 - (g.k < g.E ? (double)g.k / g.E : 1.0), g.T));
+  const double chosen = chosen_experts(g.T, g.k, g.E);
   // Pair by pair while few experts are read twice.  us in a graph, pairs / grouped,
   // by tokens: int4, 8 of 64 experts of 2048 x 1024, 2 24/37, 6 55/58, 12 87/73; 8 of
   // 128 of 4096 x 1536, 4 71/90, 8 124/140, 16 237/175;  fp4, 3 of 30 of 2336 x 1056,
   // 5 24/44, 12 43/56;  e4m3, 4 of 64 of 4096 x 2048, 2 41/51, 4 71/80, 8 126/115; 2
   // of 8 of 4096 x 14336, 1 66/71, 2 121/116.  (Grouped, 4-bit weights stream at 3 to
   // 4.6 TB/s, e4m3 ones at 5 to 5.8.)
-  if (pairs <= chosen * (d.format == HIPGEMM_W8_E4M3 ? 1.13 : 1.5)) return vec_turn(g, d, stream);
-  // Tiles of 16 tokens, two at a time where experts have more on average.
-  const int mt = pairs > 12 * g.E ? 2 : 1;
-  g.parts = down_parts(g.T, g.k, g.E, g.D, g.F, &g.part_len);
+  if (!grouped(g.D, g.F) || pairs <= chosen * (d.format == HIPGEMM_W8_E4M3 ? 1.13 : 1.5))
+    return vec_turn(g, d, stream);
+  // Tiles of 16 tokens, two at a time where experts have more on average and more
+  // rows than with one fit in LDS (sums of two tiles take room from them).
+  const int mt = pairs > 12 * g.E && up_rows(2, g.D) > up_rows(1, g.D) ? 2 : 1;
+  const DownPlan down = down_plan(g.T, g.k, g.E, g.D, g.F);
+  g.parts = down.parts;
+  g.part_len = down.len;
   // Tiles of 128 rows with two waves to a row's K where each CU has ten or more of
   // them (fewer ends of tiles per byte), of 32 rows with eight where not.
   const int wku = chosen * g.F / 64 >= 2560 ? 2 : 8;
@@ -201,7 +241,7 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
                         dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   e = launch(hk::moe_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type,
-                          mode_of(kInBf16, d.format, d.scale_type, d.group_size), mt, wkd),
+                          mode_of(kInBf16, d.format, d.scale_type, d.group_size), down.mt, wkd),
              dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   return launch((const void*)&k_moe_sum, dim3((unsigned)((g.T * (g.D / 4) + 255) / 256)), 256, g,
@@ -213,11 +253,10 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
 extern "C" size_t hipgemm_moe_workspace_size(int T, int k, int E, int D, int F) {
   if (T <= 0 || k <= 0 || k > 64 || E <= 0 || D <= 0 || F <= 0) return 0;
   const int t = turn_tokens(T, k);
-  int len;
   // (a last turn of fewer tokens can have more parts)
   size_t o = 0;
   for (int u : {t, T % t}) {
-    const size_t n = u == 0 ? 0 : (size_t)down_parts(u, k, E, D, F, &len) * u * k;
+    const size_t n = u == 0 || !grouped(D, F) ? 0 : (size_t)down_plan(u, k, E, D, F).parts * u * k;
     if (n > o) o = n;
   }
   return (size_t)t * k * F * 4 + o * D * 4;

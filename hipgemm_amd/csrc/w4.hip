@@ -64,7 +64,7 @@ bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p)
 
 constexpr int kMaxK = 1 << 26;
 constexpr long long kMaxTileRow = 1 << 23;  // 128 rows' bytes in a buffer's range
-constexpr long long kMaxRow = 1 << 25;      // 64 rows' bytes
+constexpr long long kMaxRow = 1 << 25;      // 64 rows' bytes in a buffer's range
 
 template <class Args>
 hipError_t launch(const void* fn, dim3 grid, int threads, Args& g, hipStream_t stream) {
@@ -205,7 +205,7 @@ extern "C" hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc* desc, hipStream_t s
         !aligned(d.scales, type_bytes(d.scale_type)))
       return hipErrorInvalidValue;
     if (d.ldx < d.K || d.ldx % 8 != 0 || d.ldw < d.K / 2 || d.ldw % 16 != 0 ||
-        d.ldw > kMaxRow || d.lds > kMaxRow ||
+        d.ldw > kMaxRow || d.lds > kMaxRow / type_bytes(d.scale_type) ||
         d.lds < (d.K + d.group_size - 1) / d.group_size)
       return hipErrorInvalidValue;
   }

@@ -377,7 +377,7 @@ hipError_t hipgemm_quantize_rows_e4m3(const void *x, int type, int M, int K,
  * Rows of x, q, scales and zeros are contiguous, with the strides given.
  * Requirements: K % 32 == 0, K <= 2^26, G % 32 == 0, x and q 16-byte aligned
  * with strides of a multiple of 16 bytes, the others aligned to their element;
- * out_dtype BF16, F16 or F32; ldw and lds up to 2^25.  M == 0 or N == 0 is a
+ * out_dtype BF16, F16 or F32; ldw and lds up to 2^25 bytes.  M == 0 or N == 0 is a
  * no-op, K == 0 gives activation(bias).  One launch on `stream` (one per four rows
  * where K == 0 or ldx > 2^24), no workspace.  Zero-initialise the struct and set
  * `size`.  No reference counterpart (the reference has e4m3 operands only).

@@ -213,6 +213,17 @@ def test_other_stream_graph_and_workspace(hg):
         assert torch.equal(y, ref)
 
 
+# Sizes of which a workgroup's LDS holds few rows, or none: many tokens of wide
+# experts, parts of F, and the way pair by pair beyond.
+@pytest.mark.parametrize("fmt", ["e4m3", "int4"])
+@pytest.mark.parametrize("T,E,k,D,F", [(16, 2, 1, 256, 14336), (40, 2, 1, 96, 14368),
+                                       (7, 2, 2, 64, 18592), (5, 1, 1, 128, 65568),
+                                       (33, 2, 2, 8192, 64), (20, 1, 1, 28960, 32),
+                                       (6, 1, 1, 37120, 32), (6, 1, 1, 37152, 32)])
+def test_wide(hg, T, E, k, D, F, fmt):
+    check(hg, make(T + F, T, E, k, D, F, fmt, zeros=fmt == "int4"), fmt)
+
+
 def test_repeats_are_equal(hg):
     for T in (1, 64):
         a = make(T, T, 24, 6, 512, 384, "fp4")
