@@ -47,11 +47,11 @@ struct MoeArgs {
   int waves_k, rows, wave_rows;  // k_moe_vec_*: of a workgroup, of a wave
 };
 
-// One value of h, in two parts (an infinite one has no rest).
+// One value of h, in two parts (one that is infinite, or in bf16, has no rest).
 __device__ __forceinline__ void store_h(const MoeArgs& g, int pair, int f, float v) {
   const __bf16 hi = (__bf16)v;
   const float rest = v - (float)hi;
-  const __bf16 lo = (__bf16)(rest == rest ? rest : 0.0f);
+  const __bf16 lo = (__bf16)(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.0f);
   uint16_t* h = g.h + (long long)pair * 2 * g.F + f;
   h[0] = __builtin_bit_cast(uint16_t, hi);
   h[g.F] = __builtin_bit_cast(uint16_t, lo);

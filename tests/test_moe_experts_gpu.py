@@ -224,6 +224,22 @@ def test_wide(hg, T, E, k, D, F, fmt):
     check(hg, make(T + F, T, E, k, D, F, fmt, zeros=fmt == "int4"), fmt)
 
 
+def test_h_next_to_the_largest(hg):
+    """A gate times up that is finite in fp32 and infinite in bf16 gives an
+    infinity, no NaN."""
+    a = make(5, 4, 2, 2, 32, 32)
+    a["x"].fill_(1.0)
+    for n in ("w13", "w2"):
+        a[n].copy_(torch.ones_like(a[n], dtype=torch.float32))
+    a["scales13"].fill_(float((2.0 ** 128 * (1 - 2.0 ** -12)) ** 0.5 / 32))
+    a["scales2"].fill_(1.0)
+    a["weights"].fill_(1.0)
+    for T in (1, 4):  # pair by pair, grouped
+        y = hg.moe_experts(a["x"][:T], a["ids"][:T], a["weights"][:T], a["w13"], a["scales13"],
+                           a["w2"], a["scales2"], activation=None)
+        assert bool((y == float("inf")).all())
+
+
 def test_repeats_are_equal(hg):
     for T in (1, 64):
         a = make(T, T, 24, 6, 512, 384, "fp4")
