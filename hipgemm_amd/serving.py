@@ -11,6 +11,7 @@ None of them records a gradient.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 
@@ -78,13 +79,10 @@ def _stream_handle(t, stream) -> int:
     return _torch()._C._cuda_getCurrentRawStream(t.get_device())
 
 
-def _scratch(nbytes: int, device, stream):
-    """Scratch memory for one call on `stream` (None: the current one)."""
-    torch = _torch()
-    if stream is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+def _on(stream):
+    """Memory that is allocated here belongs to `stream` (None: the current one):
+    what the current stream has freed and may still read is not written over."""
+    return contextlib.nullcontext() if stream is None else _torch().cuda.stream(stream)
 
 
 def w4_gemm_raw(desc: "W4Desc", stream: int = 0) -> int:
@@ -139,8 +137,9 @@ def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
         if zeros.dtype != torch.uint8 or zeros.shape != scales.shape or not zeros.is_cuda:
             _bad("zeros must be uint8 of the shape of scales, on the GPU")
         if zeros.stride() != scales.stride() and zeros.numel() > 1:
-            zeros = torch.empty_strided(scales.shape, scales.stride(), dtype=torch.uint8,
-                                        device=zeros.device).copy_(zeros)
+            with _on(stream):
+                zeros = torch.empty_strided(scales.shape, scales.stride(), dtype=torch.uint8,
+                                            device=zeros.device).copy_(zeros)
         zp = zeros.data_ptr()
     if not (x.is_cuda and weight.is_cuda and scales.is_cuda):
         _bad("x, weight and scales must be device tensors")
@@ -155,8 +154,12 @@ def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
         _bad("out_dtype must be bfloat16, float16 or float32")
     if out is None:
         # (a bare new_empty is the quickest there is, by 0.3 us of 8)
-        out = (x.new_empty((M, N)) if out_dtype is x.dtype else
-               x.new_empty((M, N), dtype=out_dtype))
+        if stream is None:
+            out = (x.new_empty((M, N)) if out_dtype is x.dtype else
+                   x.new_empty((M, N), dtype=out_dtype))
+        else:
+            with _on(stream):
+                out = x.new_empty((M, N), dtype=out_dtype)
     elif (out.dtype != out_dtype or tuple(out.shape) != (M, N) or not out.is_cuda
           or (N > 1 and out.stride(1) != 1)):
         _bad(f"out must be a ({M}, {N}) {out_dtype} device tensor with unit column stride")
@@ -199,9 +202,14 @@ def moe_route(logits, k: int, *, scoring: str = "softmax", renormalize: bool = T
     if code is None:
         _bad(f"scoring must be one of {sorted(MOE_SCORING)}")
     shape = (T, k if k > 0 else 0)
-    weights = (logits.new_empty(shape) if kind == 0 else
-               logits.new_empty(shape, dtype=torch.float32))
-    ids = logits.new_empty(shape, dtype=torch.int32)
+    if stream is None:
+        weights = (logits.new_empty(shape) if kind == 0 else
+                   logits.new_empty(shape, dtype=torch.float32))
+        ids = logits.new_empty(shape, dtype=torch.int32)
+    else:
+        with _on(stream):
+            weights = logits.new_empty(shape, dtype=torch.float32)
+            ids = logits.new_empty(shape, dtype=torch.int32)
     _check(lib().hipgemm_moe_route(
         logits.data_ptr(), kind, T, E, k, logits.stride(0) if T > 1 else E, code,
         int(renormalize), scale, weights.data_ptr(), ids.data_ptr(),
@@ -304,13 +312,15 @@ def moe_experts(x, ids, weights, w13, scales13, w2, scales2, *, zeros13=None,
     if ot is None:
         _bad("out_dtype must be bfloat16, float16 or float32")
     if out is None:
-        out = torch.empty((T, D), dtype=out_dtype, device=x.device)
+        with _on(stream):
+            out = torch.empty((T, D), dtype=out_dtype, device=x.device)
     elif (out.dtype != out_dtype or tuple(out.shape) != (T, D) or not out.is_cuda
           or out.stride(1) != 1):
         _bad(f"out must be a ({T}, {D}) {out_dtype} device tensor with unit column stride")
     need = _moe_ws_bytes(T, k, E, D, F)
     if workspace is None:
-        workspace = _scratch(need, x.device, stream)
+        with _on(stream):
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
     elif workspace.dtype != torch.uint8 or not workspace.is_cuda \
             or not workspace.is_contiguous() or workspace.numel() < need:
         _bad(f"workspace must be a contiguous uint8 device tensor of {need} bytes")

@@ -213,6 +213,28 @@ def test_other_stream_graph_and_workspace(hg):
         assert torch.equal(y, ref)
 
 
+def test_results_belong_to_the_stream(hg):
+    """Without `out`, results (and an experts' call's workspace) are memory of the
+    stream that writes them, not what the current stream has just freed."""
+    a = make(3, 4, 16, 4, 256, 128, "int4", zeros=True)
+    wide = a["zeros13"][0].t().contiguous().t()  # (of other strides: copied)
+    want = (hg.moe_experts(**a, format="int4"), *hg.moe_route(a["x"][:, :16], 4),
+            hg.w4_gemm(a["x"], a["w13"][0], a["scales13"][0], wide))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = (hg.moe_experts(**a, format="int4", stream=side),
+           *hg.moe_route(a["x"][:, :16], 4, stream=side),
+           hg.w4_gemm(a["x"], a["w13"][0], a["scales13"][0], wide, stream=side))
+    torch.cuda.synchronize()
+    segments = torch.cuda.memory_snapshot()
+    for x, y in zip(want, got):
+        assert torch.equal(x, y)
+        p = y.data_ptr()
+        owner = [s["stream"] for s in segments
+                 if s["address"] <= p < s["address"] + s["total_size"]]
+        assert owner == [side.cuda_stream]
+
+
 # Sizes of which a workgroup's LDS holds few rows, or none: many tokens of wide
 # experts, parts of F, and the way pair by pair beyond.
 @pytest.mark.parametrize("fmt", ["e4m3", "int4"])
