@@ -223,7 +223,16 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   // 5 24/44, 12 43/56;  e4m3, 4 of 64 of 4096 x 2048, 2 41/51, 4 71/80, 8 126/115; 2
   // of 8 of 4096 x 14336, 1 66/71, 2 121/116.  (Grouped, 4-bit weights stream at 3 to
   // 4.6 TB/s, e4m3 ones at 5 to 5.8.)
-  if (!grouped(g.D, g.F) || pairs <= chosen * (d.format == HIPGEMM_W8_E4M3 ? 1.13 : 1.5))
+  // And while what is read again is less than 64 MB: grouping is a third launch and
+  // the tables.  Pairs / grouped, MB: e4m3 10 tokens, 1 of 24 of 384 x 640, 1, 9.8/20;
+  // 2, 7 of 24 of 768 x 1536, 7, 18.6/30;  int4 3, 3 of 4 of 1536 x 384, 4, 12/24;  64, 2
+  // of 4 of 256 x 512, 24, 16/29;  e4m3 64, 4 of 8 of 256 x 256, 49, 12.5/31;  fp4 10,
+  // 5 of 16 of 4096 x 256, 54, 34/28;  32, 4 of 64 of 1024 x 512, 57, 29/36;  e4m3 41, 1
+  // of 16 of 1024 x 896, 72, 28.5/26;  int4 64, 8 of 128 of 512 x 512, 152, 50/38.
+  const bool e4m3 = d.format == HIPGEMM_W8_E4M3;
+  const double expert_bytes = 3.0 * g.D * g.F * (e4m3 ? 1.0 : 0.5);
+  if (!grouped(g.D, g.F) || pairs <= chosen * (e4m3 ? 1.13 : 1.5) ||
+      (pairs - chosen) * expert_bytes <= 64e6)
     return vec_turn(g, d, stream);
   // Tiles of 16 tokens, two at a time where experts have more on average and more
   // rows than with one fit in LDS (sums of two tiles take room from them).
@@ -232,9 +241,14 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   g.parts = down.parts;
   g.part_len = down.len;
   // Tiles of 128 rows with two waves to a row's K where each CU has ten or more of
-  // them (fewer ends of tiles per byte), of 32 rows with eight where not.
-  const int wku = chosen * g.F / 64 >= 2560 ? 2 : 8;
-  const int wkd = chosen * g.D / 128 * g.parts >= 2560 ? 2 : 8;
+  // them (fewer ends of tiles per byte), of 32 rows with eight where not, unless K is
+  // no more than one unit for each of the eight: most would wait (us, eight / two:
+  // fp4 320 x 6272, 6 of 12, 26 tokens 73/51;  int4 2048 x 1024, 8 of 64, 64 tokens
+  // 85/64;  e4m3 1024 x 512, 8 of 128, 64 tokens 64/53;  beyond, e4m3 4096 x 4096, 2 of
+  // 8, 16 tokens 82/91, 4096 x 2048, 4 of 64, 177/187).
+  const int short_k = 8 * (e4m3 ? 128 : 256);
+  const int wku = chosen * g.F / 64 >= 2560 || g.D <= short_k ? 2 : 8;
+  const int wkd = chosen * g.D / 128 * g.parts >= 2560 || g.part_len <= short_k ? 2 : 8;
   const int cus = 256;
   hipError_t e = launch(hk::moe_up(d.x_type, d.w13.zeros ? kWInt4Z : d.format, d.scale_type,
                                    mode_of(d.x_type, d.format, d.scale_type, d.group_size), mt, wku),
