@@ -90,7 +90,11 @@ bool by_tiles(const hipgemm_w4_desc& d) {
 
 // k_w4_split: groups of up to 64 rows of even lengths, and 32 columns where that
 // leaves a workgroup for each CU (16 rows, 4096 x 4096: 9.8 us for 13.4;  14336 x
-// 4096, 448 tiles: 19.6 for 16.0).
+// 4096, 448 tiles: 19.6 for 16.0).  Groups are halved while each CU still takes at
+// most one such tile: weights are decoded once more, by CUs that had nothing to do
+// (us, not halved / halved, int4: 64 x 256 x 8192 24.0/13.8, 256 x 512 x 8192
+// 25.3/16.3, 37 x 2048 x 4096 12.1/9.5, 64 x 4096 x 4096 16.3/13.0, 703 x 256 x 22144
+// 105/70, 128 x 512 x 512 6.5/4.8;  fp4 512 x 512 x 4096 15.9/12.9).
 struct SplitPlan {
   int mt, nt;
   long long tiles;
@@ -99,8 +103,11 @@ SplitPlan split_plan(int M, int N) {
   SplitPlan p;
   const int groups = (M + 63) / 64;
   p.mt = ((M + groups - 1) / groups + 15) / 16;
-  const long long tm = (M + 16 * p.mt - 1) / (16 * p.mt);
-  p.nt = tm * ((N + 31) / 32) <= 256 ? 2 : 4;
+  auto groups_of = [M](int mt) { return (long long)((M + 16 * mt - 1) / (16 * mt)); };
+  const long long narrow = (N + 31) / 32;
+  while (p.mt > 1 && groups_of((p.mt + 1) / 2) * narrow <= 256) p.mt = (p.mt + 1) / 2;
+  const long long tm = groups_of(p.mt);
+  p.nt = tm * narrow <= 256 ? 2 : 4;
   p.tiles = tm * ((N + 16 * p.nt - 1) / (16 * p.nt));
   return p;
 }

@@ -66,6 +66,16 @@ def test_shapes(hg, M, N, K, fmt):
     case(hg, M, N, K, fmt, zeros=fmt == "int4" and N % 2 == 0, seed=M + N + K)
 
 
+# Columns enough for tiles of 32, 48 and 64 rows, of 32 columns and of 64.
+@pytest.mark.parametrize("M,N", [(20, 4104), (37, 5000), (20, 8200), (40, 8200), (64, 4100),
+                                 (64, 8216), (90, 8200)])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("fmt,scale", [("int4", "bfloat16"), ("fp4", "e8m0"), ("fp4", "float16")])
+def test_tall_tiles(hg, M, N, group, fmt, scale):
+    for dtype, zeros in (("bfloat16", False), ("float16", fmt == "int4")):
+        case(hg, M, N, 1120, fmt, group, scale, zeros, dtype, seed=M + N)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("scale", ["bfloat16", "float16", "float32", "e8m0"])
 @pytest.mark.parametrize("group", [32, 64, 96, 128, 256, 4096])
