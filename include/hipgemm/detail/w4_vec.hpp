@@ -110,33 +110,43 @@ struct Vec {
     odd = kGroups && __builtin_amdgcn_ballot_w64(any) != 0;
   }
 
-  // Rows row to below end of a matrix of `row_bytes`-byte rows (zeros past end).
+  // v, of which the compiler holds nothing that it computed from it before.
+  __device__ __forceinline__ static uint32_t anew(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+  }
+
+  // Rows row to below end of a matrix, zeros past end.  Rows are stepped by the lane's
+  // offset, which the range check sees, not by the scalar one, which it may leave
+  // out: nothing past the matrix' last row is asked of memory.  The sums are made
+  // anew at every step (held over the loop they cost 14 registers and with them a
+  // wave per SIMD: 15 pairs of fp4 2336 x 1056 25.7 us for HELD).
   __device__ __forceinline__ void load(Rows& r, const uint8_t* w, long long ldw, const uint8_t* s,
                                        long long lds, const uint8_t* z, long long ldz, int row,
                                        int end) const {
     const int left = max(min(end - row, kStep), 0), rl = lane_id() / kLk;
     const auto wb = make_rsrc(w + row * ldw, (uint32_t)(left * ldw));
-    const uint32_t wo = in ? (uint32_t)(rl * ldw) + (kW == kWE4M3 ? k : k >> 1) : kOobOffset;
+    const uint32_t wo = anew(in ? (uint32_t)(rl * ldw) + (kW == kWE4M3 ? k : k >> 1) : kOobOffset);
 #pragma unroll
     for (int i = 0; i < kVecRows; ++i)
-      r.w[i] = __builtin_amdgcn_raw_buffer_load_b128(wb, wo, (uint32_t)(i * kPer * ldw), kStoreC);
+      r.w[i] = __builtin_amdgcn_raw_buffer_load_b128(wb, wo + (uint32_t)(i * kPer * ldw), 0, kStoreC);
     {
       const auto sb = make_rsrc(s + row * lds, (uint32_t)(left * lds));
-      const uint32_t so = (uint32_t)(rl * lds) + grp * type_bytes(kS);
+      const uint32_t so = anew((uint32_t)(rl * lds) + grp * type_bytes(kS));
 #pragma unroll
       for (int i = 0; i < kVecRows; ++i) {
-        const uint32_t at = (uint32_t)(i * kPer * lds);
-        if constexpr (type_bytes(kS) == 4) r.s[i] = __builtin_amdgcn_raw_buffer_load_b32(sb, so, at, 0);
+        const uint32_t at = so + (uint32_t)(i * kPer * lds);
+        if constexpr (type_bytes(kS) == 4) r.s[i] = __builtin_amdgcn_raw_buffer_load_b32(sb, at, 0, 0);
         else if constexpr (type_bytes(kS) == 2)
-          r.s[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sb, so, at, 0);
-        else r.s[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(sb, so, at, 0);
+          r.s[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sb, at, 0, 0);
+        else r.s[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(sb, at, 0, 0);
       }
       if constexpr (kW == kWInt4Z) {
         const auto zb = make_rsrc(z + row * ldz, (uint32_t)(left * ldz));
-        const uint32_t zo = (uint32_t)(rl * ldz) + grp;
+        const uint32_t zo = anew((uint32_t)(rl * ldz) + grp);
 #pragma unroll
         for (int i = 0; i < kVecRows; ++i)
-          r.z[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zb, zo, (uint32_t)(i * kPer * ldz), 0);
+          r.z[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(zb, zo + (uint32_t)(i * kPer * ldz), 0, 0);
       }
     }
   }
