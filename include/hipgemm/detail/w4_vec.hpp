@@ -120,7 +120,7 @@ struct Vec {
   // offset, which the range check sees, not by the scalar one, which it may leave
   // out: nothing past the matrix' last row is asked of memory.  The sums are made
   // anew at every step (held over the loop they cost 14 registers and with them a
-  // wave per SIMD: 15 pairs of fp4 2336 x 1056 25.7 us for HELD).
+  // wave per SIMD: 15 pairs of fp4 2336 x 1056 took 25.7 us for 23.5).
   __device__ __forceinline__ void load(Rows& r, const uint8_t* w, long long ldw, const uint8_t* s,
                                        long long lds, const uint8_t* z, long long ldz, int row,
                                        int end) const {
