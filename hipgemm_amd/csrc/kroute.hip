@@ -184,9 +184,17 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs g) {
     }
   }
 
-  const float v = value_of<kType>(mine_key);
+  // Sigmoids that are divided by their sum, of a token whose logits are all negative:
+  // each times exp(-max), which the division takes out again.  By themselves they
+  // would all be 0 below -88, and 0 / 0 no weight.
+  const float v = value_of<kType>(mine_key), ref = value_of<kType>(top);
+  const bool sigmoid = g.sigmoid && !(g.renormalize && ref < 0.0f);
   float w = 0.0f;
-  if (mine_id >= 0) w = g.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - value_of<kType>(top));
+  if (mine_id >= 0) {
+    w = expf(sigmoid ? -v : v - ref);
+    if (sigmoid) w = 1.0f / (1.0f + w);
+    else if (g.sigmoid) w /= 1.0f + expf(v);
+  }
   if (g.renormalize) total = sum_lanes<kL>(w);
   w = mine_id >= 0 ? w / total * g.scale : 0.0f;
   if (live && gl < g.k) {
