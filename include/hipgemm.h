@@ -373,7 +373,10 @@ hipError_t hipgemm_quantize_rows_e4m3(const void *x, int type, int M, int K,
  * low nibble of byte i of a row; one scale s (and zero point z, a byte, 8 where
  * zeros is NULL) per G = group_size neighbouring elements of a row, N x
  * ceil(K / G).  Products and sums are fp32 and the weights are not rounded: the
- * scale multiplies the fp32 sum over its group.  bias: N floats or NULL.
+ * scale multiplies the fp32 sum over its group.  Results that come out infinite or
+ * NaN are computed again term by term, unless their row of x holds a NaN: rows of NaN
+ * cost about three times the call, rows with an infinity up to 100 times (M > 4).
+ * bias: N floats or NULL.
  * Rows of x, q, scales and zeros are contiguous, with the strides given.
  * Requirements: K % 32 == 0, K <= 2^26, G % 32 == 0, x and q 16-byte aligned
  * with strides of a multiple of 16 bytes, the others aligned to their element;
