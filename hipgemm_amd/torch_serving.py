@@ -194,6 +194,8 @@ class W4Linear(torch.nn.Module):
                    format, group_size, activation)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.in_features:
+            raise HipGemmError(f"x must have {self.in_features} features, got {tuple(x.shape)}")
         x2 = x.reshape(-1, self.in_features)
         kw = dict(format=self.format, group_size=self.group_size, bias=self.bias,
                   activation=self.activation)
