@@ -13,7 +13,8 @@ Importing this module registers, in the ``hipgemm`` namespace:
                                 group_size=128, activation="silu",
                                 out_dtype=None)
 
-with the arguments and rules of the functions of the same names, and fake (meta)
+with the arguments and rules of the functions of the same names (but an x of any
+strides and alignment, which is copied where it has to be), and fake (meta)
 implementations, so that they trace under torch.compile, torch.export and
 FakeTensorMode.  They may be captured in CUDA graphs.  CPU tensors raise
 HipGemmError: there is no CPU path.  They record no gradient.
@@ -36,13 +37,22 @@ from .torch_ops import _plain_buffers, _plain_eager, quantize_rows
 __all__ = ["w4_gemm", "moe_route", "moe_experts", "quantize_w4", "W4Linear", "MoE"]
 
 
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x where its rows are as the kernels take them (unit stride, on 16 bytes), else
+    a copy: views of any strides are what a Linear is given."""
+    if (x.dim() == 2 and x.stride(1) == 1 and x.data_ptr() % 16 == 0 and
+            (x.shape[0] <= 1 or (x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1]))):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
 @torch.library.custom_op("hipgemm::w4_gemm", mutates_args=())
 def w4_gemm(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor,
             zeros: Optional[torch.Tensor] = None, format: str = "int4",
             group_size: int = 128, bias: Optional[torch.Tensor] = None,
             activation: str = "none",
             out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    return serving.w4_gemm(x, weight, scales, zeros, format=format,
+    return serving.w4_gemm(_rows(x), weight, scales, zeros, format=format,
                            group_size=group_size, bias=bias,
                            activation=activation, out_dtype=out_dtype)
 
@@ -87,7 +97,7 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
                 zeros2: Optional[torch.Tensor] = None, format: str = "e4m3",
                 group_size: int = 128, activation: str = "silu",
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    return serving.moe_experts(x, ids, weights, w13, scales13, w2, scales2,
+    return serving.moe_experts(_rows(x), ids, weights, w13, scales13, w2, scales2,
                                zeros13=zeros13, zeros2=zeros2, format=format,
                                group_size=group_size, activation=activation,
                                out_dtype=out_dtype)
@@ -202,7 +212,7 @@ class W4Linear(torch.nn.Module):
         # (as in Fp8Linear: the call itself where nothing watches the operations)
         if _plain_eager(x2) and _plain_buffers(self.weight, self.scales, self.zeros,
                                                self.bias):
-            y = serving.w4_gemm(x2, self.weight, self.scales, self.zeros, **kw)
+            y = serving.w4_gemm(_rows(x2), self.weight, self.scales, self.zeros, **kw)
         else:
             y = torch.ops.hipgemm.w4_gemm(x2, self.weight, self.scales, self.zeros, **kw)
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.out_features)
@@ -251,12 +261,15 @@ class MoE(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x2 = x.reshape(-1, x.shape[-1])
+        experts = (self.w13, self.scales13, self.w2, self.scales2)
+        plain = _plain_eager(x2) and _plain_buffers(self.gate, *experts)
+        if plain:
+            x2 = _rows(x2)
         logits = torch.nn.functional.linear(x2.to(self.gate.dtype), self.gate)
         route = dict(scoring=self.scoring, renormalize=self.renormalize, scale=self.scale)
         kw = dict(format=self.format, group_size=self.group_size,
                   activation=self.activation)
-        experts = (self.w13, self.scales13, self.w2, self.scales2)
-        if _plain_eager(x2) and _plain_buffers(self.gate, *experts):
+        if plain:
             weights, ids = serving.moe_route(logits, self.k, **route)
             y = serving.moe_experts(x2, ids, weights, *experts, **kw)
         else:
