@@ -148,6 +148,10 @@ def lib() -> ctypes.CDLL:
     L.hipgemm_quantize_rows_e4m3.restype = ci
     L.hipgemm_w4_gemm.argtypes = [ctypes.c_void_p, vp]
     L.hipgemm_w4_gemm.restype = ci
+    L.hipgemm_w4_select.argtypes = [vp, vp]
+    L.hipgemm_w4_select.restype = ci
+    L.hipgemm_moe_select.argtypes = [ci, ci, ci, ci, ci, ci, vp]
+    L.hipgemm_moe_select.restype = ci
     L.hipgemm_moe_experts.argtypes = [vp, vp]
     L.hipgemm_moe_experts.restype = ci
     L.hipgemm_moe_workspace_size.argtypes = [ci, ci, ci, ci, ci]

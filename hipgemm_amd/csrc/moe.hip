@@ -214,9 +214,10 @@ hipError_t vec_turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
                 kWave * ((items + turns - 1) / turns), g, stream);
 }
 
-hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
-  const int pairs = g.T * g.k;
-  const double chosen = chosen_experts(g.T, g.k, g.E);
+// The kernels of a turn.
+hipgemm_moe_plan turn_plan(int T, int k, int E, int D, int F, int format) {
+  const int pairs = T * k;
+  const double chosen = chosen_experts(T, k, E);
   // Pair by pair while few experts are read twice.  us in a graph, pairs / grouped,
   // by tokens: int4, 8 of 64 experts of 2048 x 1024, 2 24/37, 6 55/58, 12 87/73; 8 of
   // 128 of 4096 x 1536, 4 71/90, 8 124/140, 16 237/175;  fp4, 3 of 30 of 2336 x 1056,
@@ -229,17 +230,15 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   // of 4 of 256 x 512, 24, 16/29;  e4m3 64, 4 of 8 of 256 x 256, 49, 12.5/31;  fp4 10,
   // 5 of 16 of 4096 x 256, 54, 34/28;  32, 4 of 64 of 1024 x 512, 57, 29/36;  e4m3 41, 1
   // of 16 of 1024 x 896, 72, 28.5/26;  int4 64, 8 of 128 of 512 x 512, 152, 50/38.
-  const bool e4m3 = d.format == HIPGEMM_W8_E4M3;
-  const double expert_bytes = 3.0 * g.D * g.F * (e4m3 ? 1.0 : 0.5);
-  if (!grouped(g.D, g.F) || pairs <= chosen * (e4m3 ? 1.13 : 1.5) ||
+  const bool e4m3 = format == HIPGEMM_W8_E4M3;
+  const double expert_bytes = 3.0 * D * F * (e4m3 ? 1.0 : 0.5);
+  if (!grouped(D, F) || pairs <= chosen * (e4m3 ? 1.13 : 1.5) ||
       (pairs - chosen) * expert_bytes <= 64e6)
-    return vec_turn(g, d, stream);
+    return {};
   // Tiles of 16 tokens, two at a time where experts have more on average and more
   // rows than with one fit in LDS (sums of two tiles take room from them).
-  const int mt = pairs > 12 * g.E && up_rows(2, g.D) > up_rows(1, g.D) ? 2 : 1;
-  const DownPlan down = down_plan(g.T, g.k, g.E, g.D, g.F);
-  g.parts = down.parts;
-  g.part_len = down.len;
+  const int mt = pairs > 12 * E && up_rows(2, D) > up_rows(1, D) ? 2 : 1;
+  const DownPlan down = down_plan(T, k, E, D, F);
   // Tiles of 128 rows with two waves to a row's K where each CU has ten or more of
   // them (fewer ends of tiles per byte), of 32 rows with eight where not, unless K is
   // no more than one unit for each of the eight: most would wait (us, eight / two:
@@ -247,15 +246,25 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   // 85/64;  e4m3 1024 x 512, 8 of 128, 64 tokens 64/53;  beyond, e4m3 4096 x 4096, 2 of
   // 8, 16 tokens 82/91, 4096 x 2048, 4 of 64, 177/187).
   const int short_k = 8 * (e4m3 ? 128 : 256);
-  const int wku = chosen * g.F / 64 >= 2560 || g.D <= short_k ? 2 : 8;
-  const int wkd = chosen * g.D / 128 * g.parts >= 2560 || g.part_len <= short_k ? 2 : 8;
+  const int wku = chosen * F / 64 >= 2560 || D <= short_k ? 2 : 8;
+  const int wkd = chosen * D / 128 * down.parts >= 2560 || down.len <= short_k ? 2 : 8;
+  return {1, 16 * mt, wku, 16 * down.mt, wkd, down.parts, down.len};
+}
+
+hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
+  const hipgemm_moe_plan p = turn_plan(g.T, g.k, g.E, g.D, g.F, d.format);
+  if (!p.grouped) return vec_turn(g, d, stream);
+  g.parts = p.parts;
+  g.part_len = p.part_len;
   const int cus = 256;
   hipError_t e = launch(hk::moe_up(d.x_type, d.w13.zeros ? kWInt4Z : d.format, d.scale_type,
-                                   mode_of(d.x_type, d.format, d.scale_type, d.group_size), mt, wku),
+                                   mode_of(d.x_type, d.format, d.scale_type, d.group_size),
+                                   p.up_rows / 16, p.up_waves),
                         dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   e = launch(hk::moe_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type,
-                          mode_of(kInBf16, d.format, d.scale_type, d.group_size), down.mt, wkd),
+                          mode_of(kInBf16, d.format, d.scale_type, d.group_size), p.down_rows / 16,
+                          p.down_waves),
              dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   return launch((const void*)&k_moe_sum, dim3((unsigned)((g.T * (g.D / 4) + 255) / 256)), 256, g,
@@ -263,6 +272,16 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
 }
 
 }  // namespace
+
+extern "C" hipError_t hipgemm_moe_select(int T, int k, int E, int D, int F, int format,
+                                         hipgemm_moe_plan* plan) {
+  if (!plan || T < 1 || k < 1 || k > 64 || E < 1 || E > HIPGEMM_MOE_MAX_EXPERTS || D < 32 ||
+      D % 32 != 0 || D > kMaxDim || F < 32 || F % 32 != 0 || F > kMaxDim / 2 || format < 0 ||
+      format > HIPGEMM_W8_E4M3)
+    return hipErrorInvalidValue;
+  *plan = turn_plan(turn_tokens(T, k), k, E, D, F, format);
+  return hipSuccess;
+}
 
 extern "C" size_t hipgemm_moe_workspace_size(int T, int k, int E, int D, int F) {
   if (T <= 0 || k <= 0 || k > 64 || E <= 0 || D <= 0 || F <= 0) return 0;

@@ -97,7 +97,6 @@ bool by_tiles(const hipgemm_w4_desc& d) {
 // 105/70, 128 x 512 x 512 6.5/4.8;  fp4 512 x 512 x 4096 15.9/12.9).
 struct SplitPlan {
   int mt, nt;
-  long long tiles;
 };
 SplitPlan split_plan(int M, int N) {
   SplitPlan p;
@@ -108,7 +107,6 @@ SplitPlan split_plan(int M, int N) {
   while (p.mt > 1 && groups_of((p.mt + 1) / 2) * narrow <= 256) p.mt = (p.mt + 1) / 2;
   const long long tm = groups_of(p.mt);
   p.nt = tm * narrow <= 256 ? 2 : 4;
-  p.tiles = tm * ((N + 16 * p.nt - 1) / (16 * p.nt));
   return p;
 }
 
@@ -134,6 +132,16 @@ VecPlan vec_plan(int N, int K) {
   return p;
 }
 
+// The kernel of a call, and of tiles their rows and columns: vectors up to four rows;
+// and, four at a time, without any K or where rows of x lie so far apart that 64 are
+// not in a buffer's range.
+hipgemm_w4_plan plan_of(const hipgemm_w4_desc& d) {
+  if (d.M <= 4 || d.K == 0 || 2 * d.ldx > kMaxRow) return {HIPGEMM_W4_VECTORS, 0, 0};
+  if (by_tiles(d)) return {HIPGEMM_W4_TILES, kW4TileM, kW4TileN};
+  const SplitPlan p = split_plan(d.M, d.N);
+  return {HIPGEMM_W4_SPLIT, 16 * p.mt, 16 * p.nt};
+}
+
 hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
   W4Args g{};
   g.x = static_cast<const uint8_t*>(d.x);
@@ -154,9 +162,8 @@ hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
   g.act = d.activation;
   g.out = d.out_dtype;
   const int w = d.zeros ? kWInt4Z : d.format;
-  // Up to four rows;  and, four at a time, without any K or where rows of x lie so
-  // far apart that 64 are not in a buffer's range.
-  if (d.M <= 4 || d.K == 0 || 2 * d.ldx > kMaxRow) {
+  const hipgemm_w4_plan plan = plan_of(d);
+  if (plan.kernel == HIPGEMM_W4_VECTORS) {
     const VecPlan p = vec_plan(d.N, d.K);
     g.waves_k = p.waves_k;
     g.rows = p.rows;
@@ -178,20 +185,17 @@ hipError_t run(const hipgemm_w4_desc& d, hipStream_t stream) {
                        ? kInline
                    : d.group_size % 128 == 0 ? kCoarse
                                              : kFine;
-  if (by_tiles(d)) {
-    const long long tiles = (long long)((d.M + kW4TileM - 1) / kW4TileM) *
-                            ((d.N + kW4TileN - 1) / kW4TileN);
-    return launch(hk::w4_tile(d.x_type, w, d.scale_type, mode),
-                  dim3((unsigned)(tiles < 512 ? tiles : 512)), 256, g, stream);
-  }
-  const SplitPlan p = split_plan(d.M, d.N);
-  return launch(hk::w4_split(d.x_type, w, d.scale_type, mode, p.mt, p.nt),
-                dim3((unsigned)(p.tiles < 256 ? p.tiles : 256)), 256, g, stream);
+  const long long tiles = (long long)((d.M + plan.tile_rows - 1) / plan.tile_rows) *
+                          ((d.N + plan.tile_columns - 1) / plan.tile_columns);
+  const bool by = plan.kernel == HIPGEMM_W4_TILES;
+  const long long most = by ? 512 : 256;  // workgroups: two per CU, one
+  const void* fn = by ? hk::w4_tile(d.x_type, w, d.scale_type, mode)
+                      : hk::w4_split(d.x_type, w, d.scale_type, mode, plan.tile_rows / 16,
+                                     plan.tile_columns / 16);
+  return launch(fn, dim3((unsigned)(tiles < most ? tiles : most)), 256, g, stream);
 }
 
-}  // namespace
-
-extern "C" hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc* desc, hipStream_t stream) {
+hipError_t check(const hipgemm_w4_desc* desc) {
   if (!desc || desc->size != sizeof(hipgemm_w4_desc)) return hipErrorInvalidValue;
   const hipgemm_w4_desc& d = *desc;
   if (d.M < 0 || d.N < 0 || d.K < 0 || d.K % 32 != 0 || d.K > kMaxK || d.group_size <= 0 ||
@@ -216,5 +220,19 @@ extern "C" hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc* desc, hipStream_t s
         d.lds < (d.K + d.group_size - 1) / d.group_size)
       return hipErrorInvalidValue;
   }
-  return run(d, stream);
+  return hipSuccess;
+}
+
+}  // namespace
+
+extern "C" hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc* desc, hipStream_t stream) {
+  const hipError_t e = check(desc);
+  return e != hipSuccess || desc->M == 0 || desc->N == 0 ? e : run(*desc, stream);
+}
+
+extern "C" hipError_t hipgemm_w4_select(const hipgemm_w4_desc* desc, hipgemm_w4_plan* plan) {
+  const hipError_t e = check(desc);
+  if (e != hipSuccess || !plan) return hipErrorInvalidValue;
+  *plan = plan_of(*desc);
+  return hipSuccess;
 }

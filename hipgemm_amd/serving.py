@@ -18,7 +18,7 @@ import functools
 from . import (ACTIVATIONS, OUT_BF16, OUT_F16, OUT_F32, HipGemmError, _check,
                _torch, hipErrorInvalidValue, lib)
 
-__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "W4_FORMATS",
+__all__ = ["w4_gemm", "W4Desc", "w4_gemm_raw", "w4_select", "moe_select", "W4_FORMATS",
            "moe_route", "MOE_SCORING", "moe_experts", "MoeDesc", "MoeMatrix",
            "moe_experts_raw", "moe_workspace_size", "MOE_FORMATS"]
 
@@ -88,6 +88,14 @@ def _on(stream):
 def w4_gemm_raw(desc: "W4Desc", stream: int = 0) -> int:
     """Call hipgemm_w4_gemm; returns hipError_t."""
     return int(lib().hipgemm_w4_gemm(ctypes.byref(desc), stream or None))
+
+
+def w4_select(desc: "W4Desc") -> tuple:
+    """(kernel, tile rows, tile columns) that hipgemm_w4_gemm takes for a descriptor;
+    kernel: "vectors" (no tiles), "split" or "tiles"."""
+    plan = (_ci * 3)()
+    _check(lib().hipgemm_w4_select(ctypes.byref(desc), plan), "hipgemm_w4_select")
+    return (("vectors", "split", "tiles")[plan[0]], *plan[1:])
 
 
 def w4_gemm(x, weight, scales, zeros=None, *, format: str = "int4",
@@ -215,6 +223,17 @@ def moe_route(logits, k: int, *, scoring: str = "softmax", renormalize: bool = T
         int(renormalize), scale, weights.data_ptr(), ids.data_ptr(),
         _stream_handle(logits, stream)), "hipgemm_moe_route")
     return weights, ids
+
+
+def moe_select(T: int, k: int, E: int, D: int, F: int, format: str = "e4m3") -> dict:
+    """How moe_experts runs the first turn of such a call: empty pair by pair;
+    grouped, up_rows and down_rows (tokens of a tile), up_waves and down_waves (that
+    share a row's K), parts (of F, of part_len each)."""
+    plan = (_ci * 7)()
+    _check(lib().hipgemm_moe_select(T, k, E, D, F, MOE_FORMATS.get(format, -1), plan),
+           "hipgemm_moe_select")
+    names = ("up_rows", "up_waves", "down_rows", "down_waves", "parts", "part_len")
+    return dict(zip(names, plan[1:])) if plan[0] else {}
 
 
 def moe_experts_raw(desc: "MoeDesc", stream: int = 0) -> int:

@@ -407,6 +407,19 @@ typedef struct hipgemm_w4_desc {
 } hipgemm_w4_desc;
 hipError_t hipgemm_w4_gemm(const hipgemm_w4_desc *desc, hipStream_t stream);
 
+/* The kernel that hipgemm_w4_gemm runs for a descriptor, and the rows and columns of
+ * its tiles (0 for VECTORS: up to four rows of x at a time, a pass over the weights).
+ * No GPU needed; no reference counterpart. */
+enum {
+  HIPGEMM_W4_VECTORS = 0,
+  HIPGEMM_W4_SPLIT = 1, /* some rows: four waves along K */
+  HIPGEMM_W4_TILES = 2  /* many: tiles of 128 x 128 */
+};
+typedef struct hipgemm_w4_plan {
+  int kernel, tile_rows, tile_columns;
+} hipgemm_w4_plan;
+hipError_t hipgemm_w4_select(const hipgemm_w4_desc *desc, hipgemm_w4_plan *plan);
+
 /*
  * The router's choice of a mixture-of-experts layer: for each of T rows of E
  * logits (device, of type HIPGEMM_IN_*, row stride ld elements) the k largest,
@@ -476,6 +489,16 @@ typedef struct hipgemm_moe_desc {
 } hipgemm_moe_desc;
 size_t hipgemm_moe_workspace_size(int T, int k, int E, int D, int F);
 hipError_t hipgemm_moe_experts(const hipgemm_moe_desc *desc, hipStream_t stream);
+
+/* How hipgemm_moe_experts runs (the first turn of) a call of these sizes: all 0 pair by
+ * pair; grouped, the rows (tokens) of a tile and the waves that share a row's K, up and
+ * down, and the parts of F of the down product, of part_len each.  No GPU needed; no
+ * reference counterpart. */
+typedef struct hipgemm_moe_plan {
+  int grouped, up_rows, up_waves, down_rows, down_waves, parts, part_len;
+} hipgemm_moe_plan;
+hipError_t hipgemm_moe_select(int T, int k, int E, int D, int F, int format,
+                              hipgemm_moe_plan *plan);
 
 /* Workspace bytes hipgemm_fp8_gemm_bf16_ws needs for this shape and variant
  * on the current device (0: none).  No GPU work.  No reference counterpart. */
