@@ -190,7 +190,7 @@ struct Stream {
         const int k = (t - row * segs) * 512 + kl;
         if (k < ((k1 - k0 + 255) & ~255))
           *reinterpret_cast<__attribute__((address_space(3))) i32x4*>(lds + row * pt + 2 * k) =
-              k0 + k < k1 ? pair_order<kW>(v[i]) : i32x4{};
+              k0 + k < k1 ? v[i] : i32x4{};
       }
     }
   }
@@ -307,8 +307,8 @@ struct Stream {
           for (int n = 0; n < kNT; ++n) {
             const int i = kMode == kFine ? j : h;
             const float c = scale_of<kS>(sc[n][i]);
-            float off = -(kInt4Bias<kX> + 8.0f);
-            if constexpr (kW == kWInt4Z) off = -(kInt4Bias<kX> + (float)zs[n][i]);
+            float off = -8.0f;
+            if constexpr (kW == kWInt4Z) off = -(float)zs[n][i];
 #pragma unroll
             for (int m = 0; m < kMT; ++m)
 #pragma unroll

@@ -15,17 +15,14 @@
 // k_w4_tile, many rows: bound by the matrix unit and by what surrounds it.  Tiles of
 // 128 x 128 by four waves, 64 x 64 each, two stages of 40 KiB that they share, two
 // workgroups to a CU, so that one's arithmetic hides the other's waits.  2048 x 14336
-// x 4096 int4, group 128, bf16: 321 us, 750 TFLOP/s (628 by k_w4_split).
+// x 4096 int4, group 128, bf16: 297 us, 810 TFLOP/s (628 by k_w4_split).
 //
 // Per wave of 64 x 64 and step there are 64 MFMAs of 16 cycles each; the decoding
 // takes 9 instructions per 8 weights and lane (16 x 9), int4 with one scale per step
 // and row one FMA per accumulator (64): all told about as many issue slots as the
 // matrix unit takes, so neither may grow.  Hence:
-//   * int4 codes are decoded exactly, q (0-15), not q plus an offset: the code's
-//     nibble is the e4m3 number q 2^-9 (subnormal below 8, the first binade from
-//     there), so unpacked nibbles go through the e4m3 conversion with scale 2^9.
-//     They come out in their own order, and the activations need no reordering,
-//     which would cost as much as the decoding (16 operands against 16).
+//   * int4 codes are decoded in their own order (decode.hpp): reordering activations
+//     would cost as much as the decoding (16 operands against 16).
 //   * the zero point's share, -z sum(x), is the accumulator that a step's MFMAs
 //     start from: without zero points it is the same for all columns.
 // Scales as in w4_stream.hpp (kCoarse, kFine, kInline), loaded with the stage by the
@@ -49,18 +46,6 @@ constexpr int kW4TileM = 128, kW4TileN = 128, kW4TileK = 128;
 
 // (rows 0-3, 12-15 have slots 0-7, the others 8-15: xor 1 or 4 stays in these)
 __device__ __forceinline__ int x_slot(int row) { return (row + 4) & 15; }
-
-// Eight codes in their own order, exactly (int4: q).
-template <int kX, int kW>
-__device__ __forceinline__ i32x4 decode8_exact(uint32_t q, float scale) {
-  if constexpr (!is_int4(kW)) {
-    return decode8<kX, kW>(q, 0u, scale);
-  } else {
-    const uint32_t lo = q & 0x0f0f0f0fu, hi = (q >> 4) & 0x0f0f0f0fu;
-    return decode8<kX, kWE4M3>(__builtin_amdgcn_perm(hi, lo, 0x05010400u),
-                               __builtin_amdgcn_perm(hi, lo, 0x07030602u), 512.0f);
-  }
-}
 
 // Sums that came out infinite or NaN, by the definition, weight by weight: the sums
 // before the scale can overflow for an x near the largest, and an infinite one makes
@@ -218,7 +203,7 @@ struct W4Wave {
         }
 #pragma unroll
         for (int n = 0; n < kNT; ++n) {
-          const i32x4 b = decode8_exact<kX, kW>(w[n][j], 1.0f);
+          const i32x4 b = decode8<kX, kW>(w[n][j], 0u, 1.0f);
           const float c = scale_of<kS>(s4[n][j]);
 #pragma unroll
           for (int m = 0; m < kMT; ++m) {
@@ -262,7 +247,7 @@ struct W4Wave {
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const i32x4 b = decode8_exact<kX, kW>((uint32_t)q[n][j], kMode == kInline ? c : 1.0f);
+          const i32x4 b = decode8<kX, kW>((uint32_t)q[n][j], 0u, kMode == kInline ? c : 1.0f);
 #pragma unroll
           for (int m = 0; m < kMT; ++m) p[m] = mfma_16x16x32<kX>(a[j][m], b, p[m]);
         }

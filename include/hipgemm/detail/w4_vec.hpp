@@ -11,7 +11,7 @@
 // instructions in fp32.  The lanes' sums meet in a butterfly that halves the rows
 // as it halves the lanes, those of the chunks in LDS.
 //
-// The int4 excess (decode.hpp) is (bias + z) times the lane's sum of x.  Where
+// The int4 excess (decode.hpp) is z times the lane's sum of x.  Where
 // x is so large that the unscaled sums could overflow, or infinite, the wave
 // takes its weights one by one instead, so that infinities come out as the
 // definition has them.
@@ -101,7 +101,7 @@ struct Vec {
             top = fmaxf(top, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
           }
         }
-        x[m][j] = pair_order<kW>(v[m][j]);
+        x[m][j] = v[m][j];
       }
       // (fp16 stays below it unless infinite; the maximum ignores a NaN, which
       // comes out as one either way)
@@ -169,8 +169,8 @@ struct Vec {
             d[m] = dot2<kX>((uint32_t)x[m][j][e], (uint32_t)b[e], d[m]);
       }
       const float sc = scale_of<kS>(r.s[i]);
-      float off = -(kInt4Bias<kX> + 8.0f);
-      if constexpr (kW == kWInt4Z) off = -(kInt4Bias<kX> + (float)r.z[i]);
+      float off = -8.0f;
+      if constexpr (kW == kWInt4Z) off = -(float)r.z[i];
 #pragma unroll
       for (int m = 0; m < kM; ++m) {
         if constexpr (is_int4(kW)) d[m] = __builtin_fmaf(off, xs[m], d[m]);
