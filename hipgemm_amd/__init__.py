@@ -150,7 +150,7 @@ def lib() -> ctypes.CDLL:
     L.hipgemm_w4_gemm.restype = ci
     L.hipgemm_w4_select.argtypes = [vp, vp]
     L.hipgemm_w4_select.restype = ci
-    L.hipgemm_moe_select.argtypes = [ci, ci, ci, ci, ci, ci, vp]
+    L.hipgemm_moe_select.argtypes = [ci, ci, ci, ci, ci, ci, ci, vp]
     L.hipgemm_moe_select.restype = ci
     L.hipgemm_moe_experts.argtypes = [vp, vp]
     L.hipgemm_moe_experts.restype = ci

@@ -77,14 +77,14 @@ hipError_t quantize_rows(const void* x, int type, int M, int K, long long ldx,
 // x: activations' type, w: detail::kW*, s: scales' type, mode: detail::kNone,
 // kCoarse, kFine or kInline; rows: 1, 2 or 4, lk: 16
 // or 64 lanes of a row; mt: tiles of 16 rows of x (1, 2);
-// wk: waves that share a row's K (2, 8).
+// wk: waves that share a row's K (2, 8); h: parts of the experts' h (2, 3).
 const void* w4_vec(int x, int w, int s, int rows, int lk);
 const void* w4_tile(int x, int w, int s, int mode);
 const void* w4_split(int x, int w, int s, int mode, int mt, int nt);
 const void* moe_up(int x, int w, int s, int mode, int mt, int wk);
-const void* moe_down(int w, int s, int mode, int mt, int wk);
+const void* moe_down(int w, int s, int mode, int mt, int wk, int h);
 const void* moe_vec_up(int x, int w, int s, int lk);
-const void* moe_vec_down(int w, int s, int lk);
+const void* moe_vec_down(int w, int s, int lk, int h);
 // Packs [rows][ceil(K/32)] E8M0 scales (row stride ld) into MxArgs' layout.
 hipError_t mx_pack(const uint8_t* src, int rows, int K, int ld, uint8_t* dst,
                    hipStream_t stream);

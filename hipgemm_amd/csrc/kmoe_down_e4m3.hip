@@ -4,11 +4,11 @@
 namespace hipgemm {
 namespace kernels {
 
-const void* moe_down_e4m3(int s, int mode, int mt, int wk) {
-  return moe_down_of<detail::kWE4M3>(s, mode, mt, wk);
+const void* moe_down_e4m3(int s, int mode, int mt, int wk, int h) {
+  return moe_down_of<detail::kWE4M3>(s, mode, mt, wk, h);
 }
-const void* moe_vec_down_e4m3(int s, int lk) {
-  return moe_vec_down_of<detail::kWE4M3>(s, lk);
+const void* moe_vec_down_e4m3(int s, int lk, int h) {
+  return moe_vec_down_of<detail::kWE4M3>(s, lk, h);
 }
 
 }  // namespace kernels

@@ -4,11 +4,11 @@
 namespace hipgemm {
 namespace kernels {
 
-const void* moe_down_int4(int s, int mode, int mt, int wk) {
-  return moe_down_of<detail::kWInt4>(s, mode, mt, wk);
+const void* moe_down_int4(int s, int mode, int mt, int wk, int h) {
+  return moe_down_of<detail::kWInt4>(s, mode, mt, wk, h);
 }
-const void* moe_vec_down_int4(int s, int lk) {
-  return moe_vec_down_of<detail::kWInt4>(s, lk);
+const void* moe_vec_down_int4(int s, int lk, int h) {
+  return moe_vec_down_of<detail::kWInt4>(s, lk, h);
 }
 
 }  // namespace kernels

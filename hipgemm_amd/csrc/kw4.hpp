@@ -97,20 +97,27 @@ const void* moe_vec_up_of(int s, int lk) {
   });
 }
 template <int kW>
-const void* moe_vec_down_of(int s, int lk) {
-  return sel_vec<kW>(s, lk, [](auto S, auto L) {
-    return (const void*)&detail::k_moe_vec_down<kW, decltype(S)::value, decltype(L)::value>;
+const void* moe_vec_down_of(int s, int lk, int h) {
+  return sel_vec<kW>(s, lk, [h](auto S, auto L) {
+    constexpr int kS = decltype(S)::value, kLk = decltype(L)::value;
+    return h == 3 ? (const void*)&detail::k_moe_vec_down<kW, kS, kLk, 3>
+                  : (const void*)&detail::k_moe_vec_down<kW, kS, kLk, 2>;
   });
 }
 
+// h: parts of h; tiles of three are of 16 rows.
 template <int kW>
-const void* moe_down_of(int s, int mode, int mt, int wk) {
-  return sel_scales<detail::kInBf16, kW>(s, mode, [&](auto S, auto Mode) {
+const void* moe_down_of(int s, int mode, int mt, int wk, int h) {
+  return sel_scales<detail::kInBf16, kW>(s, mode, [&](auto S, auto Mode) -> const void* {
+    constexpr int kS = decltype(S)::value, kMode = decltype(Mode)::value;
+    if (h == 3)
+      return mt != 1 ? nullptr
+             : wk == 8 ? (const void*)&detail::k_moe_down<kW, kS, kMode, 1, 8, 3>
+                       : (const void*)&detail::k_moe_down<kW, kS, kMode, 1, 2, 3>;
     return sel_mt(mt, [&](auto MT) {
-      constexpr int kS = decltype(S)::value, kMode = decltype(Mode)::value;
       constexpr int kMT = decltype(MT)::value;
-      return wk == 8 ? (const void*)&detail::k_moe_down<kW, kS, kMode, kMT, 8>
-                     : (const void*)&detail::k_moe_down<kW, kS, kMode, kMT, 2>;
+      return wk == 8 ? (const void*)&detail::k_moe_down<kW, kS, kMode, kMT, 8, 2>
+                     : (const void*)&detail::k_moe_down<kW, kS, kMode, kMT, 2, 2>;
     });
   });
 }

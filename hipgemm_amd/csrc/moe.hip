@@ -13,10 +13,10 @@ namespace kernels {
 #define HIPGEMM_MOE(W)                                  \
   const void* moe_up_bf16_##W(int s, int mode, int mt, int wk); \
   const void* moe_up_f16_##W(int s, int mode, int mt, int wk);  \
-  const void* moe_down_##W(int s, int mode, int mt, int wk);    \
+  const void* moe_down_##W(int s, int mode, int mt, int wk, int h); \
   const void* moe_vec_up_bf16_##W(int s, int lk);       \
   const void* moe_vec_up_f16_##W(int s, int lk);        \
-  const void* moe_vec_down_##W(int s, int lk);
+  const void* moe_vec_down_##W(int s, int lk, int h);
 HIPGEMM_MOE(int4)
 HIPGEMM_MOE(int4z)
 HIPGEMM_MOE(fp4)
@@ -33,12 +33,12 @@ const void* moe_up(int x, int w, int s, int mode, int mt, int wk) {
     default: return b ? moe_up_bf16_e4m3(s, mode, mt, wk) : moe_up_f16_e4m3(s, mode, mt, wk);
   }
 }
-const void* moe_down(int w, int s, int mode, int mt, int wk) {
+const void* moe_down(int w, int s, int mode, int mt, int wk, int h) {
   switch (w) {
-    case detail::kWInt4: return moe_down_int4(s, mode, mt, wk);
-    case detail::kWInt4Z: return moe_down_int4z(s, mode, mt, wk);
-    case detail::kWFp4: return moe_down_fp4(s, mode, mt, wk);
-    default: return moe_down_e4m3(s, mode, mt, wk);
+    case detail::kWInt4: return moe_down_int4(s, mode, mt, wk, h);
+    case detail::kWInt4Z: return moe_down_int4z(s, mode, mt, wk, h);
+    case detail::kWFp4: return moe_down_fp4(s, mode, mt, wk, h);
+    default: return moe_down_e4m3(s, mode, mt, wk, h);
   }
 }
 const void* moe_vec_up(int x, int w, int s, int lk) {
@@ -50,12 +50,12 @@ const void* moe_vec_up(int x, int w, int s, int lk) {
     default: return b ? moe_vec_up_bf16_e4m3(s, lk) : moe_vec_up_f16_e4m3(s, lk);
   }
 }
-const void* moe_vec_down(int w, int s, int lk) {
+const void* moe_vec_down(int w, int s, int lk, int h) {
   switch (w) {
-    case detail::kWInt4: return moe_vec_down_int4(s, lk);
-    case detail::kWInt4Z: return moe_vec_down_int4z(s, lk);
-    case detail::kWFp4: return moe_vec_down_fp4(s, lk);
-    default: return moe_vec_down_e4m3(s, lk);
+    case detail::kWInt4: return moe_vec_down_int4(s, lk, h);
+    case detail::kWInt4Z: return moe_vec_down_int4z(s, lk, h);
+    case detail::kWFp4: return moe_vec_down_fp4(s, lk, h);
+    default: return moe_vec_down_e4m3(s, lk, h);
   }
 }
 
@@ -131,15 +131,18 @@ double chosen_experts(int T, int k, int E) {
 }
 
 // What a workgroup of the grouped kernels keeps in LDS is the same for all formats.
-template <int kMT, bool kLo>
-using AnyStream = Stream<kInBf16, kWE4M3, kInF32, kNone, kMT, kLo, 8, kMoeTables>;
+template <int kMT, int kParts>
+using AnyStream = Stream<kInBf16, kWE4M3, kInF32, kNone, kMT, kParts, 8, kMoeTables>;
 // Rows of x (of D elements) going up.
 int up_rows(int mt, int D) {
-  return mt == 2 ? AnyStream<2, false>::rows_that_fit(D) : AnyStream<1, false>::rows_that_fit(D);
+  return mt == 2 ? AnyStream<2, 1>::rows_that_fit(D) : AnyStream<1, 1>::rows_that_fit(D);
 }
+// Parts of h (moe.hpp).
+int h_parts(int out_dtype) { return out_dtype == HIPGEMM_OUT_F32 ? 3 : 2; }
 // Elements of h going down, over all rows.
-int down_elems(int mt) {
-  return (mt == 2 ? AnyStream<2, true>::kElems : AnyStream<1, true>::kElems) / 2;
+int down_elems(int mt, int h) {
+  return h == 3 ? AnyStream<1, 3>::kElems / 3
+                : (mt == 2 ? AnyStream<2, 2>::kElems : AnyStream<1, 2>::kElems) / 2;
 }
 
 // Whether the grouped kernels take the sizes: a row of x in LDS going up, and going
@@ -151,17 +154,17 @@ bool grouped(int D, int F) { return up_rows(1, D) >= 1 && F <= 1 << 16; }
 struct DownPlan {
   int mt, parts, len;
 };
-DownPlan down_plan(int T, int k, int E, int D, int F) {
+DownPlan down_plan(int T, int k, int E, int D, int F, int h) {
   const int pairs = T * k, steps = (F + 255) / 256;
   // Parts so short that the rows of an expert, up to half as many again as there are on
   // average, lie in LDS together: its weights are read once for them.  Not below
   // 1024, and of 32 rows only where more than 16 fit.
   const double rows = std::ceil(1.5 * pairs / chosen_experts(T, k, E));
-  int mt = pairs > 12 * E ? 2 : 1, fit;
+  int mt = pairs > 12 * E && h == 2 ? 2 : 1, fit;
   for (;; mt = 1) {
-    fit = (int)(down_elems(mt) / (rows < 16 * mt ? rows : 16 * mt)) / 256;
+    fit = (int)(down_elems(mt, h) / (rows < 16 * mt ? rows : 16 * mt)) / 256;
     if (fit < 4) fit = 4;
-    if (mt == 1 || down_elems(2) / (256 * (fit < steps ? fit : steps)) > 16) break;
+    if (mt == 1 || down_elems(2, h) / (256 * (fit < steps ? fit : steps)) > 16) break;
   }
   const int chosen = pairs < E ? pairs : E;  // experts at most
   const int tiles = chosen * ((D + 63) / 64);
@@ -209,13 +212,13 @@ hipError_t vec_turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   const int lk = vec_lanes(g.F, per_lane), chunks = chunks_of(g.F, per_lane, lk);
   const int items = chunks * g.k, turns = (items + 7) / 8;
   g.rows = kVecRows * (kWave / lk) * steps_of(g.D, g.T, kVecRows * (kWave / lk));
-  return launch(hk::moe_vec_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type, lk),
+  return launch(hk::moe_vec_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type, lk, g.h_parts),
                 dim3((unsigned)((g.D + g.rows - 1) / g.rows), (unsigned)g.T),
                 kWave * ((items + turns - 1) / turns), g, stream);
 }
 
 // The kernels of a turn.
-hipgemm_moe_plan turn_plan(int T, int k, int E, int D, int F, int format) {
+hipgemm_moe_plan turn_plan(int T, int k, int E, int D, int F, int format, int h) {
   const int pairs = T * k;
   const double chosen = chosen_experts(T, k, E);
   // Pair by pair while few experts are read twice.  us in a graph, pairs / grouped,
@@ -238,7 +241,7 @@ hipgemm_moe_plan turn_plan(int T, int k, int E, int D, int F, int format) {
   // Tiles of 16 tokens, two at a time where experts have more on average and more
   // rows than with one fit in LDS (sums of two tiles take room from them).
   const int mt = pairs > 12 * E && up_rows(2, D) > up_rows(1, D) ? 2 : 1;
-  const DownPlan down = down_plan(T, k, E, D, F);
+  const DownPlan down = down_plan(T, k, E, D, F, h);
   // Tiles of 128 rows with two waves to a row's K where each CU has ten or more of
   // them (fewer ends of tiles per byte), of 32 rows with eight where not, unless K is
   // no more than one unit for each of the eight: most would wait (us, eight / two:
@@ -252,7 +255,7 @@ hipgemm_moe_plan turn_plan(int T, int k, int E, int D, int F, int format) {
 }
 
 hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
-  const hipgemm_moe_plan p = turn_plan(g.T, g.k, g.E, g.D, g.F, d.format);
+  const hipgemm_moe_plan p = turn_plan(g.T, g.k, g.E, g.D, g.F, d.format, g.h_parts);
   if (!p.grouped) return vec_turn(g, d, stream);
   g.parts = p.parts;
   g.part_len = p.part_len;
@@ -264,7 +267,7 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
   if (e != hipSuccess) return e;
   e = launch(hk::moe_down(d.w2.zeros ? kWInt4Z : d.format, d.scale_type,
                           mode_of(kInBf16, d.format, d.scale_type, d.group_size), p.down_rows / 16,
-                          p.down_waves),
+                          p.down_waves, g.h_parts),
              dim3((unsigned)cus), 512, g, stream);
   if (e != hipSuccess) return e;
   return launch((const void*)&k_moe_sum, dim3((unsigned)((g.T * (g.D / 4) + 255) / 256)), 256, g,
@@ -274,25 +277,27 @@ hipError_t turn(MoeArgs g, const hipgemm_moe_desc& d, hipStream_t stream) {
 }  // namespace
 
 extern "C" hipError_t hipgemm_moe_select(int T, int k, int E, int D, int F, int format,
-                                         hipgemm_moe_plan* plan) {
+                                         int out_dtype, hipgemm_moe_plan* plan) {
   if (!plan || T < 1 || k < 1 || k > 64 || E < 1 || E > HIPGEMM_MOE_MAX_EXPERTS || D < 32 ||
       D % 32 != 0 || D > kMaxDim || F < 32 || F % 32 != 0 || F > kMaxDim / 2 || format < 0 ||
-      format > HIPGEMM_W8_E4M3)
+      format > HIPGEMM_W8_E4M3 || out_dtype < 0 || out_dtype > HIPGEMM_OUT_F32)
     return hipErrorInvalidValue;
-  *plan = turn_plan(turn_tokens(T, k), k, E, D, F, format);
+  *plan = turn_plan(turn_tokens(T, k), k, E, D, F, format, h_parts(out_dtype));
   return hipSuccess;
 }
 
 extern "C" size_t hipgemm_moe_workspace_size(int T, int k, int E, int D, int F) {
   if (T <= 0 || k <= 0 || k > 64 || E <= 0 || D <= 0 || F <= 0) return 0;
   const int t = turn_tokens(T, k);
-  // (a last turn of fewer tokens can have more parts)
+  // (a last turn of fewer tokens can have more parts, and h of three parts)
   size_t o = 0;
-  for (int u : {t, T % t}) {
-    const size_t n = u == 0 || !grouped(D, F) ? 0 : (size_t)down_plan(u, k, E, D, F).parts * u * k;
-    if (n > o) o = n;
-  }
-  return (size_t)t * k * F * 4 + o * D * 4;
+  for (int u : {t, T % t})
+    for (int h : {2, 3}) {
+      if (u == 0 || !grouped(D, F)) continue;
+      const size_t n = (size_t)down_plan(u, k, E, D, F, h).parts * u * k;
+      if (n > o) o = n;
+    }
+  return (size_t)t * k * F * 6 + o * D * 4;
 }
 
 extern "C" hipError_t hipgemm_moe_experts(const hipgemm_moe_desc* desc, hipStream_t stream) {
@@ -348,9 +353,10 @@ extern "C" hipError_t hipgemm_moe_experts(const hipgemm_moe_desc* desc, hipStrea
   g.G = e4m3 ? 32 : d.group_size;
   g.act = d.activation;
   g.out = d.out_dtype;
+  g.h_parts = h_parts(d.out_dtype);
   const int most = turn_tokens(d.T, d.k);
   g.h = static_cast<uint16_t*>(d.workspace);
-  g.o = reinterpret_cast<float*>(g.h + (size_t)most * d.k * 2 * d.F);
+  g.o = reinterpret_cast<float*>(g.h + (size_t)most * d.k * 3 * d.F);
   for (int t = 0; t < d.T; t += most) {
     g.T = d.T - t < most ? d.T - t : most;
     g.x = static_cast<const uint8_t*>(d.x) + (long long)t * g.ldx;

@@ -225,12 +225,14 @@ def moe_route(logits, k: int, *, scoring: str = "softmax", renormalize: bool = T
     return weights, ids
 
 
-def moe_select(T: int, k: int, E: int, D: int, F: int, format: str = "e4m3") -> dict:
-    """How moe_experts runs the first turn of such a call: empty pair by pair;
-    grouped, up_rows and down_rows (tokens of a tile), up_waves and down_waves (that
+def moe_select(T: int, k: int, E: int, D: int, F: int, format: str = "e4m3",
+               out_dtype=None) -> dict:
+    """How moe_experts runs the first turn of such a call (out_dtype: bfloat16 where
+    None): empty pair by pair; grouped, up_rows and down_rows (tokens of a tile), up_waves and down_waves (that
     share a row's K), parts (of F, of part_len each)."""
     plan = (_ci * 7)()
-    _check(lib().hipgemm_moe_select(T, k, E, D, F, MOE_FORMATS.get(format, -1), plan),
+    out = OUT_BF16 if out_dtype is None else _types()[2].get(out_dtype, -1)
+    _check(lib().hipgemm_moe_select(T, k, E, D, F, MOE_FORMATS.get(format, -1), out, plan),
            "hipgemm_moe_select")
     names = ("up_rows", "up_waves", "down_rows", "down_waves", "parts", "part_len")
     return dict(zip(names, plan[1:])) if plan[0] else {}
@@ -296,7 +298,7 @@ def moe_experts(x, ids, weights, w13, scales13, w2, scales2, *, zeros13=None,
     group_size elements of a row, (E, rows, groups), as for w4_gemm ("int4",
     "fp4").  D, F and group_size are multiples of 32.  activation: of the gate
     (None, "relu", "gelu_tanh", "silu").  out_dtype: bfloat16, float16 or float32,
-    x's where None.  Made for up to 64 tokens (each expert's weights are read once
+    x's where None; h is held to 16 significant bits, to 24 for float32 results.  Made for up to 64 tokens (each expert's weights are read once
     for up to 16 of its tokens); any number works.  workspace: a uint8 device
     tensor of moe_workspace_size bytes; allocated per call where None."""
     torch = _torch()

@@ -452,7 +452,7 @@ hipError_t hipgemm_moe_route(const void *logits, int type, int T, int E, int k,
  * row as in hipgemm_w4_gemm, or HIPGEMM_W8_E4M3 with one float scale per row
  * (scale_type F32, lds 1: E x 2F and E x D).  An id outside [0, E) is skipped: a
  * token without any gives zeros.  Sums are fp32; h is held to 16 significant
- * bits between the two kernels.  Each chosen expert's weights are read once for
+ * bits between the two kernels, to fp32's 24 where out_dtype is F32.  Each chosen expert's weights are read once for
  * up to 16 of its tokens, so it is made for a few tokens (up to 64); more go in
  * turns of at most HIPGEMM_MOE_MAX_PAIRS / k.
  * D, F, group_size multiples of 32; matrices 16-byte aligned, with row and
@@ -498,7 +498,7 @@ typedef struct hipgemm_moe_plan {
   int grouped, up_rows, up_waves, down_rows, down_waves, parts, part_len;
 } hipgemm_moe_plan;
 hipError_t hipgemm_moe_select(int T, int k, int E, int D, int F, int format,
-                              hipgemm_moe_plan *plan);
+                              int out_dtype, hipgemm_moe_plan *plan);
 
 /* Workspace bytes hipgemm_fp8_gemm_bf16_ws needs for this shape and variant
  * on the current device (0: none).  No GPU work.  No reference counterpart. */

@@ -16,8 +16,12 @@
 // in their order: no atomics, the same result every time.
 //
 // h is held as the sum of two bf16 numbers (16 significand bits; one rounding to
-// bf16 would leave an error as large as the output's own), and the second
-// kernel multiplies both parts: its matrix unit is idle most of the time.
+// bf16 would leave an error as large as the output's own), of three for fp32
+// results (24 bits, its own), and the second kernel multiplies all parts: its matrix
+// unit is idle most of the time.  16 bits leave 3e-6 of the results' rms, a
+// thousandth of a bf16 result's rounding, 24 bits 2e-7; three parts everywhere
+// would cost (us, three / two) 64 tokens, 8 of 128 of 4096 x 1536 int4 297/266, 8 of 64
+// of 2048 x 1024 85/64, one token of 2 of 8 of 4096 x 14336 59/53 (e4m3 74/70).
 #pragma once
 
 #include "w4_stream.hpp"
@@ -39,22 +43,26 @@ struct MoeArgs {
   long long w13_row, w13_expert, s13_row, s13_expert, z13_row, z13_expert;
   long long w2_row, w2_expert, s2_row, s2_expert, z2_row, z2_expert;
   uint8_t* y;
-  uint16_t* h;  // pairs x 2 x F: high parts, low parts
+  uint16_t* h;  // pairs x h_parts x F
   float* o;     // parts x pairs x D
   int T, k, E, D, F, G;
   int act, out;
+  int h_parts;  // of h: 2, 3
   int parts, part_len;  // k_moe_down: of F
   int waves_k, rows, wave_rows;  // k_moe_vec_*: of a workgroup, of a wave
 };
 
-// One value of h, in two parts (one that is infinite, or in bf16, has no rest).
+// One value of h, in its parts (one that is infinite, or in bf16, has no rest).
 __device__ __forceinline__ void store_h(const MoeArgs& g, int pair, int f, float v) {
-  const __bf16 hi = (__bf16)v;
-  const float rest = v - (float)hi;
-  const __bf16 lo = (__bf16)(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.0f);
-  uint16_t* h = g.h + (long long)pair * 2 * g.F + f;
-  h[0] = __builtin_bit_cast(uint16_t, hi);
-  h[g.F] = __builtin_bit_cast(uint16_t, lo);
+  uint16_t* h = g.h + (long long)pair * g.h_parts * g.F + f;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (i == g.h_parts) break;
+    const __bf16 part = (__bf16)v;
+    h[i * g.F] = __builtin_bit_cast(uint16_t, part);
+    v -= (float)part;
+    if (!(__builtin_fabsf(v) < __builtin_inff())) v = 0.0f;
+  }
 }
 
 // The pairs by expert: groups of up to rows_max pairs of one expert.
@@ -144,7 +152,7 @@ __device__ __forceinline__ void share(int items, int* first, int* last) {
 
 template <int kX, int kW, int kS, int kMode, int kMT, int kWK>
 __global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
-  using S = Stream<kX, kW, kS, kMode, kMT, false, kWK, kMoeTables>;
+  using S = Stream<kX, kW, kS, kMode, kMT, 1, kWK, kMoeTables>;
   constexpr int kCols = 16 * S::kWN;  // of F, of an item: gate and up rows
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::kXBytes];
   __shared__ __attribute__((aligned(1024))) uint8_t rings[S::kRingBytes];
@@ -205,9 +213,9 @@ __global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
   p.st.run(first, last, g.D, p);
 }
 
-template <int kW, int kS, int kMode, int kMT, int kWK>
+template <int kW, int kS, int kMode, int kMT, int kWK, int kH>
 __global__ __launch_bounds__(512) void k_moe_down(MoeArgs g) {
-  using S = Stream<kInBf16, kW, kS, kMode, kMT, true, kWK, kMoeTables>;
+  using S = Stream<kInBf16, kW, kS, kMode, kMT, kH, kWK, kMoeTables>;
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::kXBytes];
   __shared__ __attribute__((aligned(1024))) uint8_t rings[S::kRingBytes];
   __shared__ float sums[S::kSums];
@@ -234,7 +242,7 @@ __global__ __launch_bounds__(512) void k_moe_down(MoeArgs g) {
     }
     __device__ __forceinline__ const uint8_t* row_at(int q, int part, int m) const {
       return reinterpret_cast<const uint8_t*>(
-          g.h + ((long long)__builtin_amdgcn_readfirstlane(pair(q, m)) * 2 + part) * g.F);
+          g.h + ((long long)__builtin_amdgcn_readfirstlane(pair(q, m)) * kH + part) * g.F);
     }
     __device__ __forceinline__ void weights(int item) {
       const int q = item / tiles, e = __builtin_amdgcn_readfirstlane(t.expert[q / g.parts]);

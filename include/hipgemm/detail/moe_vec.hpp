@@ -7,8 +7,8 @@
 // there is nothing to group: blockIdx.y names the pair (or, going down, the
 // token).  Going down a workgroup takes its rows of W2 for all of the token's
 // experts, dealt to its waves by expert and chunk of F, so that the sum over the
-// experts is the sum over the waves in LDS, in a fixed order.  h is two bf16 parts
-// (moe.hpp), here two rows of x whose sums are added.
+// experts is the sum over the waves in LDS, in a fixed order.  h is kH bf16 parts
+// (moe.hpp), here rows of x whose sums are added.
 #pragma once
 
 #include "moe.hpp"
@@ -51,14 +51,14 @@ __global__ __launch_bounds__(512) void k_moe_vec_up(MoeArgs g) {
   }
 }
 
-template <int kW, int kS, int kLk>
+template <int kW, int kS, int kLk, int kH>
 __global__ __launch_bounds__(512) void k_moe_vec_down(MoeArgs g) {
-  using V = Vec<kInBf16, kW, kS, 2, kLk>;
+  using V = Vec<kInBf16, kW, kS, kH, kLk>;
   const int wave = wave_id(), tid = (int)threadIdx.x, t = (int)blockIdx.y;
   const int waves = (int)blockDim.x / kWave;
   const int r0 = (int)blockIdx.x * g.rows, r1 = min(r0 + g.rows, g.D);
-  __shared__ float part[8][2 * kVecMaxRows];
-  for (int i = tid; i < 16 * kVecMaxRows; i += (int)blockDim.x) (&part[0][0])[i] = 0.0f;
+  __shared__ float part[8][kH * kVecMaxRows];
+  for (int i = tid; i < 8 * kH * kVecMaxRows; i += (int)blockDim.x) (&part[0][0])[i] = 0.0f;
   __syncthreads();
   const int chunks = (g.F + V::kChunk - 1) / V::kChunk;
   V v;
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(512) void k_moe_vec_down(MoeArgs g) {
     const int p = t * g.k + i / chunks;
     const int e = g.ids[p];
     if (e < 0 || e >= g.E) continue;
-    const uint8_t* h = reinterpret_cast<const uint8_t*>(g.h + (long long)p * 2 * g.F);
+    const uint8_t* h = reinterpret_cast<const uint8_t*>(g.h + (long long)p * kH * g.F);
     v.pass(i % chunks * V::kChunk, g.F, g.G, [&](int m) { return h + m * 2ll * g.F; },
            g.w2 + e * g.w2_expert, g.w2_row, g.s2 + e * g.s2_expert, g.s2_row,
            kW == kWInt4Z ? g.z2 + e * g.z2_expert : nullptr, g.z2_row, r0, r1, part[wave]);
@@ -74,7 +74,9 @@ __global__ __launch_bounds__(512) void k_moe_vec_down(MoeArgs g) {
   __syncthreads();
   for (int i = tid; i < r1 - r0; i += (int)blockDim.x) {
     float f = 0.0f;
-    for (int w = 0; w < waves; ++w) f += part[w][i] + part[w][kVecMaxRows + i];
+    for (int w = 0; w < waves; ++w)
+#pragma unroll
+      for (int q = 0; q < kH; ++q) f += part[w][q * kVecMaxRows + i];
     store_result(g.y, t * g.ldy + r0 + i, g.out, f);
   }
 }

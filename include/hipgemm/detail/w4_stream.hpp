@@ -77,12 +77,11 @@ __device__ __forceinline__ uint32_t scale_raw(const uint8_t* p, int i) {
   else if constexpr (type_bytes(kS) == 2) return reinterpret_cast<const uint16_t*>(p)[i];
   else return p[i];
 }
-// kLo: activations in two parts, x = hi + lo (16 bits each).
+// kParts: activations in that many parts, x their sum (16 bits each).
 // kTables: bytes of LDS that the kernel keeps for itself.
-template <int kX, int kW, int kS, int kMode, int kMT, bool kLo, int kWK, int kTables>
+template <int kX, int kW, int kS, int kMode, int kMT, int kParts, int kWK, int kTables>
 struct Stream {
   static constexpr int kWaves = 8, kThreads = kWaves * kWave, kNT = 2;
-  static constexpr int kParts = kLo ? 2 : 1;
   static constexpr int kRows = 16 * kMT;
   static constexpr int kWN = kWaves / kWK;
   static constexpr int kTile = 32 * kWN;  // rows of weights of an item
