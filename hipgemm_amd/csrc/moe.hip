@@ -116,7 +116,7 @@ int mode_of(int x_type, int format, int scale_type, int group) {
 bool matrix_ok(const hipgemm_moe_matrix& m, int rows, int K, const hipgemm_moe_desc& d) {
   const bool e4m3 = d.format == HIPGEMM_W8_E4M3;
   const long long row = e4m3 ? K : K / 2;
-  const long long groups = e4m3 ? 1 : (K + d.group_size - 1) / d.group_size;
+  const long long groups = e4m3 ? 1 : (K - 1) / d.group_size + 1;
   return m.weight && m.scales && aligned(m.weight, 16) && m.ldw <= kMaxRow &&
          m.lds <= kMaxRow / type_bytes(d.scale_type) &&
          aligned(m.scales, type_bytes(d.scale_type)) && m.ldw >= row && m.ldw % 16 == 0 &&

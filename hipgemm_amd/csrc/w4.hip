@@ -217,7 +217,7 @@ hipError_t check(const hipgemm_w4_desc* desc) {
       return hipErrorInvalidValue;
     if (d.ldx < d.K || d.ldx % 8 != 0 || d.ldw < d.K / 2 || d.ldw % 16 != 0 ||
         d.ldw > kMaxRow || d.lds > kMaxRow / type_bytes(d.scale_type) ||
-        d.lds < (d.K + d.group_size - 1) / d.group_size)
+        d.lds < (d.K - 1) / d.group_size + 1)
       return hipErrorInvalidValue;
   }
   return hipSuccess;
