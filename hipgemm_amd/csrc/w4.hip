@@ -73,30 +73,19 @@ hipError_t launch(const void* fn, dim3 grid, int threads, Args& g, hipStream_t s
   return hipLaunchKernel(fn, grid, dim3((unsigned)threads), args, 0, stream);
 }
 
-// k_w4_split and k_w4_tile.  us in a graph, split / tile, group 128, by M:
-//   N x K            96       128       192       256
-//   5000 x 3584    32/112    39/114    40/114    71/114
-//   4096 x 4096    16/65     18/67     23/67     24/67
-//   14336 x 4096   36/66     42/68     61/68     80/68
-//   28672 x 8192  116/116   134/120   198/169   238/174
-// (tile: 40, 32, 112, 224 tiles and twice that from 192 rows): tiles from three
-// quarters of the CUs on, not of fewer rows than three quarters of a tile.
-bool by_tiles(const hipgemm_w4_desc& d) {
-  const long long tiles = (long long)((d.M + kW4TileM - 1) / kW4TileM) *
-                          ((d.N + kW4TileN - 1) / kW4TileN);
-  return d.M > 96 && tiles >= 192 && 2 * d.ldx <= kMaxTileRow && d.ldw <= kMaxTileRow &&
-         d.lds <= kMaxTileRow;
-}
-
 // k_w4_split: groups of up to 64 rows of even lengths, and 32 columns where that
 // leaves a workgroup for each CU (16 rows, 4096 x 4096: 9.8 us for 13.4;  14336 x
 // 4096, 448 tiles: 19.6 for 16.0).  Groups are halved while each CU still takes at
 // most one such tile: weights are decoded once more, by CUs that had nothing to do
 // (us, not halved / halved, int4: 64 x 256 x 8192 24.0/13.8, 256 x 512 x 8192
 // 25.3/16.3, 37 x 2048 x 4096 12.1/9.5, 64 x 4096 x 4096 16.3/13.0, 703 x 256 x 22144
-// 105/70, 128 x 512 x 512 6.5/4.8;  fp4 512 x 512 x 4096 15.9/12.9).
+// 105/70, 128 x 512 x 512 6.5/4.8;  fp4 512 x 512 x 4096 15.9/12.9).  Groups of 48 rows
+// beside those of 32 and 64 (us, 48 / 64): int4 37 x 5000 x 3584 12.4/14.5, in groups of
+// 64 18.7/22.5, 48 x 14336 x 4096 20.2/22.3, 90 x 14336 x 4096 34.6/40.3; 40 x 4096 x 4096,
+// halved to 32, alike.
 struct SplitPlan {
   int mt, nt;
+  long long tiles;
 };
 SplitPlan split_plan(int M, int N) {
   SplitPlan p;
@@ -107,7 +96,27 @@ SplitPlan split_plan(int M, int N) {
   while (p.mt > 1 && groups_of((p.mt + 1) / 2) * narrow <= 256) p.mt = (p.mt + 1) / 2;
   const long long tm = groups_of(p.mt);
   p.nt = tm * narrow <= 256 ? 2 : 4;
+  p.tiles = tm * ((N + 16 * p.nt - 1) / (16 * p.nt));
   return p;
+}
+
+// Tiles of 128 x 128 where the split kernel's take four rounds over the CUs, five where
+// the large ones are more than a workgroup per CU, and not of fewer rows than three
+// quarters of a tile.  us in a graph, split / tile, K = 4096 but as given:
+//   int4 in groups of 128
+//     rounds 3: 129 x 14336 48/62, 192 x 14336 60/63, 300 x 8192 x 8192 99/108, 384 102/107
+//     rounds 4: 97 x 28672 79/62, 256 x 14336 77/62, 1024 x 4096 83/63; 258 large tiles:
+//       129 x 16600 63/86
+//     rounds 5: 300 x 14336 95/86, 700 x 6144 98/86, 800 x 5000 x 3584 87/77
+//     more: 512 x 14336 135/90, 2048 x 4096 188/96
+//   int4 in groups of 32 with zero points: 129 x 14336 95/118, 192 117/118, 256 154/119
+//   fp4, E8M0: 192 x 14336 56/64, 256 x 12288 56/64, 256 x 14336 69/64
+//   three quarters of a tile: 96 x 28672 x 8192 112/109 (128: 131/115)
+bool by_tiles(const hipgemm_w4_desc& d, const SplitPlan& p) {
+  const long long tiles = (long long)((d.M + kW4TileM - 1) / kW4TileM) *
+                          ((d.N + kW4TileN - 1) / kW4TileN);
+  return d.M > 96 && p.tiles > 256 * (tiles <= 256 ? 3 : 4) && 2 * d.ldx <= kMaxTileRow &&
+         d.ldw <= kMaxTileRow && d.lds <= kMaxTileRow;
 }
 
 // k_w4_vec: lanes of a row, and the waves along K and rows of a workgroup.
@@ -137,8 +146,8 @@ VecPlan vec_plan(int N, int K) {
 // not in a buffer's range.
 hipgemm_w4_plan plan_of(const hipgemm_w4_desc& d) {
   if (d.M <= 4 || d.K == 0 || 2 * d.ldx > kMaxRow) return {HIPGEMM_W4_VECTORS, 0, 0};
-  if (by_tiles(d)) return {HIPGEMM_W4_TILES, kW4TileM, kW4TileN};
   const SplitPlan p = split_plan(d.M, d.N);
+  if (by_tiles(d, p)) return {HIPGEMM_W4_TILES, kW4TileM, kW4TileN};
   return {HIPGEMM_W4_SPLIT, 16 * p.mt, 16 * p.nt};
 }
 

@@ -28,8 +28,10 @@ def w4_kernel(M, N, K, ldx=None, group=128):
 # ---- which kernels (no GPU) ------------------------------------------------
 
 # 128 x 128 tiles: ragged rows and columns, fewer tiles than workgroups and more.
-TILES = [(97, 24500, 160), (129, 12300, 1120), (300, 8200, 96), (1030, 7400, 32),
+TILES = [(97, 28600, 160), (193, 12300, 1120), (300, 10300, 96), (1030, 7400, 32),
          (1100, 2700, 416)]
+# As many of the large tiles, and nearly as many, that run on the split kernel's.
+NEAR = [(97, 24500, 160), (129, 12300, 1120), (300, 8200, 96), (129, 16600, 224)]
 # Tiles of 16 rows of 64 columns, and of each height.
 SPLIT = [((5, 8200, 1120), 16, 64), ((16, 8300, 160), 16, 64), ((11, 16400, 32), 16, 64),
          ((7, 100, 416), 16, 32), ((20, 8200, 544), 32, 64), ((37, 5000, 160), 48, 32),
@@ -55,6 +57,8 @@ def test_sizes_reach_their_kernels():
     for M, N, K in TILES:
         assert w4_kernel(M, N, K) == ("tiles", 128, 128)
     assert any(-(-M // 128) * -(-N // 128) > 512 for M, N, K in TILES)
+    for size in NEAR:
+        assert w4_kernel(*size)[0] == "split"
     for size, rows, columns in SPLIT:
         assert w4_kernel(*size) == ("split", rows, columns), size
     assert w4_kernel(4, 8200, 64)[0] == w4_kernel(40, 100, 0, 64)[0] == "vectors"
@@ -87,7 +91,7 @@ def test_select_refuses():
 # ---- products of many rows --------------------------------------------------
 
 @gpu_test
-@pytest.mark.parametrize("M,N,K", TILES)
+@pytest.mark.parametrize("M,N,K", TILES + NEAR)
 @pytest.mark.parametrize("group", [32, 96, 128, 256])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 def test_w4_tiles(gpu, M, N, K, group, dtype):
@@ -114,12 +118,14 @@ def test_w4_split(gpu, size, rows, columns, group):
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu_tanh"])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float16, torch.float32])
 def test_w4_tiles_epilogue(gpu, out, act):
-    case(hg, 129, 12300, 512, bias=True, act=act, out_dtype=out, zeros=True, seed=1)
-    case(hg, 300, 8200, 224, "fp4", 32, "e8m0", bias=True, act=act, out_dtype=out, seed=2)
+    for M, N in ((129, 12300), (193, 12300)):
+        case(hg, M, N, 512, bias=True, act=act, out_dtype=out, zeros=True, seed=1)
+    for M, N in ((300, 8200), (300, 10300)):
+        case(hg, M, N, 224, "fp4", 32, "e8m0", bias=True, act=act, out_dtype=out, seed=2)
 
 
 @gpu_test
-@pytest.mark.parametrize("M,N", [(129, 12300), (1100, 2700), (13, 8300)])
+@pytest.mark.parametrize("M,N", [(129, 12300), (193, 12300), (1100, 2700), (13, 8300)])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 def test_w4_strides_and_guards(gpu, M, N, dtype):
     """Rows inside wider tensors; nothing written outside the output's window."""
@@ -140,12 +146,13 @@ def test_w4_strides_and_guards(gpu, M, N, dtype):
 
 
 @gpu_test
+@pytest.mark.parametrize("M", [129, 193])
 @pytest.mark.parametrize("fmt", ["int4", "fp4"])
-def test_w4_tiles_large_activations(gpu, fmt):
+def test_w4_tiles_large_activations(gpu, fmt, M):
     """Activations whose product with an unscaled code overflows fp32, while the
     results do not."""
     g = u.generator(3)
-    M, N, K = 129, 12300, 256
+    N, K = 12300, 256
     x = torch.zeros((M, K), device="cuda", dtype=torch.bfloat16)
     x[:, 17] = 2.0 ** 126
     x[:, 100] = -2.0 ** 125
@@ -156,7 +163,7 @@ def test_w4_tiles_large_activations(gpu, fmt):
 
 
 @gpu_test
-@pytest.mark.parametrize("M,N", [(129, 12300), (1030, 7400), (16, 8300)])
+@pytest.mark.parametrize("M,N", [(129, 12300), (193, 12300), (1030, 7400), (16, 8300)])
 def test_w4_stream_graph_and_repeats(gpu, M, N):
     g = u.generator(11)
     w, s, z = u.four_bit(g, (N,), 1024, "int4", 128, "bfloat16", True)

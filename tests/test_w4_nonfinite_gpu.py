@@ -18,7 +18,7 @@ def hg(gpu):
 
 
 # Tiles of 16 rows by four waves along K, of several row tiles, and of 128 x 128.
-@pytest.mark.parametrize("M,N", [(9, 70), (60, 4100), (200, 150), (131, 12300)])
+@pytest.mark.parametrize("M,N", [(9, 70), (60, 4100), (200, 150), (131, 12300), (193, 12300)])
 @pytest.mark.parametrize("fmt,group,scale,dtype", [
     ("int4", 128, "bfloat16", "bfloat16"), ("int4", 32, "float32", "float16"),
     ("fp4", 96, "float16", "bfloat16"), ("fp4", 32, "e8m0", "bfloat16")])
