@@ -222,17 +222,18 @@ hipgemm_moe_plan turn_plan(int T, int k, int E, int D, int F, int format, int h)
   const int pairs = T * k;
   const double chosen = chosen_experts(T, k, E);
   // Pair by pair while few experts are read twice.  us in a graph, pairs / grouped,
-  // by tokens: int4, 8 of 64 experts of 2048 x 1024, 2 24/37, 6 55/58, 12 87/73; 8 of
-  // 128 of 4096 x 1536, 4 71/90, 8 124/140, 16 237/175;  fp4, 3 of 30 of 2336 x 1056,
-  // 5 24/44, 12 43/56;  e4m3, 4 of 64 of 4096 x 2048, 2 41/51, 4 71/80, 8 126/115; 2
-  // of 8 of 4096 x 14336, 1 66/71, 2 121/116.  (Grouped, 4-bit weights stream at 3 to
-  // 4.6 TB/s, e4m3 ones at 5 to 5.8.)
+  // by tokens, ids spread evenly: int4, 8 of 64 experts of 2048 x 1024, 2 24/29, 12
+  // 86/62; 8 of 128 of 4096 x 1536, 4 71/81, 8 120/119, 16 223/175;  fp4, 3 of 30 of 2336
+  // x 1056, 5 25/40;  e4m3, 4 of 64 of 4096 x 2048, 2 41/51, 4 71/80, 8 127/115; 2 of 8
+  // of 4096 x 14336, 1 69/72, 2 121/115.  (Grouped, 4-bit weights stream at 3 to 4.6
+  // TB/s, e4m3 ones at 5 to 5.8.)
   // And while what is read again is less than 64 MB: grouping is a third launch and
-  // the tables.  Pairs / grouped, MB: e4m3 10 tokens, 1 of 24 of 384 x 640, 1, 9.8/20;
-  // 2, 7 of 24 of 768 x 1536, 7, 18.6/30;  int4 3, 3 of 4 of 1536 x 384, 4, 12/24;  64, 2
-  // of 4 of 256 x 512, 24, 16/29;  e4m3 64, 4 of 8 of 256 x 256, 49, 12.5/31;  fp4 10,
-  // 5 of 16 of 4096 x 256, 54, 34/28;  32, 4 of 64 of 1024 x 512, 57, 29/36;  e4m3 41, 1
-  // of 16 of 1024 x 896, 72, 28.5/26;  int4 64, 8 of 128 of 512 x 512, 152, 50/38.
+  // the tables.  Pairs / grouped, MB: e4m3 10 tokens, 1 of 24 of 384 x 640, 1, 9.5/20;
+  // 2, 7 of 24 of 768 x 1536, 7, 18.7/29;  int4 3, 3 of 4 of 1536 x 384, 4, 12/24;  64, 2
+  // of 4 of 256 x 512, 24, 16/29;  6, 8 of 64 of 2048 x 1024, 40, 54/51;  e4m3 64, 4 of 8
+  // of 256 x 256, 49, 12.5/33;  fp4 12, 3 of 30 of 2336 x 1056, 54, 44/53;  32, 4 of 64 of
+  // 1024 x 512, 57, 30/36;  e4m3 41, 1 of 16 of 1024 x 896, 72, 29/26;  int4 64, 8 of 128
+  // of 512 x 512, 152, 50/38.  Decided wrongly: fp4 10, 5 of 16 of 4096 x 256, 54, 34/28.
   const bool e4m3 = format == HIPGEMM_W8_E4M3;
   const double expert_bytes = 3.0 * D * F * (e4m3 ? 1.0 : 0.5);
   if (!grouped(D, F) || pairs <= chosen * (e4m3 ? 1.13 : 1.5) ||
