@@ -298,8 +298,9 @@ def moe_experts(x, ids, weights, w13, scales13, w2, scales2, *, zeros13=None,
     group_size elements of a row, (E, rows, groups), as for w4_gemm ("int4",
     "fp4").  D, F and group_size are multiples of 32.  activation: of the gate
     (None, "relu", "gelu_tanh", "silu").  out_dtype: bfloat16, float16 or float32,
-    x's where None; h is held to 16 significant bits, to 24 for float32 results.  Made for up to 64 tokens (each expert's weights are read once
-    for up to 16 of its tokens); any number works.  workspace: a uint8 device
+    x's where None; h is held to 16 significant bits, to 24 for float32 results.
+    Made for up to 64 tokens; any number works, in turns of 512 / k that each read
+    the chosen experts' weights (moe_select: how often).  workspace: a uint8 device
     tensor of moe_workspace_size bytes; allocated per call where None."""
     torch = _torch()
     x_types, _, o_types = _types()

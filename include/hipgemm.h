@@ -452,13 +452,16 @@ hipError_t hipgemm_moe_route(const void *logits, int type, int T, int E, int k,
  * row as in hipgemm_w4_gemm, or HIPGEMM_W8_E4M3 with one float scale per row
  * (scale_type F32, lds 1: E x 2F and E x D).  An id outside [0, E) is skipped: a
  * token without any gives zeros.  Sums are fp32; h is held to 16 significant
- * bits between the two kernels, to fp32's 24 where out_dtype is F32.  Each chosen expert's weights are read once for
- * up to 16 of its tokens, so it is made for a few tokens (up to 64); more go in
- * turns of at most HIPGEMM_MOE_MAX_PAIRS / k.
+ * bits between the two kernels, to fp32's 24 where out_dtype is F32.  Made for a few
+ * tokens (up to 64); more go in turns of at most HIPGEMM_MOE_MAX_PAIRS / k.  In a turn
+ * an expert's weights are read for each of its tokens while few are read twice
+ * (pair by pair: hipgemm_moe_select), else once for up to 16 or 32 of them, W13 for
+ * no more than 37120 / D.  Always pair by pair for D above 37120 or F above 65536.
  * D, F, group_size multiples of 32; matrices 16-byte aligned, with row and
  * expert strides of multiples of 16 bytes; k <= 64.  Workspace:
  * hipgemm_moe_workspace_size bytes, 16-byte aligned, of any content; calls that
- * may run concurrently must not share one.  Two or three launches per turn on `stream`.
+ * may run concurrently must not share one.  Two launches per turn on `stream`, three
+ * grouped.
  * Zero-initialise the struct and set `size`.  No reference counterpart.
  */
 enum { HIPGEMM_W8_E4M3 = 2 };

@@ -5,8 +5,10 @@
 //   k_moe_down  o[q][p] = h[p] W2[e]^T over the q-th part of F
 //   k_moe_sum   y[t] = sum_j sum_q o[q][t k + j]
 //
-// What bounds it: each chosen expert's weights are read once, whatever the
-// number of its tokens, so the first two stream weights past the few rows that
+// What bounds it: each chosen expert's weights, read once for as many of its tokens
+// as LDS has room for (going up 37120 / D rows of x, at most 16, or 32 where experts have
+// many; going down as many of h, for which F is cut into parts), so the first two
+// stream weights past the few rows that
 // need them (w4_stream.hpp: Stream), one workgroup per CU, which share the work
 // evenly: all tiles of weights of all chosen experts, in order, cut into as many
 // pieces as there are workgroups.  Which experts those are, and their pairs, each
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(512) void k_moe_up(MoeArgs g) {
       const int f0 = min((item - q * tiles) * kCols + 16 * st.set(), g.F - 16);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        st.set_tile(n, g.w13 + e * g.w13_expert + ((long long)n * g.F + f0) * g.w13_row, 16);
+        st.set_tile(n, g.w13 + e * g.w13_expert + ((long long)n * g.F + f0) * g.w13_row);
         const long long r = (long long)st.scale_tile(n) * g.F + f0 + (lane_id() & 15);
         st.sp[n] = g.s13 + e * g.s13_expert + r * g.s13_row;
         if constexpr (kW == kWInt4Z) st.zp[n] = g.z13 + e * g.z13_expert + r * g.z13_row;
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(512) void k_moe_down(MoeArgs g) {
       const int d0 = min((item - q * tiles) * S::kTile + 32 * st.set(), g.D - 32);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        st.set_tile(n, g.w2 + e * g.w2_expert + (long long)(d0 + 16 * n) * g.w2_row, 16);
+        st.set_tile(n, g.w2 + e * g.w2_expert + (long long)(d0 + 16 * n) * g.w2_row);
         const long long r = d0 + 16 * st.scale_tile(n) + (lane_id() & 15);
         st.sp[n] = g.s2 + e * g.s2_expert + r * g.s2_row;
         if constexpr (kW == kWInt4Z) st.zp[n] = g.z2 + e * g.z2_expert + r * g.z2_row;

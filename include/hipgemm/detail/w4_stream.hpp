@@ -1,6 +1,5 @@
 // Streams quantised weights past a few rows of 16-bit activations: the inner
-// part of the products with 4-bit weights for 5 rows and more, and of the
-// experts' products.
+// part of the experts' products where they are grouped (moe.hpp).
 //
 // What bounds it is the weights' bytes, 9 per CU and cycle at most, so all that
 // matters is that enough of them are on their way all the time, from the first
@@ -133,9 +132,9 @@ struct Stream {
     const int g = lane_id() >> 4;
     return kMode == kCoarse ? g >> 1 : kMode == kNone ? g & 1 : n;
   }
-  // Tile n: 16 rows at w, of which `left` exist (1 or more).
-  __device__ __forceinline__ void set_tile(int n, const uint8_t* w, int left) {
-    wb[n] = make_rsrc(w, (uint32_t)(min(left, 16)) * ldw);
+  // Tile n: 16 rows at w.
+  __device__ __forceinline__ void set_tile(int n, const uint8_t* w) {
+    wb[n] = make_rsrc(w, 16 * ldw);
   }
 
   // The unit at k to the ring's slot; past k_end nothing is fetched.  Always

@@ -8,7 +8,7 @@
 // one tile each, with stages of their own, so nobody waits for anybody until the
 // sums are added; up to 160 KiB of stages are on their way.  bf16, us in a graph:
 // 16 x 14336 x 4096 fp4 in groups of 32 16.1 (2.0 TB/s), 16 x 28672 x 8192 int4 52,
-// 64 x 14336 x 4096 int4 24, 37 x 5000 x 3584 int4 in groups of 64 21.  (With all of
+// 64 x 14336 x 4096 int4 24, 37 x 5000 x 3584 int4 in groups of 64 19.  (With all of
 // x of a group in LDS and the weights streaming past it the same took 18.6, 53, 104,
 // 35: x came in again for every 32 columns.)
 //
