@@ -198,6 +198,18 @@ def test_experts(gpu, T, E, k, D, F, fmt, zeros):
 
 
 @gpu_test
+@pytest.mark.parametrize("size", GROUPED + LIMITS)
+@pytest.mark.parametrize("fmt", ["e4m3", "int4", "fp4"])
+def test_experts_float32(gpu, size, fmt):
+    """h in three parts: fewer rows of it in LDS, more parts of F."""
+    T, E, k, D, F = size
+    assert hg.moe_select(T, k, E, D, F, fmt, torch.float32)
+    for group in (128,) if fmt == "e4m3" else (32, 128):
+        check(hg, make(T + E + k, *size, fmt, group, "e8m0" if fmt == "fp4" else "float16"), fmt,
+              group, out_dtype=torch.float32)
+
+
+@gpu_test
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("scale", ["bfloat16", "float16", "float32", "e8m0"])
 @pytest.mark.parametrize("group", [32, 64, 96, 128, 256])
