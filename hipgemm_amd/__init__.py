@@ -159,6 +159,11 @@ def lib() -> ctypes.CDLL:
     L.hipgemm_moe_route.argtypes = [vp, ci, ci, ci, ci, ctypes.c_longlong, ci,
                                     ci, ctypes.c_float, vp, vp, vp]
     L.hipgemm_moe_route.restype = ci
+    for name in ("hipgemm_linear", "hipgemm_linear_backward"):
+        getattr(L, name).argtypes = [vp, vp]
+        getattr(L, name).restype = ci
+        getattr(L, name + "_workspace_size").argtypes = [vp]
+        getattr(L, name + "_workspace_size").restype = ctypes.c_size_t
     L.hipgemm_workspace_size.argtypes = [ci, ci, ci, ci]
     L.hipgemm_workspace_size.restype = ctypes.c_size_t
     L.hipgemm_fp8_gemm_4wave_256x256x128.argtypes = [vp, vp, vp, ci, ci, ci,
@@ -659,4 +664,7 @@ def fp8_gemm_4wave_256x256x128(A, B_T, C, stream=None):
 from .serving import *  # noqa: E402,F401,F403
 from . import serving as _serving  # noqa: E402
 
-__all__ += _serving.__all__
+from .dense import *  # noqa: E402,F401,F403
+from . import dense as _dense  # noqa: E402
+
+__all__ += _serving.__all__ + _dense.__all__

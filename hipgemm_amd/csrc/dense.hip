@@ -1,0 +1,371 @@
+// hipgemm_linear and hipgemm_linear_backward: arguments, the choice of tiles, launches.
+#include "hipgemm.h"
+
+#include "kernels.hpp"
+
+#include "hipgemm/detail/dense.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+#define HIPGEMM_DENSE(L)                             \
+  const void* dense_tile_bf16_##L(int tile, bool split); \
+  const void* dense_tile_f16_##L(int tile, bool split);
+HIPGEMM_DENSE(nt)
+HIPGEMM_DENSE(nn)
+HIPGEMM_DENSE(tn)
+HIPGEMM_DENSE(gated)
+#undef HIPGEMM_DENSE
+
+const void* dense_tile(int x, int layout, int tile, bool split) {
+  const bool b = x == detail::kInBf16;
+  switch (layout) {
+    case kDenseNT: return b ? dense_tile_bf16_nt(tile, split) : dense_tile_f16_nt(tile, split);
+    case kDenseNN: return b ? dense_tile_bf16_nn(tile, split) : dense_tile_f16_nn(tile, split);
+    case kDenseTN: return b ? dense_tile_bf16_tn(tile, split) : dense_tile_f16_tn(tile, split);
+    default:
+      return b ? dense_tile_bf16_gated(tile, split) : dense_tile_f16_gated(tile, split);
+  }
+}
+
+}  // namespace kernels
+}  // namespace hipgemm
+
+namespace {
+
+using namespace hipgemm::detail;
+namespace hk = hipgemm::kernels;
+
+template <bool kGated>
+__global__ __launch_bounds__(256) void k_dense_reduce(DenseArgs g) {
+  dense_reduce_body<kGated>(g);
+}
+template <int kX, bool kGated>
+__global__ __launch_bounds__(256) void k_dense_slope(SlopeArgs g) {
+  __shared__ float sums[8 * 256];
+  dense_slope_body<kX, kGated>(g, sums);
+}
+__global__ __launch_bounds__(256) void k_dense_columns(const float* columns, int blocks, int N,
+                                                       uint8_t* out, int type) {
+  dense_columns_body(columns, blocks, N, out, type);
+}
+
+bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// 256 rows of an operand, and of a result, are addressed with 31 bits.
+constexpr long long kMaxLd = 1 << 21;
+constexpr int kMaxRows = 1 << 30;
+constexpr size_t kAlign = 256;
+size_t padded(size_t bytes) { return (bytes + kAlign - 1) / kAlign * kAlign; }
+
+template <class Args>
+hipError_t launch(const void* fn, dim3 grid, Args& g, hipStream_t stream) {
+  if (!fn) return hipErrorInvalidValue;
+  void* args[] = {&g};
+  return hipLaunchKernel(fn, grid, dim3(256), args, 0, stream);
+}
+
+// ---- one product ----------------------------------------------------------------
+
+struct Plan {
+  int tile, slices, slice_steps;
+  long long units;
+};
+Plan plan_of(int layout, int M, int N, int K) {
+  Plan p{0, 1, 0, 0};
+  const hk::TileShape s = hk::kDenseTiles[p.tile];
+  const int cols = layout == hk::kDenseGated ? s.bn / 2 : s.bn;
+  p.units = (((long long)M + s.bm - 1) / s.bm) * (((long long)N + cols - 1) / cols) * p.slices;
+  (void)K;
+  return p;
+}
+
+// Columns of a partial sum's row.
+long long partial_columns(int layout, int N) {
+  const long long n = ((long long)N + 7) & ~7ll;
+  return layout == hk::kDenseGated ? 2 * n : n;
+}
+size_t partial_bytes(int layout, const Plan& p, int M, int N) {
+  if (p.slices == 1) return 0;
+  return padded(4ull * (size_t)p.slices * (size_t)M * (size_t)partial_columns(layout, N));
+}
+
+// g: operands, sizes and epilogue; ws: partial_bytes.
+hipError_t product(int x, int layout, DenseArgs& g, void* ws, hipStream_t stream) {
+  const Plan p = plan_of(layout, g.M, g.N, g.K);
+  const hk::TileShape s = hk::kDenseTiles[p.tile];
+  const int cols = layout == hk::kDenseGated ? s.bn / 2 : s.bn;
+  g.group_m = default_group_m((g.M + s.bm - 1) / s.bm, (g.N + cols - 1) / cols);
+  g.slices = p.slices;
+  g.slice_steps = p.slice_steps;
+  g.partial = static_cast<float*>(ws);
+  g.ldpart = partial_columns(layout, g.N);
+  const long long most = 256;
+  hipError_t e = launch(hk::dense_tile(x, layout, p.tile, p.slices > 1),
+                        dim3((unsigned)(p.units < most ? p.units : most)), g, stream);
+  if (e != hipSuccess || p.slices == 1) return e;
+  const long long threads = (long long)g.M * ((g.N + 7) / 8);
+  const bool gated = layout == hk::kDenseGated;
+  const void* fn = gated ? (const void*)&k_dense_reduce<true> : (const void*)&k_dense_reduce<false>;
+  return launch(fn, dim3((unsigned)((threads + 255) / 256)), g, stream);
+}
+
+// A matrix of rows that take 16-byte accesses at columns of multiples of eight.
+bool fits16(const void* p, long long ld, int bytes) {
+  return !p || (aligned(p, 16) && ld * bytes % 16 == 0);
+}
+bool operand(const void* p, long long ld, long long columns) {
+  return p && aligned(p, 16) && ld >= columns && ld % 8 == 0 && ld <= kMaxLd;
+}
+bool result(const void* p, long long ld, long long columns, int out) {
+  return p && aligned(p, (uintptr_t)out_bytes(out)) && ld >= columns && ld <= kMaxLd;
+}
+int in_bytes(int type) { return type == kInF32 ? 4 : 2; }
+
+bool common(int M, int N, int K, int gated, int type, int act) {
+  return M >= 0 && M <= kMaxRows && N >= 0 && K >= 0 && K % 8 == 0 && (gated == 0 || gated == 1) &&
+         (!gated || N % 8 == 0) && (long long)N * (gated ? 2 : 1) <= kMaxLd && K <= kMaxLd &&
+         (type == HIPGEMM_IN_BF16 || type == HIPGEMM_IN_F16) && act >= 0 &&
+         act <= HIPGEMM_ACT_SILU;
+}
+
+// ---- forward ----------------------------------------------------------------------
+
+hipError_t check(const hipgemm_linear_desc* desc) {
+  if (!desc || desc->size != sizeof(hipgemm_linear_desc)) return hipErrorInvalidValue;
+  const hipgemm_linear_desc& d = *desc;
+  if (!common(d.M, d.N, d.K, d.gated, d.type, d.activation) || d.out_dtype < 0 ||
+      d.out_dtype > HIPGEMM_OUT_F32 || d.bias_type < 0 || d.bias_type > HIPGEMM_IN_F16 ||
+      d.residual_type < 0 || d.residual_type > HIPGEMM_IN_F16 || d.pre_dtype < 0 ||
+      d.pre_dtype > HIPGEMM_OUT_F32 || (d.gated && d.residual))
+    return hipErrorInvalidValue;
+  if (d.M == 0 || d.N == 0) return hipSuccess;
+  const long long rows = d.gated ? 2ll * d.N : d.N;
+  if (!result(d.y, d.ldy, d.N, d.out_dtype) ||
+      (d.K > 0 && (!operand(d.x, d.ldx, d.K) || !operand(d.weight, d.ldw, d.K))) ||
+      (d.bias && !aligned(d.bias, in_bytes(d.bias_type))) ||
+      (d.residual && (!aligned(d.residual, in_bytes(d.residual_type)) || d.ldr < d.N)) ||
+      (d.pre && !result(d.pre, d.ldp, rows, d.pre_dtype)))
+    return hipErrorInvalidValue;
+  return hipSuccess;
+}
+
+size_t forward_bytes(const hipgemm_linear_desc& d) {
+  const int layout = d.gated ? hk::kDenseGated : hk::kDenseNT;
+  return partial_bytes(layout, plan_of(layout, d.M, d.N, d.K), d.M, d.N);
+}
+
+hipError_t forward(const hipgemm_linear_desc& d, hipStream_t stream) {
+  const size_t need = forward_bytes(d);
+  if (need && (!d.workspace || d.workspace_bytes < need || !aligned(d.workspace, kAlign)))
+    return hipErrorInvalidValue;
+  DenseArgs g{};
+  g.a = static_cast<const uint8_t*>(d.x);
+  g.b = static_cast<const uint8_t*>(d.weight);
+  g.lda = 2 * d.ldx;
+  g.ldb = 2 * d.ldw;
+  g.up = 2 * d.ldw * d.N;
+  g.M = d.M;
+  g.N = d.N;
+  g.K = d.K;
+  DenseEpi& e = g.epi;
+  e.y = static_cast<uint8_t*>(d.y);
+  e.bias = static_cast<const uint8_t*>(d.bias);
+  e.r = static_cast<const uint8_t*>(d.residual);
+  e.pre = static_cast<uint8_t*>(d.pre);
+  e.ldy = d.ldy;
+  e.ldr = d.ldr;
+  e.ldp = d.ldp;
+  e.up = d.N;
+  e.act = d.activation;
+  e.y_type = d.out_dtype;
+  e.p_type = d.pre_dtype;
+  e.b_type = d.bias_type;
+  e.r_type = d.residual_type;
+  e.vec = d.N % 8 == 0 && fits16(d.y, d.ldy, out_bytes(d.out_dtype)) &&
+          fits16(d.residual, d.ldr, in_bytes(d.residual_type)) && fits16(d.pre, d.ldp, out_bytes(d.pre_dtype)) &&
+          fits16(d.bias, 8, 2);
+  return product(d.type, d.gated ? hk::kDenseGated : hk::kDenseNT, g, d.workspace, stream);
+}
+
+// ---- backward ---------------------------------------------------------------------
+
+hipError_t check(const hipgemm_linear_grad_desc* desc) {
+  if (!desc || desc->size != sizeof(hipgemm_linear_grad_desc)) return hipErrorInvalidValue;
+  const hipgemm_linear_grad_desc& d = *desc;
+  if (!common(d.M, d.N, d.K, d.gated, d.type, d.activation) || d.dy_type < 0 ||
+      d.dy_type > HIPGEMM_IN_F16 || d.pre_type < 0 || d.pre_type > HIPGEMM_IN_F16 || d.dx_dtype < 0 || d.dx_dtype > HIPGEMM_OUT_F32 ||
+      d.dw_dtype < 0 || d.dw_dtype > HIPGEMM_OUT_F32 || d.db_dtype < 0 ||
+      d.db_dtype > HIPGEMM_OUT_F32)
+    return hipErrorInvalidValue;
+  const long long cols = d.gated ? 2ll * d.N : d.N;
+  if (d.M > 0 && d.N > 0) {
+    if (!d.dy || !aligned(d.dy, in_bytes(d.dy_type)) || d.lddy < d.N) return hipErrorInvalidValue;
+    if ((d.gated || d.activation != HIPGEMM_ACT_NONE) &&
+        (!d.pre || !aligned(d.pre, in_bytes(d.pre_type)) || d.ldp < cols))
+      return hipErrorInvalidValue;
+    if (d.K > 0 && ((d.dx && !operand(d.weight, d.ldw, d.K)) ||
+                    (d.dw && !operand(d.x, d.ldx, d.K))))
+      return hipErrorInvalidValue;
+  }
+  if ((d.dx && !result(d.dx, d.lddx, d.K, d.dx_dtype)) ||
+      (d.dw && !result(d.dw, d.lddw, d.K, d.dw_dtype)) ||
+      (d.db && !aligned(d.db, (uintptr_t)out_bytes(d.db_dtype))))
+    return hipErrorInvalidValue;
+  return hipSuccess;
+}
+
+// Where dz is dy itself: nothing to multiply by, in the operands' type, in rows that the
+// products read as they are.
+bool as_is(const hipgemm_linear_grad_desc& d) {
+  return !d.gated && d.activation == HIPGEMM_ACT_NONE && d.dy_type == d.type && d.N % 8 == 0 &&
+         aligned(d.dy, 16) && d.lddy % 8 == 0 && d.lddy <= kMaxLd;
+}
+
+struct GradPlan {
+  long long cols, ldz;  // of dz
+  bool own;             // dz lies in the workspace
+  int blocks, rows;     // of the column sums
+  size_t dz, columns, partial;
+};
+GradPlan grad_plan(const hipgemm_linear_grad_desc& d) {
+  GradPlan p{};
+  p.cols = d.gated ? 2ll * d.N : d.N;
+  p.ldz = (p.cols + 7) & ~7ll;
+  p.own = !as_is(d) && (d.dx || d.dw);
+  // Blocks of 256 columns by `rows` rows: four to a CU, of eight rows at least.
+  const int across = (d.N + 255) / 256;
+  int blocks = across ? (1024 + across - 1) / across : 1;
+  if (blocks > (d.M + 7) / 8) blocks = (d.M + 7) / 8;
+  if (blocks < 1) blocks = 1;
+  p.rows = ((d.M + blocks - 1) / blocks + 7) / 8 * 8;
+  if (p.rows < 8) p.rows = 8;
+  p.blocks = (d.M + p.rows - 1) / p.rows;
+  if (p.blocks < 1) p.blocks = 1;
+  p.dz = p.own ? padded(2ull * (size_t)d.M * (size_t)p.ldz) : 0;
+  p.columns = d.db ? padded(4ull * (size_t)p.blocks * (size_t)p.cols) : 0;
+  size_t part = 0;
+  if (d.dx)
+    part = partial_bytes(hk::kDenseNN, plan_of(hk::kDenseNN, d.M, d.K, (int)p.cols), d.M, d.K);
+  if (d.dw) {
+    const size_t w = partial_bytes(hk::kDenseTN, plan_of(hk::kDenseTN, (int)p.cols, d.K, d.M),
+                                   (int)p.cols, d.K);
+    if (w > part) part = w;
+  }
+  p.partial = part;
+  return p;
+}
+
+void plain_epilogue(DenseArgs& g, void* y, long long ldy, int out) {
+  g.epi.y = static_cast<uint8_t*>(y);
+  g.epi.ldy = ldy;
+  g.epi.y_type = out;
+  g.epi.vec = g.N % 8 == 0 && fits16(y, ldy, out_bytes(out));
+}
+
+hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
+  const GradPlan p = grad_plan(d);
+  const size_t need = p.dz + p.columns + p.partial;
+  if (need && (!d.workspace || d.workspace_bytes < need || !aligned(d.workspace, kAlign)))
+    return hipErrorInvalidValue;
+  uint8_t* ws = static_cast<uint8_t*>(d.workspace);
+  uint8_t* dz = ws;
+  float* columns = reinterpret_cast<float*>(ws + p.dz);
+  void* partial = ws + p.dz + p.columns;
+  if (p.own || d.db) {
+    SlopeArgs s{};
+    s.dy = static_cast<const uint8_t*>(d.dy);
+    s.pre = d.activation == HIPGEMM_ACT_NONE && !d.gated ? nullptr
+                                                         : static_cast<const uint8_t*>(d.pre);
+    s.dz = p.own ? dz : nullptr;
+    s.columns = d.db ? columns : nullptr;
+    s.lddy = d.lddy;
+    s.ldp = d.ldp;
+    s.lddz = p.ldz;
+    s.M = d.M;
+    s.N = d.N;
+    s.act = d.activation;
+    s.dy_type = d.dy_type;
+    s.p_type = d.pre_type;
+    s.rows = p.rows;
+    s.vec = fits16(d.dy, d.lddy, in_bytes(d.dy_type)) && fits16(s.pre, d.ldp, in_bytes(d.pre_type));
+    const dim3 grid((unsigned)((d.N + 255) / 256), (unsigned)p.blocks);
+    const bool b = d.type == HIPGEMM_IN_BF16;
+    const void* fn = d.gated ? (b ? (const void*)&k_dense_slope<kInBf16, true>
+                                  : (const void*)&k_dense_slope<kInF16, true>)
+                             : (b ? (const void*)&k_dense_slope<kInBf16, false>
+                                  : (const void*)&k_dense_slope<kInF16, false>);
+    if (d.N > 0) {
+      const hipError_t e = launch(fn, grid, s, stream);
+      if (e != hipSuccess) return e;
+      if (d.db) {
+        int blocks = p.blocks, cols = (int)p.cols, type = d.db_dtype;
+        uint8_t* out = static_cast<uint8_t*>(d.db);
+        const float* from = columns;
+        void* args[] = {&from, &blocks, &cols, &out, &type};
+        const hipError_t e2 =
+            hipLaunchKernel((const void*)&k_dense_columns, dim3((unsigned)((cols + 255) / 256)),
+                            dim3(256), args, 0, stream);
+        if (e2 != hipSuccess) return e2;
+      }
+    }
+  }
+  const uint8_t* z = p.own ? dz : static_cast<const uint8_t*>(d.dy);
+  const long long ldz = p.own ? p.ldz : d.lddy;
+  if (d.dx && d.M > 0 && d.K > 0) {
+    DenseArgs g{};
+    g.a = z;
+    g.lda = 2 * ldz;
+    g.b = static_cast<const uint8_t*>(d.weight);
+    g.ldb = 2 * d.ldw;
+    g.M = d.M;
+    g.N = d.K;
+    g.K = (int)p.cols;
+    plain_epilogue(g, d.dx, d.lddx, d.dx_dtype);
+    const hipError_t e = product(d.type, hk::kDenseNN, g, partial, stream);
+    if (e != hipSuccess) return e;
+  }
+  if (d.dw && d.N > 0 && d.K > 0) {
+    DenseArgs g{};
+    g.a = z;
+    g.lda = 2 * ldz;
+    g.b = static_cast<const uint8_t*>(d.x);
+    g.ldb = 2 * d.ldx;
+    g.M = (int)p.cols;
+    g.N = d.K;
+    g.K = d.M;
+    plain_epilogue(g, d.dw, d.lddw, d.dw_dtype);
+    const hipError_t e = product(d.type, hk::kDenseTN, g, partial, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+extern "C" size_t hipgemm_linear_workspace_size(const hipgemm_linear_desc* desc) {
+  if (!desc || desc->size != sizeof(*desc) ||
+      !common(desc->M, desc->N, desc->K, desc->gated, desc->type, desc->activation) ||
+      desc->M == 0 || desc->N == 0)
+    return 0;
+  return forward_bytes(*desc);
+}
+
+extern "C" hipError_t hipgemm_linear(const hipgemm_linear_desc* desc, hipStream_t stream) {
+  const hipError_t e = check(desc);
+  return e != hipSuccess || desc->M == 0 || desc->N == 0 ? e : forward(*desc, stream);
+}
+
+extern "C" size_t hipgemm_linear_backward_workspace_size(const hipgemm_linear_grad_desc* desc) {
+  if (!desc || desc->size != sizeof(*desc) ||
+      !common(desc->M, desc->N, desc->K, desc->gated, desc->type, desc->activation))
+    return 0;
+  const GradPlan p = grad_plan(*desc);
+  return p.dz + p.columns + p.partial;
+}
+
+extern "C" hipError_t hipgemm_linear_backward(const hipgemm_linear_grad_desc* desc,
+                                              hipStream_t stream) {
+  const hipError_t e = check(desc);
+  return e != hipSuccess ? e : backward(*desc, stream);
+}

@@ -1,0 +1,12 @@
+// Products of bf16 operands: gate and up rows.
+#include "kdense.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* dense_tile_bf16_gated(int tile, bool split) {
+  return dense_tile_of<detail::kInBf16, false, false, true>(tile, split);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

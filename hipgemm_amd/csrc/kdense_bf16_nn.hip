@@ -1,0 +1,12 @@
+// Products of bf16 operands: the second operand across K.
+#include "kdense.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* dense_tile_bf16_nn(int tile, bool split) {
+  return dense_tile_of<detail::kInBf16, false, true, false>(tile, split);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

@@ -1,0 +1,12 @@
+// Products of f16 operands: gate and up rows.
+#include "kdense.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* dense_tile_f16_gated(int tile, bool split) {
+  return dense_tile_of<detail::kInF16, false, false, true>(tile, split);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

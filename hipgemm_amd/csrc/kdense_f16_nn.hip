@@ -1,0 +1,12 @@
+// Products of f16 operands: the second operand across K.
+#include "kdense.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* dense_tile_f16_nn(int tile, bool split) {
+  return dense_tile_of<detail::kInF16, false, true, false>(tile, split);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

@@ -1,0 +1,12 @@
+// Products of f16 operands: both operands along K.
+#include "kdense.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* dense_tile_f16_nt(int tile, bool split) {
+  return dense_tile_of<detail::kInF16, false, false, false>(tile, split);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

@@ -1,0 +1,272 @@
+"""Products of 16-bit activations with 16-bit weights and the epilogues of a
+feed-forward block, with their backward passes (include/hipgemm.h: hipgemm_linear
+and hipgemm_linear_backward), on torch tensors.
+
+linear, linear_backward              y = act(x W^T + b) + r
+gated_linear, gated_linear_backward  y = act(x Wg^T + bg) * (x Wu^T + bu)
+
+Like the rest of the package these run on the GPU only, on the current stream or
+the one given, and raise HipGemmError for arguments that they do not take.  They
+record no gradient: hipgemm_amd.torch_dense has operators and modules that do.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import functools
+
+from . import ACTIVATIONS, OUT_BF16, OUT_F16, OUT_F32, _check, _torch, lib
+from .serving import _bad, _on, _stream_handle
+
+__all__ = ["linear", "linear_backward", "gated_linear", "gated_linear_backward",
+           "LinearDesc", "LinearGradDesc", "linear_raw", "linear_backward_raw",
+           "linear_workspace_size", "linear_backward_workspace_size"]
+
+_vp, _ci, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+
+
+class LinearDesc(ctypes.Structure):
+    """hipgemm_linear_desc (include/hipgemm.h)."""
+    _fields_ = [("size", ctypes.c_size_t), ("x", _vp), ("weight", _vp), ("bias", _vp),
+                ("residual", _vp), ("y", _vp), ("pre", _vp), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t), ("ldx", _ll), ("ldw", _ll),
+                ("ldr", _ll), ("ldy", _ll), ("ldp", _ll), ("M", _ci), ("N", _ci),
+                ("K", _ci), ("gated", _ci), ("type", _ci), ("bias_type", _ci),
+                ("residual_type", _ci), ("out_dtype", _ci), ("pre_dtype", _ci),
+                ("activation", _ci)]
+
+
+class LinearGradDesc(ctypes.Structure):
+    """hipgemm_linear_grad_desc (include/hipgemm.h)."""
+    _fields_ = [("size", ctypes.c_size_t), ("dy", _vp), ("x", _vp), ("weight", _vp),
+                ("pre", _vp), ("dx", _vp), ("dw", _vp), ("db", _vp), ("workspace", _vp),
+                ("workspace_bytes", ctypes.c_size_t), ("lddy", _ll), ("ldx", _ll),
+                ("ldw", _ll), ("ldp", _ll), ("lddx", _ll), ("lddw", _ll), ("M", _ci),
+                ("N", _ci), ("K", _ci), ("gated", _ci), ("type", _ci), ("dy_type", _ci),
+                ("pre_type", _ci), ("dx_dtype", _ci), ("dw_dtype", _ci), ("db_dtype", _ci),
+                ("activation", _ci)]
+
+
+_DESC_BYTES = ctypes.sizeof(LinearDesc)
+_GRAD_BYTES = ctypes.sizeof(LinearGradDesc)
+
+
+@functools.lru_cache(maxsize=1)
+def _types():
+    """Codes by dtype: operands, inputs, outputs."""
+    t = _torch()
+    return ({t.bfloat16: 1, t.float16: 2}, {t.float32: 0, t.bfloat16: 1, t.float16: 2},
+            {t.bfloat16: OUT_BF16, t.float16: OUT_F16, t.float32: OUT_F32})
+
+
+def linear_raw(desc: "LinearDesc", stream: int = 0) -> int:
+    """Call hipgemm_linear; returns hipError_t."""
+    return int(lib().hipgemm_linear(ctypes.byref(desc), stream or None))
+
+
+def linear_backward_raw(desc: "LinearGradDesc", stream: int = 0) -> int:
+    """Call hipgemm_linear_backward; returns hipError_t."""
+    return int(lib().hipgemm_linear_backward(ctypes.byref(desc), stream or None))
+
+
+def linear_workspace_size(desc: "LinearDesc") -> int:
+    """Workspace bytes hipgemm_linear needs for a descriptor."""
+    return int(lib().hipgemm_linear_workspace_size(ctypes.byref(desc)))
+
+
+def linear_backward_workspace_size(desc: "LinearGradDesc") -> int:
+    """Workspace bytes hipgemm_linear_backward needs for a descriptor."""
+    return int(lib().hipgemm_linear_backward_workspace_size(ctypes.byref(desc)))
+
+
+def _device(dev, stream):
+    """The tensors' device as the current one."""
+    if stream is not None and stream.device != dev:
+        _bad(f"stream is on {stream.device}, x on {dev}")
+    if dev.index == _torch()._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return _torch().cuda.device(dev)
+
+
+def _operand(t, name, dtype, device):
+    """The row stride of a matrix that the products read as it is."""
+    if t.dim() != 2 or t.dtype != dtype or t.device != device:
+        _bad(f"{name} must be a 2-D {dtype} tensor on {device}, got {tuple(t.shape)} "
+             f"{t.dtype} on {t.device}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        _bad(f"{name} must have unit stride along its rows")
+    ld = t.stride(0) if rows > 1 else cols
+    if rows and cols and (t.data_ptr() % 16 or ld % 8 or ld < cols):
+        _bad(f"rows of {name} must start on 16 bytes")
+    return ld
+
+
+def _matrix(t, name, shape, dtypes, device):
+    """The code of a (M, N) matrix' type and its row stride."""
+    code = dtypes.get(t.dtype)
+    if code is None or tuple(t.shape) != shape or t.device != device:
+        _bad(f"{name} must be a {shape} bfloat16, float16 or float32 tensor on {device}, got "
+             f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if shape[1] > 1 and t.stride(1) != 1:
+        _bad(f"{name} must have unit stride along its rows")
+    ld = t.stride(0) if shape[0] > 1 else shape[1]
+    if ld < shape[1]:
+        _bad(f"rows of {name} must not overlap")
+    return code, ld
+
+
+def _sizes(x, weight, gated):
+    operands = _types()[0]
+    code = operands.get(x.dtype)
+    if code is None or x.dim() != 2 or not x.is_cuda:
+        _bad(f"x must be a 2-D bfloat16 or float16 device tensor, got {x.dtype} on {x.device}")
+    if weight.dim() != 2 or weight.shape[1] != x.shape[1]:
+        _bad(f"K mismatch: x {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    (M, K), N = x.shape, weight.shape[0]
+    if K % 8:
+        _bad(f"K must be a multiple of 8, got {K}")
+    if gated:
+        if N % 16:
+            _bad(f"weight must have 2 N rows, N a multiple of 8, got {N}")
+        N //= 2
+    return code, M, N, K
+
+
+def _forward(x, weight, bias, activation, residual, out_dtype, out, save_pre, gated, stream):
+    torch = _torch()
+    _, inputs, outputs = _types()
+    code, M, N, K = _sizes(x, weight, gated)
+    dev = x.device
+    ldx = _operand(x, "x", x.dtype, dev)
+    ldw = _operand(weight, "weight", x.dtype, dev)
+    rows = weight.shape[0]
+    if activation not in ACTIVATIONS:
+        _bad(f"activation must be one of {sorted(a for a in ACTIVATIONS if a)}")
+    bp = bt = rp = rt = ldr = 0
+    if bias is not None:
+        bt = inputs.get(bias.dtype)
+        if (bt is None or tuple(bias.shape) != (rows,) or bias.device != dev
+                or (rows > 1 and bias.stride(0) != 1)):
+            _bad(f"bias must be a contiguous bfloat16, float16 or float32 vector of {rows} "
+                 f"elements on {dev}")
+        bp = bias.data_ptr()
+    if residual is not None:
+        rt, ldr = _matrix(residual, "residual", (M, N), inputs, dev)
+        rp = residual.data_ptr()
+    out_dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    ot = outputs.get(out_dtype)
+    if ot is None:
+        _bad("out_dtype must be bfloat16, float16 or float32")
+    pre_dtype = torch.float32 if save_pre is True else save_pre or torch.float32
+    pt = outputs.get(pre_dtype)
+    if pt is None:
+        _bad("save_pre must be True, False, bfloat16, float16 or float32")
+    with _on(stream):
+        if out is None:
+            out = x.new_empty((M, N), dtype=out_dtype)
+            ldy = N
+        else:
+            if out.dtype != out_dtype:
+                _bad(f"out must be {out_dtype}")
+            ldy = _matrix(out, "out", (M, N), outputs, dev)[1]
+        pre = x.new_empty((M, rows), dtype=pre_dtype) if save_pre else None
+        d = LinearDesc(_DESC_BYTES, x.data_ptr(), weight.data_ptr(), bp, rp, out.data_ptr(),
+                       pre.data_ptr() if save_pre else 0, 0, 0, ldx, ldw, ldr, ldy, rows, M,
+                       N, K, int(gated), code, bt, rt, ot, pt, ACTIVATIONS[activation])
+        need = lib().hipgemm_linear_workspace_size(ctypes.byref(d))
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            d.workspace, d.workspace_bytes = workspace.data_ptr(), need
+    with _device(dev, stream):
+        _check(lib().hipgemm_linear(ctypes.byref(d), _stream_handle(x, stream)),
+               "hipgemm_linear")
+    return (out, pre) if save_pre else out
+
+
+def _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias, grad_dtype,
+              gated, stream):
+    torch = _torch()
+    _, inputs, outputs = _types()
+    code, M, N, K = _sizes(x, weight, gated)
+    dev = x.device
+    ldx = _operand(x, "x", x.dtype, dev)
+    ldw = _operand(weight, "weight", x.dtype, dev)
+    rows = weight.shape[0]
+    if activation not in ACTIVATIONS:
+        _bad(f"activation must be one of {sorted(a for a in ACTIVATIONS if a)}")
+    dyt, lddy = _matrix(dy, "dy", (M, N), inputs, dev)
+    pp = pt = ldp = 0
+    if gated or ACTIVATIONS[activation]:
+        if pre is None:
+            _bad("pre of the forward pass (save_pre) is needed")
+        pt, ldp = _matrix(pre, "pre", (M, rows), inputs, dev)
+        pp = pre.data_ptr()
+    grad_dtype = grad_dtype or x.dtype
+    ot = outputs.get(grad_dtype)
+    if ot is None:
+        _bad("grad_dtype must be bfloat16, float16 or float32")
+    with _on(stream):
+        dx = x.new_empty((M, K)) if need_x else None
+        dw = x.new_empty((rows, K), dtype=grad_dtype) if need_weight else None
+        db = x.new_empty(rows, dtype=grad_dtype) if need_bias else None
+        dp, wp, bp = (0 if t is None else t.data_ptr() for t in (dx, dw, db))
+        d = LinearGradDesc(_GRAD_BYTES, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), pp, dp,
+                           wp, bp, 0, 0, lddy, ldx, ldw, ldp, K, K, M, N, K, int(gated), code,
+                           dyt, pt, outputs[x.dtype], ot, ot, ACTIVATIONS[activation])
+        need = lib().hipgemm_linear_backward_workspace_size(ctypes.byref(d))
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            d.workspace, d.workspace_bytes = workspace.data_ptr(), need
+    with _device(dev, stream):
+        _check(lib().hipgemm_linear_backward(ctypes.byref(d), _stream_handle(x, stream)),
+               "hipgemm_linear_backward")
+    return dx, dw, db
+
+
+def linear(x, weight, *, bias=None, activation=None, residual=None, out_dtype=None,
+           out=None, save_pre=False, stream=None):
+    """out[m, n] = round(act(z[m, n]) + residual[m, n]), z = x @ weight.T + bias.
+
+    x (M, K) and weight (N, K): both bfloat16 or both float16, K a multiple of 8, rows of
+    unit stride that start on 16 bytes.  bias (N) and residual (M, N): bfloat16, float16
+    or float32.  activation as for gemm().  out_dtype: bfloat16, float16 or float32, x's
+    where None.  out may be residual itself.  Sums are fp32, and everything after them
+    until the one rounding.  save_pre: returns (out, z), as linear_backward takes it: z in
+    float32 where True, or of the type given (x's halves its memory and adds a rounding to
+    the gradients)."""
+    return _forward(x, weight, bias, activation, residual, out_dtype, out, save_pre, False,
+                    stream)
+
+
+def gated_linear(x, weight, *, bias=None, activation="silu", out_dtype=None, out=None,
+                 save_pre=False, stream=None):
+    """out[m, n] = round(act(z[m, n]) * z[m, N + n]), z = x @ weight.T + bias: the gate and
+    up projections of a gated MLP, its activation and the product in one kernel.
+
+    weight (2N, K): gate rows, then up rows (as moe_experts' w13), N a multiple of 8; bias
+    (2N).  The rest as for linear; save_pre returns (out, z (M, 2N))."""
+    return _forward(x, weight, bias, activation, None, out_dtype, out, save_pre, True, stream)
+
+
+def linear_backward(dy, x, weight, pre=None, *, activation=None, need_x: bool = True,
+                    need_weight: bool = True, need_bias: bool = False, grad_dtype=None,
+                    stream=None):
+    """(dx, dweight, dbias) of linear, None where not needed: dz = dy * act'(z), dx = dz @
+    weight, dweight = dz.T @ x, dbias = dz.sum(0).  (The residual's gradient is dy.)
+
+    dy (M, N): bfloat16, float16 or float32.  pre: linear's z (save_pre); not needed without
+    an activation.  dx has x's type, dweight and dbias grad_dtype (bfloat16, float16 or
+    float32; x's type where None).  dz is rounded to x's type for the two products; sums are
+    fp32."""
+    return _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias,
+                     grad_dtype, False, stream)
+
+
+def gated_linear_backward(dy, x, weight, pre, *, activation="silu", need_x: bool = True,
+                          need_weight: bool = True, need_bias: bool = False,
+                          grad_dtype=None, stream=None):
+    """(dx, dweight, dbias) of gated_linear, None where not needed; as linear_backward, with
+    [dg | du] = [dy * u * act'(g) | dy * act(g)] for dz, z = [g | u]."""
+    return _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias,
+                     grad_dtype, True, stream)

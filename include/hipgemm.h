@@ -503,6 +503,84 @@ typedef struct hipgemm_moe_plan {
 hipError_t hipgemm_moe_select(int T, int k, int E, int D, int F, int format,
                               int out_dtype, hipgemm_moe_plan *plan);
 
+/*
+ * Products of 16-bit activations with 16-bit weights, and what a feed-forward block
+ * does with them:
+ *
+ *   z[m, n] = sum_k x[m, k] weight[n, k] + bias[n]
+ *   y[m, n] = round_out(activation(z[m, n]) + residual[m, n])
+ *
+ * gated: weight holds N gate rows, then N up rows (bias likewise), and
+ *
+ *   y[m, n] = round_out(activation(z[m, n]) * z[m, N + n])
+ *
+ * x is M x K, weight N x K (gated 2N x K), both of `type`, bf16 or fp16; products and
+ * sums are fp32.  bias, residual (not gated) and pre may be NULL; pre receives z (gated:
+ * both halves, M x 2N) as pre_dtype, for the backward pass.  bias_type,
+ * residual_type: HIPGEMM_IN_*.  Rows are contiguous, with the strides given.
+ * Requirements: K % 8 == 0, gated N % 8 == 0;  x and weight 16-byte aligned with row
+ * strides of a multiple of 8;  the others aligned to their element (16 bytes, strides
+ * of a multiple of 16 bytes and N % 8 == 0 are faster);  M <= 2^30, K, rows of weight
+ * and strides of x and weight up to 2^21.  residual may be y itself.  M == 0 or N == 0 is a no-op;
+ * K == 0 is a sum of nothing.  Workspace: hipgemm_linear_workspace_size bytes (0 for
+ * most calls), 256-byte aligned, of any content; calls that may run concurrently must not
+ * share one.  Zero-initialise the struct and set `size`.  No reference counterpart (the
+ * reference has e4m3 operands only).
+ */
+typedef struct hipgemm_linear_desc {
+  size_t size;
+  const void *x, *weight;
+  const void *bias, *residual; /* or NULL */
+  void *y;
+  void *pre;                   /* or NULL */
+  void *workspace;
+  size_t workspace_bytes;
+  long long ldx, ldw, ldr, ldy, ldp; /* elements */
+  int M, N, K;
+  int gated;                   /* 0 or 1 */
+  int type;                    /* HIPGEMM_IN_BF16 or HIPGEMM_IN_F16 */
+  int bias_type, residual_type; /* HIPGEMM_IN_* */
+  int out_dtype, pre_dtype;    /* HIPGEMM_OUT_BF16, _F16 or _F32 */
+  int activation;              /* HIPGEMM_ACT_* */
+} hipgemm_linear_desc;
+size_t hipgemm_linear_workspace_size(const hipgemm_linear_desc *desc);
+hipError_t hipgemm_linear(const hipgemm_linear_desc *desc, hipStream_t stream);
+
+/*
+ * Its backward pass: of dy, the gradient of y (M x N, dy_type HIPGEMM_IN_*),
+ *
+ *   dz = dy activation'(z)     gated, z = [g | u]: [dy u activation'(g) | dy activation(g)]
+ *   dx = dz weight             M x K
+ *   dw = dz^T x                N x K (gated 2N x K)
+ *   db[n] = sum_m dz[m, n]     N (gated 2N)
+ *
+ * each where its pointer is not NULL.  (The residual's gradient is dy.)  z is read from
+ * pre (pre_type HIPGEMM_IN_*), as the forward pass left it; not needed where activation is NONE and not
+ * gated.  dz is rounded to `type` for the two products, not for db; sums are fp32, in an
+ * order that depends on the sizes only.  Slopes: relu'(0) = 0.  With M == 0, dw and db
+ * are zeros.  Requirements as above; dy, pre: aligned to their element.  Workspace:
+ * hipgemm_linear_backward_workspace_size bytes for the descriptor (its pointers, strides
+ * and types matter), as above.  No reference counterpart.
+ */
+typedef struct hipgemm_linear_grad_desc {
+  size_t size;
+  const void *dy, *x, *weight;
+  const void *pre;             /* or NULL */
+  void *dx, *dw, *db;          /* or NULL */
+  void *workspace;
+  size_t workspace_bytes;
+  long long lddy, ldx, ldw, ldp, lddx, lddw; /* elements */
+  int M, N, K;
+  int gated;
+  int type;                    /* of x and weight */
+  int dy_type, pre_type;       /* HIPGEMM_IN_* */
+  int dx_dtype, dw_dtype, db_dtype; /* HIPGEMM_OUT_BF16, _F16 or _F32 */
+  int activation;
+} hipgemm_linear_grad_desc;
+size_t hipgemm_linear_backward_workspace_size(const hipgemm_linear_grad_desc *desc);
+hipError_t hipgemm_linear_backward(const hipgemm_linear_grad_desc *desc,
+                                   hipStream_t stream);
+
 /* Workspace bytes hipgemm_fp8_gemm_bf16_ws needs for this shape and variant
  * on the current device (0: none).  No GPU work.  No reference counterpart. */
 size_t hipgemm_workspace_size(int M, int N, int K, int variant);

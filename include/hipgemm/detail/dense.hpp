@@ -1,0 +1,732 @@
+// Products of 16-bit operands, fp32 sums, with the epilogues of a feed-forward
+// block, and the two products of its backward pass:
+//
+//   forward   z[m, n]  = sum_k x[m, k] w[n, k]            both along K
+//   of x      dx[m, k] = sum_n dz[m, n] w[n, k]           w across its rows
+//   of w      dw[n, k] = sum_m dz[m, n] x[m, k]           both across their rows
+//
+// One kernel body serves the three: C (M x N) = sum over K of A(m, k) B(n, k), each
+// operand either in rows along K (kCol false: element (m, k) at m ld + k) or across
+// (kCol true: at k ld + m).  Nothing is transposed in memory: tiles go to LDS as they
+// lie, and an operand that lies across K is turned on its way from LDS to registers
+// (ds_read_b64_tr_b16: sixteen lanes read four k of sixteen columns, and each gets
+// one column's four).
+//
+// Work decomposition: one workgroup = 4 waves (one per SIMD), persistent over the
+// tiles (tile_walk / grouped_tile, layout.hpp).  Wave w owns the BM / 2 x BN / 2 part
+// (w / 2, w % 2) of a tile as FA x FB blocks of 16 x 16 (v_mfma_f32_16x16x32).
+// kGated: of a tile's BN rows of B, half are gate rows and half the up rows of the
+// same columns, interleaved so that each wave holds both sums of its columns and
+// forms act(g) u from its own registers.
+//
+// A step is 64 elements of K: 128 bytes of a row, whole lines.  S stages of LDS
+// hold steps, brought by DMA (buffer_load_dwordx4 ... lds) S steps ahead.  A step runs
+// as two halves with a set of registers each:
+//   half 0 of step k: MFMA of set 0 | read set 1: half 1 of step k
+//   barrier: every wave's reads of step k are done, step k + 1 has landed
+//   half 1 of step k: MFMA of set 1 | read set 0: half 0 of step k + 1,
+//                                   | DMA of step k + S into step k's stage
+// The sequence runs on across tiles: what lies past a tile's last step is the next
+// tile's first.  Steps of a tile are padded to at least S (padding reads zeros).
+//
+// K order inside a step: lane group g = lane / 16 takes the eight k from 16 g + 8 h in
+// half h, in both layouts: slots 2 g + h of a row (layout.hpp: no bank conflicts), or
+// the LDS rows 16 g + 8 h .. + 7 of an operand that lies across.  There the 16-byte
+// slot s of row k is stored at s ^ col_xor(k): the four rows that sixteen lanes read
+// and the next lane group's four lie in different banks.
+//
+// kSplit: work units are (tile, K-slice) pairs that write their fp32 sums to
+// `partial`; k_dense_reduce adds them in order and finishes.
+//
+// Epilogue: sums through the wave's own LDS stage, 16 rows at a time, to eight
+// neighbouring columns of a lane: bias, activation, residual and all stores go 16 bytes
+// per lane; single elements, neighbouring lanes side by side, where sizes, strides
+// or addresses do not allow 16 bytes.
+#pragma once
+
+#include "arch.hpp"
+#include "decode.hpp"
+#include "epilogue.hpp"
+#include "layout.hpp"
+
+namespace hipgemm {
+namespace detail {
+
+// What becomes of the sums (types: kOut*, kIn*; strides in elements).
+struct DenseEpi {
+  uint8_t* y;
+  const uint8_t* bias;  // or null; gated: N gate values, then N up values
+  const uint8_t* r;     // residual or null
+  uint8_t* pre;         // sums with bias, or null
+  long long ldy, ldr, ldp;
+  long long up;         // gated: columns from a gate sum to its up sum, in pre
+  int act, y_type, p_type, b_type, r_type;
+  int vec;              // 16-byte accesses fit
+};
+
+struct DenseArgs {
+  const uint8_t *a, *b;
+  long long lda, ldb;  // bytes
+  long long up;        // gated: bytes from a gate row of B to its up row
+  int M, N, K;         // result rows and columns, and the sum's length
+  int group_m;
+  int slices, slice_steps;  // kSplit: K-slices of 64 slice_steps
+  float* partial;           // slices x M x ldpart
+  long long ldpart;
+  DenseEpi epi;
+};
+
+template <int BM, int BN, int S>
+struct CfgDense {
+  static constexpr int kBM = BM, kBN = BN, kStages = S;
+  static constexpr int kBK = 64, kRow = 2 * kBK;  // elements, bytes of a step
+  static constexpr int kWM = BM / 2, kWN = BN / 2;
+  static constexpr int kFA = kWM / 16, kFB = kWN / 16;
+  static constexpr int kAStage = kBM * kRow;
+  static constexpr int kStage = (kBM + kBN) * kRow;
+  static constexpr int kOutStage = 16 * kWN * 4;  // of a wave
+  static constexpr int kOutBase = S * kStage;
+  static constexpr int kLdsBytes = kOutBase + 4 * kOutStage;
+  static constexpr int kDmaA = BM / 32, kDmaB = BN / 32;  // per wave and step
+  static constexpr int kDma = kDmaA + kDmaB;
+  static_assert(kLdsBytes <= 160 * 1024, "LDS");
+};
+
+// ---- eight neighbouring elements, or one ------------------------------------
+
+__device__ __forceinline__ float widen(uint32_t h, int type) {
+  return type == kInBf16 ? __builtin_bit_cast(float, h << 16)
+                         : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+// Rounded to the 16-bit type, to nearest even.
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi, bool bf16) {
+  return bf16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+}
+__device__ __forceinline__ void load8(const uint8_t* p, long long at, int type,
+                                      float (&v)[8]) {
+  if (type == kInF32) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * at);
+    const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4 * at + 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+  } else {
+    const i32x4 a = *reinterpret_cast<const i32x4*>(p + 2 * at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t d = (uint32_t)a[e];
+      if (type == kInBf16) {
+        v[2 * e] = __builtin_bit_cast(float, d << 16);
+        v[2 * e + 1] = __builtin_bit_cast(float, d & 0xffff0000u);
+      } else {
+        v[2 * e] = widen(d & 0xffffu, type);
+        v[2 * e + 1] = widen(d >> 16, type);
+      }
+    }
+  }
+}
+__device__ __forceinline__ float load1(const uint8_t* p, long long at, int type) {
+  if (type == kInF32) return *reinterpret_cast<const float*>(p + 4 * at);
+  return widen(*reinterpret_cast<const uint16_t*>(p + 2 * at), type);
+}
+// A store of 16 bytes, and the wait states of store_b128 (arch.hpp).
+__device__ __forceinline__ void store16(uint8_t* p, i32x4 v) {
+  *reinterpret_cast<i32x4*>(p) = v;
+  asm volatile("s_nop 1" ::: "memory");
+}
+__device__ __forceinline__ void store8(uint8_t* p, long long at, int out,
+                                       const float (&v)[8]) {
+  if (out == kOutF32) {
+    store16(p + 4 * at, __builtin_bit_cast(i32x4, f32x4{v[0], v[1], v[2], v[3]}));
+    store16(p + 4 * at + 16, __builtin_bit_cast(i32x4, f32x4{v[4], v[5], v[6], v[7]}));
+  } else {
+    const bool b = out == kOutBf16;
+    store16(p + 2 * at, i32x4{(int)narrow2(v[0], v[1], b), (int)narrow2(v[2], v[3], b),
+                              (int)narrow2(v[4], v[5], b), (int)narrow2(v[6], v[7], b)});
+  }
+}
+__device__ __forceinline__ void store1(uint8_t* p, long long at, int out, float v) {
+  if (out == kOutF32) *reinterpret_cast<float*>(p + 4 * at) = v;
+  else *reinterpret_cast<uint16_t*>(p + 2 * at) = (uint16_t)narrow2(v, 0.0f, out == kOutBf16);
+}
+
+__device__ __forceinline__ float activate(float v, int act) {
+  return act == kActRelu ? relu(v) : act == kActSilu ? silu(v) : act == kActGeluTanh ? gelu_tanh(v) : v;
+}
+__device__ __forceinline__ void activate8(float (&v)[8], int act) {
+  if (act == kActRelu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = relu(v[e]);
+  } else if (act == kActSilu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = silu(v[e]);
+  } else if (act == kActGeluTanh) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = gelu_tanh(v[e]);
+  }
+}
+
+// Eight columns from `col` of row `row`: v (gated: gate sums, u the up sums).
+template <bool kGated>
+__device__ __forceinline__ void finish8(const DenseEpi& e, long long row, int col, int N,
+                                        float (&v)[8], float (&u)[8]) {
+  if (e.bias) {
+    float b[8];
+    load8(e.bias, col, e.b_type, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += b[i];
+    if constexpr (kGated) {
+      load8(e.bias, (long long)N + col, e.b_type, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] += b[i];
+    }
+  }
+  if (e.pre) {
+    store8(e.pre, row * e.ldp + col, e.p_type, v);
+    if constexpr (kGated) store8(e.pre, row * e.ldp + e.up + col, e.p_type, u);
+  }
+  activate8(v, e.act);
+  if constexpr (kGated) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= u[i];
+  }
+  if (e.r) {
+    float r[8];
+    load8(e.r, row * e.ldr + col, e.r_type, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += r[i];
+  }
+  store8(e.y, row * e.ldy + col, e.y_type, v);
+}
+template <bool kGated>
+__device__ __forceinline__ void finish1(const DenseEpi& e, long long row, int col, int N,
+                                        float v, float u) {
+  if (e.bias) {
+    v += load1(e.bias, col, e.b_type);
+    if constexpr (kGated) u += load1(e.bias, (long long)N + col, e.b_type);
+  }
+  if (e.pre) {
+    store1(e.pre, row * e.ldp + col, e.p_type, v);
+    if constexpr (kGated) store1(e.pre, row * e.ldp + e.up + col, e.p_type, u);
+  }
+  v = activate(v, e.act);
+  if constexpr (kGated) v *= u;
+  if (e.r) v += load1(e.r, row * e.ldr + col, e.r_type);
+  store1(e.y, row * e.ldy + col, e.y_type, v);
+}
+
+// ---- tiles --------------------------------------------------------------------
+
+__host__ __device__ constexpr int col_xor(int k) { return 2 * ((k & 3) | (((k >> 4) & 1) << 2)); }
+
+using s16x4 = short __attribute__((ext_vector_type(4)));
+using s16x8 = short __attribute__((ext_vector_type(8)));
+
+// Sixteen lanes give the addresses of four columns' elements in each of four rows (lane
+// i: row i / 4, columns 4 (i % 4) ..); lane i gets column i's four.  (__restrict: a
+// read without any aliasing information is made to wait for every DMA in flight.)
+__device__ __forceinline__ s16x4 lds_read_across(const lds_u8* __restrict p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)p);
+}
+
+// c += a b, in place.  Written as an instruction of its own: given the builtin, the
+// register allocator moves accumulators about inside the K loop (36 to 180
+// v_accvgpr_* of a step's 128 MFMA, 256 x 256 tiles).  The compiler does not see a matrix
+// instruction here: operands are waited for (wait_lgkmcnt) before their first use, and
+// mfma_drain() stands between the last one and the first read of a sum.
+template <int kX>
+__device__ __forceinline__ void mfma_acc(i32x4 a, i32x4 b, f32x4& c) {
+  if constexpr (kX == kInBf16)
+    asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else
+    asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+
+template <class Cfg, int kX, bool kACol, bool kBCol, bool kGated, bool kSplit>
+__device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds) {
+  constexpr int S = Cfg::kStages, FA = Cfg::kFA, FB = Cfg::kFB;
+  constexpr int kBK = Cfg::kBK, kDma = Cfg::kDma;
+  constexpr int kMfma = FA * FB;  // of a half
+  constexpr int kReadA = kACol ? 2 : 1, kReadB = kBCol ? 2 : 1;  // of a fragment
+  constexpr int kReads = kReadA * FA + kReadB * FB;
+  // MFMA of half 0 that are issued after the barrier: they read registers only and
+  // keep the matrix unit busy while the waves meet.
+  constexpr int kTail = 2, kHead = kMfma - kTail;
+  constexpr int kPer = (kReads + kHead - 1) / kHead;  // reads after one MFMA
+  constexpr int kDmaAt = kReads + kDma <= kHead ? kReads : 0;
+  constexpr int kWNr = kGated ? Cfg::kWN / 2 : Cfg::kWN;  // result columns of a wave
+  constexpr int kBNr = 2 * kWNr;
+  static_assert((S - 2) * kDma < 64, "vmcnt range");
+  static_assert(!kGated || !kBCol, "gated: weights along K");
+  const int lane = lane_id(), wave = wave_id();
+  const int wm = wave >> 1, wn = wave & 1;
+  const int tiles_m = (g.M + Cfg::kBM - 1) / Cfg::kBM;
+  const int tiles_n = (g.N + kBNr - 1) / kBNr;
+  const int tiles = tiles_m * tiles_n;
+  const int units = kSplit ? tiles * g.slices : tiles;
+  const int steps = kSplit ? g.slice_steps : (int)(((long long)g.K + kBK - 1) / kBK);
+  const int steps_pad = max(S, steps);
+  const TileWalk walk = tile_walk(blockIdx.x, gridDim.x, units);
+  int t = walk.first;
+  if (t >= walk.end) return;
+
+  // ---- DMA lane geometry -------------------------------------------------------
+  // Along K: instruction q of wave w covers rows (4 q + w) 8 .. + 8, lane l row l / 8,
+  // slot l % 8, which holds chunk (l % 8) ^ slot_xor(row).
+  // Across: 1 KiB of rows of 2 BM bytes, lane l 16 bytes each; slot s of row k holds
+  // the columns' chunk s ^ col_xor(k).
+  const int drow = lane >> 3;
+  const int dchunk = (lane & 7) ^ slot_xor(8 * (wave & 1) + drow);
+  auto lane_off = [&](bool col, int width, long long ld, int q) -> uint32_t {
+    if (!col) return (uint32_t)((4 * q + wave) * 8 + drow) * (uint32_t)ld + dchunk * 16;
+    const int slots = width / 8, k = (4 * q + wave) * (64 / slots) + lane / slots;
+    return (uint32_t)k * (uint32_t)ld + (((lane % slots) ^ col_xor(k)) * 16);
+  };
+  // Gated: row R of the tile's BN rows is column kWNr (R / kWN) + R % kWNr, of the up
+  // half where R % kWN >= kWNr: whole instructions (eight rows) of one half.
+  auto is_up = [&](int q) { return kGated && ((4 * q + wave) * 8) % Cfg::kWN >= kWNr; };
+  uint32_t voff_a[Cfg::kDmaA], voff_b[Cfg::kDmaB];
+#pragma unroll
+  for (int q = 0; q < Cfg::kDmaA; ++q) voff_a[q] = lane_off(kACol, Cfg::kBM, g.lda, q);
+#pragma unroll
+  for (int q = 0; q < Cfg::kDmaB; ++q) {
+    if constexpr (kGated) {
+      const int R = (4 * q + wave) * 8;
+      voff_b[q] = (uint32_t)(kWNr * (R / Cfg::kWN) + R % kWNr + drow) * (uint32_t)g.ldb +
+                  dchunk * 16;
+    } else {
+      voff_b[q] = lane_off(kBCol, Cfg::kBN, g.ldb, q);
+    }
+  }
+
+  // (Kept in registers: otherwise computed anew in every step.)
+#pragma unroll
+  for (int q = 0; q < Cfg::kDmaA; ++q) asm volatile("" : "+v"(voff_a[q]));
+#pragma unroll
+  for (int q = 0; q < Cfg::kDmaB; ++q) asm volatile("" : "+v"(voff_b[q]));
+
+  // A unit's operands: along K the rows' resource; across, the columns' address, from
+  // which each step's resource is made (rows past the sum's end read zero).
+  struct Src {
+    __amdgpu_buffer_rsrc_t a, b, b2;
+    const uint8_t *pa, *pb;
+    uint32_t ca, cb;  // across: bytes of a row from pa, pb
+    int k0, kend;
+  };
+  auto rows_of = [](const uint8_t* p, long long ld, int first, int have, int most) {
+    const int n = min(most, have - first);
+    return make_rsrc(p + (long long)first * ld, (uint32_t)n * (uint32_t)ld);
+  };
+  auto src_of = [&](int unit) {
+    Src s;
+    if (unit >= walk.end) {
+      s.a = s.b = s.b2 = make_rsrc(g.a, 0u);
+      s.pa = s.pb = g.a;
+      s.ca = s.cb = 0;
+      s.k0 = s.kend = 0;
+      return s;
+    }
+    const int tile = kSplit ? unit % tiles : unit;
+    const int slice = kSplit ? __builtin_amdgcn_readfirstlane(unit / tiles) : 0;
+    const TileCoord c = grouped_tile_u(tile, tiles_m, tiles_n, g.group_m);
+    const int m0 = c.m * Cfg::kBM, n0 = c.n * kBNr;
+    s.k0 = kSplit ? slice * steps * kBK : 0;
+    s.kend = kSplit ? (int)min((long long)g.K, (long long)s.k0 + (long long)steps * kBK) : g.K;
+    s.a = s.b = s.b2 = make_rsrc(g.a, 0u);
+    s.pa = g.a;
+    s.pb = g.b;
+    s.ca = s.cb = 0;
+    if constexpr (kACol) {
+      s.pa = g.a + 2ll * m0;
+      s.ca = (uint32_t)(2 * (((g.M + 7) & ~7) - m0));
+    } else {
+      s.a = rows_of(g.a, g.lda, m0, g.M, Cfg::kBM);
+    }
+    if constexpr (kBCol) {
+      s.pb = g.b + 2ll * n0;
+      s.cb = (uint32_t)(2 * (((g.N + 7) & ~7) - n0));
+    } else {
+      s.b = rows_of(g.b, g.ldb, n0, g.N, kBNr);
+      if constexpr (kGated) s.b2 = rows_of(g.b + g.up, g.ldb, n0, g.N, kBNr);
+    }
+    return s;
+  };
+  Src cur = src_of(t), nxt = src_of(t + walk.stride);
+
+  struct Step {
+    __amdgpu_buffer_rsrc_t a, b, b2;
+    uint32_t soff, oob;
+  };
+  // Step d of the unit, or past its end step d - steps_pad of the next.
+  auto step_src = [&](int d) {
+    const bool next = d >= steps_pad;
+    const int k = (next ? nxt.k0 : cur.k0) + (next ? d - steps_pad : d) * kBK;
+    const int kend = next ? nxt.kend : cur.kend;
+    Step s;
+    uint32_t soff = (uint32_t)k * 2u;
+    asm volatile("" : "+s"(soff));
+    s.soff = soff;
+    s.oob = 0;
+    if constexpr (!kACol || !kBCol) s.oob = k + dchunk * 8 < kend ? 0u : kOobOffset;
+    auto across = [&](const uint8_t* p, long long ld, uint32_t cols) {
+      const int rows = min(kBK, kend - k);
+      return make_rsrc(p + (long long)k * ld,
+                       rows > 0 ? (uint32_t)(rows - 1) * (uint32_t)ld + cols : 0u);
+    };
+    if constexpr (kACol) s.a = across(next ? nxt.pa : cur.pa, g.lda, next ? nxt.ca : cur.ca);
+    else s.a = next ? nxt.a : cur.a;
+    if constexpr (kBCol) s.b = across(next ? nxt.pb : cur.pb, g.ldb, next ? nxt.cb : cur.cb);
+    else s.b = next ? nxt.b : cur.b;
+    s.b2 = s.b;
+    if constexpr (kGated) s.b2 = next ? nxt.b2 : cur.b2;
+    return s;
+  };
+  auto dma_one = [&](const Step& s, int dst, int n) {
+    const bool is_a = n < Cfg::kDmaA;
+    const int q = is_a ? n : n - Cfg::kDmaA;
+    lds_u8* to = lds + dst + (is_a ? 0 : Cfg::kAStage) + (4 * q + wave) * 1024;
+    const uint32_t vo = is_a ? voff_a[q] : voff_b[q];
+    const bool col = is_a ? kACol : kBCol;
+    const uint32_t v = col ? vo : vo | s.oob;
+    const uint32_t so = col ? 0u : s.soff;
+    if (is_a) dma16(s.a, to, v, so);
+    else dma16(is_up(q) ? s.b2 : s.b, to, v, so);
+  };
+
+  // ---- fragments ---------------------------------------------------------------
+  const int r16 = lane & 15, grp = lane >> 4;
+  // Along K: row r16 of the fragment, slot 2 grp + h.
+  const uint32_t row_a = (uint32_t)((wm * Cfg::kWM + r16) * Cfg::kRow);
+  const uint32_t row_b = (uint32_t)(Cfg::kAStage + (wn * Cfg::kWN + r16) * Cfg::kRow);
+  uint32_t slot[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) slot[h] = (uint32_t)(((2 * grp + h) ^ slot_xor(r16)) * 16);
+  // Across: LDS row 16 grp + 8 h + 4 p + r16 / 4, columns 16 f + 4 (r16 % 4) .. + 3.
+  const int krow = 16 * grp + (r16 >> 2);
+  const int kx = col_xor(krow);
+  const uint32_t sub = (uint32_t)((((r16 & 3) >> 1) * 16) + (r16 & 1) * 8);
+  uint32_t col_a[FA], col_b[FB];
+#pragma unroll
+  for (int f = 0; f < FA; ++f)
+    col_a[f] = (uint32_t)(krow * 2 * Cfg::kBM) + sub + (uint32_t)(((2 * (wm * FA + f)) ^ kx) * 16);
+#pragma unroll
+  for (int f = 0; f < FB; ++f)
+    col_b[f] = (uint32_t)(Cfg::kAStage + krow * 2 * Cfg::kBN) + sub +
+               (uint32_t)(((2 * (wn * FB + f)) ^ kx) * 16);
+
+  s16x4 fa[2][FA][2], fb[2][FB][2];
+  // Read n of half h of the step in the stage at `st`, in the order in which the MFMA
+  // need them: A 0, every B, the other A.
+  auto read_one = [&](int st, int h, int n) {
+    constexpr int kFirst = kReadA, kMid = kReadA + kReadB * FB;
+    const bool is_b = n >= kFirst && n < kMid;
+    const int m = is_b ? n - kFirst : n < kFirst ? n : n - kReadB * FB;
+    const int per = is_b ? kReadB : kReadA;
+    const int f = m / per, p = m % per;
+    s16x4(&to)[2] = is_b ? fb[h][f] : fa[h][f];
+    if (is_b ? kBCol : kACol) {
+      const int width = is_b ? 2 * Cfg::kBN : 2 * Cfg::kBM;
+      const lds_u8* from = lds + st + (is_b ? col_b[f] : col_a[f]) + (8 * h + 4 * p) * width;
+      to[p] = lds_read_across(from);
+    } else {
+      const lds_u8* from = lds + st + (is_b ? row_b : row_a) + slot[h] + f * 16 * Cfg::kRow;
+      const s16x8 v = __builtin_bit_cast(s16x8, lds_read16(from));
+      to[0] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+      to[1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+    }
+  };
+  auto frag = [](const s16x4 (&p)[2]) {
+    return __builtin_bit_cast(i32x4, __builtin_shufflevector(p[0], p[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f32x4 acc[FA][FB];
+  // Blocks row by row, odd rows right to left (neighbouring MFMA share an operand).
+  auto mfma = [&](int h, int n) {
+    const int i = n / FB, j = i % 2 ? FB - 1 - n % FB : n % FB;
+    mfma_acc<kX>(frag(fb[h][j]), frag(fa[h][i]), acc[i][j]);
+  };
+  auto half0 = [&](int st) {
+    wait_lgkmcnt<0>();
+#pragma unroll
+    for (int n = 0; n < kHead; ++n) {
+      mfma(0, n);
+#pragma unroll
+      for (int r = 0; r < kPer; ++r)
+        if (n * kPer + r < kReads) read_one(st, 1, n * kPer + r);
+      sched_fence();
+    }
+  };
+  auto half1 = [&](int st, int rst, int d) {
+    const Step src = step_src(d);
+#pragma unroll
+    for (int n = kHead; n < kMfma; ++n) mfma(0, n);
+    sched_fence();
+#pragma unroll
+    for (int n = 0; n < kMfma; ++n) {
+      mfma(1, n);
+#pragma unroll
+      for (int r = 0; r < kPer; ++r)
+        if (n * kPer + r < kReads) read_one(rst, 0, n * kPer + r);
+#pragma unroll
+      for (int q = 0; q < kDma; ++q)
+        if (kDmaAt + q * (kMfma - kDmaAt) / kDma == n) dma_one(src, st, q);
+      sched_fence();
+    }
+  };
+  auto next_stage = [](int s) {
+    s += Cfg::kStage;
+    return s == S * Cfg::kStage ? 0 : s;
+  };
+  int st = 0;
+  auto step = [&](int k) {
+    const int rst = next_stage(st);
+    half0(st);
+    // Step k + 1 has landed: newer are the DMA of S - 2 steps.
+    wait_lgkmcnt<0>();
+    wait_vmcnt<(S - 2) * kDma>();
+    barrier();
+    half1(st, rst, k + S);
+    st = rst;
+  };
+
+#pragma unroll
+  for (int d = 0; d < S; ++d) {
+    const Step src = step_src(d);
+#pragma unroll
+    for (int n = 0; n < kDma; ++n) dma_one(src, d * Cfg::kStage, n);
+  }
+  wait_vmcnt<(S - 1) * kDma>();
+  barrier();
+#pragma unroll
+  for (int n = 0; n < kReads; ++n) read_one(0, 0, n);
+
+  lds_u8* const stg = lds + Cfg::kOutBase + wave * Cfg::kOutStage;
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+      for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{};
+    for (int k = 0; k < steps_pad; ++k) step(k);
+
+    // ---- epilogue --------------------------------------------------------------
+    mfma_drain();
+    const int tile = kSplit ? t % tiles : t;
+    const TileCoord tc = grouped_tile_u(tile, tiles_m, tiles_n, g.group_m);
+    const int row0 = tc.m * Cfg::kBM + wm * Cfg::kWM, col0 = tc.n * kBNr + wn * kWNr;
+    int el = lane;
+    asm volatile("" : "+v"(el));
+    constexpr int kChunkRow = Cfg::kWN * 4;  // bytes of a staged row
+    auto at = [&](int r, int chunk) { return stg + r * kChunkRow + ((chunk ^ (r & 7)) * 16); };
+    // (Rolled, the accumulators picked by branches: unrolled the epilogue is FA times
+    // the code, and its array stays in memory.)
+#pragma nounroll
+    for (int i = 0; i < FA; ++i) {
+#pragma unroll
+      for (int b = 0; b < FA; ++b)
+        if (b == i) {
+#pragma unroll
+          for (int j = 0; j < FB; ++j)
+            *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(
+                at(el & 15, 4 * j + (el >> 4))) = acc[b][j];
+        }
+      compiler_fence();
+      auto read8 = [&](int r, int chunk, float (&v)[8]) {
+        const f32x4 a = __builtin_bit_cast(f32x4, lds_read16(at(r, chunk)));
+        const f32x4 b = __builtin_bit_cast(f32x4, lds_read16(at(r, chunk + 1)));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+      };
+      constexpr int kUnits = kWNr / 8, kRows = 64 / kUnits;
+      if (kSplit || g.epi.vec) {
+#pragma unroll
+        for (int q = 0; q < 16 / kRows; ++q) {
+          const int r = q * kRows + el / kUnits, c = el % kUnits;
+          const int row = row0 + 16 * i + r, col = col0 + 8 * c;
+          float v[8], u[8] = {};
+          read8(r, 2 * c, v);
+          if constexpr (kGated) read8(r, kWNr / 4 + 2 * c, u);
+          if (row < g.M && col < g.N) {
+            if constexpr (kSplit) {
+              const int slice = t / tiles;
+              uint8_t* p = reinterpret_cast<uint8_t*>(g.partial);
+              const long long o = ((long long)slice * g.M + row) * g.ldpart + col;
+              store8(p, o, kOutF32, v);
+              if constexpr (kGated) store8(p, o + g.ldpart / 2, kOutF32, u);
+            } else {
+              finish8<kGated>(g.epi, row, col, g.N, v, u);
+            }
+          }
+        }
+      } else {
+        for (int q = 0; q < 16 * kWNr / 64; ++q) {
+          const int r = (64 * q + el) / kWNr, c = (64 * q + el) % kWNr;
+          const int row = row0 + 16 * i + r, col = col0 + c;
+          auto read1 = [&](int x) {
+            return __builtin_bit_cast(float, lds_read4(at(r, x >> 2) + (x & 3) * 4));
+          };
+          if (row < g.M && col < g.N)
+            finish1<kGated>(g.epi, row, col, g.N, read1(c), kGated ? read1(kWNr + c) : 0.0f);
+        }
+      }
+      compiler_fence();
+    }
+    t += walk.stride;
+    if (t >= walk.end) break;
+    cur = nxt;
+    nxt = src_of(t + walk.stride);
+  }
+  // The look-ahead's DMA (empty ranges) still write LDS.
+  wait_vmcnt<0>();
+}
+
+// ---- K-slices' sums -----------------------------------------------------------
+
+// A thread per row and eight columns: slices in order, then the epilogue.
+template <bool kGated>
+__device__ __forceinline__ void dense_reduce_body(const DenseArgs& g) {
+  const int units = (g.N + 7) / 8;
+  const long long x = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long row = x / units;
+  const int col = 8 * (int)(x % units);
+  if (row >= g.M) return;
+  float v[8] = {}, u[8] = {};
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(g.partial);
+  for (int s = 0; s < g.slices; ++s) {
+    const long long o = ((long long)s * g.M + row) * g.ldpart + col;
+    float w[8];
+    load8(p, o, kInF32, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += w[e];
+    if constexpr (kGated) {
+      load8(p, o + g.ldpart / 2, kInF32, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] += w[e];
+    }
+  }
+  if (g.epi.vec) {
+    finish8<kGated>(g.epi, row, col, g.N, v, u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (col + e < g.N) finish1<kGated>(g.epi, row, col + e, g.N, v[e], u[e]);
+  }
+}
+
+// ---- gradients of the sums ----------------------------------------------------
+
+// The activation's derivative at z, its limits at infinities (NaN stays NaN):
+//   relu  z > 0
+//   silu  s (1 + z (1 - s)),            s = 1 / (1 + e^-z)
+//   gelu  s (1 + z (1 - s) 2 u'(z)),    s = 1 / (1 + e^(-2 u)),
+//         u' = sqrt(2/pi) (1 + 3 0.044715 z^2)
+// with z held to +-96 in the second factors, past which s or 1 - s is zero in fp32.
+__device__ __forceinline__ float slope(float z, int act) {
+  if (act == kActRelu) return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+  if (act == kActNone) return 1.0f;
+  const float c = __builtin_fminf(__builtin_fmaxf(z, -96.0f), 96.0f);
+  float s, d = c;
+  if (act == kActSilu) {
+    s = __builtin_amdgcn_rcpf(1.0f + exp_fast(-c));
+  } else {
+    constexpr float k = 0.7978845608028654f;
+    const float c2 = c * c;
+    const float u2 = 2.0f * k * c * __builtin_fmaf(c2, 0.044715f, 1.0f);
+    s = __builtin_amdgcn_rcpf(1.0f + exp_fast(-u2));
+    d = 2.0f * k * c * __builtin_fmaf(c2, 3.0f * 0.044715f, 1.0f);
+  }
+  return z != z ? z : s * __builtin_fmaf(d, 1.0f - s, 1.0f);
+}
+
+struct SlopeArgs {
+  const uint8_t *dy, *pre;
+  uint8_t* dz;     // or null
+  float* columns;  // gridDim.y x width sums of dz over a block's rows, or null
+  long long lddy, ldp, lddz;
+  int M, N;        // of dy; dz has 2 N columns where gated
+  int act, dy_type, p_type;
+  int rows;        // of a block
+  int vec;         // dy and pre in 16-byte accesses
+};
+
+// dz = dy act'(z);  gated, z = [g | u]: [dy u act'(g) | dy act(g)].  Rounded to the
+// operands' type, as the matrix instructions take it; column sums are of the values
+// before that, in fp32.  A thread has eight columns and every eighth row of the block's.
+// Columns from N to the padded row's end are written as zeros.
+template <int kX, bool kGated>
+__device__ __forceinline__ void dense_slope_body(const SlopeArgs& g, float* sums) {
+  constexpr int kParts = kGated ? 2 : 1;
+  constexpr int kOut = kX == kInBf16 ? kOutBf16 : kOutF16;
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int col = 8 * (32 * blockIdx.x + tx);
+  const long long first = (long long)blockIdx.y * g.rows;
+  const long long end = min((long long)g.M, first + g.rows);
+  const bool live = col < g.N;
+  const bool whole = g.vec && col + 8 <= g.N;
+  float sum[kParts][8] = {};
+  if (live)
+    for (long long row = first + ty; row < end; row += 8) {
+      float dy[8] = {}, z[8] = {}, u[8] = {};
+      if (whole) {
+        load8(g.dy, row * g.lddy + col, g.dy_type, dy);
+        if (g.pre) load8(g.pre, row * g.ldp + col, g.p_type, z);
+        if constexpr (kGated) load8(g.pre, row * g.ldp + g.N + col, g.p_type, u);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (col + e < g.N) {
+            dy[e] = load1(g.dy, row * g.lddy + col + e, g.dy_type);
+            if (g.pre) z[e] = load1(g.pre, row * g.ldp + col + e, g.p_type);
+            if constexpr (kGated) u[e] = load1(g.pre, row * g.ldp + g.N + col + e, g.p_type);
+          }
+      }
+      float d[8];
+      if constexpr (kGated) {
+        float a[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          d[e] = dy[e] * u[e] * slope(z[e], g.act);
+          a[e] = z[e];
+        }
+        activate8(a, g.act);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          a[e] *= dy[e];
+          sum[kParts - 1][e] += a[e];
+        }
+        if (g.dz) store8(g.dz, row * g.lddz + g.N + col, kOut, a);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = dy[e] * slope(z[e], g.act);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[0][e] += d[e];
+      if (g.dz) store8(g.dz, row * g.lddz + col, kOut, d);
+    }
+  if (!g.columns) return;
+  // The block's eight sums of each column, in order.
+#pragma unroll
+  for (int p = 0; p < kParts; ++p) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[ty * 256 + 8 * tx + e] = sum[p][e];
+    __syncthreads();
+    const int c = 256 * blockIdx.x + threadIdx.x;
+    float s = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) s += sums[y * 256 + threadIdx.x];
+    if (c < g.N) g.columns[((long long)blockIdx.y * kParts + p) * g.N + c] = s;
+  }
+}
+
+// out[c] = sum over blocks of columns[b][c], in order.
+__device__ __forceinline__ void dense_columns_body(const float* columns, int blocks, int N,
+                                                   uint8_t* out, int type) {
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= N) return;
+  float s = 0.0f;
+  for (int b = 0; b < blocks; ++b) s += columns[(long long)b * N + c];
+  store1(out, c, type, s);
+}
+
+}  // namespace detail
+}  // namespace hipgemm
