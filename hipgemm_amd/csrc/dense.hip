@@ -12,15 +12,17 @@ namespace kernels {
   const void* dense_tile_bf16_##L(int tile, bool split); \
   const void* dense_tile_f16_##L(int tile, bool split);
 HIPGEMM_DENSE(nt)
+HIPGEMM_DENSE(res)
 HIPGEMM_DENSE(nn)
 HIPGEMM_DENSE(tn)
 HIPGEMM_DENSE(gated)
 #undef HIPGEMM_DENSE
 
-const void* dense_tile(int x, int layout, int tile, bool split) {
+const void* dense_tile(int x, int kind, int tile, bool split) {
   const bool b = x == detail::kInBf16;
-  switch (layout) {
+  switch (kind) {
     case kDenseNT: return b ? dense_tile_bf16_nt(tile, split) : dense_tile_f16_nt(tile, split);
+    case kDenseRes: return b ? dense_tile_bf16_res(tile, split) : dense_tile_f16_res(tile, split);
     case kDenseNN: return b ? dense_tile_bf16_nn(tile, split) : dense_tile_f16_nn(tile, split);
     case kDenseTN: return b ? dense_tile_bf16_tn(tile, split) : dense_tile_f16_tn(tile, split);
     default:
@@ -36,9 +38,9 @@ namespace {
 using namespace hipgemm::detail;
 namespace hk = hipgemm::kernels;
 
-template <bool kGated>
+template <int kEpi>
 __global__ __launch_bounds__(256) void k_dense_reduce(DenseArgs g) {
-  dense_reduce_body<kGated>(g);
+  dense_reduce_body<kEpi>(g);
 }
 template <int kX, bool kGated>
 __global__ __launch_bounds__(256) void k_dense_slope(SlopeArgs g) {
@@ -71,49 +73,51 @@ struct Plan {
   int tile, slices, slice_steps;
   long long units;
 };
-Plan plan_of(int layout, int M, int N, int K) {
+Plan plan_of(int kind, int M, int N, int K) {
   Plan p{0, 1, 0, 0};
-  const hk::TileShape s = hk::kDenseTiles[p.tile];
-  const int cols = layout == hk::kDenseGated ? s.bn / 2 : s.bn;
-  p.units = (((long long)M + s.bm - 1) / s.bm) * (((long long)N + cols - 1) / cols) * p.slices;
+  auto units = [&](int tile) {
+    const hk::TileShape s = hk::kDenseTiles[tile];
+    const int cols = kind == hk::kDenseGated ? s.bn / 2 : s.bn;
+    return (((long long)M + s.bm - 1) / s.bm) * (((long long)N + cols - 1) / cols);
+  };
+  if (units(1) >= 160) p.tile = 1;
+  p.units = units(p.tile) * p.slices;
   (void)K;
   return p;
 }
 
 // Columns of a partial sum's row.
-long long partial_columns(int layout, int N) {
+long long partial_columns(int kind, int N) {
   const long long n = ((long long)N + 7) & ~7ll;
-  return layout == hk::kDenseGated ? 2 * n : n;
+  return kind == hk::kDenseGated ? 2 * n : n;
 }
-size_t partial_bytes(int layout, const Plan& p, int M, int N) {
+size_t partial_bytes(int kind, const Plan& p, int M, int N) {
   if (p.slices == 1) return 0;
-  return padded(4ull * (size_t)p.slices * (size_t)M * (size_t)partial_columns(layout, N));
+  return padded(4ull * (size_t)p.slices * (size_t)M * (size_t)partial_columns(kind, N));
 }
 
 // g: operands, sizes and epilogue; ws: partial_bytes.
-hipError_t product(int x, int layout, DenseArgs& g, void* ws, hipStream_t stream) {
-  const Plan p = plan_of(layout, g.M, g.N, g.K);
+hipError_t product(int x, int kind, DenseArgs& g, void* ws, hipStream_t stream) {
+  const Plan p = plan_of(kind, g.M, g.N, g.K);
   const hk::TileShape s = hk::kDenseTiles[p.tile];
-  const int cols = layout == hk::kDenseGated ? s.bn / 2 : s.bn;
+  const int cols = kind == hk::kDenseGated ? s.bn / 2 : s.bn;
   g.group_m = default_group_m((g.M + s.bm - 1) / s.bm, (g.N + cols - 1) / cols);
   g.slices = p.slices;
   g.slice_steps = p.slice_steps;
   g.partial = static_cast<float*>(ws);
-  g.ldpart = partial_columns(layout, g.N);
+  g.ldpart = partial_columns(kind, g.N);
   const long long most = 256;
-  hipError_t e = launch(hk::dense_tile(x, layout, p.tile, p.slices > 1),
+  hipError_t e = launch(hk::dense_tile(x, kind, p.tile, p.slices > 1),
                         dim3((unsigned)(p.units < most ? p.units : most)), g, stream);
   if (e != hipSuccess || p.slices == 1) return e;
   const long long threads = (long long)g.M * ((g.N + 7) / 8);
-  const bool gated = layout == hk::kDenseGated;
-  const void* fn = gated ? (const void*)&k_dense_reduce<true> : (const void*)&k_dense_reduce<false>;
+  const void* fn = kind == hk::kDenseGated ? (const void*)&k_dense_reduce<kEpiGated>
+                   : kind == hk::kDenseRes ? (const void*)&k_dense_reduce<kEpiResidual>
+                   : kind == hk::kDenseNT  ? (const void*)&k_dense_reduce<kEpiLinear>
+                                           : (const void*)&k_dense_reduce<kEpiPlain>;
   return launch(fn, dim3((unsigned)((threads + 255) / 256)), g, stream);
 }
 
-// A matrix of rows that take 16-byte accesses at columns of multiples of eight.
-bool fits16(const void* p, long long ld, int bytes) {
-  return !p || (aligned(p, 16) && ld * bytes % 16 == 0);
-}
 bool operand(const void* p, long long ld, long long columns) {
   return p && aligned(p, 16) && ld >= columns && ld % 8 == 0 && ld <= kMaxLd;
 }
@@ -150,9 +154,13 @@ hipError_t check(const hipgemm_linear_desc* desc) {
   return hipSuccess;
 }
 
+int kind_of(const hipgemm_linear_desc& d) {
+  return d.gated ? hk::kDenseGated : d.residual ? hk::kDenseRes : hk::kDenseNT;
+}
+
 size_t forward_bytes(const hipgemm_linear_desc& d) {
-  const int layout = d.gated ? hk::kDenseGated : hk::kDenseNT;
-  return partial_bytes(layout, plan_of(layout, d.M, d.N, d.K), d.M, d.N);
+  const int kind = kind_of(d);
+  return partial_bytes(kind, plan_of(kind, d.M, d.N, d.K), d.M, d.N);
 }
 
 hipError_t forward(const hipgemm_linear_desc& d, hipStream_t stream) {
@@ -182,10 +190,7 @@ hipError_t forward(const hipgemm_linear_desc& d, hipStream_t stream) {
   e.p_type = d.pre_dtype;
   e.b_type = d.bias_type;
   e.r_type = d.residual_type;
-  e.vec = d.N % 8 == 0 && fits16(d.y, d.ldy, out_bytes(d.out_dtype)) &&
-          fits16(d.residual, d.ldr, in_bytes(d.residual_type)) && fits16(d.pre, d.ldp, out_bytes(d.pre_dtype)) &&
-          fits16(d.bias, 8, 2);
-  return product(d.type, d.gated ? hk::kDenseGated : hk::kDenseNT, g, d.workspace, stream);
+  return product(d.type, kind_of(d), g, d.workspace, stream);
 }
 
 // ---- backward ---------------------------------------------------------------------
@@ -260,7 +265,6 @@ void plain_epilogue(DenseArgs& g, void* y, long long ldy, int out) {
   g.epi.y = static_cast<uint8_t*>(y);
   g.epi.ldy = ldy;
   g.epi.y_type = out;
-  g.epi.vec = g.N % 8 == 0 && fits16(y, ldy, out_bytes(out));
 }
 
 hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
@@ -288,7 +292,6 @@ hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
     s.dy_type = d.dy_type;
     s.p_type = d.pre_type;
     s.rows = p.rows;
-    s.vec = fits16(d.dy, d.lddy, in_bytes(d.dy_type)) && fits16(s.pre, d.ldp, in_bytes(d.pre_type));
     const dim3 grid((unsigned)((d.N + 255) / 256), (unsigned)p.blocks);
     const bool b = d.type == HIPGEMM_IN_BF16;
     const void* fn = d.gated ? (b ? (const void*)&k_dense_slope<kInBf16, true>

@@ -5,7 +5,7 @@ namespace hipgemm {
 namespace kernels {
 
 const void* dense_tile_bf16_gated(int tile, bool split) {
-  return dense_tile_of<detail::kInBf16, false, false, true>(tile, split);
+  return dense_tile_of<detail::kInBf16, false, false, detail::kEpiGated>(tile, split);
 }
 
 }  // namespace kernels

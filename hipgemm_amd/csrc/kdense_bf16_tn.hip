@@ -5,7 +5,7 @@ namespace hipgemm {
 namespace kernels {
 
 const void* dense_tile_bf16_tn(int tile, bool split) {
-  return dense_tile_of<detail::kInBf16, true, true, false>(tile, split);
+  return dense_tile_of<detail::kInBf16, true, true, detail::kEpiPlain>(tile, split);
 }
 
 }  // namespace kernels

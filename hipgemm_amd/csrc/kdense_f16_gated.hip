@@ -5,7 +5,7 @@ namespace hipgemm {
 namespace kernels {
 
 const void* dense_tile_f16_gated(int tile, bool split) {
-  return dense_tile_of<detail::kInF16, false, false, true>(tile, split);
+  return dense_tile_of<detail::kInF16, false, false, detail::kEpiGated>(tile, split);
 }
 
 }  // namespace kernels

@@ -5,7 +5,7 @@ namespace hipgemm {
 namespace kernels {
 
 const void* dense_tile_f16_nn(int tile, bool split) {
-  return dense_tile_of<detail::kInF16, false, true, false>(tile, split);
+  return dense_tile_of<detail::kInF16, false, true, detail::kEpiPlain>(tile, split);
 }
 
 }  // namespace kernels

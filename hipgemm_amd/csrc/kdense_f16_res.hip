@@ -1,0 +1,12 @@
+// Products of f16 operands: both operands along K, with a residual.
+#include "kdense.hpp"
+
+namespace hipgemm {
+namespace kernels {
+
+const void* dense_tile_f16_res(int tile, bool split) {
+  return dense_tile_of<detail::kInF16, false, false, detail::kEpiResidual>(tile, split);
+}
+
+}  // namespace kernels
+}  // namespace hipgemm

@@ -85,11 +85,11 @@ const void* moe_up(int x, int w, int s, int mode, int mt, int wk);
 const void* moe_down(int w, int s, int mode, int mt, int wk, int h);
 const void* moe_vec_up(int x, int w, int s, int lk);
 const void* moe_vec_down(int w, int s, int lk, int h);
-// Products of 16-bit operands (kdense_*.hip).  layout: kDenseNT (both along K),
-// kDenseNN (the second across), kDenseTN (both across), kDenseGated (both along, gate
-// and up rows); tile: index of kDenseTiles.
-enum { kDenseNT = 0, kDenseNN = 1, kDenseTN = 2, kDenseGated = 3 };
-const void* dense_tile(int x, int layout, int tile, bool split);
+// Products of 16-bit operands (kdense_*.hip).  kind: kDenseNT (both along K),
+// kDenseRes (and a residual), kDenseNN (the second across K), kDenseTN (both across),
+// kDenseGated (both along, gate and up rows); tile: index of kDenseTiles.
+enum { kDenseNT = 0, kDenseRes = 1, kDenseNN = 2, kDenseTN = 3, kDenseGated = 4 };
+const void* dense_tile(int x, int kind, int tile, bool split);
 // Packs [rows][ceil(K/32)] E8M0 scales (row stride ld) into MxArgs' layout.
 hipError_t mx_pack(const uint8_t* src, int rows, int K, int ld, uint8_t* dst,
                    hipStream_t stream);
@@ -144,8 +144,8 @@ constexpr int kNumTiles = 3, kNumNarrow = 2;
 constexpr TileShape kTiles[kNumTiles] = {{128, 256}, {192, 192}, {192, 128}};
 constexpr TileShape kNarrow[kNumNarrow] = {{128, 64}, {64, 64}};
 // Tiles of the products of 16-bit operands.
-constexpr int kNumDenseTiles = 1;
-constexpr TileShape kDenseTiles[kNumDenseTiles] = {{128, 128}};
+constexpr int kNumDenseTiles = 2;
+constexpr TileShape kDenseTiles[kNumDenseTiles] = {{128, 128}, {256, 256}};
 template <class F>
 const void* sel_tile(int t, F&& f) {
   switch (t) {

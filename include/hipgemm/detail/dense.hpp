@@ -38,11 +38,13 @@
 // kSplit: work units are (tile, K-slice) pairs that write their fp32 sums to
 // `partial`; k_dense_reduce adds them in order and finishes.
 //
-// Epilogue: sums through the wave's own LDS stage, 16 rows at a time, to eight
-// neighbouring columns of a lane: bias, activation, residual and all stores go 16 bytes
-// per lane; single elements, neighbouring lanes side by side, where sizes, strides
-// or addresses do not allow 16 bytes.
+// Epilogue: two neighbouring blocks' sums change places between lane groups
+// (v_permlane16_swap), so that a lane has eight columns of a row: bias, activation, residual
+// and all stores go 16 bytes per lane, 64 bytes of a row side by side, at any address.
+// Only where N ends inside a lane's eight columns they go one by one.
 #pragma once
+
+#include <utility>
 
 #include "arch.hpp"
 #include "decode.hpp"
@@ -51,6 +53,12 @@
 
 namespace hipgemm {
 namespace detail {
+
+// kEpi: what the sums become.
+constexpr int kEpiPlain = 0;     // stored
+constexpr int kEpiLinear = 1;    // bias, pre, activation
+constexpr int kEpiResidual = 2;  // and a residual
+constexpr int kEpiGated = 3;     // bias, pre, activation, product
 
 // What becomes of the sums (types: kOut*, kIn*; strides in elements).
 struct DenseEpi {
@@ -61,7 +69,6 @@ struct DenseEpi {
   long long ldy, ldr, ldp;
   long long up;         // gated: columns from a gate sum to its up sum, in pre
   int act, y_type, p_type, b_type, r_type;
-  int vec;              // 16-byte accesses fit
 };
 
 struct DenseArgs {
@@ -84,9 +91,7 @@ struct CfgDense {
   static constexpr int kFA = kWM / 16, kFB = kWN / 16;
   static constexpr int kAStage = kBM * kRow;
   static constexpr int kStage = (kBM + kBN) * kRow;
-  static constexpr int kOutStage = 16 * kWN * 4;  // of a wave
-  static constexpr int kOutBase = S * kStage;
-  static constexpr int kLdsBytes = kOutBase + 4 * kOutStage;
+  static constexpr int kLdsBytes = S * kStage;
   static constexpr int kDmaA = BM / 32, kDmaB = BN / 32;  // per wave and step
   static constexpr int kDma = kDmaA + kDmaB;
   static_assert(kLdsBytes <= 160 * 1024, "LDS");
@@ -102,18 +107,31 @@ __device__ __forceinline__ float widen(uint32_t h, int type) {
 __device__ __forceinline__ uint32_t narrow2(float lo, float hi, bool bf16) {
   return bf16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
 }
-__device__ __forceinline__ void load8(const uint8_t* p, long long at, int type,
-                                      float (&v)[8]) {
+// Sixteen bytes at an address that is a multiple of an element (the memory system takes
+// any; the type says so to the compiler).
+struct __attribute__((packed, aligned(2))) Any16 {
+  i32x4 v;
+};
+__device__ __forceinline__ i32x4 load16(const uint8_t* p) {
+  return reinterpret_cast<const Any16*>(p)->v;
+}
+// Eight elements as they lie in memory: 16-bit ones in a, fp32 in a and b.
+struct Raw8 {
+  i32x4 a, b;
+};
+__device__ __forceinline__ Raw8 raw8(const uint8_t* p, long long at, int type) {
+  if (type == kInF32) return Raw8{load16(p + 4 * at), load16(p + 4 * at + 16)};
+  return Raw8{load16(p + 2 * at), i32x4{}};
+}
+__device__ __forceinline__ void widen8(const Raw8& r, int type, float (&v)[8]) {
   if (type == kInF32) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * at);
-    const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4 * at + 16);
+    const f32x4 a = __builtin_bit_cast(f32x4, r.a), b = __builtin_bit_cast(f32x4, r.b);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
   } else {
-    const i32x4 a = *reinterpret_cast<const i32x4*>(p + 2 * at);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t d = (uint32_t)a[e];
+      const uint32_t d = (uint32_t)r.a[e];
       if (type == kInBf16) {
         v[2 * e] = __builtin_bit_cast(float, d << 16);
         v[2 * e + 1] = __builtin_bit_cast(float, d & 0xffff0000u);
@@ -124,13 +142,17 @@ __device__ __forceinline__ void load8(const uint8_t* p, long long at, int type,
     }
   }
 }
+__device__ __forceinline__ void load8(const uint8_t* p, long long at, int type,
+                                      float (&v)[8]) {
+  widen8(raw8(p, at, type), type, v);
+}
 __device__ __forceinline__ float load1(const uint8_t* p, long long at, int type) {
   if (type == kInF32) return *reinterpret_cast<const float*>(p + 4 * at);
   return widen(*reinterpret_cast<const uint16_t*>(p + 2 * at), type);
 }
 // A store of 16 bytes, and the wait states of store_b128 (arch.hpp).
 __device__ __forceinline__ void store16(uint8_t* p, i32x4 v) {
-  *reinterpret_cast<i32x4*>(p) = v;
+  reinterpret_cast<Any16*>(p)->v = v;
   asm volatile("s_nop 1" ::: "memory");
 }
 __device__ __forceinline__ void store8(uint8_t* p, long long at, int out,
@@ -165,58 +187,73 @@ __device__ __forceinline__ void activate8(float (&v)[8], int act) {
   }
 }
 
-// Eight columns from `col` of row `row`: v (gated: gate sums, u the up sums).
-template <bool kGated>
-__device__ __forceinline__ void finish8(const DenseEpi& e, long long row, int col, int N,
-                                        float (&v)[8], float (&u)[8]) {
-  if (e.bias) {
-    float b[8];
-    load8(e.bias, col, e.b_type, b);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += b[i];
-    if constexpr (kGated) {
-      load8(e.bias, (long long)N + col, e.b_type, b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] += b[i];
+// Element offsets of a row's first column here in the result, the residual and pre.
+struct DenseAt {
+  long long y, r, p;
+};
+__device__ __forceinline__ DenseAt dense_at(const DenseEpi& e, long long row, int col) {
+  return DenseAt{row * e.ldy + col, row * e.ldr + col, row * e.ldp + col};
+}
+
+// Eight columns from `at` + c: v (gated: gate sums, u the up sums), with the bias; r: the
+// residual, if there is one.
+template <int kEpi>
+__device__ __forceinline__ void finish8(const DenseEpi& e, const DenseAt& at, int c,
+                                        float (&v)[8], float (&u)[8], const Raw8& r) {
+  if constexpr (kEpi != kEpiPlain) {
+    if (e.pre) {
+      store8(e.pre, at.p + c, e.p_type, v);
+      if constexpr (kEpi == kEpiGated) store8(e.pre, at.p + e.up + c, e.p_type, u);
     }
+    activate8(v, e.act);
   }
-  if (e.pre) {
-    store8(e.pre, row * e.ldp + col, e.p_type, v);
-    if constexpr (kGated) store8(e.pre, row * e.ldp + e.up + col, e.p_type, u);
-  }
-  activate8(v, e.act);
-  if constexpr (kGated) {
+  if constexpr (kEpi == kEpiGated) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= u[i];
   }
-  if (e.r) {
-    float r[8];
-    load8(e.r, row * e.ldr + col, e.r_type, r);
+  if constexpr (kEpi == kEpiResidual) {
+    float w[8];
+    widen8(r, e.r_type, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += r[i];
+    for (int i = 0; i < 8; ++i) v[i] += w[i];
   }
-  store8(e.y, row * e.ldy + col, e.y_type, v);
+  store8(e.y, at.y + c, e.y_type, v);
 }
-template <bool kGated>
-__device__ __forceinline__ void finish1(const DenseEpi& e, long long row, int col, int N,
-                                        float v, float u) {
-  if (e.bias) {
-    v += load1(e.bias, col, e.b_type);
-    if constexpr (kGated) u += load1(e.bias, (long long)N + col, e.b_type);
+// One column; v, u without the bias.
+template <int kEpi>
+__device__ __forceinline__ void finish1(const DenseEpi& e, const DenseAt& at, int c, int col,
+                                        int N, float v, float u) {
+  if constexpr (kEpi != kEpiPlain) {
+    if (e.bias) {
+      v += load1(e.bias, col, e.b_type);
+      if constexpr (kEpi == kEpiGated) u += load1(e.bias, (long long)N + col, e.b_type);
+    }
+    if (e.pre) {
+      store1(e.pre, at.p + c, e.p_type, v);
+      if constexpr (kEpi == kEpiGated) store1(e.pre, at.p + e.up + c, e.p_type, u);
+    }
+    v = activate(v, e.act);
   }
-  if (e.pre) {
-    store1(e.pre, row * e.ldp + col, e.p_type, v);
-    if constexpr (kGated) store1(e.pre, row * e.ldp + e.up + col, e.p_type, u);
-  }
-  v = activate(v, e.act);
-  if constexpr (kGated) v *= u;
-  if (e.r) v += load1(e.r, row * e.ldr + col, e.r_type);
-  store1(e.y, row * e.ldy + col, e.y_type, v);
+  if constexpr (kEpi == kEpiGated) v *= u;
+  if constexpr (kEpi == kEpiResidual) v += load1(e.r, at.r + c, e.r_type);
+  store1(e.y, at.y + c, e.y_type, v);
 }
 
 // ---- tiles --------------------------------------------------------------------
 
 __host__ __device__ constexpr int col_xor(int k) { return 2 * ((k & 3) | (((k >> 4) & 1) << 2)); }
+
+// f(0), .., f(N - 1) with constants.
+template <int N, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+  [&]<int... I>(std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+  }(std::make_integer_sequence<int, N>{});
+}
+// Of `count` things spread evenly over `span` places from 0, those before place n.
+constexpr int due(int n, int span, int count) {
+  return n <= 0 ? 0 : n >= span ? count : (n * count + span - 1) / span;
+}
 
 using s16x4 = short __attribute__((ext_vector_type(4)));
 using s16x8 = short __attribute__((ext_vector_type(8)));
@@ -242,8 +279,9 @@ __device__ __forceinline__ void mfma_acc(i32x4 a, i32x4 b, f32x4& c) {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
-template <class Cfg, int kX, bool kACol, bool kBCol, bool kGated, bool kSplit>
+template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi, bool kSplit>
 __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds) {
+  constexpr bool kGated = kEpi == kEpiGated, kRes = kEpi == kEpiResidual;
   constexpr int S = Cfg::kStages, FA = Cfg::kFA, FB = Cfg::kFB;
   constexpr int kBK = Cfg::kBK, kDma = Cfg::kDma;
   constexpr int kMfma = FA * FB;  // of a half
@@ -251,9 +289,8 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   constexpr int kReads = kReadA * FA + kReadB * FB;
   // MFMA of half 0 that are issued after the barrier: they read registers only and
   // keep the matrix unit busy while the waves meet.
-  constexpr int kTail = 2, kHead = kMfma - kTail;
-  constexpr int kPer = (kReads + kHead - 1) / kHead;  // reads after one MFMA
-  constexpr int kDmaAt = kReads + kDma <= kHead ? kReads : 0;
+  constexpr int kTail = kMfma >= 16 ? 2 : 0, kHead = kMfma - kTail;
+  constexpr int kSpan = kMfma * 48 / 64;
   constexpr int kWNr = kGated ? Cfg::kWN / 2 : Cfg::kWN;  // result columns of a wave
   constexpr int kBNr = 2 * kWNr;
   static_assert((S - 2) * kDma < 64, "vmcnt range");
@@ -445,45 +482,49 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     const int i = n / FB, j = i % 2 ? FB - 1 - n % FB : n % FB;
     mfma_acc<kX>(frag(fb[h][j]), frag(fa[h][i]), acc[i][j]);
   };
+  // Each MFMA of a half is followed by the reads and DMA that are due: reads spread over
+  // three quarters of its MFMA, DMA over all of half 1 (256 x 256 x K 14336 / 4096, both in rows,
+  // TFLOP/s: 1552 / 1409; reads one after each of the first sixteen MFMA and DMA after them
+  // 1543 / 1385, across K 1315 for 1410: LDS is busy three quarters of the time, bursts
+  // queue).
   auto half0 = [&](int st) {
     wait_lgkmcnt<0>();
-#pragma unroll
-    for (int n = 0; n < kHead; ++n) {
+    static_for<kHead>([&](auto n) {
       mfma(0, n);
-#pragma unroll
-      for (int r = 0; r < kPer; ++r)
-        if (n * kPer + r < kReads) read_one(st, 1, n * kPer + r);
+      static_for<due(n + 1, kSpan, kReads) - due(n, kSpan, kReads)>(
+          [&](auto r) { read_one(st, 1, due(n, kSpan, kReads) + r); });
       sched_fence();
-    }
+    });
   };
   auto half1 = [&](int st, int rst, int d) {
     const Step src = step_src(d);
-#pragma unroll
-    for (int n = kHead; n < kMfma; ++n) mfma(0, n);
+    static_for<kTail>([&](auto n) { mfma(0, kHead + n); });
     sched_fence();
-#pragma unroll
-    for (int n = 0; n < kMfma; ++n) {
+    static_for<kMfma>([&](auto n) {
       mfma(1, n);
-#pragma unroll
-      for (int r = 0; r < kPer; ++r)
-        if (n * kPer + r < kReads) read_one(rst, 0, n * kPer + r);
-#pragma unroll
-      for (int q = 0; q < kDma; ++q)
-        if (kDmaAt + q * (kMfma - kDmaAt) / kDma == n) dma_one(src, st, q);
+      static_for<due(n + 1, kSpan, kReads) - due(n, kSpan, kReads)>(
+          [&](auto r) { read_one(rst, 0, due(n, kSpan, kReads) + r); });
+      static_for<due(n + 1, kMfma, kDma) - due(n, kMfma, kDma)>(
+          [&](auto q) { dma_one(src, st, due(n, kMfma, kDma) + q); });
       sched_fence();
-    }
+    });
   };
   auto next_stage = [](int s) {
     s += Cfg::kStage;
     return s == S * Cfg::kStage ? 0 : s;
   };
   int st = 0;
+  bool stored = false;  // the previous tile was whole: all its stores were issued
+  constexpr int kStores = FA * FB / (kGated ? 4 : 2);  // at least
+  static_assert((S - 2) * kDma + kStores < 64, "vmcnt range");
   auto step = [&](int k) {
     const int rst = next_stage(st);
     half0(st);
-    // Step k + 1 has landed: newer are the DMA of S - 2 steps.
+    // Step k + 1 has landed: newer are the DMA of S - 2 steps, and in a tile's first S - 1
+    // steps the stores of the one before.
     wait_lgkmcnt<0>();
-    wait_vmcnt<(S - 2) * kDma>();
+    if (stored && k < S - 1) wait_vmcnt<(S - 2) * kDma + kStores>();
+    else wait_vmcnt<(S - 2) * kDma>();
     barrier();
     half1(st, rst, k + S);
     st = rst;
@@ -500,12 +541,16 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
 #pragma unroll
   for (int n = 0; n < kReads; ++n) read_one(0, 0, n);
 
-  lds_u8* const stg = lds + Cfg::kOutBase + wave * Cfg::kOutStage;
   for (;;) {
 #pragma unroll
     for (int i = 0; i < FA; ++i)
 #pragma unroll
-      for (int j = 0; j < FB; ++j) acc[i][j] = f32x4{};
+      for (int j = 0; j < FB; ++j) {
+        acc[i][j] = f32x4{};
+        asm volatile("" : "+a"(acc[i][j]));
+      }
+    // Two wait states from the last zero's write to the first matrix instruction.
+    asm volatile("s_nop 3");
     for (int k = 0; k < steps_pad; ++k) step(k);
 
     // ---- epilogue --------------------------------------------------------------
@@ -515,61 +560,105 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     const int row0 = tc.m * Cfg::kBM + wm * Cfg::kWM, col0 = tc.n * kBNr + wn * kWNr;
     int el = lane;
     asm volatile("" : "+v"(el));
-    constexpr int kChunkRow = Cfg::kWN * 4;  // bytes of a staged row
-    auto at = [&](int r, int chunk) { return stg + r * kChunkRow + ((chunk ^ (r & 7)) * 16); };
+    const DenseEpi& e = g.epi;
+    // Pair p of blocks: the lane's eight columns from col_l + 32 p (gated: of the gate where
+    // p < kResults, of the up half after).
+    constexpr int kPairs = FB / 2, kResults = kGated ? kPairs / 2 : kPairs;
+    int row_l = row0 + (el & 15);
+    int col_l = col0 + 16 * ((el >> 4) & 1) + 8 * (el >> 5);
+    auto whole = [&](int p) { return col_l + 32 * p + 8 <= g.N; };
+    float bias[kPairs][8] = {};
+    const bool biased = !kSplit && kEpi != kEpiPlain && e.bias;
+    if (biased) {
+#pragma unroll
+      for (int p = 0; p < kPairs; ++p)
+        if (whole(p % kResults))
+          load8(e.bias, (long long)(p / kResults) * g.N + col_l + 32 * (p % kResults), e.b_type,
+                bias[p]);
+      // No load may look pending where the K loop starts again: the compiler would have
+      // every step wait for all DMA before it uses the register.
+#pragma unroll
+      for (int p = 0; p < kPairs; ++p)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) asm volatile("" : "+v"(bias[p][x]));
+    }
+    Raw8 res[kResults] = {};
+    auto residual = [&](int row, long long at, int p) {
+      if (row < g.M && whole(p)) res[p] = raw8(e.r, at + 32 * p, e.r_type);
+    };
+    if constexpr (kRes) {
+#pragma unroll
+      for (int p = 0; p < kResults; ++p) residual(row_l, row_l * e.ldr + col_l, p);
+    }
     // (Rolled, the accumulators picked by branches: unrolled the epilogue is FA times
     // the code, and its array stays in memory.)
 #pragma nounroll
     for (int i = 0; i < FA; ++i) {
+      f32x4 blk[FB];
 #pragma unroll
       for (int b = 0; b < FA; ++b)
         if (b == i) {
+          // (Opaque: their elements are read here, not ahead of the loop, where nothing
+          // would keep the reads behind mfma_drain.)
 #pragma unroll
-          for (int j = 0; j < FB; ++j)
-            *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(
-                at(el & 15, 4 * j + (el >> 4))) = acc[b][j];
+          for (int j = 0; j < FB; ++j) asm volatile("" : "+a"(acc[b][j]));
+#pragma unroll
+          for (int j = 0; j < FB; ++j) blk[j] = acc[b][j];
         }
-      compiler_fence();
-      auto read8 = [&](int r, int chunk, float (&v)[8]) {
-        const f32x4 a = __builtin_bit_cast(f32x4, lds_read16(at(r, chunk)));
-        const f32x4 b = __builtin_bit_cast(f32x4, lds_read16(at(r, chunk + 1)));
+      // Lane group g has columns 4 g .. + 3 of two neighbouring blocks; after the swap
+      // of its odd 16 lanes with the other's even ones, eight of one block.
+      float v[kPairs][8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
-      };
-      constexpr int kUnits = kWNr / 8, kRows = 64 / kUnits;
-      if (kSplit || g.epi.vec) {
+      for (int p = 0; p < kPairs; ++p) {
+        // (Bit casts of whole vectors: of one element they yield element 0.)
+        const i32x4 b0 = __builtin_bit_cast(i32x4, blk[2 * p]);
+        const i32x4 b1 = __builtin_bit_cast(i32x4, blk[2 * p + 1]);
 #pragma unroll
-        for (int q = 0; q < 16 / kRows; ++q) {
-          const int r = q * kRows + el / kUnits, c = el % kUnits;
-          const int row = row0 + 16 * i + r, col = col0 + 8 * c;
-          float v[8], u[8] = {};
-          read8(r, 2 * c, v);
-          if constexpr (kGated) read8(r, kWNr / 4 + 2 * c, u);
-          if (row < g.M && col < g.N) {
-            if constexpr (kSplit) {
-              const int slice = t / tiles;
-              uint8_t* p = reinterpret_cast<uint8_t*>(g.partial);
-              const long long o = ((long long)slice * g.M + row) * g.ldpart + col;
-              store8(p, o, kOutF32, v);
-              if constexpr (kGated) store8(p, o + g.ldpart / 2, kOutF32, u);
-            } else {
-              finish8<kGated>(g.epi, row, col, g.N, v, u);
-            }
-          }
-        }
-      } else {
-        for (int q = 0; q < 16 * kWNr / 64; ++q) {
-          const int r = (64 * q + el) / kWNr, c = (64 * q + el) % kWNr;
-          const int row = row0 + 16 * i + r, col = col0 + c;
-          auto read1 = [&](int x) {
-            return __builtin_bit_cast(float, lds_read4(at(r, x >> 2) + (x & 3) * 4));
-          };
-          if (row < g.M && col < g.N)
-            finish1<kGated>(g.epi, row, col, g.N, read1(c), kGated ? read1(kWNr + c) : 0.0f);
+        for (int x = 0; x < 4; ++x) {
+          const auto s2 =
+              __builtin_amdgcn_permlane16_swap((uint32_t)b0[x], (uint32_t)b1[x], false, false);
+          const uint32_t lo = s2[0], hi = s2[1];
+          v[p][x] = __builtin_bit_cast(float, lo);
+          v[p][4 + x] = __builtin_bit_cast(float, hi);
         }
       }
-      compiler_fence();
+      // (Opaque: addresses are made here, not all of them before the loop.)
+      asm volatile("" : "+v"(row_l), "+v"(col_l));
+      if (row_l < g.M) {
+        const DenseAt at = dense_at(e, row_l, col_l);
+        const long long part = ((long long)(kSplit ? t / tiles : 0) * g.M + row_l) * g.ldpart + col_l;
+#pragma unroll
+        for (int p = 0; p < kResults; ++p) {
+          const int col = col_l + 32 * p;
+          float(&u)[8] = v[kGated ? p + kResults : p];
+          if constexpr (kSplit) {
+            if (col < g.N) {
+              uint8_t* to = reinterpret_cast<uint8_t*>(g.partial);
+              store8(to, part + 32 * p, kOutF32, v[p]);
+              if constexpr (kGated) store8(to, part + g.ldpart / 2 + 32 * p, kOutF32, u);
+            }
+          } else if (whole(p)) {
+            if (biased) {
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                v[p][x] += bias[p][x];
+                if constexpr (kGated) u[x] += bias[p + kResults][x];
+              }
+            }
+            finish8<kEpi>(e, at, 32 * p, v[p], u, res[p]);
+            if (kRes && i + 1 < FA) residual(row_l + 16, at.r + 16 * e.ldr, p);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              if (col + x < g.N) finish1<kEpi>(e, at, 32 * p + x, col + x, g.N, v[p][x], u[x]);
+          }
+        }
+      }
+      row_l += 16;
     }
+    // (As for the bias.)
+    if constexpr (kRes) wait_vmcnt<0>();
+    stored = row0 + Cfg::kWM <= g.M && col0 + kWNr <= g.N;
     t += walk.stride;
     if (t >= walk.end) break;
     cur = nxt;
@@ -582,8 +671,9 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
 // ---- K-slices' sums -----------------------------------------------------------
 
 // A thread per row and eight columns: slices in order, then the epilogue.
-template <bool kGated>
+template <int kEpi>
 __device__ __forceinline__ void dense_reduce_body(const DenseArgs& g) {
+  constexpr bool kGated = kEpi == kEpiGated;
   const int units = (g.N + 7) / 8;
   const long long x = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   const long long row = x / units;
@@ -603,12 +693,27 @@ __device__ __forceinline__ void dense_reduce_body(const DenseArgs& g) {
       for (int e = 0; e < 8; ++e) u[e] += w[e];
     }
   }
-  if (g.epi.vec) {
-    finish8<kGated>(g.epi, row, col, g.N, v, u);
+  const DenseEpi& e = g.epi;
+  const DenseAt at = dense_at(e, row, col);
+  if (col + 8 <= g.N) {
+    if (kEpi != kEpiPlain && e.bias) {
+      float b[8];
+      load8(e.bias, col, e.b_type, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += b[i];
+      if constexpr (kGated) {
+        load8(e.bias, (long long)g.N + col, e.b_type, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] += b[i];
+      }
+    }
+    Raw8 r{};
+    if constexpr (kEpi == kEpiResidual) r = raw8(e.r, at.r, e.r_type);
+    finish8<kEpi>(e, at, 0, v, u, r);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (col + e < g.N) finish1<kGated>(g.epi, row, col + e, g.N, v[e], u[e]);
+    for (int i = 0; i < 8; ++i)
+      if (col + i < g.N) finish1<kEpi>(e, at, i, col + i, g.N, v[i], u[i]);
   }
 }
 
@@ -645,7 +750,6 @@ struct SlopeArgs {
   int M, N;        // of dy; dz has 2 N columns where gated
   int act, dy_type, p_type;
   int rows;        // of a block
-  int vec;         // dy and pre in 16-byte accesses
 };
 
 // dz = dy act'(z);  gated, z = [g | u]: [dy u act'(g) | dy act(g)].  Rounded to the
@@ -661,7 +765,7 @@ __device__ __forceinline__ void dense_slope_body(const SlopeArgs& g, float* sums
   const long long first = (long long)blockIdx.y * g.rows;
   const long long end = min((long long)g.M, first + g.rows);
   const bool live = col < g.N;
-  const bool whole = g.vec && col + 8 <= g.N;
+  const bool whole = col + 8 <= g.N;
   float sum[kParts][8] = {};
   if (live)
     for (long long row = first + ty; row < end; row += 8) {
