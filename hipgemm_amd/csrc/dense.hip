@@ -9,8 +9,8 @@ namespace hipgemm {
 namespace kernels {
 
 #define HIPGEMM_DENSE(L)                             \
-  const void* dense_tile_bf16_##L(int tile, bool split); \
-  const void* dense_tile_f16_##L(int tile, bool split);
+  const void* dense_tile_bf16_##L(int tile, int mode); \
+  const void* dense_tile_f16_##L(int tile, int mode);
 HIPGEMM_DENSE(nt)
 HIPGEMM_DENSE(res)
 HIPGEMM_DENSE(nn)
@@ -18,15 +18,15 @@ HIPGEMM_DENSE(tn)
 HIPGEMM_DENSE(gated)
 #undef HIPGEMM_DENSE
 
-const void* dense_tile(int x, int kind, int tile, bool split) {
+const void* dense_tile(int x, int kind, int tile, int mode) {
   const bool b = x == detail::kInBf16;
   switch (kind) {
-    case kDenseNT: return b ? dense_tile_bf16_nt(tile, split) : dense_tile_f16_nt(tile, split);
-    case kDenseRes: return b ? dense_tile_bf16_res(tile, split) : dense_tile_f16_res(tile, split);
-    case kDenseNN: return b ? dense_tile_bf16_nn(tile, split) : dense_tile_f16_nn(tile, split);
-    case kDenseTN: return b ? dense_tile_bf16_tn(tile, split) : dense_tile_f16_tn(tile, split);
+    case kDenseNT: return b ? dense_tile_bf16_nt(tile, mode) : dense_tile_f16_nt(tile, mode);
+    case kDenseRes: return b ? dense_tile_bf16_res(tile, mode) : dense_tile_f16_res(tile, mode);
+    case kDenseNN: return b ? dense_tile_bf16_nn(tile, mode) : dense_tile_f16_nn(tile, mode);
+    case kDenseTN: return b ? dense_tile_bf16_tn(tile, mode) : dense_tile_f16_tn(tile, mode);
     default:
-      return b ? dense_tile_bf16_gated(tile, split) : dense_tile_f16_gated(tile, split);
+      return b ? dense_tile_bf16_gated(tile, mode) : dense_tile_f16_gated(tile, mode);
   }
 }
 
@@ -70,20 +70,91 @@ hipError_t launch(const void* fn, dim3 grid, Args& g, hipStream_t stream) {
 // ---- one product ----------------------------------------------------------------
 
 struct Plan {
-  int tile, slices, slice_steps;
+  int tile;  // index of kDenseTiles, or -1: a few rows
+  int slices, slice_steps;
   long long units;
 };
+
+// Estimated times, us.  A tile's step of 64 along K by how the operands lie, and its end,
+// with every CU at work on operands that come from memory: 128 x 128, 256 x 256, 64 x 128,
+// 256 x 128.  Measured against every tile and 1, 2, 4, 8 slices on 190 shapes, the choice is
+// within 5 % of the best at the median (us, chosen / best):
+//   forward   64 x 4096 x 4096 14.6/14.6 (rows; tiles 16.5), 96 x 4096 x 14336 34.0/34.0 (128 x 128
+//             in 8 slices; 64 x 128 37.4), 512 x 14336 x 4096 65/64 (256 x 128; 128 x 128 83),
+//             1024 x 4096 x 4096 39.7/39.7 (128 x 128; 256 x 128 54.9)
+//   of x      777 x 14336 x 4096 108/106 (256 x 128 in 2 slices; 128 x 128 128)
+//   of w      4096 x 14336 x 4096 391/391 (256 x 256; 256 x 128 432)
+struct TileTime {
+  double forward, of_x, of_w, end;
+};
+constexpr TileTime kTime[hk::kNumDenseTiles] = {{0.57, 0.55, 0.58, 1.5},
+                                                {1.55, 1.55, 1.50, 5.0},
+                                                {0.40, 0.42, 0.0, 1.0},
+                                                {0.85, 0.85, 0.96, 3.0}};
+constexpr double kLaunch = 4.0, kSplitLaunch = 3.5;
+constexpr double kBytesPerUs = 5.0e6;      // from memory
+constexpr double kCuBytesPerUs = 75.0e3;   // into one CU
+constexpr int kCus = 256;
+
+double split_us(int slices, int M, int N, bool gated) {
+  if (slices == 1) return 0.0;
+  return kSplitLaunch + 8.0 * slices * M * (double)N * (gated ? 2 : 1) / kBytesPerUs;
+}
+
+// A few rows: what a CU has to fetch (x again for every 16 rows of weights), or the weights
+// from memory, and more of both with more rows.
+double rows_us(int M, int N, int K, bool gated, int slices) {
+  const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  const double rows = N * (gated ? 2.0 : 1.0);
+  const long long groups = (long long)((rows + 15) / 16) * slices;
+  const double cu = (double)((groups + kCus - 1) / kCus) * 32.0 * (1 + mt) * K / slices;
+  const double us = cu / kCuBytesPerUs, memory = 2.0 * rows * K / kBytesPerUs;
+  return kLaunch + (us > memory ? us : memory) * (0.9 + 0.1 * mt) + split_us(slices, M, N, gated);
+}
+
+// The fewest estimated us: rounds of tiles over the CUs, no less than the operands' bytes
+// take, and for K-slices the way of their sums through memory.
 Plan plan_of(int kind, int M, int N, int K) {
-  Plan p{0, 1, 0, 0};
-  auto units = [&](int tile) {
-    const hk::TileShape s = hk::kDenseTiles[tile];
-    const int cols = kind == hk::kDenseGated ? s.bn / 2 : s.bn;
-    return (((long long)M + s.bm - 1) / s.bm) * (((long long)N + cols - 1) / cols);
-  };
-  if (units(1) >= 160) p.tile = 1;
-  p.units = units(p.tile) * p.slices;
-  (void)K;
-  return p;
+  const int steps = (int)(((long long)K + 63) / 64);
+  const bool gated = kind == hk::kDenseGated;
+  const bool forward = gated || kind == hk::kDenseNT || kind == hk::kDenseRes;
+  Plan best{0, 1, steps, 0};
+  double least = 1e300;
+  if (forward && M <= 64)
+    for (int slices = 1; slices <= 4 && steps >= 16 * (slices - 1); slices *= 2) {
+      const double us = rows_us(M, N, K, gated, slices);
+      if (us < least) {
+        least = us;
+        best = {-1, slices, (steps + slices - 1) / slices, 0};
+      }
+    }
+  // (Nothing beats it: it is a pass over the weights.)
+  if (forward && M <= 16) return best;
+  const double memory =
+      2.0 * ((double)M + N * (gated ? 2.0 : 1.0)) * K / kBytesPerUs;
+  for (int t = 0; t < hk::kNumDenseTiles; ++t) {
+    if (kind == hk::kDenseTN && t == 2) continue;
+    const hk::TileShape s = hk::kDenseTiles[t];
+    const int cols = gated ? s.bn / 2 : s.bn;
+    const long long tiles =
+        (((long long)M + s.bm - 1) / s.bm) * (((long long)N + cols - 1) / cols);
+    const double step = forward                ? kTime[t].forward
+                        : kind == hk::kDenseNN ? kTime[t].of_x
+                                               : kTime[t].of_w;
+    for (int slices = 1; slices <= 16; ++slices) {
+      if (slices > 1 && (tiles * slices > 2 * kCus || steps < 4 * slices)) break;
+      const int each = (steps + slices - 1) / slices;
+      const long long units = tiles * slices;
+      const double work = (double)((units + kCus - 1) / kCus) * (each * step + kTime[t].end);
+      const double us =
+          kLaunch + (work > memory ? work : memory) + split_us(slices, M, N, gated);
+      if (us < least) {
+        least = us;
+        best = {t, slices, each, units};
+      }
+    }
+  }
+  return best;
 }
 
 // Columns of a partial sum's row.
@@ -99,16 +170,23 @@ size_t partial_bytes(int kind, const Plan& p, int M, int N) {
 // g: operands, sizes and epilogue; ws: partial_bytes.
 hipError_t product(int x, int kind, DenseArgs& g, void* ws, hipStream_t stream) {
   const Plan p = plan_of(kind, g.M, g.N, g.K);
-  const hk::TileShape s = hk::kDenseTiles[p.tile];
-  const int cols = kind == hk::kDenseGated ? s.bn / 2 : s.bn;
-  g.group_m = default_group_m((g.M + s.bm - 1) / s.bm, (g.N + cols - 1) / cols);
   g.slices = p.slices;
   g.slice_steps = p.slice_steps;
   g.partial = static_cast<float*>(ws);
   g.ldpart = partial_columns(kind, g.N);
-  const long long most = 256;
-  hipError_t e = launch(hk::dense_tile(x, kind, p.tile, p.slices > 1),
-                        dim3((unsigned)(p.units < most ? p.units : most)), g, stream);
+  hipError_t e;
+  if (p.tile < 0) {
+    const int cols = kind == hk::kDenseGated ? 8 : 16;
+    e = launch(hk::dense_rows(x, kind, g.M <= 16 ? 1 : g.M <= 32 ? 2 : 4),
+               dim3((unsigned)((g.N + cols - 1) / cols), (unsigned)p.slices), g, stream);
+  } else {
+    const hk::TileShape s = hk::kDenseTiles[p.tile];
+    const int cols = kind == hk::kDenseGated ? s.bn / 2 : s.bn;
+    g.group_m = default_group_m((g.M + s.bm - 1) / s.bm, (g.N + cols - 1) / cols);
+    const int once = s.bm == 64 && g.M <= 64 && kind != hk::kDenseNN ? hk::kDenseOnce : 0;
+    e = launch(hk::dense_tile(x, kind, p.tile, once | (p.slices > 1 ? hk::kDenseSplit : 0)),
+               dim3((unsigned)(p.units < kCus ? p.units : kCus)), g, stream);
+  }
   if (e != hipSuccess || p.slices == 1) return e;
   const long long threads = (long long)g.M * ((g.N + 7) / 8);
   const void* fn = kind == hk::kDenseGated ? (const void*)&k_dense_reduce<kEpiGated>

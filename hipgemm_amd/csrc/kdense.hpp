@@ -9,24 +9,44 @@
 namespace hipgemm {
 namespace kernels {
 
-template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi, bool kSplit>
+template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi, bool kSplit, bool kOnce>
 __global__ __launch_bounds__(256, 1) void k_dense_tile(detail::DenseArgs g) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsBytes];
-  detail::dense_tile_body<Cfg, kX, kACol, kBCol, kEpi, kSplit>(g, (detail::lds_u8*)lds);
+  detail::dense_tile_body<Cfg, kX, kACol, kBCol, kEpi, kSplit, kOnce>(g, (detail::lds_u8*)lds);
+}
+
+template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi>
+const void* dense_tile_mode(int mode) {
+  // (Sums in slices know of the gate only.)
+  constexpr int kPart = kEpi == detail::kEpiGated ? kEpi : detail::kEpiPlain;
+  constexpr bool kOnce = Cfg::kBM == 64 && !kBCol;
+  switch (mode) {
+    case 0: return (const void*)&k_dense_tile<Cfg, kX, kACol, kBCol, kEpi, false, false>;
+    case kDenseSplit:
+      return (const void*)&k_dense_tile<Cfg, kX, kACol, kBCol, kPart, true, false>;
+    case kDenseOnce:
+      if constexpr (kOnce)
+        return (const void*)&k_dense_tile<Cfg, kX, kACol, kBCol, kEpi, false, true>;
+      return nullptr;
+    default:
+      if constexpr (kOnce)
+        return (const void*)&k_dense_tile<Cfg, kX, kACol, kBCol, kPart, true, true>;
+      return nullptr;
+  }
 }
 
 // tile: index of kDenseTiles.
 template <int kX, bool kACol, bool kBCol, int kEpi>
-const void* dense_tile_of(int tile, bool split) {
+const void* dense_tile_of(int tile, int mode) {
+  using namespace detail;
   auto of = [&](auto cfg) {
-    return sel2(split, [&](auto s) {
-      return (const void*)&k_dense_tile<decltype(cfg), kX, kACol, kBCol, kEpi,
-                                        decltype(s)::value>;
-    });
+    return dense_tile_mode<decltype(cfg), kX, kACol, kBCol, kEpi>(mode);
   };
   switch (tile) {
-    case 0: return of(detail::CfgDense<kDenseTiles[0].bm, kDenseTiles[0].bn, 4>{});
-    case 1: return of(detail::CfgDense<kDenseTiles[1].bm, kDenseTiles[1].bn, 2>{});
+    case 0: return of(CfgDense<kDenseTiles[0].bm, kDenseTiles[0].bn, 4>{});
+    case 1: return of(CfgDense<kDenseTiles[1].bm, kDenseTiles[1].bn, 2>{});
+    case 2: return kACol ? nullptr : of(CfgDense<kDenseTiles[2].bm, kDenseTiles[2].bn, 6>{});
+    case 3: return of(CfgDense<kDenseTiles[3].bm, kDenseTiles[3].bn, 3>{});
     default: return nullptr;
   }
 }

@@ -4,8 +4,8 @@
 namespace hipgemm {
 namespace kernels {
 
-const void* dense_tile_bf16_res(int tile, bool split) {
-  return dense_tile_of<detail::kInBf16, false, false, detail::kEpiResidual>(tile, split);
+const void* dense_tile_bf16_res(int tile, int mode) {
+  return dense_tile_of<detail::kInBf16, false, false, detail::kEpiResidual>(tile, mode);
 }
 
 }  // namespace kernels

@@ -4,8 +4,8 @@
 namespace hipgemm {
 namespace kernels {
 
-const void* dense_tile_f16_nn(int tile, bool split) {
-  return dense_tile_of<detail::kInF16, false, true, detail::kEpiPlain>(tile, split);
+const void* dense_tile_f16_nn(int tile, int mode) {
+  return dense_tile_of<detail::kInF16, false, true, detail::kEpiPlain>(tile, mode);
 }
 
 }  // namespace kernels

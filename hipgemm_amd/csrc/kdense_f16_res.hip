@@ -4,8 +4,8 @@
 namespace hipgemm {
 namespace kernels {
 
-const void* dense_tile_f16_res(int tile, bool split) {
-  return dense_tile_of<detail::kInF16, false, false, detail::kEpiResidual>(tile, split);
+const void* dense_tile_f16_res(int tile, int mode) {
+  return dense_tile_of<detail::kInF16, false, false, detail::kEpiResidual>(tile, mode);
 }
 
 }  // namespace kernels

@@ -89,7 +89,11 @@ const void* moe_vec_down(int w, int s, int lk, int h);
 // kDenseRes (and a residual), kDenseNN (the second across K), kDenseTN (both across),
 // kDenseGated (both along, gate and up rows); tile: index of kDenseTiles.
 enum { kDenseNT = 0, kDenseRes = 1, kDenseNN = 2, kDenseTN = 3, kDenseGated = 4 };
-const void* dense_tile(int x, int kind, int tile, bool split);
+const void* dense_tile(int x, int kind, int tile, int mode);
+// mode: bit 0 K-slices, bit 1 the second operand is read once (one row of tiles).
+enum { kDenseSplit = 1, kDenseOnce = 2 };
+// A few rows (kdense_rows.hip); mt: tiles of 16 rows of x (1, 2, 4).
+const void* dense_rows(int x, int kind, int mt);
 // Packs [rows][ceil(K/32)] E8M0 scales (row stride ld) into MxArgs' layout.
 hipError_t mx_pack(const uint8_t* src, int rows, int K, int ld, uint8_t* dst,
                    hipStream_t stream);
@@ -144,8 +148,8 @@ constexpr int kNumTiles = 3, kNumNarrow = 2;
 constexpr TileShape kTiles[kNumTiles] = {{128, 256}, {192, 192}, {192, 128}};
 constexpr TileShape kNarrow[kNumNarrow] = {{128, 64}, {64, 64}};
 // Tiles of the products of 16-bit operands.
-constexpr int kNumDenseTiles = 2;
-constexpr TileShape kDenseTiles[kNumDenseTiles] = {{128, 128}, {256, 256}};
+constexpr int kNumDenseTiles = 4;
+constexpr TileShape kDenseTiles[kNumDenseTiles] = {{128, 128}, {256, 256}, {64, 128}, {256, 128}};
 template <class F>
 const void* sel_tile(int t, F&& f) {
   switch (t) {

@@ -279,7 +279,7 @@ __device__ __forceinline__ void mfma_acc(i32x4 a, i32x4 b, f32x4& c) {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
-template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi, bool kSplit>
+template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi, bool kSplit, bool kOnce = false>
 __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds) {
   constexpr bool kGated = kEpi == kEpiGated, kRes = kEpi == kEpiResidual;
   constexpr int S = Cfg::kStages, FA = Cfg::kFA, FB = Cfg::kFB;
@@ -427,6 +427,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     const uint32_t v = col ? vo : vo | s.oob;
     const uint32_t so = col ? 0u : s.soff;
     if (is_a) dma16(s.a, to, v, so);
+    else if (kOnce) dma16_nt(is_up(q) ? s.b2 : s.b, to, v, so);
     else dma16(is_up(q) ? s.b2 : s.b, to, v, so);
   };
 
