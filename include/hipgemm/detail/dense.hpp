@@ -349,6 +349,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     const uint8_t *pa, *pb;
     uint32_t ca, cb;  // across: bytes of a row from pa, pb
     int k0, kend;
+    int full, rot;  // whole steps, and the one it starts at
   };
   auto rows_of = [](const uint8_t* p, long long ld, int first, int have, int most) {
     const int n = min(most, have - first);
@@ -360,7 +361,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
       s.a = s.b = s.b2 = make_rsrc(g.a, 0u);
       s.pa = s.pb = g.a;
       s.ca = s.cb = 0;
-      s.k0 = s.kend = 0;
+      s.k0 = s.kend = s.full = s.rot = 0;
       return s;
     }
     const int tile = kSplit ? unit % tiles : unit;
@@ -369,6 +370,8 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     const int m0 = c.m * Cfg::kBM, n0 = c.n * kBNr;
     s.k0 = kSplit ? slice * steps * kBK : 0;
     s.kend = kSplit ? (int)min((long long)g.K, (long long)s.k0 + (long long)steps * kBK) : g.K;
+    s.full = max(0, s.kend - s.k0) / kBK;
+    s.rot = (int)((blockIdx.x & 7u) * (unsigned)s.full / 8u);
     s.a = s.b = s.b2 = make_rsrc(g.a, 0u);
     s.pa = g.a;
     s.pb = g.b;
@@ -397,7 +400,10 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   // Step d of the unit, or past its end step d - steps_pad of the next.
   auto step_src = [&](int d) {
     const bool next = d >= steps_pad;
-    const int k = (next ? nxt.k0 : cur.k0) + (next ? d - steps_pad : d) * kBK;
+    const int at = next ? d - steps_pad : d, full = next ? nxt.full : cur.full;
+    int turned = at + (next ? nxt.rot : cur.rot);
+    if (turned >= full) turned -= full;
+    const int k = (next ? nxt.k0 : cur.k0) + (at < full ? turned : at) * kBK;
     const int kend = next ? nxt.kend : cur.kend;
     Step s;
     uint32_t soff = (uint32_t)k * 2u;

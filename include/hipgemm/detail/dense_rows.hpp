@@ -64,8 +64,10 @@ __device__ __forceinline__ void dense_rows_body(const DenseArgs& g, lds_u8* lds)
   const __amdgpu_buffer_rsrc_t ru =
       kGated ? make_rsrc(w0 + g.up, (uint32_t)rows * (uint32_t)g.ldb) : rw;
   const __amdgpu_buffer_rsrc_t rx = make_rsrc(g.a, (uint32_t)g.M * (uint32_t)g.lda);
+  const int rot = (int)((blockIdx.x & 7u) * (unsigned)mine / 8u);
   auto fetch = [&](int s, int stage) {
-    const int k = (first + wave + 4 * s) * 64;
+    const int turned = s + rot < mine ? s + rot : s + rot - mine;
+    const int k = (first + wave + 4 * turned) * 64;
     uint32_t oob[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p)
