@@ -11,7 +11,6 @@ record no gradient: hipgemm_amd.torch_dense has operators and modules that do.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 
@@ -79,24 +78,36 @@ def linear_backward_workspace_size(desc: "LinearGradDesc") -> int:
     return int(lib().hipgemm_linear_backward_workspace_size(ctypes.byref(desc)))
 
 
-def _device(dev, stream):
-    """The tensors' device as the current one."""
-    if stream is not None and stream.device != dev:
-        _bad(f"stream is on {stream.device}, x on {dev}")
-    if dev.index == _torch()._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return _torch().cuda.device(dev)
+def _launch(call, what, desc, x, stream):
+    """call(desc, stream) with x's device as the current one."""
+    torch = _torch()
+    dev = x.device
+    if dev.index == torch._C._cuda_getDevice():
+        return _check(call(ctypes.byref(desc), _stream_handle(x, stream)), what)
+    with torch.cuda.device(dev):
+        _check(call(ctypes.byref(desc), _stream_handle(x, stream)), what)
+
+
+@functools.lru_cache(maxsize=4096)
+def _forward_bytes(M, N, K, kind, device):
+    """Workspace of a forward call (a pure function of its sizes; kind: 0 linear, 1 with a
+    residual, 2 gated)."""
+    d = LinearDesc(size=_DESC_BYTES, M=M, N=N, K=K, gated=int(kind == 2), type=1,
+                   residual=int(kind == 1))
+    return linear_workspace_size(d)
 
 
 def _operand(t, name, dtype, device):
     """The row stride of a matrix that the products read as it is."""
-    if t.dim() != 2 or t.dtype != dtype or t.device != device:
+    if t.dtype is not dtype or t.dim() != 2 or t.device != device:
         _bad(f"{name} must be a 2-D {dtype} tensor on {device}, got {tuple(t.shape)} "
              f"{t.dtype} on {t.device}")
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    ld, unit = t.stride()
+    if cols > 1 and unit != 1:
         _bad(f"{name} must have unit stride along its rows")
-    ld = t.stride(0) if rows > 1 else cols
+    if rows <= 1:
+        ld = cols
     if rows and cols and (t.data_ptr() % 16 or ld % 8 or ld < cols):
         _bad(f"rows of {name} must start on 16 bytes")
     return ld
@@ -162,26 +173,36 @@ def _forward(x, weight, bias, activation, residual, out_dtype, out, save_pre, ga
     pt = outputs.get(pre_dtype)
     if pt is None:
         _bad("save_pre must be True, False, bfloat16, float16 or float32")
-    with _on(stream):
-        if out is None:
-            out = x.new_empty((M, N), dtype=out_dtype)
-            ldy = N
-        else:
-            if out.dtype != out_dtype:
-                _bad(f"out must be {out_dtype}")
-            ldy = _matrix(out, "out", (M, N), outputs, dev)[1]
-        pre = x.new_empty((M, rows), dtype=pre_dtype) if save_pre else None
-        d = LinearDesc(_DESC_BYTES, x.data_ptr(), weight.data_ptr(), bp, rp, out.data_ptr(),
-                       pre.data_ptr() if save_pre else 0, 0, 0, ldx, ldw, ldr, ldy, rows, M,
-                       N, K, int(gated), code, bt, rt, ot, pt, ACTIVATIONS[activation])
-        need = lib().hipgemm_linear_workspace_size(ctypes.byref(d))
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-            d.workspace, d.workspace_bytes = workspace.data_ptr(), need
-    with _device(dev, stream):
-        _check(lib().hipgemm_linear(ctypes.byref(d), _stream_handle(x, stream)),
-               "hipgemm_linear")
+    if stream is not None:
+        if stream.device != dev:
+            _bad(f"stream is on {stream.device}, x on {dev}")
+        with torch.cuda.stream(stream):
+            memory = _forward_memory(x, M, N, K, rows, out, out_dtype, pre_dtype, save_pre, rp,
+                                     gated)
+    else:
+        memory = _forward_memory(x, M, N, K, rows, out, out_dtype, pre_dtype, save_pre, rp, gated)
+    out, ldy, pre, workspace, need = memory
+    d = LinearDesc(_DESC_BYTES, x.data_ptr(), weight.data_ptr(), bp, rp, out.data_ptr(),
+                   0 if pre is None else pre.data_ptr(),
+                   workspace.data_ptr() if need else 0, need, ldx, ldw, ldr, ldy, rows, M, N, K,
+                   int(gated), code, bt, rt, ot, pt, ACTIVATIONS[activation])
+    _launch(lib().hipgemm_linear, "hipgemm_linear", d, x, stream)
     return (out, pre) if save_pre else out
+
+
+def _forward_memory(x, M, N, K, rows, out, out_dtype, pre_dtype, save_pre, residual, gated):
+    """(out, its row stride, pre, workspace, its bytes): what of them has to be allocated is the
+    current stream's."""
+    if out is None:
+        out, ldy = x.new_empty((M, N), dtype=out_dtype), N
+    else:
+        if out.dtype != out_dtype:
+            _bad(f"out must be {out_dtype}")
+        ldy = _matrix(out, "out", (M, N), _types()[2], x.device)[1]
+    pre = x.new_empty((M, rows), dtype=pre_dtype) if save_pre else None
+    need = _forward_bytes(M, N, K, 2 if gated else 1 if residual else 0, x.device.index)
+    workspace = x.new_empty(need, dtype=_torch().uint8) if need else None
+    return out, ldy, pre, workspace, need
 
 
 def _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias, grad_dtype,
@@ -202,6 +223,8 @@ def _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias, gr
             _bad("pre of the forward pass (save_pre) is needed")
         pt, ldp = _matrix(pre, "pre", (M, rows), inputs, dev)
         pp = pre.data_ptr()
+    if stream is not None and stream.device != dev:
+        _bad(f"stream is on {stream.device}, x on {dev}")
     grad_dtype = grad_dtype or x.dtype
     ot = outputs.get(grad_dtype)
     if ot is None:
@@ -218,9 +241,7 @@ def _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias, gr
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
             d.workspace, d.workspace_bytes = workspace.data_ptr(), need
-    with _device(dev, stream):
-        _check(lib().hipgemm_linear_backward(ctypes.byref(d), _stream_handle(x, stream)),
-               "hipgemm_linear_backward")
+    _launch(lib().hipgemm_linear_backward, "hipgemm_linear_backward", d, x, stream)
     return dx, dw, db
 
 

@@ -29,6 +29,21 @@
 // The sequence runs on across tiles: what lies past a tile's last step is the next
 // tile's first.  Steps of a tile are padded to at least S (padding reads zeros).
 //
+// 256 x 256 tiles have room for two stages only, and a step's DMA (16 KiB of each wave's,
+// 64 bytes a cycle) keep the memory path busy for half of its matrix instructions' time: all of
+// them issued in half 1 have half a step to land, which is too little where operands come from
+// memory (4096 x 4096 x 14336 341 us, with operands in the caches 314; by quarters 317, 315).
+// There a step runs as four quarters, 4 x 4
+// blocks by the whole step each, with one set of registers for each half of the rows (low,
+// high) of A and B, read anew as soon as its second use is over, and a fourth of the DMA:
+//   Q00: A low  x B low  | read B high of k     | DMA A low  of k + 2
+//   Q01: A low  x B high | read A high of k     | DMA B low  of k + 2
+//   Q10: A high x B low  | read A low  of k + 1 | DMA B high of k + 2
+//   Q11: A high x B high | read B low  of k + 1 | DMA A high of k + 2
+// Q00 and Q10 start with a barrier; what they and the quarter after read was fetched five or
+// six quarters before, and what is fetched over was read two quarters before, across a
+// barrier.  At each barrier the sixteen newest DMA may be in flight.
+//
 // K order inside a step: lane group g = lane / 16 takes the eight k from 16 g + 8 h in
 // half h, in both layouts: slots 2 g + h of a row (layout.hpp: no bank conflicts), or
 // the LDS rows 16 g + 8 h .. + 7 of an operand that lies across.  There the 16-byte
@@ -92,6 +107,10 @@ struct CfgDense {
   static constexpr int kAStage = kBM * kRow;
   static constexpr int kStage = (kBM + kBN) * kRow;
   static constexpr int kLdsBytes = S * kStage;
+  // The schedule by quarter steps (dense_tile_body), for tiles whose registers and LDS
+  // hold no more than a step and the next.
+  static constexpr bool kQuarters = BM == 256 && BN == 256;
+  static_assert(!kQuarters || S == 2, "two stages");
   static constexpr int kDmaA = BM / 32, kDmaB = BN / 32;  // per wave and step
   static constexpr int kDma = kDmaA + kDmaB;
   static_assert(kLdsBytes <= 160 * 1024, "LDS");
@@ -291,6 +310,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   // keep the matrix unit busy while the waves meet.
   constexpr int kTail = kMfma >= 16 ? 2 : 0, kHead = kMfma - kTail;
   constexpr int kSpan = kMfma * 48 / 64;
+  constexpr bool kQ = Cfg::kQuarters;
   constexpr int kWNr = kGated ? Cfg::kWN / 2 : Cfg::kWN;  // result columns of a wave
   constexpr int kBNr = 2 * kWNr;
   static_assert((S - 2) * kDma < 64, "vmcnt range");
@@ -316,6 +336,10 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   const int dchunk = (lane & 7) ^ slot_xor(8 * (wave & 1) + drow);
   auto lane_off = [&](bool col, int width, long long ld, int q) -> uint32_t {
     if (!col) return (uint32_t)((4 * q + wave) * 8 + drow) * (uint32_t)ld + dchunk * 16;
+    if constexpr (kQ) {  // two halves of the columns, below
+      const int k = (4 * (q % 4) + wave) * 4 + lane / 16, c = (lane % 16) ^ col_xor(k);
+      return (uint32_t)k * (uint32_t)ld + (c % 8 + 16 * (c / 8) + 8 * (q / 4)) * 16;
+    }
     const int slots = width / 8, k = (4 * q + wave) * (64 / slots) + lane / slots;
     return (uint32_t)k * (uint32_t)ld + (((lane % slots) ^ col_xor(k)) * 16);
   };
@@ -337,10 +361,28 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   }
 
   // (Kept in registers: otherwise computed anew in every step.)
+  auto keep = [&]() {
 #pragma unroll
-  for (int q = 0; q < Cfg::kDmaA; ++q) asm volatile("" : "+v"(voff_a[q]));
+    for (int q = 0; q < Cfg::kDmaA; ++q) asm volatile("" : "+v"(voff_a[q]));
 #pragma unroll
-  for (int q = 0; q < Cfg::kDmaB; ++q) asm volatile("" : "+v"(voff_b[q]));
+    for (int q = 0; q < Cfg::kDmaB; ++q) asm volatile("" : "+v"(voff_b[q]));
+  };
+  keep();
+  // The same for a step that is not whole: offsets of lanes past the sum's end lie outside.
+  // They change only where such a step comes or goes (2 % at 4096 x 4096 x 14336 against
+  // a mask for every DMA).
+  bool masked = false;
+  auto mask = [&](uint32_t oob) {
+    if constexpr (!kACol) {
+#pragma unroll
+      for (int q = 0; q < Cfg::kDmaA; ++q) voff_a[q] = (voff_a[q] & ~kOobOffset) | oob;
+    }
+    if constexpr (!kBCol) {
+#pragma unroll
+      for (int q = 0; q < Cfg::kDmaB; ++q) voff_b[q] = (voff_b[q] & ~kOobOffset) | oob;
+    }
+    keep();
+  };
 
   // A unit's operands: along K the rows' resource; across, the columns' address, from
   // which each step's resource is made (rows past the sum's end read zero).
@@ -395,7 +437,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
 
   struct Step {
     __amdgpu_buffer_rsrc_t a, b, b2;
-    uint32_t soff, oob;
+    uint32_t soff;
   };
   // Step d of the unit, or past its end step d - steps_pad of the next.
   auto step_src = [&](int d) {
@@ -409,8 +451,12 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     uint32_t soff = (uint32_t)k * 2u;
     asm volatile("" : "+s"(soff));
     s.soff = soff;
-    s.oob = 0;
-    if constexpr (!kACol || !kBCol) s.oob = k + dchunk * 8 < kend ? 0u : kOobOffset;
+    if constexpr (!kACol || !kBCol) {
+      if (at >= full || masked) {
+        mask(k + dchunk * 8 < kend ? 0u : kOobOffset);
+        masked = at >= full;
+      }
+    }
     auto across = [&](const uint8_t* p, long long ld, uint32_t cols) {
       const int rows = min(kBK, kend - k);
       return make_rsrc(p + (long long)k * ld,
@@ -430,11 +476,10 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     lds_u8* to = lds + dst + (is_a ? 0 : Cfg::kAStage) + (4 * q + wave) * 1024;
     const uint32_t vo = is_a ? voff_a[q] : voff_b[q];
     const bool col = is_a ? kACol : kBCol;
-    const uint32_t v = col ? vo : vo | s.oob;
     const uint32_t so = col ? 0u : s.soff;
-    if (is_a) dma16(s.a, to, v, so);
-    else if (kOnce) dma16_nt(is_up(q) ? s.b2 : s.b, to, v, so);
-    else dma16(is_up(q) ? s.b2 : s.b, to, v, so);
+    if (is_a) dma16(s.a, to, vo, so);
+    else if (kOnce) dma16_nt(is_up(q) ? s.b2 : s.b, to, vo, so);
+    else dma16(is_up(q) ? s.b2 : s.b, to, vo, so);
   };
 
   // ---- fragments ---------------------------------------------------------------
@@ -449,35 +494,40 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   const int krow = 16 * grp + (r16 >> 2);
   const int kx = col_xor(krow);
   const uint32_t sub = (uint32_t)((((r16 & 3) >> 1) * 16) + (r16 & 1) * 8);
-  uint32_t col_a[FA], col_b[FB];
+  // (By quarters: LDS rows of 128 columns, those of one half of both waves'.)
+  constexpr int kParts = kQ ? 2 : 1, kCA = FA / kParts, kCB = FB / kParts;
+  constexpr int kWideA = 2 * Cfg::kBM / kParts, kWideB = 2 * Cfg::kBN / kParts;
+  uint32_t col_a[kCA], col_b[kCB];
 #pragma unroll
-  for (int f = 0; f < FA; ++f)
-    col_a[f] = (uint32_t)(krow * 2 * Cfg::kBM) + sub + (uint32_t)(((2 * (wm * FA + f)) ^ kx) * 16);
+  for (int f = 0; f < kCA; ++f)
+    col_a[f] = (uint32_t)(krow * kWideA) + sub + (uint32_t)(((2 * (wm * kCA + f)) ^ kx) * 16);
 #pragma unroll
-  for (int f = 0; f < FB; ++f)
-    col_b[f] = (uint32_t)(Cfg::kAStage + krow * 2 * Cfg::kBN) + sub +
-               (uint32_t)(((2 * (wn * FB + f)) ^ kx) * 16);
+  for (int f = 0; f < kCB; ++f)
+    col_b[f] = (uint32_t)(Cfg::kAStage + krow * kWideB) + sub +
+               (uint32_t)(((2 * (wn * kCB + f)) ^ kx) * 16);
 
   s16x4 fa[2][FA][2], fb[2][FB][2];
-  // Read n of half h of the step in the stage at `st`, in the order in which the MFMA
-  // need them: A 0, every B, the other A.
-  auto read_one = [&](int st, int h, int n) {
-    constexpr int kFirst = kReadA, kMid = kReadA + kReadB * FB;
-    const bool is_b = n >= kFirst && n < kMid;
-    const int m = is_b ? n - kFirst : n < kFirst ? n : n - kReadB * FB;
-    const int per = is_b ? kReadB : kReadA;
-    const int f = m / per, p = m % per;
+  // Fragment f of an operand, half h of the step in the stage at `st`, part p of it.
+  auto read = [&](bool is_b, int st, int h, int f, int p) {
     s16x4(&to)[2] = is_b ? fb[h][f] : fa[h][f];
     if (is_b ? kBCol : kACol) {
-      const int width = is_b ? 2 * Cfg::kBN : 2 * Cfg::kBM;
-      const lds_u8* from = lds + st + (is_b ? col_b[f] : col_a[f]) + (8 * h + 4 * p) * width;
-      to[p] = lds_read_across(from);
+      const int width = is_b ? kWideB : kWideA, c = f % (is_b ? kCB : kCA);
+      const int part = f / (is_b ? kCB : kCA) * kBK * width;
+      to[p] = lds_read_across(lds + st + (is_b ? col_b[c] : col_a[c]) + part + (8 * h + 4 * p) * width);
     } else {
       const lds_u8* from = lds + st + (is_b ? row_b : row_a) + slot[h] + f * 16 * Cfg::kRow;
       const s16x8 v = __builtin_bit_cast(s16x8, lds_read16(from));
       to[0] = __builtin_shufflevector(v, v, 0, 1, 2, 3);
       to[1] = __builtin_shufflevector(v, v, 4, 5, 6, 7);
     }
+  };
+  // Read n of half h, in the order in which the MFMA need them: A 0, every B, the other A.
+  auto read_one = [&](int st, int h, int n) {
+    constexpr int kFirst = kReadA, kMid = kReadA + kReadB * FB;
+    const bool is_b = n >= kFirst && n < kMid;
+    const int m = is_b ? n - kFirst : n < kFirst ? n : n - kReadB * FB;
+    const int per = is_b ? kReadB : kReadA;
+    read(is_b, st, h, m / per, m % per);
   };
   auto frag = [](const s16x4 (&p)[2]) {
     return __builtin_bit_cast(i32x4, __builtin_shufflevector(p[0], p[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -524,7 +574,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   bool stored = false;  // the previous tile was whole: all its stores were issued
   constexpr int kStores = FA * FB / (kGated ? 4 : 2);  // at least
   static_assert((S - 2) * kDma + kStores < 64, "vmcnt range");
-  auto step = [&](int k) {
+  auto step_halves = [&](int k) {
     const int rst = next_stage(st);
     half0(st);
     // Step k + 1 has landed: newer are the DMA of S - 2 steps, and in a tile's first S - 1
@@ -537,16 +587,100 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     st = rst;
   };
 
+  // ---- by quarters -------------------------------------------------------------
+  constexpr int kQMfma = 32, kQTail = 2;
+  static_assert(!kQ || (FA == 8 && FB == 8 && kDma == 16), "quarters of 4 x 4 blocks");
+  auto mfma_q = [&](int qi, int qj, int n) {
+    const int h = n / 16, i = n % 16 / 4, j = i % 2 ? 3 - n % 4 : n % 4;
+    mfma_acc<kX>(frag(fb[h][4 * qj + j]), frag(fa[h][4 * qi + i]), acc[4 * qi + i][4 * qj + j]);
+  };
+  // Reads go with the first half of a quarter's matrix instructions, DMA with the second.
+  // Blocks (qi, qj); reads of part rhi of operand rb (0: A, 1: B) from the stage at rst;
+  // DMA of part dhi of operand db into the stage at dst.
+  auto quarter = [&](int qi, int qj, auto rb, int rhi, int rst, auto db, int dhi, int dst,
+                     const Step& src) {
+    constexpr bool kRB = decltype(rb)::value, kDB = decltype(db)::value;
+    constexpr int per = kRB ? kReadB : kReadA, reads = 8 * per;
+    static_for<kQMfma - kQTail>([&](auto n) {
+      mfma_q(qi, qj, n);
+      static_for<due(n + 1, 16, reads) - due(n, 16, reads)>([&](auto r) {
+        constexpr int x = due(n, 16, reads) + r;
+        read(kRB, rst, x / per / 4, 4 * rhi + x / per % 4, x % per);
+      });
+      static_for<due(n - 15, 16, 4) - due(n - 16, 16, 4)>([&](auto d) {
+        constexpr int x = due(n - 16, 16, 4) + d;
+        const int q = (kDB ? kBCol : kACol) ? 4 * dhi + x : x % 2 + 4 * (x / 2) + 2 * dhi;
+        dma_one(src, dst, kDB ? Cfg::kDmaA + q : q);
+      });
+      sched_fence();
+    });
+  };
+  auto tail_q = [&](int qi, int qj) {
+    static_for<kQTail>([&](auto n) { mfma_q(qi, qj, kQMfma - kQTail + n); });
+    sched_fence();
+  };
+  auto step_quarters = [&](int k) {
+    const std::false_type A{};
+    const std::true_type B{};
+    const int nst = next_stage(st);
+    wait_lgkmcnt<0>();
+    if (stored && k < 2) wait_vmcnt<16 + kStores>();
+    else wait_vmcnt<16>();
+    barrier();
+    const Step src = step_src(k + 2);
+    if (k > 0) tail_q(1, 1);
+    quarter(0, 0, B, 1, st, A, 0, st, src);
+    wait_lgkmcnt<0>();
+    tail_q(0, 0);
+    quarter(0, 1, A, 1, st, B, 0, st, src);
+    wait_lgkmcnt<0>();
+    if (stored && k == 0) wait_vmcnt<16 + kStores>();
+    else wait_vmcnt<16>();
+    barrier();
+    tail_q(0, 1);
+    quarter(1, 0, A, 0, nst, B, 1, st, src);
+    wait_lgkmcnt<0>();
+    tail_q(1, 0);
+    quarter(1, 1, B, 0, nst, A, 1, st, src);
+    st = nst;
+  };
+
+  if constexpr (kQ) {
+    // In the order of the loop: A low, B low, B high, A high.
 #pragma unroll
-  for (int d = 0; d < S; ++d) {
-    const Step src = step_src(d);
+    for (int d = 0; d < 2; ++d) {
+      const Step src = step_src(d);
 #pragma unroll
-    for (int n = 0; n < kDma; ++n) dma_one(src, d * Cfg::kStage, n);
+      for (int n = 0; n < 16; ++n) {
+        const bool is_b = n >= 4 && n < 12;
+        const int hi = n >= 8, x = n % 4;
+        const int q = (is_b ? kBCol : kACol) ? 4 * hi + x : x % 2 + 4 * (x / 2) + 2 * hi;
+        dma_one(src, d * Cfg::kStage, is_b ? Cfg::kDmaA + q : q);
+      }
+    }
+    wait_vmcnt<16>();
+    barrier();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+#pragma unroll
+        for (int p = 0; p < kReadA; ++p) read(false, 0, h, f, p);
+#pragma unroll
+        for (int p = 0; p < kReadB; ++p) read(true, 0, h, f, p);
+      }
+  } else {
+#pragma unroll
+    for (int d = 0; d < S; ++d) {
+      const Step src = step_src(d);
+#pragma unroll
+      for (int n = 0; n < kDma; ++n) dma_one(src, d * Cfg::kStage, n);
+    }
+    wait_vmcnt<(S - 1) * kDma>();
+    barrier();
+#pragma unroll
+    for (int n = 0; n < kReads; ++n) read_one(0, 0, n);
   }
-  wait_vmcnt<(S - 1) * kDma>();
-  barrier();
-#pragma unroll
-  for (int n = 0; n < kReads; ++n) read_one(0, 0, n);
 
   for (;;) {
 #pragma unroll
@@ -558,7 +692,12 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
       }
     // Two wait states from the last zero's write to the first matrix instruction.
     asm volatile("s_nop 3");
-    for (int k = 0; k < steps_pad; ++k) step(k);
+    if constexpr (kQ) {
+      for (int k = 0; k < steps_pad; ++k) step_quarters(k);
+      tail_q(1, 1);
+    } else {
+      for (int k = 0; k < steps_pad; ++k) step_halves(k);
+    }
 
     // ---- epilogue --------------------------------------------------------------
     mfma_drain();
@@ -749,6 +888,7 @@ __device__ __forceinline__ float slope(float z, int act) {
   return z != z ? z : s * __builtin_fmaf(d, 1.0f - s, 1.0f);
 }
 
+constexpr int kSlopeColumns = 256;  // of a workgroup
 struct SlopeArgs {
   const uint8_t *dy, *pre;
   uint8_t* dz;     // or null
@@ -767,75 +907,98 @@ template <int kX, bool kGated>
 __device__ __forceinline__ void dense_slope_body(const SlopeArgs& g, float* sums) {
   constexpr int kParts = kGated ? 2 : 1;
   constexpr int kOut = kX == kInBf16 ? kOutBf16 : kOutF16;
-  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-  const int col = 8 * (32 * blockIdx.x + tx);
+  constexpr int kTx = kSlopeColumns / 8, kTy = 256 / kTx;
+  const int tx = threadIdx.x % kTx, ty = threadIdx.x / kTx;
+  const int col = 8 * (kTx * blockIdx.x + tx);
   const long long first = (long long)blockIdx.y * g.rows;
   const long long end = min((long long)g.M, first + g.rows);
   const bool live = col < g.N;
   const bool whole = col + 8 <= g.N;
   float sum[kParts][8] = {};
-  if (live)
-    for (long long row = first + ty; row < end; row += 8) {
-      float dy[8] = {}, z[8] = {}, u[8] = {};
-      if (whole) {
-        load8(g.dy, row * g.lddy + col, g.dy_type, dy);
-        if (g.pre) load8(g.pre, row * g.ldp + col, g.p_type, z);
-        if constexpr (kGated) load8(g.pre, row * g.ldp + g.N + col, g.p_type, u);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (col + e < g.N) {
-            dy[e] = load1(g.dy, row * g.lddy + col + e, g.dy_type);
-            if (g.pre) z[e] = load1(g.pre, row * g.ldp + col + e, g.p_type);
-            if constexpr (kGated) u[e] = load1(g.pre, row * g.ldp + g.N + col + e, g.p_type);
-          }
-      }
-      float d[8];
-      if constexpr (kGated) {
-        float a[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          d[e] = dy[e] * u[e] * slope(z[e], g.act);
-          a[e] = z[e];
-        }
-        activate8(a, g.act);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          a[e] *= dy[e];
-          sum[kParts - 1][e] += a[e];
-        }
-        if (g.dz) store8(g.dz, row * g.lddz + g.N + col, kOut, a);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = dy[e] * slope(z[e], g.act);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum[0][e] += d[e];
-      if (g.dz) store8(g.dz, row * g.lddz + col, kOut, d);
+  struct Row {
+    Raw8 dy, z, u;
+  };
+  auto fetch = [&](long long row) {
+    Row r{};
+    if (whole) {
+      r.dy = raw8(g.dy, row * g.lddy + col, g.dy_type);
+      if (g.pre) r.z = raw8(g.pre, row * g.ldp + col, g.p_type);
+      if constexpr (kGated) r.u = raw8(g.pre, row * g.ldp + g.N + col, g.p_type);
     }
+    return r;
+  };
+  auto finish = [&](long long row, const Row& r) {
+    float dy[8] = {}, z[8] = {}, u[8] = {};
+    if (whole) {
+      widen8(r.dy, g.dy_type, dy);
+      if (g.pre) widen8(r.z, g.p_type, z);
+      if constexpr (kGated) widen8(r.u, g.p_type, u);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < g.N) {
+          dy[e] = load1(g.dy, row * g.lddy + col + e, g.dy_type);
+          if (g.pre) z[e] = load1(g.pre, row * g.ldp + col + e, g.p_type);
+          if constexpr (kGated) u[e] = load1(g.pre, row * g.ldp + g.N + col + e, g.p_type);
+        }
+    }
+    float d[8];
+    if constexpr (kGated) {
+      float a[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        d[e] = dy[e] * u[e] * slope(z[e], g.act);
+        a[e] = z[e];
+      }
+      activate8(a, g.act);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        a[e] *= dy[e];
+        sum[kParts - 1][e] += a[e];
+      }
+      if (g.dz) store8(g.dz, row * g.lddz + g.N + col, kOut, a);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[e] = dy[e] * slope(z[e], g.act);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[0][e] += d[e];
+    if (g.dz) store8(g.dz, row * g.lddz + col, kOut, d);
+  };
+  if (live)
+    for (long long row = first + ty; row < end; row += kTy) finish(row, fetch(row));
   if (!g.columns) return;
-  // The block's eight sums of each column, in order.
+  // The block's sums of each column, in order.
 #pragma unroll
   for (int p = 0; p < kParts; ++p) {
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[ty * 256 + 8 * tx + e] = sum[p][e];
+    for (int e = 0; e < 8; ++e) sums[ty * kSlopeColumns + 8 * tx + e] = sum[p][e];
     __syncthreads();
-    const int c = 256 * blockIdx.x + threadIdx.x;
-    float s = 0.0f;
+    for (int x = threadIdx.x; x < kSlopeColumns; x += 256) {
+      const int c = kSlopeColumns * blockIdx.x + x;
+      float s = 0.0f;
 #pragma unroll
-    for (int y = 0; y < 8; ++y) s += sums[y * 256 + threadIdx.x];
-    if (c < g.N) g.columns[((long long)blockIdx.y * kParts + p) * g.N + c] = s;
+      for (int y = 0; y < kTy; ++y) s += sums[y * kSlopeColumns + x];
+      if (c < g.N) g.columns[((long long)blockIdx.y * kParts + p) * g.N + c] = s;
+    }
   }
 }
 
-// out[c] = sum over blocks of columns[b][c], in order.
+// out[c] = sum over blocks of columns[b][c]: sixteen columns of a workgroup, a sixteenth of
+// the blocks each thread, whose sums are added in order.
 __device__ __forceinline__ void dense_columns_body(const float* columns, int blocks, int N,
-                                                   uint8_t* out, int type) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= N) return;
+                                                   uint8_t* out, int type, float* sums) {
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, c = 16 * blockIdx.x + tx;
   float s = 0.0f;
-  for (int b = 0; b < blocks; ++b) s += columns[(long long)b * N + c];
+  if (c < N)
+#pragma unroll 4
+    for (int b = ty; b < blocks; b += 16) s += columns[(long long)b * N + c];
+  sums[threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.x >= 16 || c >= N) return;
+#pragma unroll
+  for (int y = 1; y < 16; ++y) s += sums[16 * y + tx];
   store1(out, c, type, s);
 }
 
