@@ -206,7 +206,7 @@ def _forward_memory(x, M, N, K, rows, out, out_dtype, pre_dtype, save_pre, resid
 
 
 def _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias, grad_dtype,
-              gated, stream):
+              bias_dtype, gated, stream):
     torch = _torch()
     _, inputs, outputs = _types()
     code, M, N, K = _sizes(x, weight, gated)
@@ -229,14 +229,18 @@ def _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias, gr
     ot = outputs.get(grad_dtype)
     if ot is None:
         _bad("grad_dtype must be bfloat16, float16 or float32")
+    bias_dtype = bias_dtype or grad_dtype
+    bt = outputs.get(bias_dtype)
+    if bt is None:
+        _bad("bias_dtype must be bfloat16, float16 or float32")
     with _on(stream):
         dx = x.new_empty((M, K)) if need_x else None
         dw = x.new_empty((rows, K), dtype=grad_dtype) if need_weight else None
-        db = x.new_empty(rows, dtype=grad_dtype) if need_bias else None
+        db = x.new_empty(rows, dtype=bias_dtype) if need_bias else None
         dp, wp, bp = (0 if t is None else t.data_ptr() for t in (dx, dw, db))
         d = LinearGradDesc(_GRAD_BYTES, dy.data_ptr(), x.data_ptr(), weight.data_ptr(), pp, dp,
                            wp, bp, 0, 0, lddy, ldx, ldw, ldp, K, K, M, N, K, int(gated), code,
-                           dyt, pt, outputs[x.dtype], ot, ot, ACTIVATIONS[activation])
+                           dyt, pt, outputs[x.dtype], ot, bt, ACTIVATIONS[activation])
         need = lib().hipgemm_linear_backward_workspace_size(ctypes.byref(d))
         if need:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
@@ -272,22 +276,22 @@ def gated_linear(x, weight, *, bias=None, activation="silu", out_dtype=None, out
 
 def linear_backward(dy, x, weight, pre=None, *, activation=None, need_x: bool = True,
                     need_weight: bool = True, need_bias: bool = False, grad_dtype=None,
-                    stream=None):
+                    bias_dtype=None, stream=None):
     """(dx, dweight, dbias) of linear, None where not needed: dz = dy * act'(z), dx = dz @
     weight, dweight = dz.T @ x, dbias = dz.sum(0).  (The residual's gradient is dy.)
 
     dy (M, N): bfloat16, float16 or float32.  pre: linear's z (save_pre); not needed without
-    an activation.  dx has x's type, dweight and dbias grad_dtype (bfloat16, float16 or
-    float32; x's type where None).  dz is rounded to x's type for the two products; sums are
+    an activation.  dx has x's type, dweight grad_dtype (bfloat16, float16 or float32; x's
+    type where None) and dbias bias_dtype (grad_dtype where None).  dz is rounded to x's type for the two products; sums are
     fp32."""
     return _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias,
-                     grad_dtype, False, stream)
+                     grad_dtype, bias_dtype, False, stream)
 
 
 def gated_linear_backward(dy, x, weight, pre, *, activation="silu", need_x: bool = True,
                           need_weight: bool = True, need_bias: bool = False,
-                          grad_dtype=None, stream=None):
+                          grad_dtype=None, bias_dtype=None, stream=None):
     """(dx, dweight, dbias) of gated_linear, None where not needed; as linear_backward, with
     [dg | du] = [dy * u * act'(g) | dy * act(g)] for dz, z = [g | u]."""
     return _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias,
-                     grad_dtype, True, stream)
+                     grad_dtype, bias_dtype, True, stream)
