@@ -53,6 +53,7 @@ __global__ __launch_bounds__(256) void k_dense_columns(const float* columns, int
   dense_columns_body(columns, blocks, N, out, type, sums);
 }
 
+int in_bytes(int type) { return type == kInF32 ? 4 : 2; }
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 // 256 rows of an operand, and of a result, are addressed with 31 bits.
@@ -74,17 +75,19 @@ struct Plan {
   int tile;  // index of kDenseTiles, or -1: a few rows
   int slices, slice_steps;
   long long units;
+  double us;
+  int first;  // columns that 256 x 256 tiles do ahead of this plan, which is for the rest
 };
 
 // Estimated times, us.  A tile's step of 64 along K by how the operands lie, and its end,
 // with every CU at work on operands that come from memory: 128 x 128, 256 x 256, 64 x 128,
-// 256 x 128.  Measured against every tile and 1, 2, 4, 8 slices on 190 shapes, the choice is
-// within 5 % of the best at the median (us, chosen / best):
-//   forward   64 x 4096 x 4096 14.6/14.6 (rows; tiles 16.5), 96 x 4096 x 14336 34.0/34.0 (128 x 128
-//             in 8 slices; 64 x 128 37.4), 512 x 14336 x 4096 65/64 (256 x 128; 128 x 128 83),
-//             1024 x 4096 x 4096 39.7/39.7 (128 x 128; 256 x 128 54.9)
-//   of x      777 x 14336 x 4096 108/106 (256 x 128 in 2 slices; 128 x 128 128)
-//   of w      4096 x 14336 x 4096 391/391 (256 x 256; 256 x 128 432)
+// 256 x 128.  Against every tile and 1, 2, 4, 8 slices on 148 shapes the choice is within 1 % of
+// the best at the median, 3 % in the mean (us, chosen / another):
+//   forward   64 x 4096 x 4096 15 (rows) / 32 (64 x 128), 64 x 14336 x 4096 29 (64 x 128 in 2 slices)
+//             / 46 (rows), 128 x 4096 x 14336 39 (128 x 128 in 8 slices) / 48 (in 4), 512 x 14336 x
+//             4096 65 (256 x 128) / 83 (128 x 128), 1024 x 4096 x 4096 40 (128 x 128) / 55 (256 x 128)
+//   of x      777 x 14336 x 4096 108 (256 x 128 in 2 slices) / 128 (128 x 128)
+//   of w      4096 x 14336 x 4096 391 (256 x 256) / 432 (256 x 128)
 struct TileTime {
   double forward, of_x, of_w, end;
 };
@@ -93,46 +96,44 @@ constexpr TileTime kTime[hk::kNumDenseTiles] = {{0.57, 0.55, 0.58, 1.5},
                                                 {0.40, 0.42, 0.0, 1.0},
                                                 {0.85, 0.85, 0.96, 3.0}};
 constexpr double kLaunch = 4.0, kSplitLaunch = 3.5;
-constexpr double kBytesPerUs = 5.0e6;      // from memory
-constexpr double kCuBytesPerUs = 75.0e3;   // into one CU
+constexpr double kBytesPerUs = 5.0e6;          // from memory: a few rows
+constexpr double kSumBytesPerUs = 9.0e6;       // sums of K-slices, both ways
+constexpr double kTileBytesPerUs = 5.7e6;      // the operands of tiles
+constexpr double kCuMemoryBytesPerUs = 28.0e3;  // from memory, into one CU among few at work
+constexpr double kCuBytesPerUs = 75.0e3;       // into one CU, the most of it from a cache
 constexpr int kCus = 256;
 
 double split_us(int slices, int M, int N, bool gated) {
   if (slices == 1) return 0.0;
-  return kSplitLaunch + 8.0 * slices * M * (double)N * (gated ? 2 : 1) / kBytesPerUs;
+  return kSplitLaunch + 0.3 * slices + 8.0 * slices * M * (double)N * (gated ? 2 : 1) / kSumBytesPerUs;
 }
 
 // A few rows: what a CU has to fetch (x again for every 16 rows of weights), or the weights
-// from memory, and more of both with more rows.
+// from memory, and more of both with more rows (gated 14336 x 4096, one row 37 us, 16 rows 51,
+// 32 rows 61, 64 rows 80; tiles of 64 x 128 take 41 to 47).
 double rows_us(int M, int N, int K, bool gated, int slices) {
   const int mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
   const double rows = N * (gated ? 2.0 : 1.0);
   const long long groups = (long long)((rows + 15) / 16) * slices;
   const double cu = (double)((groups + kCus - 1) / kCus) * 32.0 * (1 + mt) * K / slices;
   const double us = cu / kCuBytesPerUs, memory = 2.0 * rows * K / kBytesPerUs;
-  return kLaunch + (us > memory ? us : memory) * (0.9 + 0.1 * mt) + split_us(slices, M, N, gated);
+  const double more = M <= 16 ? 0.7 + 0.3 / 16 * M : 0.9 + 0.1 * mt;
+  return kLaunch + (us > memory ? us : memory) * more + split_us(slices, M, N, gated);
 }
 
 // The fewest estimated us: rounds of tiles over the CUs, no less than the operands' bytes
 // take, and for K-slices the way of their sums through memory.
-Plan plan_of(int kind, int M, int N, int K) {
+Plan plan_whole(int kind, int M, int N, int K) {
   const int steps = (int)(((long long)K + 63) / 64);
   const bool gated = kind == hk::kDenseGated;
   const bool forward = gated || kind == hk::kDenseNT || kind == hk::kDenseRes;
-  Plan best{0, 1, steps, 0};
-  double least = 1e300;
+  Plan best{0, 1, steps, 0, 1e300, 0};
   if (forward && M <= 64)
     for (int slices = 1; slices <= 4 && steps >= 16 * (slices - 1); slices *= 2) {
       const double us = rows_us(M, N, K, gated, slices);
-      if (us < least) {
-        least = us;
-        best = {-1, slices, (steps + slices - 1) / slices, 0};
-      }
+      if (us < best.us) best = {-1, slices, (steps + slices - 1) / slices, 0, us, 0};
     }
-  // (Nothing beats it: it is a pass over the weights.)
-  if (forward && M <= 16) return best;
-  const double memory =
-      2.0 * ((double)M + N * (gated ? 2.0 : 1.0)) * K / kBytesPerUs;
+  const double bytes = 2.0 * ((double)M + N * (gated ? 2.0 : 1.0)) * K;
   for (int t = 0; t < hk::kNumDenseTiles; ++t) {
     if (kind == hk::kDenseTN && t == 2) continue;
     const hk::TileShape s = hk::kDenseTiles[t];
@@ -146,14 +147,48 @@ Plan plan_of(int kind, int M, int N, int K) {
       if (slices > 1 && (tiles * slices > 2 * kCus || steps < 4 * slices)) break;
       const int each = (steps + slices - 1) / slices;
       const long long units = tiles * slices;
-      const double work = (double)((units + kCus - 1) / kCus) * (each * step + kTime[t].end);
+      // Where CUs stay without a tile the clock rises (1531 x 4096 x 14336, 256 x 256 in 2 slices
+      // on 192 CUs: 163 us; 256 x 128 191).
+      const double clock = t == 1 && units <= kCus * 3 / 4 ? 0.85 : 1.0;
+      const double work =
+          (double)((units + kCus - 1) / kCus) * (each * step * clock + kTime[t].end);
+      const double pull = (double)(units < kCus ? units : kCus) * kCuMemoryBytesPerUs;
+      const double memory = bytes / (pull < kTileBytesPerUs ? pull : kTileBytesPerUs);
       const double us =
           kLaunch + (work > memory ? work : memory) + split_us(slices, M, N, gated);
-      if (us < least) {
-        least = us;
-        best = {t, slices, each, units};
-      }
+      if (us < best.us) best = {t, slices, each, units, us, 0};
     }
+  }
+  return best;
+}
+
+// Where 256 x 256 tiles leave a last round that is not full, their whole rounds' columns by
+// them and the rest as it goes best by itself, in a second launch (us, whole / in two: 6000 x 3000 x
+// 8192 308/261, 1531 x 14336 x 4096 172/165).  Only for a fifth at least: CUs without a tile leave
+// the others their power (2500 x 16384 x 4096, 2.5 rounds, 307/330; gated 2048 x 14336 x 4096, 3.5
+// rounds, 427/425 to 490).
+constexpr double kGain = 1.2;
+Plan plan_of(int kind, int M, int N, int K) {
+  Plan best = plan_whole(kind, M, N, K);
+  constexpr int kBig = 1;
+  const hk::TileShape s = hk::kDenseTiles[kBig];
+  const int cols = kind == hk::kDenseGated ? s.bn / 2 : s.bn;
+  const long long down = ((long long)M + s.bm - 1) / s.bm;
+  const long long across = ((long long)N + cols - 1) / cols;
+  if (best.tile < 0 || down * across <= kCus) return best;
+  const double step = kind == hk::kDenseNN   ? kTime[kBig].of_x
+                      : kind == hk::kDenseTN ? kTime[kBig].of_w
+                                             : kTime[kBig].forward;
+  const double round = ((K + 63ll) / 64) * step + kTime[kBig].end;
+  const long long rounds = down * across / kCus;
+  const long long first = rounds * kCus / down;  // columns of tiles
+  if (first < 1 || first >= across) return best;
+  const Plan rest = plan_whole(kind, M, (int)(N - first * cols), K);
+  const double us = rest.us + (double)((down * first + kCus - 1) / kCus) * round;
+  if (us * kGain < best.us) {
+    best = rest;
+    best.us = us;
+    best.first = (int)(first * cols);
   }
   return best;
 }
@@ -165,12 +200,34 @@ long long partial_columns(int kind, int N) {
 }
 size_t partial_bytes(int kind, const Plan& p, int M, int N) {
   if (p.slices == 1) return 0;
-  return padded(4ull * (size_t)p.slices * (size_t)M * (size_t)partial_columns(kind, N));
+  return padded(4ull * (size_t)p.slices * (size_t)M * (size_t)partial_columns(kind, N - p.first));
 }
+
+hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream);
 
 // g: operands, sizes and epilogue; ws: partial_bytes.
 hipError_t product(int x, int kind, DenseArgs& g, void* ws, hipStream_t stream) {
   const Plan p = plan_of(kind, g.M, g.N, g.K);
+  if (!p.first) return run(x, kind, p, g, ws, stream);
+  DenseArgs part = g;
+  part.N = p.first;
+  const int cols = kind == hk::kDenseGated ? 128 : 256;
+  const hipError_t e = run(
+      x, kind,
+      Plan{1, 1, 0, ((g.M + 255ll) / 256) * (p.first / cols), 0.0, 0}, part, nullptr, stream);
+  if (e != hipSuccess) return e;
+  const bool across = kind == hk::kDenseNN || kind == hk::kDenseTN;
+  g.b += across ? 2ll * p.first : p.first * g.ldb;
+  DenseEpi& o = g.epi;
+  o.y += (long long)p.first * out_bytes(o.y_type);
+  if (o.r) o.r += (long long)p.first * in_bytes(o.r_type);
+  if (o.pre) o.pre += (long long)p.first * out_bytes(o.p_type);
+  if (o.bias) o.bias += (long long)p.first * in_bytes(o.b_type);
+  g.N -= p.first;
+  return run(x, kind, p, g, ws, stream);
+}
+
+hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream) {
   g.slices = p.slices;
   g.slice_steps = p.slice_steps;
   g.partial = static_cast<float*>(ws);
@@ -203,7 +260,6 @@ bool operand(const void* p, long long ld, long long columns) {
 bool result(const void* p, long long ld, long long columns, int out) {
   return p && aligned(p, (uintptr_t)out_bytes(out)) && ld >= columns && ld <= kMaxLd;
 }
-int in_bytes(int type) { return type == kInF32 ? 4 : 2; }
 
 bool common(int M, int N, int K, int gated, int type, int act) {
   return M >= 0 && M <= kMaxRows && N >= 0 && K >= 0 && K % 8 == 0 && (gated == 0 || gated == 1) &&

@@ -78,11 +78,11 @@ constexpr int kEpiGated = 3;     // bias, pre, activation, product
 // What becomes of the sums (types: kOut*, kIn*; strides in elements).
 struct DenseEpi {
   uint8_t* y;
-  const uint8_t* bias;  // or null; gated: N gate values, then N up values
+  const uint8_t* bias;  // or null
   const uint8_t* r;     // residual or null
   uint8_t* pre;         // sums with bias, or null
   long long ldy, ldr, ldp;
-  long long up;         // gated: columns from a gate sum to its up sum, in pre
+  long long up;         // gated: columns from a gate sum to its up sum, in pre and bias
   int act, y_type, p_type, b_type, r_type;
 };
 
@@ -241,11 +241,11 @@ __device__ __forceinline__ void finish8(const DenseEpi& e, const DenseAt& at, in
 // One column; v, u without the bias.
 template <int kEpi>
 __device__ __forceinline__ void finish1(const DenseEpi& e, const DenseAt& at, int c, int col,
-                                        int N, float v, float u) {
+                                        float v, float u) {
   if constexpr (kEpi != kEpiPlain) {
     if (e.bias) {
       v += load1(e.bias, col, e.b_type);
-      if constexpr (kEpi == kEpiGated) u += load1(e.bias, (long long)N + col, e.b_type);
+      if constexpr (kEpi == kEpiGated) u += load1(e.bias, e.up + col, e.b_type);
     }
     if (e.pre) {
       store1(e.pre, at.p + c, e.p_type, v);
@@ -719,8 +719,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
 #pragma unroll
       for (int p = 0; p < kPairs; ++p)
         if (whole(p % kResults))
-          load8(e.bias, (long long)(p / kResults) * g.N + col_l + 32 * (p % kResults), e.b_type,
-                bias[p]);
+          load8(e.bias, (p / kResults) * e.up + col_l + 32 * (p % kResults), e.b_type, bias[p]);
       // No load may look pending where the K loop starts again: the compiler would have
       // every step wait for all DMA before it uses the register.
 #pragma unroll
@@ -796,7 +795,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
           } else {
 #pragma unroll
             for (int x = 0; x < 8; ++x)
-              if (col + x < g.N) finish1<kEpi>(e, at, 32 * p + x, col + x, g.N, v[p][x], u[x]);
+              if (col + x < g.N) finish1<kEpi>(e, at, 32 * p + x, col + x, v[p][x], u[x]);
           }
         }
       }
@@ -848,7 +847,7 @@ __device__ __forceinline__ void dense_reduce_body(const DenseArgs& g) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += b[i];
       if constexpr (kGated) {
-        load8(e.bias, (long long)g.N + col, e.b_type, b);
+        load8(e.bias, e.up + col, e.b_type, b);
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] += b[i];
       }
@@ -859,7 +858,7 @@ __device__ __forceinline__ void dense_reduce_body(const DenseArgs& g) {
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (col + i < g.N) finish1<kEpi>(e, at, i, col + i, g.N, v[i], u[i]);
+      if (col + i < g.N) finish1<kEpi>(e, at, i, col + i, v[i], u[i]);
   }
 }
 

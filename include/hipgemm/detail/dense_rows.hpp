@@ -148,7 +148,7 @@ __device__ __forceinline__ void dense_rows_body(const DenseArgs& g, lds_u8* lds)
       to[0] = v;
       if constexpr (kGated) to[g.ldpart / 2] = u;
     } else {
-      finish1<kEpi>(g.epi, dense_at(g.epi, row, col), 0, col, g.N, v, u);
+      finish1<kEpi>(g.epi, dense_at(g.epi, row, col), 0, col, v, u);
     }
   }
 }
