@@ -175,8 +175,12 @@ def _call(x, weight, bias, activation, residual, out_dtype, gated):
     if x.dim() != 2:
         lead = x.shape[:-1]
         if residual is not None:
-            residual = residual.reshape(-1, residual.shape[-1])
-        y = _call(x.reshape(-1, x.shape[-1]), weight, bias, activation, residual, out_dtype, gated)
+            if residual.shape[:-1] != lead:
+                raise HipGemmError(f"residual must be {(*lead, weight.shape[0])}, got "
+                                   f"{tuple(residual.shape)}")
+            residual = residual.unsqueeze(0).flatten(0, -2)
+        y = _call(x.unsqueeze(0).flatten(0, -2), weight, bias, activation, residual, out_dtype,
+                  gated)
         return y.reshape(*lead, y.shape[-1])
     _check_shapes(x, weight, bias, activation, residual, gated)
     if _wanted(x, weight, bias, residual):

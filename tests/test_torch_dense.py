@@ -251,3 +251,27 @@ def test_example(gpu):
         step()
         with torch.no_grad():
             assert torch.equal(sy, block(x[:1], residual=x[:1]))
+
+
+def test_leading_dimensions():
+    """Those of the residual are x's own, not any that hold as many rows."""
+    w = torch.empty(48, 64, dtype=BF, device="meta")
+    x = torch.empty(2, 3, 64, dtype=BF, device="meta")
+    for shape in ((3, 2, 48), (6, 48), (1, 3, 48)):
+        with pytest.raises(hg.HipGemmError, match="residual"):
+            td.linear(x, w, residual=torch.empty(shape, dtype=BF, device="meta"))
+    r = torch.empty(2, 3, 48, dtype=BF, device="meta")
+    assert td.linear(x, w, residual=r).shape == (2, 3, 48)
+    assert td.linear(x[0, 0], w, residual=torch.empty(48, dtype=BF, device="meta")).shape == (48,)
+    # and of no elements
+    for lead, k in (((0, 3), 64), ((2, 0), 64), ((2, 3), 0)):
+        y = td.gated_linear(torch.empty(*lead, k, dtype=BF, device="meta"), w[:, :k])
+        assert y.shape == (*lead, 24)
+
+
+def test_differentiable_once():
+    x = torch.empty(5, 64, dtype=BF, device="meta", requires_grad=True)
+    w = torch.empty(48, 64, dtype=BF, device="meta", requires_grad=True)
+    g, = torch.autograd.grad(td.gated_linear(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), w)
