@@ -164,6 +164,8 @@ def lib() -> ctypes.CDLL:
         getattr(L, name).restype = ci
         getattr(L, name + "_workspace_size").argtypes = [vp]
         getattr(L, name + "_workspace_size").restype = ctypes.c_size_t
+        getattr(L, name + "_select").argtypes = [vp, vp]
+        getattr(L, name + "_select").restype = ci
     L.hipgemm_workspace_size.argtypes = [ci, ci, ci, ci]
     L.hipgemm_workspace_size.restype = ctypes.c_size_t
     L.hipgemm_fp8_gemm_4wave_256x256x128.argtypes = [vp, vp, vp, ci, ci, ci,

@@ -334,9 +334,9 @@ hipError_t check(const hipgemm_linear_grad_desc* desc) {
   if (!desc || desc->size != sizeof(hipgemm_linear_grad_desc)) return hipErrorInvalidValue;
   const hipgemm_linear_grad_desc& d = *desc;
   if (!common(d.M, d.N, d.K, d.gated, d.type, d.activation) || d.dy_type < 0 ||
-      d.dy_type > HIPGEMM_IN_F16 || d.pre_type < 0 || d.pre_type > HIPGEMM_IN_F16 || d.dx_dtype < 0 || d.dx_dtype > HIPGEMM_OUT_F32 ||
-      d.dw_dtype < 0 || d.dw_dtype > HIPGEMM_OUT_F32 || d.db_dtype < 0 ||
-      d.db_dtype > HIPGEMM_OUT_F32)
+      d.dy_type > HIPGEMM_IN_F16 || d.pre_type < 0 || d.pre_type > HIPGEMM_IN_F16 ||
+      d.dx_dtype < 0 || d.dx_dtype > HIPGEMM_OUT_F32 || d.dw_dtype < 0 ||
+      d.dw_dtype > HIPGEMM_OUT_F32 || d.db_dtype < 0 || d.db_dtype > HIPGEMM_OUT_F32)
     return hipErrorInvalidValue;
   const long long cols = d.gated ? 2ll * d.N : d.N;
   if (d.M > 0 && d.N > 0) {
@@ -360,6 +360,13 @@ hipError_t check(const hipgemm_linear_grad_desc* desc) {
 bool as_is(const hipgemm_linear_grad_desc& d) {
   return !d.gated && d.activation == HIPGEMM_ACT_NONE && d.dy_type == d.type && d.N % 8 == 0 &&
          aligned(d.dy, 16) && d.lddy % 8 == 0 && d.lddy <= kMaxLd;
+}
+
+Plan plan_of_x(const hipgemm_linear_grad_desc& d) {
+  return plan_of(hk::kDenseNN, d.M, d.K, d.gated ? 2 * d.N : d.N);
+}
+Plan plan_of_w(const hipgemm_linear_grad_desc& d) {
+  return plan_of(hk::kDenseTN, d.gated ? 2 * d.N : d.N, d.K, d.M);
 }
 
 struct GradPlan {
@@ -387,11 +394,9 @@ GradPlan grad_plan(const hipgemm_linear_grad_desc& d) {
   p.dz = p.own ? padded(2ull * (size_t)d.M * (size_t)p.ldz) : 0;
   p.columns = d.db ? padded(4ull * (size_t)p.blocks * (size_t)p.cols) : 0;
   size_t part = 0;
-  if (d.dx)
-    part = partial_bytes(hk::kDenseNN, plan_of(hk::kDenseNN, d.M, d.K, (int)p.cols), d.M, d.K);
+  if (d.dx) part = partial_bytes(hk::kDenseNN, plan_of_x(d), d.M, d.K);
   if (d.dw) {
-    const size_t w = partial_bytes(hk::kDenseTN, plan_of(hk::kDenseTN, (int)p.cols, d.K, d.M),
-                                   (int)p.cols, d.K);
+    const size_t w = partial_bytes(hk::kDenseTN, plan_of_w(d), (int)p.cols, d.K);
     if (w > part) part = w;
   }
   p.partial = part;
@@ -481,6 +486,11 @@ hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
   return hipSuccess;
 }
 
+hipgemm_linear_plan shown(const Plan& p) {
+  if (p.tile < 0) return {0, 0, p.slices, p.first};
+  return {hk::kDenseTiles[p.tile].bm, hk::kDenseTiles[p.tile].bn, p.slices, p.first};
+}
+
 }  // namespace
 
 extern "C" size_t hipgemm_linear_workspace_size(const hipgemm_linear_desc* desc) {
@@ -508,4 +518,26 @@ extern "C" hipError_t hipgemm_linear_backward(const hipgemm_linear_grad_desc* de
                                               hipStream_t stream) {
   const hipError_t e = check(desc);
   return e != hipSuccess ? e : backward(*desc, stream);
+}
+
+extern "C" hipError_t hipgemm_linear_select(const hipgemm_linear_desc* desc,
+                                            hipgemm_linear_plan* plan) {
+  if (!plan || !desc || desc->size != sizeof(*desc) ||
+      !common(desc->M, desc->N, desc->K, desc->gated, desc->type, desc->activation))
+    return hipErrorInvalidValue;
+  *plan = {};
+  if (desc->M > 0 && desc->N > 0)
+    *plan = shown(plan_of(kind_of(*desc), desc->M, desc->N, desc->K));
+  return hipSuccess;
+}
+
+extern "C" hipError_t hipgemm_linear_backward_select(const hipgemm_linear_grad_desc* desc,
+                                                     hipgemm_linear_plan plan[2]) {
+  if (!plan || !desc || desc->size != sizeof(*desc) ||
+      !common(desc->M, desc->N, desc->K, desc->gated, desc->type, desc->activation))
+    return hipErrorInvalidValue;
+  plan[0] = plan[1] = {};
+  if (desc->dx && desc->M > 0 && desc->K > 0) plan[0] = shown(plan_of_x(*desc));
+  if (desc->dw && desc->N > 0 && desc->K > 0) plan[1] = shown(plan_of_w(*desc));
+  return hipSuccess;
 }

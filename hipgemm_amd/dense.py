@@ -19,7 +19,8 @@ from .serving import _bad, _on, _stream_handle
 
 __all__ = ["linear", "linear_backward", "gated_linear", "gated_linear_backward",
            "LinearDesc", "LinearGradDesc", "linear_raw", "linear_backward_raw",
-           "linear_workspace_size", "linear_backward_workspace_size"]
+           "linear_workspace_size", "linear_backward_workspace_size", "linear_select",
+           "linear_backward_select"]
 
 _vp, _ci, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 
@@ -76,6 +77,22 @@ def linear_workspace_size(desc: "LinearDesc") -> int:
 def linear_backward_workspace_size(desc: "LinearGradDesc") -> int:
     """Workspace bytes hipgemm_linear_backward needs for a descriptor."""
     return int(lib().hipgemm_linear_backward_workspace_size(ctypes.byref(desc)))
+
+
+def linear_select(desc: "LinearDesc") -> tuple:
+    """(tile rows, tile columns, slices along K, first columns) that hipgemm_linear takes for
+    a descriptor's sizes (include/hipgemm.h); tile rows 0: the kernel of a few rows."""
+    plan = (_ci * 4)()
+    _check(lib().hipgemm_linear_select(ctypes.byref(desc), plan), "hipgemm_linear_select")
+    return tuple(plan)
+
+
+def linear_backward_select(desc: "LinearGradDesc") -> tuple:
+    """The same of hipgemm_linear_backward's two products: (of dx, of dw)."""
+    plan = (_ci * 8)()
+    _check(lib().hipgemm_linear_backward_select(ctypes.byref(desc), plan),
+           "hipgemm_linear_backward_select")
+    return tuple(plan[:4]), tuple(plan[4:])
 
 
 def _launch(call, what, desc, x, stream):
@@ -256,10 +273,10 @@ def linear(x, weight, *, bias=None, activation=None, residual=None, out_dtype=No
     x (M, K) and weight (N, K): both bfloat16 or both float16, K a multiple of 8, rows of
     unit stride that start on 16 bytes.  bias (N) and residual (M, N): bfloat16, float16
     or float32.  activation as for gemm().  out_dtype: bfloat16, float16 or float32, x's
-    where None.  out may be residual itself.  Sums are fp32, and everything after them
-    until the one rounding.  save_pre: returns (out, z), as linear_backward takes it: z in
-    float32 where True, or of the type given (x's halves its memory and adds a rounding to
-    the gradients)."""
+    where None.  out may be residual itself and overlaps nothing else.  Sums are fp32, and
+    everything after them until the one rounding.  save_pre: returns (out, z), as
+    linear_backward takes it: z in float32 where True, or of the type given (x's halves its
+    memory and adds a rounding to the gradients)."""
     return _forward(x, weight, bias, activation, residual, out_dtype, out, save_pre, False,
                     stream)
 
@@ -282,8 +299,8 @@ def linear_backward(dy, x, weight, pre=None, *, activation=None, need_x: bool = 
 
     dy (M, N): bfloat16, float16 or float32.  pre: linear's z (save_pre); not needed without
     an activation.  dx has x's type, dweight grad_dtype (bfloat16, float16 or float32; x's
-    type where None) and dbias bias_dtype (grad_dtype where None).  dz is rounded to x's type for the two products; sums are
-    fp32."""
+    type where None) and dbias bias_dtype (grad_dtype where None).  dz is rounded to x's type
+    for the two products; sums are fp32."""
     return _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias,
                      grad_dtype, bias_dtype, False, stream)
 

@@ -521,11 +521,11 @@ hipError_t hipgemm_moe_select(int T, int k, int E, int D, int F, int format,
  * Requirements: K % 8 == 0, gated N % 8 == 0;  x and weight 16-byte aligned with row
  * strides of a multiple of 8;  the others aligned to their element (16 bytes, strides
  * of a multiple of 16 bytes and N % 8 == 0 are faster);  M <= 2^30, K, rows of weight
- * and strides of x and weight up to 2^21.  residual may be y itself.  M == 0 or N == 0 is a no-op;
- * K == 0 is a sum of nothing.  Workspace: hipgemm_linear_workspace_size bytes (0 for
- * most calls), 256-byte aligned, of any content; calls that may run concurrently must not
- * share one.  Zero-initialise the struct and set `size`.  No reference counterpart (the
- * reference has e4m3 operands only).
+ * and strides of x and weight up to 2^21.  residual may be y itself; otherwise what is
+ * written overlaps nothing else.  M == 0 or N == 0 is a no-op;  K == 0 is a sum of nothing.
+ * Workspace: hipgemm_linear_workspace_size bytes (0 for most calls), 256-byte aligned, of
+ * any content; calls that may run concurrently must not share one.  Zero-initialise the
+ * struct and set `size`.  No reference counterpart (the reference has e4m3 operands only).
  */
 typedef struct hipgemm_linear_desc {
   size_t size;
@@ -555,10 +555,10 @@ hipError_t hipgemm_linear(const hipgemm_linear_desc *desc, hipStream_t stream);
  *   db[n] = sum_m dz[m, n]     N (gated 2N)
  *
  * each where its pointer is not NULL.  (The residual's gradient is dy.)  z is read from
- * pre (pre_type HIPGEMM_IN_*), as the forward pass left it; not needed where activation is NONE and not
- * gated.  dz is rounded to `type` for the two products, not for db; sums are fp32, in an
- * order that depends on the sizes only.  Slopes: relu'(0) = 0.  With M == 0, dw and db
- * are zeros.  Requirements as above; dy, pre: aligned to their element.  Workspace:
+ * pre (pre_type HIPGEMM_IN_*), as the forward pass left it; not needed where activation is
+ * NONE and not gated.  dz is rounded to `type` for the two products, not for db; sums are
+ * fp32, in an order that depends on the sizes only.  Slopes: relu'(0) = 0.  With M == 0, dw
+ * and db are zeros.  Requirements as above; dy, pre: aligned to their element.  Workspace:
  * hipgemm_linear_backward_workspace_size bytes for the descriptor (its pointers, strides
  * and types matter), as above.  No reference counterpart.
  */
@@ -580,6 +580,19 @@ typedef struct hipgemm_linear_grad_desc {
 size_t hipgemm_linear_backward_workspace_size(const hipgemm_linear_grad_desc *desc);
 hipError_t hipgemm_linear_backward(const hipgemm_linear_grad_desc *desc,
                                    hipStream_t stream);
+
+/* The kernels that hipgemm_linear and hipgemm_linear_backward's products (dx, dw; all 0
+ * where not asked for) run for a descriptor's sizes: tiles of tile_rows x tile_columns
+ * results (gated: of gate and up columns together), or tile_rows 0 for the kernel of a few
+ * rows; the slices along K, whose sums are added by a second kernel; and the first columns
+ * (0: none) that tiles of 256 x 256 do in a launch of their own.  No GPU needed; no
+ * reference counterpart. */
+typedef struct hipgemm_linear_plan {
+  int tile_rows, tile_columns, slices, first_columns;
+} hipgemm_linear_plan;
+hipError_t hipgemm_linear_select(const hipgemm_linear_desc *desc, hipgemm_linear_plan *plan);
+hipError_t hipgemm_linear_backward_select(const hipgemm_linear_grad_desc *desc,
+                                          hipgemm_linear_plan plan[2]);
 
 /* Workspace bytes hipgemm_fp8_gemm_bf16_ws needs for this shape and variant
  * on the current device (0: none).  No GPU work.  No reference counterpart. */
