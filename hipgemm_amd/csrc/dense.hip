@@ -163,11 +163,11 @@ Plan plan_whole(int kind, int M, int N, int K) {
 }
 
 // Where 256 x 256 tiles leave a last round that is not full, their whole rounds' columns by
-// them and the rest as it goes best by itself, in a second launch (us, whole / in two: 6000 x 3000 x
-// 8192 308/261, 1531 x 14336 x 4096 172/165).  Only for a fifth at least: CUs without a tile leave
-// the others their power (2500 x 16384 x 4096, 2.5 rounds, 307/330; gated 2048 x 14336 x 4096, 3.5
-// rounds, 427/425 to 490).
-constexpr double kGain = 1.2;
+// them and the rest as it goes best by itself, in smaller tiles or slices, in a second launch
+// (us, whole / in two: 6000 x 3000 x 8192 307/253, 4096 x 5120 x 5120 213/172, gated 2048 x 14336 x
+// 4096 409/373, 1531 x 14336 x 4096 170/158, 4096 x 6144 x 2048 101/96).  Two launches by estimates
+// that differ by less than kGain did not differ, or were slower.
+constexpr double kGain = 1.04;
 Plan plan_of(int kind, int M, int N, int K) {
   Plan best = plan_whole(kind, M, N, K);
   constexpr int kBig = 1;
@@ -185,7 +185,7 @@ Plan plan_of(int kind, int M, int N, int K) {
   if (first < 1 || first >= across) return best;
   const Plan rest = plan_whole(kind, M, (int)(N - first * cols), K);
   const double us = rest.us + (double)((down * first + kCus - 1) / kCus) * round;
-  if (us * kGain < best.us) {
+  if (us * kGain < best.us && (rest.tile != kBig || rest.slices > 1)) {
     best = rest;
     best.us = us;
     best.first = (int)(first * cols);
