@@ -81,8 +81,8 @@ struct Plan {
 
 // Estimated times, us.  A tile's step of 64 along K by how the operands lie, and its end,
 // with every CU at work on operands that come from memory: 128 x 128, 256 x 256, 64 x 128,
-// 256 x 128.  Against every tile and 1, 2, 4, 8 slices on 148 shapes the choice is within 1 % of
-// the best at the median, 3 % in the mean (us, chosen / another):
+// 256 x 128.  Against every tile and 1, 2, 4, 8 slices on 127 shapes the choice is the best one at
+// the median and within 1.5 % in the mean (us, chosen / another):
 //   forward   64 x 4096 x 4096 15 (rows) / 32 (64 x 128), 64 x 14336 x 4096 29 (64 x 128 in 2 slices)
 //             / 46 (rows), 128 x 4096 x 14336 39 (128 x 128 in 8 slices) / 48 (in 4), 512 x 14336 x
 //             4096 65 (256 x 128) / 83 (128 x 128), 1024 x 4096 x 4096 40 (128 x 128) / 55 (256 x 128)
@@ -99,13 +99,14 @@ constexpr double kLaunch = 4.0, kSplitLaunch = 3.5;
 constexpr double kBytesPerUs = 5.0e6;          // from memory: a few rows
 constexpr double kSumBytesPerUs = 9.0e6;       // sums of K-slices, both ways
 constexpr double kTileBytesPerUs = 5.7e6;      // the operands of tiles
-constexpr double kCuMemoryBytesPerUs = 28.0e3;  // from memory, into one CU among few at work
+constexpr double kPanelBytesPerUs = 33.5e3;    // 128 rows from memory, to the CUs that read them
 constexpr double kCuBytesPerUs = 75.0e3;       // into one CU, the most of it from a cache
 constexpr int kCus = 256;
 
 double split_us(int slices, int M, int N, bool gated) {
   if (slices == 1) return 0.0;
-  return kSplitLaunch + 0.3 * slices + 8.0 * slices * M * (double)N * (gated ? 2 : 1) / kSumBytesPerUs;
+  const double bytes = 8.0 * slices * M * (double)N * (gated ? 2 : 1);
+  return kSplitLaunch + 0.3 * slices + bytes / kSumBytesPerUs;
 }
 
 // A few rows: what a CU has to fetch (x again for every 16 rows of weights), or the weights
@@ -133,13 +134,15 @@ Plan plan_whole(int kind, int M, int N, int K) {
       const double us = rows_us(M, N, K, gated, slices);
       if (us < best.us) best = {-1, slices, (steps + slices - 1) / slices, 0, us, 0};
     }
-  const double bytes = 2.0 * ((double)M + N * (gated ? 2.0 : 1.0)) * K;
+  const double b_bytes = 2.0 * N * (gated ? 2.0 : 1.0) * K;
+  const double whole_us = (2.0 * M * K + b_bytes) / kTileBytesPerUs;
   for (int t = 0; t < hk::kNumDenseTiles; ++t) {
     if (kind == hk::kDenseTN && t == 2) continue;
     const hk::TileShape s = hk::kDenseTiles[t];
     const int cols = gated ? s.bn / 2 : s.bn;
-    const long long tiles =
-        (((long long)M + s.bm - 1) / s.bm) * (((long long)N + cols - 1) / cols);
+    const long long tiles_n = ((long long)N + cols - 1) / cols;
+    const long long tiles = (((long long)M + s.bm - 1) / s.bm) * tiles_n;
+    if (tiles == 0) continue;
     const double step = forward                ? kTime[t].forward
                         : kind == hk::kDenseNN ? kTime[t].of_x
                                                : kTime[t].of_w;
@@ -152,8 +155,11 @@ Plan plan_whole(int kind, int M, int N, int K) {
       const double clock = t == 1 && units <= kCus * 3 / 4 ? 0.85 : 1.0;
       const double work =
           (double)((units + kCus - 1) / kCus) * (each * step * clock + kTime[t].end);
-      const double pull = (double)(units < kCus ? units : kCus) * kCuMemoryBytesPerUs;
-      const double memory = bytes / (pull < kTileBytesPerUs ? pull : kTileBytesPerUs);
+      // B by as many panels at once as are at work: tiles above each other share one (128 x
+      // 14336 x 4096, 224 CUs: 64 x 128 39.5 us, 128 x 128 in 2 slices 34.9).
+      const double panels = (double)(units < kCus ? units : kCus) * tiles_n / tiles * s.bn / 128;
+      const double panels_us = b_bytes / (panels * kPanelBytesPerUs);
+      const double memory = whole_us > panels_us ? whole_us : panels_us;
       const double us =
           kLaunch + (work > memory ? work : memory) + split_us(slices, M, N, gated);
       if (us < best.us) best = {t, slices, each, units, us, 0};
