@@ -83,9 +83,10 @@ struct Plan {
 // with every CU at work on operands that come from memory: 128 x 128, 256 x 256, 64 x 128,
 // 256 x 128.  Against every tile and 1, 2, 4, 8 slices on 127 shapes the choice is the best one at
 // the median and within 1.5 % in the mean (us, chosen / another):
-//   forward   64 x 4096 x 4096 15 (rows) / 32 (64 x 128), 64 x 14336 x 4096 29 (64 x 128 in 2 slices)
-//             / 46 (rows), 128 x 4096 x 14336 39 (128 x 128 in 8 slices) / 48 (in 4), 512 x 14336 x
-//             4096 65 (256 x 128) / 83 (128 x 128), 1024 x 4096 x 4096 40 (128 x 128) / 55 (256 x 128)
+//   forward   64 x 4096 x 4096 15 (rows) / 32 (64 x 128), 64 x 14336 x 4096 29 (64 x 128 in 2
+//             slices) / 46 (rows), 128 x 4096 x 14336 39 (128 x 128 in 8 slices) / 48 (in 4), 512 x
+//             14336 x 4096 65 (256 x 128) / 83 (128 x 128), 1024 x 4096 x 4096 40 (128 x 128) / 55
+//             (256 x 128)
 //   of x      777 x 14336 x 4096 108 (256 x 128 in 2 slices) / 128 (128 x 128)
 //   of w      4096 x 14336 x 4096 391 (256 x 256) / 432 (256 x 128)
 struct TileTime {
@@ -134,6 +135,8 @@ Plan plan_whole(int kind, int M, int N, int K) {
       const double us = rows_us(M, N, K, gated, slices);
       if (us < best.us) best = {-1, slices, (steps + slices - 1) / slices, 0, us, 0};
     }
+  // (Of one row to four nothing else is as fast: a pass over the weights.)
+  if (forward && M <= 4) return best;
   const double b_bytes = 2.0 * N * (gated ? 2.0 : 1.0) * K;
   const double whole_us = (2.0 * M * K + b_bytes) / kTileBytesPerUs;
   for (int t = 0; t < hk::kNumDenseTiles; ++t) {
@@ -212,8 +215,7 @@ size_t partial_bytes(int kind, const Plan& p, int M, int N) {
 hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream);
 
 // g: operands, sizes and epilogue; ws: partial_bytes.
-hipError_t product(int x, int kind, DenseArgs& g, void* ws, hipStream_t stream) {
-  const Plan p = plan_of(kind, g.M, g.N, g.K);
+hipError_t product(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream) {
   if (!p.first) return run(x, kind, p, g, ws, stream);
   DenseArgs part = g;
   part.N = p.first;
@@ -305,7 +307,9 @@ size_t forward_bytes(const hipgemm_linear_desc& d) {
 }
 
 hipError_t forward(const hipgemm_linear_desc& d, hipStream_t stream) {
-  const size_t need = forward_bytes(d);
+  const int kind = kind_of(d);
+  const Plan p = plan_of(kind, d.M, d.N, d.K);
+  const size_t need = partial_bytes(kind, p, d.M, d.N);
   if (need && (!d.workspace || d.workspace_bytes < need || !aligned(d.workspace, kAlign)))
     return hipErrorInvalidValue;
   DenseArgs g{};
@@ -331,7 +335,7 @@ hipError_t forward(const hipgemm_linear_desc& d, hipStream_t stream) {
   e.p_type = d.pre_dtype;
   e.b_type = d.bias_type;
   e.r_type = d.residual_type;
-  return product(d.type, kind_of(d), g, d.workspace, stream);
+  return product(d.type, kind, p, g, d.workspace, stream);
 }
 
 // ---- backward ---------------------------------------------------------------------
@@ -368,18 +372,12 @@ bool as_is(const hipgemm_linear_grad_desc& d) {
          aligned(d.dy, 16) && d.lddy % 8 == 0 && d.lddy <= kMaxLd;
 }
 
-Plan plan_of_x(const hipgemm_linear_grad_desc& d) {
-  return plan_of(hk::kDenseNN, d.M, d.K, d.gated ? 2 * d.N : d.N);
-}
-Plan plan_of_w(const hipgemm_linear_grad_desc& d) {
-  return plan_of(hk::kDenseTN, d.gated ? 2 * d.N : d.N, d.K, d.M);
-}
-
 struct GradPlan {
   long long cols, ldz;  // of dz
   bool own;             // dz lies in the workspace
   int blocks, rows;     // of the column sums
   size_t dz, columns, partial;
+  Plan of_x, of_w;
 };
 GradPlan grad_plan(const hipgemm_linear_grad_desc& d) {
   GradPlan p{};
@@ -400,9 +398,13 @@ GradPlan grad_plan(const hipgemm_linear_grad_desc& d) {
   p.dz = p.own ? padded(2ull * (size_t)d.M * (size_t)p.ldz) : 0;
   p.columns = d.db ? padded(4ull * (size_t)p.blocks * (size_t)p.cols) : 0;
   size_t part = 0;
-  if (d.dx) part = partial_bytes(hk::kDenseNN, plan_of_x(d), d.M, d.K);
+  if (d.dx) {
+    p.of_x = plan_of(hk::kDenseNN, d.M, d.K, (int)p.cols);
+    part = partial_bytes(hk::kDenseNN, p.of_x, d.M, d.K);
+  }
   if (d.dw) {
-    const size_t w = partial_bytes(hk::kDenseTN, plan_of_w(d), (int)p.cols, d.K);
+    p.of_w = plan_of(hk::kDenseTN, (int)p.cols, d.K, d.M);
+    const size_t w = partial_bytes(hk::kDenseTN, p.of_w, (int)p.cols, d.K);
     if (w > part) part = w;
   }
   p.partial = part;
@@ -473,7 +475,7 @@ hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
     g.N = d.K;
     g.K = (int)p.cols;
     plain_epilogue(g, d.dx, d.lddx, d.dx_dtype);
-    const hipError_t e = product(d.type, hk::kDenseNN, g, partial, stream);
+    const hipError_t e = product(d.type, hk::kDenseNN, p.of_x, g, partial, stream);
     if (e != hipSuccess) return e;
   }
   if (d.dw && d.N > 0 && d.K > 0) {
@@ -486,7 +488,7 @@ hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
     g.N = d.K;
     g.K = d.M;
     plain_epilogue(g, d.dw, d.lddw, d.dw_dtype);
-    const hipError_t e = product(d.type, hk::kDenseTN, g, partial, stream);
+    const hipError_t e = product(d.type, hk::kDenseTN, p.of_w, g, partial, stream);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
@@ -542,8 +544,9 @@ extern "C" hipError_t hipgemm_linear_backward_select(const hipgemm_linear_grad_d
   if (!plan || !desc || desc->size != sizeof(*desc) ||
       !common(desc->M, desc->N, desc->K, desc->gated, desc->type, desc->activation))
     return hipErrorInvalidValue;
+  const GradPlan p = grad_plan(*desc);
   plan[0] = plan[1] = {};
-  if (desc->dx && desc->M > 0 && desc->K > 0) plan[0] = shown(plan_of_x(*desc));
-  if (desc->dw && desc->N > 0 && desc->K > 0) plan[1] = shown(plan_of_w(*desc));
+  if (desc->dx && desc->M > 0 && desc->K > 0) plan[0] = shown(p.of_x);
+  if (desc->dw && desc->N > 0 && desc->K > 0) plan[1] = shown(p.of_w);
   return hipSuccess;
 }

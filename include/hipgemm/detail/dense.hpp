@@ -25,7 +25,12 @@
 //   half 0 of step k: MFMA of set 0 | read set 1: half 1 of step k
 //   barrier: every wave's reads of step k are done, step k + 1 has landed
 //   half 1 of step k: MFMA of set 1 | read set 0: half 0 of step k + 1,
-//                                   | DMA of step k + S into step k's stage
+//                                   | DMA of step k + S into step k's stage, the first half
+//   half 0 of step k + 1            | the other half
+// A CU takes in 64 bytes a cycle, which is as long as a step's MFMA in tiles of 128 x 128 and
+// longer in smaller ones, and a wave that issues into a full queue waits: all of a step's DMA
+// in half 1 made it the longer half (256 x 128, one workgroup alone at K 8192 89 us, spread 78;
+// 2048 x 4096 x 4096 60.6 / 59.0).
 // The sequence runs on across tiles: what lies past a tile's last step is the next
 // tile's first.  Steps of a tile are padded to at least S (padding reads zeros).
 //
@@ -191,7 +196,10 @@ __device__ __forceinline__ void store1(uint8_t* p, long long at, int out, float 
 }
 
 __device__ __forceinline__ float activate(float v, int act) {
-  return act == kActRelu ? relu(v) : act == kActSilu ? silu(v) : act == kActGeluTanh ? gelu_tanh(v) : v;
+  return act == kActRelu       ? relu(v)
+         : act == kActSilu     ? silu(v)
+         : act == kActGeluTanh ? gelu_tanh(v)
+                               : v;
 }
 __device__ __forceinline__ void activate8(float (&v)[8], int act) {
   if (act == kActRelu) {
@@ -513,7 +521,8 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     if (is_b ? kBCol : kACol) {
       const int width = is_b ? kWideB : kWideA, c = f % (is_b ? kCB : kCA);
       const int part = f / (is_b ? kCB : kCA) * kBK * width;
-      to[p] = lds_read_across(lds + st + (is_b ? col_b[c] : col_a[c]) + part + (8 * h + 4 * p) * width);
+      to[p] = lds_read_across(lds + st + (is_b ? col_b[c] : col_a[c]) + part +
+                              (8 * h + 4 * p) * width);
     } else {
       const lds_u8* from = lds + st + (is_b ? row_b : row_a) + slot[h] + f * 16 * Cfg::kRow;
       const s16x8 v = __builtin_bit_cast(s16x8, lds_read16(from));
@@ -540,29 +549,33 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     mfma_acc<kX>(frag(fb[h][j]), frag(fa[h][i]), acc[i][j]);
   };
   // Each MFMA of a half is followed by the reads and DMA that are due: reads spread over
-  // three quarters of its MFMA, DMA over all of half 1 (256 x 256 x K 14336 / 4096, both in rows,
+  // three quarters of its MFMA, DMA over all (256 x 256 x K 14336 / 4096 by halves, both in rows,
   // TFLOP/s: 1552 / 1409; reads one after each of the first sixteen MFMA and DMA after them
-  // 1543 / 1385, across K 1315 for 1410: LDS is busy three quarters of the time, bursts
-  // queue).
-  auto half0 = [&](int st) {
+  // 1543 / 1385, across K 1315 for 1410: bursts queue).
+  // A step's DMA of which half 1 issues the first kFirst, and half 0 of the next the others.
+  constexpr int kFirst = (kDma + 1) / 2, kRest = kDma - kFirst;
+  Step src;
+  auto half0 = [&](int st, int last) {
     wait_lgkmcnt<0>();
     static_for<kHead>([&](auto n) {
       mfma(0, n);
       static_for<due(n + 1, kSpan, kReads) - due(n, kSpan, kReads)>(
           [&](auto r) { read_one(st, 1, due(n, kSpan, kReads) + r); });
+      static_for<due(n + 1, kHead, kRest) - due(n, kHead, kRest)>(
+          [&](auto q) { dma_one(src, last, kFirst + due(n, kHead, kRest) + q); });
       sched_fence();
     });
   };
   auto half1 = [&](int st, int rst, int d) {
-    const Step src = step_src(d);
+    src = step_src(d);
     static_for<kTail>([&](auto n) { mfma(0, kHead + n); });
     sched_fence();
     static_for<kMfma>([&](auto n) {
       mfma(1, n);
       static_for<due(n + 1, kSpan, kReads) - due(n, kSpan, kReads)>(
           [&](auto r) { read_one(rst, 0, due(n, kSpan, kReads) + r); });
-      static_for<due(n + 1, kMfma, kDma) - due(n, kMfma, kDma)>(
-          [&](auto q) { dma_one(src, st, due(n, kMfma, kDma) + q); });
+      static_for<due(n + 1, kMfma, kFirst) - due(n, kMfma, kFirst)>(
+          [&](auto q) { dma_one(src, st, due(n, kMfma, kFirst) + q); });
       sched_fence();
     });
   };
@@ -570,20 +583,21 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     s += Cfg::kStage;
     return s == S * Cfg::kStage ? 0 : s;
   };
-  int st = 0;
+  int st = 0, last = (S - 1) * Cfg::kStage;
   bool stored = false;  // the previous tile was whole: all its stores were issued
   constexpr int kStores = FA * FB / (kGated ? 4 : 2);  // at least
   static_assert((S - 2) * kDma + kStores < 64, "vmcnt range");
   auto step_halves = [&](int k) {
     const int rst = next_stage(st);
-    half0(st);
-    // Step k + 1 has landed: newer are the DMA of S - 2 steps, and in a tile's first S - 1
+    half0(st, last);
+    // Step k + 1 has landed: newer are the DMA of S - 2 steps, and in a tile's first S - 2
     // steps the stores of the one before.
     wait_lgkmcnt<0>();
-    if (stored && k < S - 1) wait_vmcnt<(S - 2) * kDma + kStores>();
+    if (stored && k < S - 2) wait_vmcnt<(S - 2) * kDma + kStores>();
     else wait_vmcnt<(S - 2) * kDma>();
     barrier();
     half1(st, rst, k + S);
+    last = st;
     st = rst;
   };
 
@@ -672,11 +686,11 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   } else {
 #pragma unroll
     for (int d = 0; d < S; ++d) {
-      const Step src = step_src(d);
+      src = step_src(d);
 #pragma unroll
-      for (int n = 0; n < kDma; ++n) dma_one(src, d * Cfg::kStage, n);
+      for (int n = 0; n < (d < S - 1 ? kDma : kFirst); ++n) dma_one(src, d * Cfg::kStage, n);
     }
-    wait_vmcnt<(S - 1) * kDma>();
+    wait_vmcnt<(S - 2) * kDma + kFirst>();
     barrier();
 #pragma unroll
     for (int n = 0; n < kReads; ++n) read_one(0, 0, n);
@@ -771,7 +785,8 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
       asm volatile("" : "+v"(row_l), "+v"(col_l));
       if (row_l < g.M) {
         const DenseAt at = dense_at(e, row_l, col_l);
-        const long long part = ((long long)(kSplit ? t / tiles : 0) * g.M + row_l) * g.ldpart + col_l;
+        const long long part =
+            ((long long)(kSplit ? t / tiles : 0) * g.M + row_l) * g.ldpart + col_l;
 #pragma unroll
         for (int p = 0; p < kResults; ++p) {
           const int col = col_l + 32 * p;
