@@ -59,3 +59,12 @@ def test_refusals():
     with pytest.raises(hg.HipGemmError):
         hg.linear_select(d)
     assert hg.lib().hipgemm_linear_select(ctypes.byref(forward(8, 8, 8)), None) == 1
+
+
+def test_packed_descriptor():
+    """The calls' packed bytes are the structure's."""
+    from hipgemm_amd.dense import _linear_desc
+    values = [ctypes.sizeof(hg.LinearDesc)] + [3 + 1000 ** 3 * i for i in range(13)]
+    values += list(range(100, 110))
+    assert len(values) == len(hg.LinearDesc._fields_)
+    assert _linear_desc(*values) == bytes(hg.LinearDesc(*values))
