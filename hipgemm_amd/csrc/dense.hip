@@ -18,6 +18,12 @@ HIPGEMM_DENSE(tn)
 HIPGEMM_DENSE(gated)
 #undef HIPGEMM_DENSE
 
+const void* dense_pair_bf16();
+const void* dense_pair_f16();
+const void* dense_pair(int x) {
+  return x == detail::kInBf16 ? dense_pair_bf16() : dense_pair_f16();
+}
+
 const void* dense_tile(int x, int kind, int tile, int mode) {
   const bool b = x == detail::kInBf16;
   switch (kind) {
@@ -378,7 +384,30 @@ struct GradPlan {
   int blocks, rows;     // of the column sums
   size_t dz, columns, partial;
   Plan of_x, of_w;
+  bool together;        // of_x and of_w in one launch
 };
+
+// Both products in tiles of 128 x 128 that have a CU each, or one after the other: by sizes
+// alone, so that a gradient is the same with and without the others, and where neither alone
+// takes more than kAlone times its best.
+constexpr double kAlone = 1.6;
+void pair_plan(const hipgemm_linear_grad_desc& d, GradPlan& p) {
+  p.of_x = plan_of(hk::kDenseNN, d.M, d.K, (int)p.cols);
+  p.of_w = plan_of(hk::kDenseTN, (int)p.cols, d.K, d.M);
+  const hk::TileShape s = hk::kDenseTiles[0];
+  const long long across = ((long long)d.K + s.bn - 1) / s.bn;
+  const long long x = (((long long)d.M + s.bm - 1) / s.bm) * across;
+  const long long w = ((p.cols + s.bm - 1) / s.bm) * across;
+  const int steps_x = (int)((p.cols + 63) / 64), steps_w = (int)(((long long)d.M + 63) / 64);
+  const double of_x = kLaunch + steps_x * kTime[0].of_x + kTime[0].end;
+  const double of_w = kLaunch + steps_w * kTime[0].of_w + kTime[0].end;
+  const double us = of_x > of_w ? of_x : of_w;
+  p.together = x > 0 && w > 0 && x + w <= kCus && us < p.of_x.us + p.of_w.us &&
+               of_x <= kAlone * p.of_x.us && of_w <= kAlone * p.of_w.us;
+  if (!p.together) return;
+  p.of_x = {0, 1, steps_x, x, us, 0};
+  p.of_w = {0, 1, steps_w, w, us, 0};
+}
 GradPlan grad_plan(const hipgemm_linear_grad_desc& d) {
   GradPlan p{};
   p.cols = d.gated ? 2ll * d.N : d.N;
@@ -397,13 +426,10 @@ GradPlan grad_plan(const hipgemm_linear_grad_desc& d) {
   if (p.blocks < 1) p.blocks = 1;
   p.dz = p.own ? padded(2ull * (size_t)d.M * (size_t)p.ldz) : 0;
   p.columns = d.db ? padded(4ull * (size_t)p.blocks * (size_t)p.cols) : 0;
+  pair_plan(d, p);
   size_t part = 0;
-  if (d.dx) {
-    p.of_x = plan_of(hk::kDenseNN, d.M, d.K, (int)p.cols);
-    part = partial_bytes(hk::kDenseNN, p.of_x, d.M, d.K);
-  }
+  if (d.dx) part = partial_bytes(hk::kDenseNN, p.of_x, d.M, d.K);
   if (d.dw) {
-    p.of_w = plan_of(hk::kDenseTN, (int)p.cols, d.K, d.M);
     const size_t w = partial_bytes(hk::kDenseTN, p.of_w, (int)p.cols, d.K);
     if (w > part) part = w;
   }
@@ -465,33 +491,34 @@ hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
   }
   const uint8_t* z = p.own ? dz : static_cast<const uint8_t*>(d.dy);
   const long long ldz = p.own ? p.ldz : d.lddy;
-  if (d.dx && d.M > 0 && d.K > 0) {
-    DenseArgs g{};
-    g.a = z;
-    g.lda = 2 * ldz;
-    g.b = static_cast<const uint8_t*>(d.weight);
-    g.ldb = 2 * d.ldw;
-    g.M = d.M;
-    g.N = d.K;
-    g.K = (int)p.cols;
-    plain_epilogue(g, d.dx, d.lddx, d.dx_dtype);
-    const hipError_t e = product(d.type, hk::kDenseNN, p.of_x, g, partial, stream);
+  const bool of_x = d.dx && d.M > 0 && d.K > 0, of_w = d.dw && d.N > 0 && d.K > 0;
+  DenseArgs x{}, w{};
+  x.a = w.a = z;
+  x.lda = w.lda = 2 * ldz;
+  x.b = static_cast<const uint8_t*>(d.weight);
+  x.ldb = 2 * d.ldw;
+  w.b = static_cast<const uint8_t*>(d.x);
+  w.ldb = 2 * d.ldx;
+  x.M = w.K = d.M;
+  x.K = w.M = (int)p.cols;
+  x.N = w.N = d.K;
+  plain_epilogue(x, d.dx, d.lddx, d.dx_dtype);
+  plain_epilogue(w, d.dw, d.lddw, d.dw_dtype);
+  if (of_x && of_w && p.together) {
+    const hk::TileShape s = hk::kDenseTiles[0];
+    const int across = (d.K + s.bn - 1) / s.bn;
+    x.slices = w.slices = 1;
+    x.group_m = default_group_m((x.M + s.bm - 1) / s.bm, across);
+    w.group_m = default_group_m((w.M + s.bm - 1) / s.bm, across);
+    DensePair pair{x, w, (int)p.of_x.units};
+    return launch(hk::dense_pair(d.type), dim3((unsigned)(p.of_x.units + p.of_w.units)), pair,
+                  stream);
+  }
+  if (of_x) {
+    const hipError_t e = product(d.type, hk::kDenseNN, p.of_x, x, partial, stream);
     if (e != hipSuccess) return e;
   }
-  if (d.dw && d.N > 0 && d.K > 0) {
-    DenseArgs g{};
-    g.a = z;
-    g.lda = 2 * ldz;
-    g.b = static_cast<const uint8_t*>(d.x);
-    g.ldb = 2 * d.ldx;
-    g.M = (int)p.cols;
-    g.N = d.K;
-    g.K = d.M;
-    plain_epilogue(g, d.dw, d.lddw, d.dw_dtype);
-    const hipError_t e = product(d.type, hk::kDenseTN, p.of_w, g, partial, stream);
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
+  return of_w ? product(d.type, hk::kDenseTN, p.of_w, w, partial, stream) : hipSuccess;
 }
 
 hipgemm_linear_plan shown(const Plan& p) {

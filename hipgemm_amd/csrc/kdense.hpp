@@ -12,7 +12,23 @@ namespace kernels {
 template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi, bool kSplit, bool kOnce>
 __global__ __launch_bounds__(256, 1) void k_dense_tile(detail::DenseArgs g) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsBytes];
-  detail::dense_tile_body<Cfg, kX, kACol, kBCol, kEpi, kSplit, kOnce>(g, (detail::lds_u8*)lds);
+  detail::dense_tile_body<Cfg, kX, kACol, kBCol, kEpi, kSplit, kOnce>(
+      g, (detail::lds_u8*)lds, blockIdx.x, gridDim.x);
+}
+
+// The two products of a backward pass, in tiles that have a CU each: half of the chip is all
+// that either takes (1531 x 2001 x 1000: 18 and 17 us one after the other, 24 together).
+template <int kX>
+__global__ __launch_bounds__(256, 1) void k_dense_tile_pair(detail::DensePair g) {
+  using Cfg = detail::CfgDense<kDenseTiles[0].bm, kDenseTiles[0].bn, 4>;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[Cfg::kLdsBytes];
+  const int b = blockIdx.x;
+  if (b < g.first)
+    detail::dense_tile_body<Cfg, kX, false, true, detail::kEpiPlain, false>(
+        g.x, (detail::lds_u8*)lds, b, g.first);
+  else
+    detail::dense_tile_body<Cfg, kX, true, true, detail::kEpiPlain, false>(
+        g.w, (detail::lds_u8*)lds, b - g.first, gridDim.x - g.first);
 }
 
 template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi>

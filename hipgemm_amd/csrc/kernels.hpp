@@ -90,6 +90,8 @@ const void* moe_vec_down(int w, int s, int lk, int h);
 // kDenseGated (both along, gate and up rows); tile: index of kDenseTiles.
 enum { kDenseNT = 0, kDenseRes = 1, kDenseNN = 2, kDenseTN = 3, kDenseGated = 4 };
 const void* dense_tile(int x, int kind, int tile, int mode);
+// kDenseNN and kDenseTN in one launch, tiles of kDenseTiles[0].
+const void* dense_pair(int x);
 // mode: bit 0 K-slices, bit 1 the second operand is read once (one row of tiles).
 enum { kDenseSplit = 1, kDenseOnce = 2 };
 // A few rows (kdense_rows.hip); mt: tiles of 16 rows of x (1, 2, 4).

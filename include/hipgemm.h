@@ -585,7 +585,8 @@ hipError_t hipgemm_linear_backward(const hipgemm_linear_grad_desc *desc,
  * where not asked for) run for a descriptor's sizes: tiles of tile_rows x tile_columns
  * results (gated: of gate and up columns together), or tile_rows 0 for the kernel of a few
  * rows; the slices along K, whose sums are added by a second kernel; and the first columns
- * (0: none) that tiles of 256 x 256 do in a launch of their own.  No GPU needed; no
+ * (0: none) that tiles of 256 x 256 do in a launch of their own.  (dx and dw both whole in
+ * tiles of 128 x 128, not more than the CUs together: one launch.)  No GPU needed; no
  * reference counterpart. */
 typedef struct hipgemm_linear_plan {
   int tile_rows, tile_columns, slices, first_columns;

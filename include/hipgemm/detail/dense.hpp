@@ -103,6 +103,12 @@ struct DenseArgs {
   DenseEpi epi;
 };
 
+// Two products of one launch: `first` workgroups for x, the others for w.
+struct DensePair {
+  DenseArgs x, w;
+  int first;
+};
+
 template <int BM, int BN, int S>
 struct CfgDense {
   static constexpr int kBM = BM, kBN = BN, kStages = S;
@@ -307,7 +313,8 @@ __device__ __forceinline__ void mfma_acc(i32x4 a, i32x4 b, f32x4& c) {
 }
 
 template <class Cfg, int kX, bool kACol, bool kBCol, int kEpi, bool kSplit, bool kOnce = false>
-__device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds) {
+__device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds, int block,
+                                                int blocks) {
   constexpr bool kGated = kEpi == kEpiGated, kRes = kEpi == kEpiResidual;
   constexpr int S = Cfg::kStages, FA = Cfg::kFA, FB = Cfg::kFB;
   constexpr int kBK = Cfg::kBK, kDma = Cfg::kDma;
@@ -331,7 +338,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
   const int units = kSplit ? tiles * g.slices : tiles;
   const int steps = kSplit ? g.slice_steps : (int)(((long long)g.K + kBK - 1) / kBK);
   const int steps_pad = max(S, steps);
-  const TileWalk walk = tile_walk(blockIdx.x, gridDim.x, units);
+  const TileWalk walk = tile_walk(block, blocks, units);
   int t = walk.first;
   if (t >= walk.end) return;
 
@@ -421,7 +428,7 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds)
     s.k0 = kSplit ? slice * steps * kBK : 0;
     s.kend = kSplit ? (int)min((long long)g.K, (long long)s.k0 + (long long)steps * kBK) : g.K;
     s.full = max(0, s.kend - s.k0) / kBK;
-    s.rot = (int)((blockIdx.x & 7u) * (unsigned)s.full / 8u);
+    s.rot = (int)(((unsigned)block & 7u) * (unsigned)s.full / 8u);
     s.a = s.b = s.b2 = make_rsrc(g.a, 0u);
     s.pa = g.a;
     s.pb = g.b;

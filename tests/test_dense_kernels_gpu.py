@@ -92,11 +92,10 @@ def test_forward_kernels(gpu, want, linear, gated, kind):
 
 # (kernel of dx or None, of dw or None), gated, sizes; kernels as above
 BACKWARD = [
-    (((64, 128, False, False), (128, 128, False, False)), False, (5, 5, 200)),
+    (((64, 128, False, False), (128, 128, True, False)), True, (2307, 520, 264)),
     (((64, 128, True, False), None), True, (131, 1032, 264)),
-    (((64, 128, True, False), None), False, (333, 1029, 264)),
-    ((None, (128, 128, True, False)), True, (1531, 520, 264)),
-    ((None, (128, 128, True, False)), False, (1531, 1029, 200)),
+    (((64, 128, True, False), None), False, (333, 4101, 264)),
+    (((64, 128, False, False), (128, 128, True, False)), False, (4099, 1029, 200)),
     (((128, 128, False, False), None), False, (2051, 133, 1032)),
     (((128, 128, True, False), None), True, (77, 2056, 4104)),
     (((256, 128, False, False), None), False, (2051, 133, 2056)),
@@ -133,6 +132,33 @@ def test_backward_kernels(gpu, want, gated, size):
         bounds = backward64(dy, x, w, pre, "silu", gated, grad)
         for name, t in zip(("dx", "dw", "db"), grads):
             check(name, t, *bounds[name])
+
+
+@pytest.mark.parametrize("M,N,K,gated", ((5, 5, 200, False), (1029, 605, 264, False),
+                                         (77, 5, 4104, False), (777, 136, 1000, True),
+                                         (1531, 2001, 1000, False), (1, 8, 8, True)))
+def test_both_products_in_one_launch(gpu, M, N, K, gated):
+    """Whole tiles of 128 x 128 with a CU each; a gradient alone has the same bits."""
+    plans = backward_plans(M, N, K, gated)
+    assert plans == ((128, 128, 1, 0),) * 2
+    rows = 2 * N if gated else N
+    assert (-(-M // 128) + -(-rows // 128)) * -(-K // 128) <= 256
+    f = hg.gated_linear_backward if gated else hg.linear_backward
+    for i, dtype in enumerate((BF, HF)):
+        g = torch.Generator(device="cuda").manual_seed(M + i)
+        x, w = amid(M, K, 1.0, dtype, g), amid(rows, K, K ** -0.5, dtype, g)
+        pre, dy = amid(M, rows, 1.0, F32, g), amid(M, N, 1.0, dtype, g, beside=3)
+        grad = (F32, dtype)[i]
+        torch.cuda.empty_cache()
+        scratch = torch.full((1 << 28,), NAN, device="cuda")
+        del scratch
+        both = f(dy, x, w, pre, activation="silu", need_bias=True, grad_dtype=grad)
+        bounds = backward64(dy, x, w, pre, "silu", gated, grad)
+        for name, t in zip(("dx", "dw", "db"), both):
+            check(name, t, *bounds[name])
+        dx, _, _ = f(dy, x, w, pre, activation="silu", need_weight=False, grad_dtype=grad)
+        _, dw, _ = f(dy, x, w, pre, activation="silu", need_x=False, grad_dtype=grad)
+        assert torch.equal(dx, both[0]) and torch.equal(dw, both[1])
 
 
 @pytest.mark.parametrize("M,N,K", ((70, 72, 136), (777, 200, 1032), (9, 1032, 264)))
