@@ -11,6 +11,7 @@ record no gradient: hipgemm_amd.torch_dense has operators and modules that do.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import struct
@@ -49,8 +50,11 @@ class LinearGradDesc(ctypes.Structure):
 
 
 _DESC_BYTES = ctypes.sizeof(LinearDesc)
-# A LinearDesc's bytes, in a fifth of the time that the structure takes to fill.
+# The structures' bytes, in a fifth of the time that they take to fill.
 _linear_desc = struct.Struct("@N7PN5q10i").pack
+_grad_desc = struct.Struct("@N8PN6q11i0q").pack
+_MAX_LD = 1 << 21  # of rows that the products read
+_NOTHING = contextlib.nullcontext()
 _GRAD_BYTES = ctypes.sizeof(LinearGradDesc)
 
 
@@ -118,6 +122,18 @@ def _forward_bytes(M, N, K, kind, device):
     d = LinearDesc(size=_DESC_BYTES, M=M, N=N, K=K, gated=int(kind == 2), type=1,
                    residual=int(kind == 1))
     return linear_workspace_size(d)
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_bytes(M, N, K, gated, code, act, dyt, aligned, whole, need_x, need_weight,
+                    need_bias, device):
+    """Workspace of a backward call, of whose addresses and strides only those of dy matter:
+    whether it starts on 16 bytes, and its rows (`whole`)."""
+    d = LinearGradDesc(size=_GRAD_BYTES, M=M, N=N, K=K, gated=int(gated), type=code,
+                       activation=act, dy_type=dyt, dy=16 if aligned else 2,
+                       lddy=8 if whole else 1, dx=int(need_x), dw=int(need_weight),
+                       db=int(need_bias))
+    return linear_backward_workspace_size(d)
 
 
 def _operand(t, name, dtype, index):
@@ -255,20 +271,19 @@ def _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias, gr
     bt = outputs.get(bias_dtype)
     if bt is None:
         _bad("bias_dtype must be bfloat16, float16 or float32")
-    with _on(stream):
+    act = ACTIVATIONS[activation]
+    need = _backward_bytes(M, N, K, gated, code, act, dyt, dyp % 16 == 0,
+                           lddy % 8 == 0 and lddy <= _MAX_LD, need_x, need_weight, need_bias, index)
+    with _on(stream) if stream is not None else _NOTHING:
         dx = x.new_empty((M, K)) if need_x else None
         dw = x.new_empty((rows, K), dtype=grad_dtype) if need_weight else None
         db = x.new_empty(rows, dtype=bias_dtype) if need_bias else None
-        dxp, dwp, dbp = (0 if t is None else t.data_ptr() for t in (dx, dw, db))
-        d = LinearGradDesc(_GRAD_BYTES, dyp, xp, wp, pp, dxp, dwp, dbp, 0, 0, lddy, ldx, ldw,
-                           ldp, K, K, M, N, K, int(gated), code, dyt, pt, outputs[x.dtype], ot,
-                           bt, ACTIVATIONS[activation])
-        at = ctypes.byref(d)
-        need = lib().hipgemm_linear_backward_workspace_size(at)
-        if need:
-            workspace = x.new_empty(need, dtype=torch.uint8)
-            d.workspace, d.workspace_bytes = workspace.data_ptr(), need
-    _launch(lib().hipgemm_linear_backward, "hipgemm_linear_backward", at, index, stream)
+        workspace = x.new_empty(need, dtype=torch.uint8) if need else None
+    d = _grad_desc(_GRAD_BYTES, dyp, xp, wp, pp, 0 if dx is None else dx.data_ptr(),
+                   0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
+                   workspace.data_ptr() if need else 0, need, lddy, ldx, ldw, ldp, K, K, M, N, K,
+                   int(gated), code, dyt, pt, outputs[x.dtype], ot, bt, act)
+    _launch(lib().hipgemm_linear_backward, "hipgemm_linear_backward", d, index, stream)
     return dx, dw, db
 
 

@@ -68,3 +68,26 @@ def test_packed_descriptor():
     values += list(range(100, 110))
     assert len(values) == len(hg.LinearDesc._fields_)
     assert _linear_desc(*values) == bytes(hg.LinearDesc(*values))
+    from hipgemm_amd.dense import _grad_desc
+    values = [ctypes.sizeof(hg.LinearGradDesc)] + [3 + 1000 ** 3 * i for i in range(15)]
+    values += list(range(100, 111))
+    assert len(values) == len(hg.LinearGradDesc._fields_)
+    assert _grad_desc(*values) == bytes(hg.LinearGradDesc(*values))
+
+
+def test_backward_workspace_by_kind():
+    """The cached sizes are those of the descriptors themselves."""
+    from hipgemm_amd.dense import _backward_bytes
+    size = ctypes.sizeof(hg.LinearGradDesc)
+    for M, N, K in ((1, 8, 8), (77, 264, 520), (333, 2056, 4104), (2051, 520, 264)):
+        for act, gated, dyt in ((0, 0, 1), (2, 0, 1), (0, 0, 0), (2, 1, 1)):
+            for dy in (4096, 4098, 4104):
+                for lddy in (N, N + 8, N + 1, (1 << 21) + 8):
+                    for needs in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1)):
+                        d = hg.LinearGradDesc(size=size, M=M, N=N, K=K, gated=gated, type=1,
+                                              activation=act, dy_type=dyt, dy=dy, lddy=lddy,
+                                              dx=needs[0], dw=needs[1], db=needs[2])
+                        whole = lddy % 8 == 0 and lddy <= 1 << 21
+                        got = _backward_bytes(M, N, K, bool(gated), 1, act, dyt, dy % 16 == 0,
+                                              whole, *map(bool, needs), 0)
+                        assert got == hg.linear_backward_workspace_size(d)
