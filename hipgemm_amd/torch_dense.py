@@ -14,10 +14,12 @@ bias of any strides and alignment, which are copied where they have to be), and 
 FakeTensorMode.  They may be captured in CUDA graphs.  CPU tensors raise HipGemmError:
 there is no CPU path.
 
-linear and gated_linear here are differentiable (once): where a gradient is wanted the
-forward pass keeps z in float32 (linear only with an activation) and the backward pass is
-hipgemm's linear_backward or gated_linear_backward.  Gradients come in their tensors'
-types; sums and z are fp32, dz is rounded to x's type.  A backward pass may be captured into
+linear and gated_linear here are differentiable, once and in reverse mode: where a gradient
+is wanted the forward pass keeps z in float32 (linear only with an activation) and the
+backward pass is hipgemm's linear_backward or gated_linear_backward.  Gradients come in
+their tensors' types; sums and z are fp32, dz is rounded to x's type.  The operators
+themselves record no gradient.  Tensors with a tangent of forward mode raise HipGemmError,
+and the operators wherever forward mode is on.  A backward pass may be captured into
 a graph, with leaves of its own: p.detach().requires_grad_() of each parameter, over the same
 memory.  (Leaves that an eager graph still alive has too end the process inside torch at the
 capture's end, whatever the operators: their accumulation belongs to that graph's stream.)
@@ -30,6 +32,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ACTIVATIONS, HipGemmError, dense
 from .torch_ops import _plain_buffers, _plain_eager
@@ -65,10 +68,34 @@ def _check_shapes(x, weight, bias, activation, residual, gated):
     return n
 
 
+def _refuse_tangents():
+    raise HipGemmError("linear and gated_linear have no forward-mode derivative")
+
+
+def _tangents(*tensors) -> bool:
+    """A tensor carries a tangent, or hides behind a transform whether it does; call it where
+    forward mode is on."""
+    return any(t is not None and (torch._C._functorch.is_functorch_wrapped_tensor(t)
+                                  or forward_ad.unpack_dual(t).tangent is not None)
+               for t in tensors)
+
+
+def _forward_mode() -> bool:
+    return forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
+
+
+def _op_checks():
+    """What an operator's body is given has lost its tangents, and torch would take them for
+    zeros.  (Calls whose tensors have been looked at turn forward mode off.)"""
+    if _forward_mode():
+        _refuse_tangents()
+
+
 @torch.library.custom_op("hipgemm::linear", mutates_args=())
 def _linear_op(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                activation: str = "none", residual: Optional[torch.Tensor] = None,
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    _op_checks()
     return dense.linear(_rows(x), _rows(weight), bias=_unit(bias), activation=activation,
                         residual=_unit(residual), out_dtype=out_dtype)
 
@@ -82,6 +109,7 @@ def _linear_fake(x, weight, bias=None, activation="none", residual=None, out_dty
 @torch.library.custom_op("hipgemm::gated_linear", mutates_args=())
 def _gated_op(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
               activation: str = "silu", out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    _op_checks()
     return dense.gated_linear(_rows(x), _rows(weight), bias=_unit(bias), activation=activation,
                               out_dtype=out_dtype)
 
@@ -99,6 +127,7 @@ def _linear_pre(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                 activation: str, residual: Optional[torch.Tensor],
                 out_dtype: Optional[torch.dtype],
                 gated: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    _op_checks()
     x, weight, bias = _rows(x), _rows(weight), _unit(bias)
     if gated:
         return dense.gated_linear(x, weight, bias=bias, activation=activation,
@@ -123,6 +152,7 @@ def _linear_grad(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, pre: t
                  activation: str, gated: bool, need_x: bool, need_weight: bool,
                  need_bias: bool, bias_dtype: torch.dtype
                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _op_checks()
     back = dense.gated_linear_backward if gated else dense.linear_backward
     dx, dw, db = back(_unit(dy), _rows(x), _rows(weight), pre if pre.dim() == 2 else None,
                       activation=activation, need_x=need_x, need_weight=need_weight,
@@ -151,6 +181,11 @@ def _setup(ctx, inputs, output):
 
 def _backward(ctx, dy, _):
     x, weight, pre = ctx.saved_tensors
+    if _forward_mode():
+        if _tangents(dy, x, weight):
+            _refuse_tangents()
+        with forward_ad._set_fwd_grad_enabled(False):
+            return _backward(ctx, dy, _)
     need = ctx.needs_input_grad
     dx = dw = db = dr = None
     if any(need[:3]):
@@ -171,6 +206,11 @@ def _wanted(*tensors) -> bool:
 
 
 def _call(x, weight, bias, activation, residual, out_dtype, gated):
+    if _forward_mode():
+        if _tangents(x, weight, bias, residual):
+            _refuse_tangents()
+        with forward_ad._set_fwd_grad_enabled(False):
+            return _call(x, weight, bias, activation, residual, out_dtype, gated)
     activation = activation or "none"
     if x.dim() != 2:
         lead = x.shape[:-1]
