@@ -213,16 +213,26 @@ long long partial_columns(int kind, int N) {
   const long long n = ((long long)N + 7) & ~7ll;
   return kind == hk::kDenseGated ? 2 * n : n;
 }
-size_t partial_bytes(int kind, const Plan& p, int M, int N) {
-  if (p.slices == 1) return 0;
-  return padded(4ull * (size_t)p.slices * (size_t)M * (size_t)partial_columns(kind, N - p.first));
+size_t partial_bytes(int kind, const Plan& p, int M, int N, int parts = 1) {
+  const int slices = parts * p.slices;
+  if (slices == 1) return 0;
+  return padded(4ull * (size_t)slices * (size_t)M * (size_t)partial_columns(kind, N - p.first));
 }
 
-hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream);
+// dz in parts (dense_slope_body) of so many bytes each.
+struct Parts {
+  int n = 1;
+  long long bytes = 0;
+  float scale = 1.0f;
+};
+
+hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream,
+               const Parts& parts = {});
 
 // g: operands, sizes and epilogue; ws: partial_bytes.
-hipError_t product(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream) {
-  if (!p.first) return run(x, kind, p, g, ws, stream);
+hipError_t product(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream,
+                   const Parts& parts = {}) {
+  if (!p.first) return run(x, kind, p, g, ws, stream, parts);
   DenseArgs part = g;
   part.N = p.first;
   const int cols = kind == hk::kDenseGated ? 128 : 256;
@@ -241,7 +251,10 @@ hipError_t product(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipSt
   return run(x, kind, p, g, ws, stream);
 }
 
-hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream) {
+// With parts of A, each part's sums go to `partial` as further slices.
+hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream_t stream,
+               const Parts& parts) {
+  const bool split = p.slices > 1 || parts.n > 1;
   g.slices = p.slices;
   g.slice_steps = p.slice_steps;
   g.partial = static_cast<float*>(ws);
@@ -256,10 +269,22 @@ hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream
     const int cols = kind == hk::kDenseGated ? s.bn / 2 : s.bn;
     g.group_m = default_group_m((g.M + s.bm - 1) / s.bm, (g.N + cols - 1) / cols);
     const int once = s.bm == 64 && g.M <= 64 && kind != hk::kDenseNN ? hk::kDenseOnce : 0;
-    e = launch(hk::dense_tile(x, kind, p.tile, once | (p.slices > 1 ? hk::kDenseSplit : 0)),
-               dim3((unsigned)(p.units < kCus ? p.units : kCus)), g, stream);
+    const void* fn = hk::dense_tile(x, kind, p.tile, once | (split ? hk::kDenseSplit : 0));
+    const dim3 grid((unsigned)(p.units < kCus ? p.units : kCus));
+    e = launch(fn, grid, g, stream);
+    for (int n = 1; n < parts.n && e == hipSuccess; ++n) {
+      g.a += parts.bytes;
+      g.partial += (long long)p.slices * g.M * g.ldpart;
+      e = launch(fn, grid, g, stream);
+    }
+    g.partial = static_cast<float*>(ws);
   }
-  if (e != hipSuccess || p.slices == 1) return e;
+  if (e != hipSuccess || !split) return e;
+  if (parts.n > 1) {
+    g.part_slices = p.slices;
+    g.part_scale = parts.scale;
+    g.slices = parts.n * p.slices;
+  }
   const long long threads = (long long)g.M * ((g.N + 7) / 8);
   const void* fn = kind == hk::kDenseGated ? (const void*)&k_dense_reduce<kEpiGated>
                    : kind == hk::kDenseRes ? (const void*)&k_dense_reduce<kEpiResidual>
@@ -382,6 +407,8 @@ struct GradPlan {
   long long cols, ldz;  // of dz
   bool own;             // dz lies in the workspace
   int blocks, rows;     // of the column sums
+  int parts_x, parts_w; // of dz, that dx and dw are sums over
+  long long plane;      // elements of a part
   size_t dz, columns, partial;
   Plan of_x, of_w;
   bool together;        // of_x and of_w in one launch
@@ -404,9 +431,14 @@ void pair_plan(const hipgemm_linear_grad_desc& d, GradPlan& p) {
   const double us = of_x > of_w ? of_x : of_w;
   p.together = x > 0 && w > 0 && x + w <= kCus && us < p.of_x.us + p.of_w.us &&
                of_x <= kAlone * p.of_x.us && of_w <= kAlone * p.of_w.us;
-  if (!p.together) return;
-  p.of_x = {0, 1, steps_x, x, us, 0};
-  p.of_w = {0, 1, steps_w, w, us, 0};
+  if (p.together) {
+    p.of_x = {0, 1, steps_x, x, us, 0};
+    p.of_w = {0, 1, steps_w, w, us, 0};
+  }
+  // (Sums over parts go through memory: no columns apart, no launch with another product.)
+  if (p.parts_x > 1) p.of_x = plan_whole(hk::kDenseNN, d.M, d.K, (int)p.cols);
+  if (p.parts_w > 1) p.of_w = plan_whole(hk::kDenseTN, (int)p.cols, d.K, d.M);
+  if (p.parts_x > 1 || p.parts_w > 1) p.together = false;
 }
 GradPlan grad_plan(const hipgemm_linear_grad_desc& d) {
   GradPlan p{};
@@ -424,13 +456,18 @@ GradPlan grad_plan(const hipgemm_linear_grad_desc& d) {
   if (p.rows < 8) p.rows = 8;
   p.blocks = (d.M + p.rows - 1) / p.rows;
   if (p.blocks < 1) p.blocks = 1;
-  p.dz = p.own ? padded(2ull * (size_t)d.M * (size_t)p.ldz) : 0;
+  const int parts = d.type == HIPGEMM_IN_BF16 ? 3 : 2;
+  p.parts_x = !as_is(d) && d.dx && d.dx_dtype == HIPGEMM_OUT_F32 ? parts : 1;
+  p.parts_w = !as_is(d) && d.dw && d.dw_dtype == HIPGEMM_OUT_F32 ? parts : 1;
+  const size_t plane = padded(2ull * (size_t)d.M * (size_t)p.ldz);
+  p.plane = (long long)(plane / 2);
+  p.dz = p.own ? plane * (size_t)(p.parts_x > p.parts_w ? p.parts_x : p.parts_w) : 0;
   p.columns = d.db ? padded(4ull * (size_t)p.blocks * (size_t)p.cols) : 0;
   pair_plan(d, p);
   size_t part = 0;
-  if (d.dx) part = partial_bytes(hk::kDenseNN, p.of_x, d.M, d.K);
+  if (d.dx) part = partial_bytes(hk::kDenseNN, p.of_x, d.M, d.K, p.parts_x);
   if (d.dw) {
-    const size_t w = partial_bytes(hk::kDenseTN, p.of_w, (int)p.cols, d.K);
+    const size_t w = partial_bytes(hk::kDenseTN, p.of_w, (int)p.cols, d.K, p.parts_w);
     if (w > part) part = w;
   }
   p.partial = part;
@@ -468,6 +505,8 @@ hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
     s.dy_type = d.dy_type;
     s.p_type = d.pre_type;
     s.rows = p.rows;
+    s.parts = p.parts_x > p.parts_w ? p.parts_x : p.parts_w;
+    s.plane = p.plane;
     const dim3 grid((unsigned)((d.N + kSlopeColumns - 1) / kSlopeColumns), (unsigned)p.blocks);
     const bool b = d.type == HIPGEMM_IN_BF16;
     const void* fn = d.gated ? (b ? (const void*)&k_dense_slope<kInBf16, true>
@@ -514,11 +553,15 @@ hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
     return launch(hk::dense_pair(d.type), dim3((unsigned)(p.of_x.units + p.of_w.units)), pair,
                   stream);
   }
+  const float scale = d.type == HIPGEMM_IN_BF16 ? 1.0f / kRest<kInBf16> : 1.0f / kRest<kInF16>;
   if (of_x) {
-    const hipError_t e = product(d.type, hk::kDenseNN, p.of_x, x, partial, stream);
+    const hipError_t e = product(d.type, hk::kDenseNN, p.of_x, x, partial, stream,
+                                 Parts{p.parts_x, 2 * p.plane, scale});
     if (e != hipSuccess) return e;
   }
-  return of_w ? product(d.type, hk::kDenseTN, p.of_w, w, partial, stream) : hipSuccess;
+  return of_w ? product(d.type, hk::kDenseTN, p.of_w, w, partial, stream,
+                        Parts{p.parts_w, 2 * p.plane, scale})
+              : hipSuccess;
 }
 
 hipgemm_linear_plan shown(const Plan& p) {

@@ -126,13 +126,14 @@ def _forward_bytes(M, N, K, kind, device):
 
 @functools.lru_cache(maxsize=4096)
 def _backward_bytes(M, N, K, gated, code, act, dyt, aligned, whole, need_x, need_weight,
-                    need_bias, device):
+                    need_bias, device, dw_type=OUT_BF16):
     """Workspace of a backward call, of whose addresses and strides only those of dy matter:
-    whether it starts on 16 bytes, and its rows (`whole`)."""
+    whether it starts on 16 bytes, and its rows (`whole`); and of whose results' types that of
+    dw, since dx has the operands'."""
     d = LinearGradDesc(size=_GRAD_BYTES, M=M, N=N, K=K, gated=int(gated), type=code,
                        activation=act, dy_type=dyt, dy=16 if aligned else 2,
                        lddy=8 if whole else 1, dx=int(need_x), dw=int(need_weight),
-                       db=int(need_bias))
+                       db=int(need_bias), dw_dtype=dw_type)
     return linear_backward_workspace_size(d)
 
 
@@ -273,7 +274,8 @@ def _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias, gr
         _bad("bias_dtype must be bfloat16, float16 or float32")
     act = ACTIVATIONS[activation]
     need = _backward_bytes(M, N, K, gated, code, act, dyt, dyp % 16 == 0,
-                           lddy % 8 == 0 and lddy <= _MAX_LD, need_x, need_weight, need_bias, index)
+                           lddy % 8 == 0 and lddy <= _MAX_LD, need_x, need_weight, need_bias, index,
+                           ot)
     with _on(stream) if stream is not None else _NOTHING:
         dx = x.new_empty((M, K)) if need_x else None
         dw = x.new_empty((rows, K), dtype=grad_dtype) if need_weight else None
@@ -321,7 +323,8 @@ def linear_backward(dy, x, weight, pre=None, *, activation=None, need_x: bool = 
     dy (M, N): bfloat16, float16 or float32.  pre: linear's z (save_pre); not needed without
     an activation.  dx has x's type, dweight grad_dtype (bfloat16, float16 or float32; x's
     type where None) and dbias bias_dtype (grad_dtype where None).  dz is rounded to x's type
-    for the two products; sums are fp32."""
+    for the two products, half a step of every term; a float32 dweight is summed over dz in 24
+    bits instead, at three times (bfloat16) or twice the operations.  Sums are fp32."""
     return _backward(dy, x, weight, pre, activation, need_x, need_weight, need_bias,
                      grad_dtype, bias_dtype, False, stream)
 

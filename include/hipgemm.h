@@ -556,8 +556,10 @@ hipError_t hipgemm_linear(const hipgemm_linear_desc *desc, hipStream_t stream);
  *
  * each where its pointer is not NULL.  (The residual's gradient is dy.)  z is read from
  * pre (pre_type HIPGEMM_IN_*), as the forward pass left it; not needed where activation is
- * NONE and not gated.  dz is rounded to `type` for the two products, not for db; sums are
- * fp32, in an order that depends on the sizes only.  Slopes: relu'(0) = 0.  With M == 0, dw
+ * NONE and not gated.  dz is rounded to `type` for the products of 16-bit results, and held
+ * to fp32's 24 bits for float32 ones (in parts of `type`, three of bf16 or two of fp16, with
+ * a product each; values past fp16's range are infinite) and for db; sums are fp32, in an
+ * order that depends on sizes and types only.  Slopes: relu'(0) = 0.  With M == 0, dw
  * and db are zeros.  Requirements as above; dy, pre: aligned to their element.  Workspace:
  * hipgemm_linear_backward_workspace_size bytes for the descriptor (its pointers, strides
  * and types matter), as above.  No reference counterpart.
@@ -586,8 +588,9 @@ hipError_t hipgemm_linear_backward(const hipgemm_linear_grad_desc *desc,
  * results (gated: of gate and up columns together), or tile_rows 0 for the kernel of a few
  * rows; the slices along K, whose sums are added by a second kernel; and the first columns
  * (0: none) that tiles of 256 x 256 do in a launch of their own.  (dx and dw both whole in
- * tiles of 128 x 128, not more than the CUs together: one launch.)  No GPU needed; no
- * reference counterpart. */
+ * tiles of 128 x 128, not more than the CUs together: one launch.  A float32 dx or dw: the
+ * kernel of each part of dz, all added by a second.)  No GPU needed; no reference
+ * counterpart. */
 typedef struct hipgemm_linear_plan {
   int tile_rows, tile_columns, slices, first_columns;
 } hipgemm_linear_plan;

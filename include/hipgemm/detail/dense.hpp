@@ -100,6 +100,8 @@ struct DenseArgs {
   int slices, slice_steps;  // kSplit: K-slices of 64 slice_steps
   float* partial;           // slices x M x ldpart
   long long ldpart;
+  int part_slices;          // slices of a part of dz (dense_slope_body), or 0: of the whole
+  float part_scale;         // of a part's sums to those of the part before
   DenseEpi epi;
 };
 
@@ -858,7 +860,9 @@ __device__ __forceinline__ void dense_tile_body(const DenseArgs& g, lds_u8* lds,
 
 // ---- K-slices' sums -----------------------------------------------------------
 
-// A thread per row and eight columns: slices in order, then the epilogue.
+// A thread per row and eight columns: slices in order, then the epilogue.  Where the slices
+// are those of dz's parts, each part's sums count part_scale of the one before; an infinite or
+// NaN sum of the first part is the result (rests of zero times an infinite operand are NaN).
 template <int kEpi>
 __device__ __forceinline__ void dense_reduce_body(const DenseArgs& g) {
   constexpr bool kGated = kEpi == kEpiGated;
@@ -869,10 +873,28 @@ __device__ __forceinline__ void dense_reduce_body(const DenseArgs& g) {
   if (row >= g.M) return;
   float v[8] = {}, u[8] = {};
   const uint8_t* p = reinterpret_cast<const uint8_t*>(g.partial);
+  float scale = 1.0f;
+  bool finite[8] = {};
   for (int s = 0; s < g.slices; ++s) {
     const long long o = ((long long)s * g.M + row) * g.ldpart + col;
     float w[8];
     load8(p, o, kInF32, w);
+    if constexpr (kEpi == kEpiPlain) {
+      if (g.part_slices && s && s % g.part_slices == 0) {
+        if (s == g.part_slices) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            finite[e] = __builtin_fabsf(v[e]) < __builtin_inff();
+        }
+        scale *= g.part_scale;
+      }
+      if (g.part_slices) {
+        const bool rest = s >= g.part_slices;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w[e] = rest && !finite[e] ? 0.0f : w[e] * scale;
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += w[e];
     if constexpr (kGated) {
@@ -939,11 +961,32 @@ struct SlopeArgs {
   int M, N;        // of dy; dz has 2 N columns where gated
   int act, dy_type, p_type;
   int rows;        // of a block
+  int parts;       // of dz: matrices of `plane` elements
+  long long plane;
 };
 
+// What rounding to the operands' type left of v, times kRest (one that is infinite or NaN
+// leaves nothing).  Rests of fp16 values are scaled into its range.
+template <int kX>
+constexpr float kRest = kX == kInBf16 ? 1.0f : 2048.0f;
+template <int kX>
+__device__ __forceinline__ void rest8(float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const uint32_t d = narrow2(v[e], v[e + 1], kX == kInBf16);
+    const float lo = v[e] - widen(d & 0xffffu, kX), hi = v[e + 1] - widen(d >> 16, kX);
+    v[e] = __builtin_fabsf(lo) < __builtin_inff() ? lo * kRest<kX> : 0.0f;
+    v[e + 1] = __builtin_fabsf(hi) < __builtin_inff() ? hi * kRest<kX> : 0.0f;
+  }
+}
+
 // dz = dy act'(z);  gated, z = [g | u]: [dy u act'(g) | dy act(g)].  Rounded to the
-// operands' type, as the matrix instructions take it; column sums are of the values
-// before that, in fp32.  A thread has eight columns and every eighth row of the block's.
+// operands' type, as the matrix instructions take it: half a step of every term of dx and dw,
+// which are rounded to that type themselves.  For float32 results dz has further parts, each
+// the rest that rounding the one before left, to 24 bits (bf16: three parts, fp16: two), and
+// the products are sums over them (4096 x 16384 x 4096 bf16, dx and dw: 916 us, with dw in
+// float32 1938).  Column sums are of the values before rounding, in fp32.
+// A thread has eight columns and every eighth row of the block's.
 // Columns from N to the padded row's end are written as zeros.
 template <int kX, bool kGated>
 __device__ __forceinline__ void dense_slope_body(const SlopeArgs& g, float* sums) {
@@ -968,6 +1011,13 @@ __device__ __forceinline__ void dense_slope_body(const SlopeArgs& g, float* sums
       if constexpr (kGated) r.u = raw8(g.pre, row * g.ldp + g.N + col, g.p_type);
     }
     return r;
+  };
+  auto store = [&](long long at, float (&v)[8]) {
+    store8(g.dz, at, kOut, v);
+    for (int p = 1; p < g.parts; ++p) {
+      rest8<kX>(v);
+      store8(g.dz, p * g.plane + at, kOut, v);
+    }
   };
   auto finish = [&](long long row, const Row& r) {
     float dy[8] = {}, z[8] = {}, u[8] = {};
@@ -998,14 +1048,14 @@ __device__ __forceinline__ void dense_slope_body(const SlopeArgs& g, float* sums
         a[e] *= dy[e];
         sum[kParts - 1][e] += a[e];
       }
-      if (g.dz) store8(g.dz, row * g.lddz + g.N + col, kOut, a);
+      if (g.dz) store(row * g.lddz + g.N + col, a);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = dy[e] * slope(z[e], g.act);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[0][e] += d[e];
-    if (g.dz) store8(g.dz, row * g.lddz + col, kOut, d);
+    if (g.dz) store(row * g.lddz + col, d);
   };
   if (live)
     for (long long row = first + ty; row < end; row += kTy) finish(row, fetch(row));
