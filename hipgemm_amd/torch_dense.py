@@ -177,6 +177,8 @@ def _setup(ctx, inputs, output):
     ctx.bias_dtype = x.dtype if bias is None else bias.dtype
     ctx.residual_dtype = None if residual is None else residual.dtype
     ctx.mark_non_differentiable(output[1])
+    # z has no gradient: none is made (zeros of z's size, in float32, for every pass).
+    ctx.set_materialize_grads(False)
 
 
 def _backward(ctx, dy, _):
@@ -188,6 +190,8 @@ def _backward(ctx, dy, _):
             return _backward(ctx, dy, _)
     need = ctx.needs_input_grad
     dx = dw = db = dr = None
+    if dy is None:
+        return (None,) * 7
     if any(need[:3]):
         dx, dw, db = torch.ops.hipgemm.linear_backward(
             dy, x, weight, pre, ctx.activation, ctx.gated, need[0], need[1], need[2],
