@@ -149,8 +149,9 @@ def _operand(t, name, dtype, index):
         _bad(f"{name} must have unit stride along its rows")
     if rows <= 1:
         ld = cols
-    if (at % 16 or ld % 8 or ld < cols) and rows and cols:
-        _bad(f"rows of {name} must start on 16 bytes")
+    if (at % 16 or ld % 8 or not cols <= ld <= _MAX_LD) and rows and cols:
+        _bad(f"rows of {name} must start on 16 bytes, not overlap and be at most {_MAX_LD} "
+             f"elements apart, got a stride of {ld}")
     return ld, at
 
 
@@ -294,7 +295,7 @@ def linear(x, weight, *, bias=None, activation=None, residual=None, out_dtype=No
     """out[m, n] = round(act(z[m, n]) + residual[m, n]), z = x @ weight.T + bias.
 
     x (M, K) and weight (N, K): both bfloat16 or both float16, K a multiple of 8, rows of
-    unit stride that start on 16 bytes.  bias (N) and residual (M, N): bfloat16, float16
+    unit stride that start on 16 bytes, 2^21 elements apart at most.  bias (N) and residual (M, N): bfloat16, float16
     or float32.  activation as for gemm().  out_dtype: bfloat16, float16 or float32, x's
     where None.  out may be residual itself and overlaps nothing else.  Sums are fp32, and
     everything after them until the one rounding.  save_pre: returns (out, z), as

@@ -36,9 +36,17 @@ from torch.autograd import forward_ad
 
 from . import ACTIVATIONS, HipGemmError, dense
 from .torch_ops import _plain_buffers, _plain_eager
-from .torch_serving import _rows
+from .torch_serving import _rows as _aligned_rows
 
 __all__ = ["linear", "gated_linear", "DenseLinear", "GatedMLP"]
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x where its rows are as the products take them, else a copy: also of rows further apart
+    than they address, as the last token's of each of several long sequences."""
+    if x.dim() == 2 and x.shape[0] > 1 and x.stride(0) > dense._MAX_LD:
+        return x.clone(memory_format=torch.contiguous_format)
+    return _aligned_rows(x)
 
 
 def _unit(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
