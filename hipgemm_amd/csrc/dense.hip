@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void k_dense_columns(const float* columns, int
 int in_bytes(int type) { return type == kInF32 ? 4 : 2; }
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// 256 rows of an operand, and of a result, are addressed with 31 bits.
+// 256 rows of an operand are addressed with 31 bits (results, dy and z with 64).
 constexpr long long kMaxLd = 1 << 21;
 constexpr int kMaxRows = 1 << 30;
 constexpr size_t kAlign = 256;
@@ -297,7 +297,7 @@ bool operand(const void* p, long long ld, long long columns) {
   return p && aligned(p, 16) && ld >= columns && ld % 8 == 0 && ld <= kMaxLd;
 }
 bool result(const void* p, long long ld, long long columns, int out) {
-  return p && aligned(p, (uintptr_t)out_bytes(out)) && ld >= columns && ld <= kMaxLd;
+  return p && aligned(p, (uintptr_t)out_bytes(out)) && ld >= columns;
 }
 
 bool common(int M, int N, int K, int gated, int type, int act) {
