@@ -76,6 +76,26 @@ def _check_shapes(x, weight, bias, activation, residual, gated):
     return n
 
 
+def _fake_shapes(x, weight, bias, activation, residual, out_dtype, gated):
+    """_check_shapes, and what the kernels refuse by types and devices: a trace refuses what
+    the call itself would."""
+    n = _check_shapes(x, weight, bias, activation, residual, gated)
+    operands, inputs, outputs = dense._types()
+    if x.dtype not in operands or weight.dtype != x.dtype:
+        raise HipGemmError(f"x and weight must both be bfloat16 or float16, got {x.dtype} and "
+                           f"{weight.dtype}")
+    if x.shape[1] % 8:
+        raise HipGemmError(f"K must be a multiple of 8, got {x.shape[1]}")
+    for name, t in (("bias", bias), ("residual", residual)):
+        if t is not None and t.dtype not in inputs:
+            raise HipGemmError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if out_dtype is not None and out_dtype not in outputs:
+        raise HipGemmError("out_dtype must be bfloat16, float16 or float32")
+    if any(t is not None and t.device != x.device for t in (weight, bias, residual)):
+        raise HipGemmError(f"all tensors must be on {x.device}")
+    return n
+
+
 def _refuse_tangents():
     raise HipGemmError("linear and gated_linear have no forward-mode derivative")
 
@@ -110,7 +130,7 @@ def _linear_op(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
 @_linear_op.register_fake
 def _linear_fake(x, weight, bias=None, activation="none", residual=None, out_dtype=None):
-    n = _check_shapes(x, weight, bias, activation, residual, False)
+    n = _fake_shapes(x, weight, bias, activation, residual, out_dtype, False)
     return x.new_empty((x.shape[0], n), dtype=out_dtype or x.dtype)
 
 
@@ -124,7 +144,7 @@ def _gated_op(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor
 
 @_gated_op.register_fake
 def _gated_fake(x, weight, bias=None, activation="silu", out_dtype=None):
-    n = _check_shapes(x, weight, bias, activation, None, True)
+    n = _fake_shapes(x, weight, bias, activation, None, out_dtype, True)
     return x.new_empty((x.shape[0], n), dtype=out_dtype or x.dtype)
 
 
@@ -149,7 +169,7 @@ def _linear_pre(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
 
 @_linear_pre.register_fake
 def _linear_pre_fake(x, weight, bias, activation, residual, out_dtype, gated):
-    n = _check_shapes(x, weight, bias, activation, residual, gated)
+    n = _fake_shapes(x, weight, bias, activation, residual, out_dtype, gated)
     pre = (x.shape[0], weight.shape[0]) if gated or ACTIVATIONS[activation] else (0,)
     return (x.new_empty((x.shape[0], n), dtype=out_dtype or x.dtype),
             x.new_empty(pre, dtype=torch.float32))
