@@ -346,9 +346,13 @@ hipError_t forward(const hipgemm_linear_desc& d, hipStream_t stream) {
   DenseArgs g{};
   g.a = static_cast<const uint8_t*>(d.x);
   g.b = static_cast<const uint8_t*>(d.weight);
-  g.lda = 2 * d.ldx;
-  g.ldb = 2 * d.ldw;
-  g.up = 2 * d.ldw * d.N;
+  // Strides of operands without elements may be anything and are not looked at: ranges of
+  // buffers are made of them, which have to be empty.
+  if (d.K > 0) {
+    g.lda = 2 * d.ldx;
+    g.ldb = 2 * d.ldw;
+    g.up = 2 * d.ldw * d.N;
+  }
   g.M = d.M;
   g.N = d.N;
   g.K = d.K;
@@ -533,11 +537,11 @@ hipError_t backward(const hipgemm_linear_grad_desc& d, hipStream_t stream) {
   const bool of_x = d.dx && d.M > 0 && d.K > 0, of_w = d.dw && d.N > 0 && d.K > 0;
   DenseArgs x{}, w{};
   x.a = w.a = z;
-  x.lda = w.lda = 2 * ldz;
+  if (d.M > 0 && d.N > 0) x.lda = w.lda = 2 * ldz;  // (as in forward)
   x.b = static_cast<const uint8_t*>(d.weight);
-  x.ldb = 2 * d.ldw;
+  if (d.N > 0) x.ldb = 2 * d.ldw;
   w.b = static_cast<const uint8_t*>(d.x);
-  w.ldb = 2 * d.ldx;
+  if (d.M > 0) w.ldb = 2 * d.ldx;
   x.M = w.K = d.M;
   x.K = w.M = (int)p.cols;
   x.N = w.N = d.K;
