@@ -420,8 +420,12 @@ struct GradPlan {
 
 // Both products in tiles of 128 x 128 that have a CU each, or one after the other: by sizes
 // alone, so that a gradient is the same with and without the others, and where neither alone
-// takes more than kAlone times its best.
-constexpr double kAlone = 1.6;
+// takes more than kAlone times its best by the estimates (bf16, with dz, us: both / the slowed one
+// alone, one after the other and together;  of dx at 1.22 times its best, 1531 x 2001 x 1000:
+// 42.8, 32.2 / 25.1, 31.8;  gated 1.19, 2048 x 704 x 1024: 38.4, 30.0 / 20.7, 23.9;  of dw at 1.44,
+// 2048 x 512 x 1024: 24.2, 19.8 / 16.8, 19.2;  past it, of dx gated at 1.56, 777 x 1400 x 1000: 39.8,
+// 37.3 / 25.8, 36.3;  1.84, 1024 x 1408 x 512: 35.5, 32.9 / 23.2, 32.5).
+constexpr double kAlone = 1.5;
 void pair_plan(const hipgemm_linear_grad_desc& d, GradPlan& p) {
   p.of_x = plan_of(hk::kDenseNN, d.M, d.K, (int)p.cols);
   p.of_w = plan_of(hk::kDenseTN, (int)p.cols, d.K, d.M);
