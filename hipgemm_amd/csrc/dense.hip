@@ -268,6 +268,9 @@ hipError_t run(int x, int kind, const Plan& p, DenseArgs& g, void* ws, hipStream
     const hk::TileShape s = hk::kDenseTiles[p.tile];
     const int cols = kind == hk::kDenseGated ? s.bn / 2 : s.bn;
     g.group_m = default_group_m((g.M + s.bm - 1) / s.bm, (g.N + cols - 1) / cols);
+    // Weights that one row of tiles reads once go past the caches (us, with / without: 17 x 8192 x
+    // 8192 29.7 / 32.5, gated 32 x 4096 x 8192 36.0 / 38.5, 64 x 8192 x 28672 117.4 / 120.5, 64 x 4096 x
+    // 14336 36.5 / 37.1; nowhere slower by more than 1 %).
     const int once = s.bm == 64 && g.M <= 64 && kind != hk::kDenseNN ? hk::kDenseOnce : 0;
     const void* fn = hk::dense_tile(x, kind, p.tile, once | (split ? hk::kDenseSplit : 0));
     const dim3 grid((unsigned)(p.units < kCus ? p.units : kCus));
